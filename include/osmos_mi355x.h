@@ -13,6 +13,7 @@
 #include "osmos/gpu/q4x_ops.h"
 #include "osmos/gpu/q8.h"
 #include "osmos/gpu/quant.h"
+#include "osmos_attn.h"
 
 #define OSMOS_LANE_MAX_PAIRS 4096 /* osmos_lane_tables' most (token, expert) pairs a step */
 

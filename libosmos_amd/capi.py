@@ -90,6 +90,48 @@ SIGS.update({
 })
 
 
+# include/osmos_attn.h
+
+class OsmosKv(ctypes.Structure):
+    _fields_ = [("data", P), ("scale", P), ("type", U32), ("layers", U32), ("pages", U32), ("page", U32), ("heads", U32),
+                ("dim", U32)]
+
+
+class OsmosKvStep(ctypes.Structure):
+    _fields_ = [("start", P), ("len", P), ("table", P), ("seq", P), ("n_seq", U32), ("n_tok", U32), ("max_tok", U32),
+                ("max_len", U32), ("seqs", U32), ("table_stride", U32)]
+
+
+class OsmosAttn(ctypes.Structure):
+    _fields_ = [("q", P), ("out", P), ("lse", P), ("q_stride", U64), ("q_head", U64), ("out_stride", U64),
+                ("out_head", U64), ("q_type", U32), ("out_type", U32), ("heads", U32), ("window", U32), ("scale", F32)]
+
+
+class OsmosKvRows(ctypes.Structure):
+    _fields_ = [("k", P), ("v", P), ("k_stride", U64), ("k_head", U64), ("v_stride", U64), ("v_head", U64), ("type", U32),
+                ("heads", U32), ("dim", U32)]
+
+
+class OsmosKvPool(ctypes.Structure):
+    _fields_ = [("ref", P), ("len", P), ("table", P), ("scratch", P), ("seqs", U32), ("table_stride", U32)]
+
+
+_KV, _ST, _AT, _PL = (ctypes.POINTER(t) for t in (OsmosKv, OsmosKvStep, OsmosAttn, OsmosKvPool))
+SIGS.update({
+    "osmos_kv_bytes": (U64, [_KV]),
+    "osmos_kv_append": (B, [_KV, U32, _ST, U32, P, U64, P, U64, P]),
+    "osmos_attn_workspace": (U64, [_AT, U32, U32, _ST]),
+    "osmos_attn_prompt": (B, [_AT, ctypes.POINTER(OsmosKvRows), _ST, P, U64, P]),
+    "osmos_attn_chunk": (B, [_AT, _KV, U32, _ST, P, U64, P]),
+    "osmos_attn_token": (B, [_AT, _KV, U32, _ST, P, U64, P]),
+    "osmos_kv_scratch": (U64, [_KV]),
+    "osmos_kv_grow": (B, [_KV, _PL, P, P, U32, P, P]),
+    "osmos_kv_fork": (B, [_KV, _PL, P, P, U32, P, P]),
+    "osmos_kv_free": (B, [_KV, _PL, P, U32, P]),
+    "osmos_kv_compact": (B, [_KV, _PL, P, P]),
+    "osmos_kv_copy": (B, [_KV, P, P, U32, P]),
+})
+
 
 # include/osmos/gpu/quant.h
 QUANT_Q5_K = 13
