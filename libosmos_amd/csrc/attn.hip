@@ -29,6 +29,440 @@ struct Kv {
   const float* scale;
 };
 
+// ---- the two 16-bit types the products are taken in ----
+typedef kv::f32x4 f32x4;
+typedef kv::u32x2 u32x2;
+typedef kv::u32x4 u32x4;
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+
+template <bool BF> struct Unit;
+template <> struct Unit<false> {
+  typedef _Float16 e;
+  typedef kv::f16x8 v8;
+  static __device__ inline f32x4 mfma16(v8 a, v8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
+  static __device__ inline f16x2 f8_low(uint32_t w) { return __builtin_amdgcn_cvt_scalef32_pk_f16_fp8((int) w, 1.0f, false); }
+  static __device__ inline f16x2 f8_high(uint32_t w) { return __builtin_amdgcn_cvt_scalef32_pk_f16_fp8((int) w, 1.0f, true); }
+};
+template <> struct Unit<true> {
+  typedef __bf16 e;
+  typedef kv::bf16x8 v8;
+  static __device__ inline f32x4 mfma16(v8 a, v8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
+  static __device__ inline bf16x2 f8_low(uint32_t w) { return __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((int) w, 1.0f, false); }
+  static __device__ inline bf16x2 f8_high(uint32_t w) { return __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((int) w, 1.0f, true); }
+};
+
+// 8 e4m3 values (two words) in the products' type: exact in either
+template <bool BF>
+__device__ inline typename Unit<BF>::v8 from_f8(u32x2 w) {
+  typename Unit<BF>::v8 r;
+#pragma unroll
+  for (int i = 0; i < 2; i++) {
+    const auto a = Unit<BF>::f8_low(w[i]), b = Unit<BF>::f8_high(w[i]);
+    r[4 * i] = a[0], r[4 * i + 1] = a[1], r[4 * i + 2] = b[0], r[4 * i + 3] = b[1];
+  }
+  return r;
+}
+
+// 8 values of q from `at` on in the products' type (an F32 q's rounded once)
+template <bool BF>
+__device__ inline typename Unit<BF>::v8 q8(const Args& a, uint64_t at) {
+  float x[8];
+  if (a.q_type == OSMOS_F32) kv::load8<OSMOS_F32>(a.q + at * 4, x);
+  else if (a.q_type == OSMOS_F16) kv::load8<OSMOS_F16>(a.q + at * 2, x);
+  else kv::load8<OSMOS_BF16>(a.q + at * 2, x);
+  typename Unit<BF>::v8 r;
+#pragma unroll
+  for (int i = 0; i < 8; i++) r[i] = (typename Unit<BF>::e) x[i];
+  return r;
+}
+
+__device__ inline void put4(const Args& a, uint64_t at, f32x4 y) {
+  if (a.out_type == OSMOS_F32) {
+    *(f32x4*) (a.out + at * 4) = y;
+  } else if (a.out_type == OSMOS_F16) {
+    typedef _Float16 h4 __attribute__((ext_vector_type(4)));
+    *(h4*) (a.out + at * 2) = h4{(_Float16) y[0], (_Float16) y[1], (_Float16) y[2], (_Float16) y[3]};
+  } else {
+    typedef __bf16 b4 __attribute__((ext_vector_type(4)));
+    *(b4*) (a.out + at * 2) = b4{(__bf16) y[0], (__bf16) y[1], (__bf16) y[2], (__bf16) y[3]};
+  }
+}
+
+// the greatest (or the sum) over the four lanes that share lane % 16
+__device__ inline float max_rows(float x) {
+  auto a = __builtin_amdgcn_permlane16_swap(__float_as_int(x), __float_as_int(x), false, false);
+  x = fmaxf(__int_as_float(a[0]), __int_as_float(a[1]));
+  auto b = __builtin_amdgcn_permlane32_swap(__float_as_int(x), __float_as_int(x), false, false);
+  return fmaxf(__int_as_float(b[0]), __int_as_float(b[1]));
+}
+__device__ inline float sum_rows(float x) {
+  auto a = __builtin_amdgcn_permlane16_swap(__float_as_int(x), __float_as_int(x), false, false);
+  x = __int_as_float(a[0]) + __int_as_float(a[1]);
+  auto b = __builtin_amdgcn_permlane32_swap(__float_as_int(x), __float_as_int(x), false, false);
+  return __int_as_float(b[0]) + __int_as_float(b[1]);
+}
+
+constexpr float kLog2E = 1.44269504088896341f, kLn2 = 0.693147180559945309f;
+// a maximum as what is subtracted: of nothing (-infinity), zero, so that exp2 of the difference is 0 and not NaN
+__device__ inline float finite_max(float m) { return m == -__builtin_inff() ? 0.0f : m; }
+
+// ---- one row a sequence (osmos_attn_token) ----
+// scores and outputs are computed transposed, S^T = K Q^T and O^T = V^T P^T, on v_mfma_f32_16x16x32 with up to 16 of a kv
+// head's query heads as columns: then a lane holds one query head's scores (of 8 keys of a tile of 32), its maximum, sum
+// and scaling are the lane's own, and the accumulator's layout of P^T is the B operand's of the second product but for the
+// order of the keys, which the V rows' order takes up. K goes straight from memory into the A operand's registers (a lane 16 bytes of
+// one key's row); V passes through the wave's own LDS tile, as its columns are wanted: written as it lies (16-byte pieces
+// rotated by row so that the transposing reads meet no bank twice), read by ds_read_tr.
+// a workgroup is 4 waves over one chunk of a sequence's keys for one kv head; wave w takes the tiles w, w + 4, ..: no
+// barrier until the waves' results are joined. the next tile's rows are loaded while this one is worked on, and the page
+// ids of the one after.
+template <bool F8, int D> struct TokenTile {
+  static constexpr int kSize = F8 ? 1 : 2;
+  static constexpr int kRow = D * kSize;                        // bytes of a V row in LDS
+  static constexpr int kPieces = kRow / 64;                     // 16-byte pieces a lane loads of a row
+  static constexpr int kOut = 16 * (D + 4) * 4;                 // a wave's result for the join
+  static constexpr int kLds = 32 * kRow > kOut ? 32 * kRow : kOut;
+  // the place of piece c of row r
+  static __device__ inline int at(int r, int c) {
+    constexpr int pieces = kRow / 16, rows = kRow < 256 ? 256 / kRow : 1;
+    const int turn = F8 ? r / rows : 2 * (r / rows);
+    return r * kRow + ((c ^ (turn & (pieces < 16 ? pieces - 1 : 15))) * 16);
+  }
+};
+
+// the keys of a sequence's row from the first tile on that its window reaches
+__device__ inline int first_key(const Seq& q, uint32_t window) { return window && q.len > (int) window ? q.len - (int) window : 0; }
+__device__ inline int keys_of(const Seq& q, uint32_t window) {
+  const int n = q.end - (first_key(q, window) & ~31);
+  return q.rows < 1 || n < 0 ? 0 : n;
+}
+
+// the step's work cut into chunks of one length, so that `want` of them hold all its keys (at least kLeast keys each, whole
+// 128s: a tile for each wave): workgroup `index` takes chunk c of sequence s's n. every workgroup reads all lengths, 64 a
+// round, and finds its place by their running sum, as no one else knows them; at most want + n_seq chunks.
+constexpr uint32_t kLeast = 256;
+struct Work {
+  uint32_t s, c, n, chunk;
+};
+__device__ inline bool find_work(const Step& st, uint32_t page, uint32_t window, uint32_t want, uint32_t index, Work& w) {
+  const uint32_t lane = threadIdx.x & 63;
+  auto keys_at = [&](uint32_t s, bool& row) {
+    row = false;
+    if (s >= st.n_seq) return 0;
+    const Seq q = sequence(st, s, page);
+    row = q.rows >= 1;
+    return keys_of(q, window);
+  };
+  uint64_t total = 0;
+  bool row0 = false;
+  int keys0 = 0;
+  for (uint32_t s = 0; s < st.n_seq; s += 64) {
+    bool row;
+    const int k = keys_at(s + lane, row);
+    if (s == 0) row0 = row, keys0 = k;
+    total += (uint32_t) k;
+  }
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) total += __shfl_xor(total, o);
+  const uint64_t even = (total + want - 1) / want;
+  w.chunk = even < kLeast ? kLeast : (uint32_t) ((even + 127) / 128 * 128);
+  uint32_t before = 0;
+  for (uint32_t s = 0; s < st.n_seq; s += 64) {
+    bool row = row0;
+    int k = keys0;
+    if (s) k = keys_at(s + lane, row);
+    const uint32_t n = !row ? 0 : k <= (int) w.chunk ? 1 : ((uint32_t) k + w.chunk - 1) / w.chunk;
+    uint32_t x = n;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+      const uint32_t y = __shfl_up(x, o);
+      if ((int) lane >= o) x += y;
+    }
+    const uint64_t past = __ballot(before + x > index);
+    if (past) {
+      const int at = __builtin_ctzll(past);
+      w.s = s + (uint32_t) at;
+      w.n = (uint32_t) __builtin_amdgcn_readlane((int) n, at);
+      w.c = index - (before + (uint32_t) __builtin_amdgcn_readlane((int) x, at) - w.n);
+      return true;
+    }
+    before += (uint32_t) __builtin_amdgcn_readlane((int) x, 63);
+  }
+  return false;
+}
+
+template <bool BF, bool F8, int D>
+__global__ __launch_bounds__(256, D > 128 ? 1 : 2) void token_kernel(Args a, Kv kv, Step st, uint32_t want, uint32_t tiles,
+                                                                   uint32_t* __restrict__ cut, float* __restrict__ part) {
+  typedef Unit<BF> U;
+  typedef typename U::v8 v8;
+  typedef TokenTile<F8, D> T;
+  constexpr int kSteps = D / 32, kDims = D / 16;
+  __shared__ __attribute__((aligned(16))) uint8_t lds[4][T::kLds];
+  __shared__ float ml[4][2][16];
+  const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x / 64, r = lane & 15, quad = lane / 16;
+  uint32_t b = blockIdx.x;
+  const uint32_t mt = b % tiles;
+  b /= tiles;
+  const uint32_t g = b % kv.heads;
+  b /= kv.heads;
+  Work work;
+  if (!find_work(st, kv.page, a.window, want, b, work)) return;
+  const uint32_t s = work.s;
+  const Seq seq = sequence(st, s, kv.page);
+  const int begin = first_key(seq, a.window), from = (begin & ~31) + (int) (work.c * work.chunk);
+  const int to = seq.end - from > (int) work.chunk ? from + (int) work.chunk : seq.end;
+  if (cut && work.c == 0 && g == 0 && mt == 0 && threadIdx.x == 0) cut[2 * s] = b, cut[2 * s + 1] = work.n;
+  const uint32_t row = (uint32_t) (seq.row0 + seq.rows - 1);
+  const uint32_t heads = a.group - mt * 16 < 16 ? a.group - mt * 16 : 16, head0 = g * a.group + mt * 16;
+
+  // Q^T as the B operand: column lane % 16, 8 dims a lane of each step's 32; of 8-bit keys a lane loads 16 dims at once,
+  // so that two steps share 64 dims
+  v8 q[kSteps];
+#pragma unroll
+  for (int i = 0; i < kSteps; i++) {
+    const uint32_t d = F8 ? (uint32_t) (64 * (i / 2) + 16 * quad + 8 * (i % 2)) : (uint32_t) (32 * i + 8 * quad);
+    q[i] = v8{};
+    if (r < heads && d < a.dim) q[i] = q8<BF>(a, row * a.qs + (head0 + r) * a.qh + d);
+  }
+  const float unit = a.scale * kLog2E * (F8 && kv.scale ? kv.scale[g] : 1.0f);
+
+  f32x4 o[kDims];
+#pragma unroll
+  for (int i = 0; i < kDims; i++) o[i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+  float m = -__builtin_inff(), l = 0.0f;
+
+  const uint32_t dim_bytes = a.dim * T::kSize;
+  // the two rows of a tile that a lane loads: its page ids (-1: none) and, from them, its rows' places
+  const uint32_t shift = 31 - __builtin_clz(kv.page);
+  auto ids = [&](int j0, int (&id)[2]) {
+#pragma unroll
+    for (int i = 0; i < 2; i++) {
+      const int j = j0 + 16 * i + (int) r;
+      id[i] = j < to && j >= begin ? seq.table[(uint32_t) j >> shift] : -1;
+    }
+  };
+  u32x4 kr[2][T::kPieces], vr[2][T::kPieces];
+  bool in[2];
+  auto load = [&](int j0, const int (&id)[2]) {
+#pragma unroll
+    for (int i = 0; i < 2; i++) {
+      in[i] = (uint32_t) id[i] < kv.pages;
+      const uint32_t slot = (uint32_t) (j0 + 16 * i + (int) r) & (kv.page - 1);
+      const uint64_t at = (((uint64_t) (in[i] ? (uint32_t) id[i] : 0u) * kv.heads + g) * kv.page + slot) * dim_bytes;
+#pragma unroll
+      for (int p = 0; p < T::kPieces; p++) {
+        const uint32_t d = 64 * p + 16 * quad;
+        kr[i][p] = vr[i][p] = u32x4{0, 0, 0, 0};
+        if (in[i] && d < dim_bytes) {
+          kr[i][p] = gload<u32x4>(kv.k + at + d);
+          vr[i][p] = gload<u32x4>(kv.v + at + d);
+        }
+      }
+    }
+  };
+
+  uint8_t* tile = lds[wave];
+  int id[2];
+  const int first = from + 32 * (int) wave;
+  if (first < to) {
+    ids(first, id);
+    load(first, id);
+    ids(first + 128, id);
+  }
+  for (int j0 = first; j0 < to; j0 += 128) {
+    // V's rows into LDS (zeros for keys that are masked: what lies there has no influence)
+    const uint32_t low = (uint32_t) __ballot(in[0]) & 0xFFFF, high = (uint32_t) __ballot(in[1]) & 0xFFFF;
+    const uint32_t live = low | high << 16;
+#pragma unroll
+    for (int i = 0; i < 2; i++)
+#pragma unroll
+      for (int p = 0; p < T::kPieces; p++) *(u32x4*) (tile + T::at(16 * i + r, 4 * p + quad)) = vr[i][p];
+    // S^T: two tiles of 16 keys
+    f32x4 x[2];
+#pragma unroll
+    for (int i = 0; i < 2; i++) {
+      x[i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+      for (int k = 0; k < kSteps; k++) {
+        v8 ka;
+        if constexpr (F8) ka = from_f8<BF>(u32x2{kr[i][k / 2][2 * (k % 2)], kr[i][k / 2][2 * (k % 2) + 1]});
+        else ka = __builtin_bit_cast(v8, kr[i][k]);
+        x[i] = U::mfma16(ka, q[k], x[i]);
+      }
+    }
+    if (j0 + 128 < to) {
+      load(j0 + 128, id);
+      ids(j0 + 256, id);
+    }
+    __builtin_amdgcn_sched_barrier(0);  // (the loads go out before the softmax)
+#pragma unroll
+    for (int i = 0; i < 2; i++)
+#pragma unroll
+      for (int j = 0; j < 4; j++) x[i][j] *= unit;
+    if (live != 0xFFFFFFFFu) {
+#pragma unroll
+      for (int i = 0; i < 2; i++)
+#pragma unroll
+        for (int j = 0; j < 4; j++)
+          if (!(live >> (16 * i + 4 * quad + j) & 1)) x[i][j] = -__builtin_inff();
+    }
+    float top = fmaxf(fmaxf(fmaxf(x[0][0], x[0][1]), fmaxf(x[0][2], x[0][3])), fmaxf(fmaxf(x[1][0], x[1][1]), fmaxf(x[1][2], x[1][3])));
+    top = fmaxf(m, max_rows(top));
+    const float base = finite_max(top), fade = __builtin_amdgcn_exp2f(m - base);
+    m = top;
+    v8 p;
+    float sum = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 2; i++)
+#pragma unroll
+      for (int j = 0; j < 4; j++) {
+        const float e = __builtin_amdgcn_exp2f(x[i][j] - base);
+        sum += e;
+        p[4 * i + j] = (typename U::e) e;
+      }
+    l = __builtin_fmaf(l, fade, sum);
+#pragma unroll
+    for (int t = 0; t < kDims; t++) o[t] *= fade;
+    // O^T: V^T's columns of keys 4 quad + 0 .. 3 and 16 + 4 quad + 0 .. 3, as P^T's lanes hold them
+#pragma unroll
+    for (int t = 0; t < kDims; t++) {
+      v8 va;
+      if constexpr (F8) {
+        typedef int i32x2 __attribute__((ext_vector_type(2)));
+        const int e = (int) (r / 2), key = e < 4 ? 4 * (int) quad + e : 12 + 4 * (int) quad + e;
+        const auto w = __builtin_amdgcn_ds_read_tr8_b64_v2i32((__attribute__((address_space(3))) i32x2*) (tile + T::at(key, t) + 8 * (r & 1)));
+        va = from_f8<BF>(u32x2{(uint32_t) w[0], (uint32_t) w[1]});
+      } else {
+        typedef short s16x4 __attribute__((ext_vector_type(4)));
+        const int key = 4 * (int) quad + (int) (r / 4), piece = 2 * t + (int) (r & 3) / 2, part8 = 8 * (r & 1);
+        const s16x4 w0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*) (tile + T::at(key, piece) + part8));
+        const s16x4 w1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*) (tile + T::at(key + 16, piece) + part8));
+        va = __builtin_bit_cast(v8, __builtin_shufflevector(w0, w1, 0, 1, 2, 3, 4, 5, 6, 7));
+      }
+      o[t] = U::mfma16(va, p, o[t]);
+    }
+  }
+
+  // the waves' results joined: each scaled to the greatest maximum, then summed in the waves' order
+  l = sum_rows(l);
+  if (quad == 0) ml[wave][0][r] = m, ml[wave][1][r] = l;
+  __syncthreads();
+  float top = fmaxf(fmaxf(ml[0][0][r], ml[1][0][r]), fmaxf(ml[2][0][r], ml[3][0][r]));
+  const float base = finite_max(top), mine = __builtin_amdgcn_exp2f(m - base);
+  float* out = (float*) lds[wave];
+#pragma unroll
+  for (int t = 0; t < kDims; t++) *(f32x4*) (out + r * (D + 4) + 16 * t + 4 * quad) = o[t] * mine;
+  __syncthreads();
+  const float v_scale = F8 && kv.scale ? kv.scale[kv.heads + g] : 1.0f;
+  for (uint32_t i = threadIdx.x; i < heads * (D / 4); i += 256) {
+    const uint32_t h = i / (D / 4), d = i % (D / 4) * 4;
+    f32x4 y = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    float sum = 0.0f, top_h = fmaxf(fmaxf(ml[0][0][h], ml[1][0][h]), fmaxf(ml[2][0][h], ml[3][0][h]));
+#pragma unroll
+    for (int w = 0; w < 4; w++) {
+      y += *(const f32x4*) ((const float*) lds[w] + h * (D + 4) + d);
+      sum = __builtin_fmaf(ml[w][1][h], __builtin_amdgcn_exp2f(ml[w][0][h] - finite_max(top_h)), sum);
+    }
+    if (work.n == 1) {
+      if (d < a.dim) put4(a, row * a.os + (head0 + h) * a.oh + d, y * (sum == 0.0f ? 0.0f : v_scale / sum));
+      if (a.lse && d == 0) a.lse[(uint64_t) row * a.heads + head0 + h] = (top_h + log2f(sum)) * kLn2;
+    } else {
+      float* to_part = part + ((uint64_t) b * a.heads + head0 + h) * (D + 4);
+      *(f32x4*) (to_part + d) = y * v_scale;
+      if (d == 0) to_part[D] = top_h, to_part[D + 1] = sum;
+    }
+  }
+}
+
+// the chunks' results of a row and head joined, in the chunks' order: a workgroup D / 4 threads of 4 dims in 256 / (D / 4)
+// groups, each group every so many chunks, then the groups in order
+template <int D>
+__global__ __launch_bounds__(256) void join_kernel(Args a, Step st, uint32_t page,
+                                                   const uint32_t* __restrict__ cut, const float* __restrict__ part) {
+  constexpr uint32_t kLanes = D / 4, kGroups = 256 / kLanes;
+  __shared__ f32x4 sum4[kGroups][kLanes];
+  __shared__ float top_of[kGroups], sum_of[kGroups];
+  const uint32_t h = blockIdx.x % a.heads, s = blockIdx.x / a.heads, i = threadIdx.x % kLanes, k = threadIdx.x / kLanes;
+  const Seq seq = sequence(st, s, page);
+  if (seq.rows < 1) return;
+  const uint32_t n = cut[2 * s + 1], row = (uint32_t) (seq.row0 + seq.rows - 1);
+  if (n == 1) return;  // (written by its only chunk's workgroup)
+  const float* p = part + ((uint64_t) cut[2 * s] * a.heads + h) * (D + 4);
+  float m = -__builtin_inff(), l = 0.0f;
+  f32x4 y = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 4
+  for (uint32_t c = k; c < n; c += kGroups) {
+    const float* pc = p + (uint64_t) c * a.heads * (D + 4);
+    const f32x4 o = *(const f32x4*) (pc + 4 * i);
+    const float mc = pc[D], lc = pc[D + 1];
+    const float top = fmaxf(m, mc), base = finite_max(top), f = __builtin_amdgcn_exp2f(m - base), fc = __builtin_amdgcn_exp2f(mc - base);
+    y = y * f + o * fc;
+    l = l * f + lc * fc;
+    m = top;
+  }
+  sum4[k][i] = y;
+  if (i == 0) top_of[k] = m, sum_of[k] = l;
+  __syncthreads();
+  if (k) return;
+  float top = -__builtin_inff();
+#pragma unroll
+  for (uint32_t w = 0; w < kGroups; w++) top = fmaxf(top, top_of[w]);
+  y = f32x4{0.0f, 0.0f, 0.0f, 0.0f}, l = 0.0f;
+#pragma unroll
+  for (uint32_t w = 0; w < kGroups; w++) {
+    const float f = __builtin_amdgcn_exp2f(top_of[w] - finite_max(top));
+    y += sum4[w][i] * f;
+    l += sum_of[w] * f;
+  }
+  if (4 * i < a.dim) put4(a, row * a.os + h * a.oh + 4 * i, y * (l == 0.0f ? 0.0f : 1.0f / l));
+  if (a.lse && i == 0) a.lse[(uint64_t) row * a.heads + h] = (top + log2f(l)) * kLn2;
+}
+
+// how a token step is launched: the chunks that the sequences are cut into for each kv head and 16 of its query heads, and
+// the workspace: where each sequence's chunks begin and how many they are, then the chunks' results
+constexpr uint32_t kWant = 1024;
+struct Cut {
+  uint32_t want, most, tiles, dim;  // most: chunks there can be
+  bool split;                       // whether a sequence can have more than one
+  uint64_t head;                    // the workspace's bytes before the results
+};
+inline Cut cut_of(const OsmosAttn* a, uint32_t kv_heads, uint32_t dim, const OsmosKvStep* st) {
+  Cut c;
+  c.tiles = (a->heads / kv_heads + 15) / 16;
+  c.dim = dim <= 64 ? 64 : dim <= 128 ? 128 : 256;
+  c.want = kWant / (kv_heads * c.tiles) ? kWant / (kv_heads * c.tiles) : 1;
+  const uint64_t keys = a->window && a->window + 31ull < st->max_len ? a->window + 31ull : st->max_len;
+  c.split = keys > kLeast;
+  const uint64_t each = st->n_seq * ((keys + kLeast - 1) / kLeast), even = (uint64_t) c.want + st->n_seq;
+  c.most = (uint32_t) (each < even ? each : even);
+  c.head = (st->n_seq * 8ull + 255) / 256 * 256;
+  return c;
+}
+inline uint64_t token_bytes(const OsmosAttn* a, const Cut& c) {
+  return c.split ? c.head + (uint64_t) c.most * a->heads * (c.dim + 4) * 4 : 0;
+}
+
+template <bool BF, bool F8>
+bool run_token(const Args& a, const Kv& k, const Step& st, const Cut& c, uint8_t* workspace, hipStream_t stream) {
+  const uint64_t blocks = (uint64_t) c.most * k.heads * c.tiles, rows = (uint64_t) st.n_seq * a.heads;
+  if (blocks > 0x7FFFFFFFull || rows > 0x7FFFFFFFull) return false;
+  auto* kernel = c.dim == 64 ? token_kernel<BF, F8, 64> : c.dim == 128 ? token_kernel<BF, F8, 128> : token_kernel<BF, F8, 256>;
+  uint32_t* cut = c.split ? (uint32_t*) workspace : nullptr;
+  float* part = (float*) (workspace + c.head);
+  kernel<<<(uint32_t) blocks, 256, 0, stream>>>(a, k, st, c.want, c.tiles, cut, part);
+  if (hipGetLastError() != hipSuccess) return false;
+  if (c.split) {
+    auto* join = c.dim == 64 ? join_kernel<64> : c.dim == 128 ? join_kernel<128> : join_kernel<256>;
+    join<<<(uint32_t) rows, 256, 0, stream>>>(a, st, k.page, cut, part);
+  }
+  return hipGetLastError() == hipSuccess;
+}
+
+// whether the products are taken in bf16
+__host__ __device__ inline bool in_bf16(uint32_t kv_type, uint32_t q_type) { return kv_type == OSMOS_BF16 || (kv_type == OSMOS_F8 && q_type == OSMOS_BF16); }
+
 __device__ inline float value(uint32_t type, const uint8_t* p, uint64_t i) {
   if (type == OSMOS_F32) return ((const float*) p)[i];
   if (type == OSMOS_F16) return (float) ((const _Float16*) p)[i];
@@ -47,7 +481,7 @@ __global__ __launch_bounds__(64) void row_kernel(Args a, Kv kv, Step st) {
   const int pos = seq.len - (seq.row0 + seq.rows - (int) t);
   const int end = pos + 1 < seq.end ? pos + 1 : seq.end;
   const int begin = a.window && pos + 1 > (int) a.window ? pos + 1 - (int) a.window : 0;
-  const bool bf = kv.type == OSMOS_BF16 || (kv.type == OSMOS_F8 && a.q_type == OSMOS_BF16);  // the products' type
+  const bool bf = in_bf16(kv.type, a.q_type);
   for (uint32_t d = lane; d < a.dim; d += 64) {
     const float x = value(a.q_type, a.q, t * a.qs + h * a.qh + d);
     qv[d] = bf ? (float) (__bf16) x : (float) (_Float16) x;
@@ -135,8 +569,8 @@ using namespace osm;
 
 extern "C" OSM_API uint64_t osmos_attn_workspace(const OsmosAttn* a, uint32_t kv_heads, uint32_t dim,
                                                  const OsmosKvStep* step) {
-  (void) a, (void) kv_heads, (void) dim, (void) step;
-  return 0;
+  if (!a || !a->heads || !kv_heads || a->heads % kv_heads || !dim || dim > OSMOS_ATTN_MAX_DIM || !step) return 0;
+  return step->max_tok == 1 && step->len ? attn::token_bytes(a, attn::cut_of(a, kv_heads, dim, step)) : 0;
 }
 
 extern "C" OSM_API bool osmos_attn_prompt(const OsmosAttn* a, const OsmosKvRows* r, const OsmosKvStep* step,
@@ -160,8 +594,14 @@ extern "C" OSM_API bool osmos_attn_chunk(const OsmosAttn* a, const OsmosKv* kv, 
 
 extern "C" OSM_API bool osmos_attn_token(const OsmosAttn* a, const OsmosKv* kv, uint32_t layer, const OsmosKvStep* step,
                                          void* workspace, uint64_t workspace_bytes, void* stream) {
-  (void) workspace, (void) workspace_bytes;
   if (!kv::cache_ok(kv) || layer >= kv->layers || !attn::args_ok(a, kv->heads, kv->dim) || !kv::step_ok(step, true)) return false;
   if (step->max_tok != 1) return false;
-  return attn::run_rows(a, attn::pages_of(kv, layer), kv->dim, step, stream);
+  const attn::Cut c = attn::cut_of(a, kv->heads, kv->dim, step);
+  const uint64_t need = attn::token_bytes(a, c);
+  if (need && (!workspace || (uintptr_t) workspace % 256 || workspace_bytes < need)) return false;
+  const bool bf = attn::in_bf16(kv->type, a->q_type), f8 = kv->type == OSMOS_F8;
+  auto* run = bf ? (f8 ? attn::run_token<true, true> : attn::run_token<true, false>)
+                 : (f8 ? attn::run_token<false, true> : attn::run_token<false, false>);
+  return run(attn::args_of(a, kv->heads, kv->dim), attn::pages_of(kv, layer), kv::step_of(step), c, (uint8_t*) workspace,
+             (hipStream_t) stream);
 }

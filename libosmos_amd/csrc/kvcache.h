@@ -133,7 +133,7 @@ inline bool step_ok(const OsmosKvStep* st, bool paged) {
     return false;
   if (!paged) return true;
   return st->len && st->table && st->table_stride && st->seqs && (st->seq || st->n_seq <= st->seqs) && st->max_len &&
-         st->max_len <= 0x7FFFFFFFu;
+         st->max_len <= 0x7FFF0000u;
 }
 inline Step step_of(const OsmosKvStep* st) {
   return Step{st->start, st->len, st->table, st->seq, st->n_seq, st->n_tok, st->max_len, st->seqs, st->table_stride};
