@@ -64,17 +64,27 @@ __device__ inline typename Unit<BF>::v8 from_f8(u32x2 w) {
   return r;
 }
 
-// 8 values of q from `at` on in the products' type (an F32 q's rounded once)
-template <bool BF>
-__device__ inline typename Unit<BF>::v8 q8(const Args& a, uint64_t at) {
-  float x[8];
-  if (a.q_type == OSMOS_F32) kv::load8<OSMOS_F32>(a.q + at * 4, x);
-  else if (a.q_type == OSMOS_F16) kv::load8<OSMOS_F16>(a.q + at * 2, x);
-  else kv::load8<OSMOS_BF16>(a.q + at * 2, x);
-  typename Unit<BF>::v8 r;
+// a lane's values of a query head as the B operand of N steps, 8 dims each from at(i) on, in the products' type (an F32 q's
+// rounded once), negated for a negative scale; zeros where `in` is false or past the dims
+template <bool BF, int N, uint32_t T, class At>
+__device__ inline void q_steps(const uint8_t* p, uint32_t dim, bool in, float sign, At at, typename Unit<BF>::v8 (&q)[N]) {
+  float x[N][8];
 #pragma unroll
-  for (int i = 0; i < 8; i++) r[i] = (typename Unit<BF>::e) x[i];
-  return r;
+  for (int i = 0; i < N; i++) kv::load8<T>(p + (at(i) < dim ? at(i) : 0) * kv::size_of(T), x[i]);
+#pragma unroll
+  for (int i = 0; i < N; i++) {
+    const float f = in && at(i) < dim ? sign : 0.0f;
+#pragma unroll
+    for (int j = 0; j < 8; j++) q[i][j] = f == 0.0f ? (typename Unit<BF>::e) 0.0f : (typename Unit<BF>::e) (x[i][j] * f);
+  }
+}
+template <bool BF, int N, class At>
+__device__ inline void load_q(const Args& a, uint64_t row, uint32_t head, bool in, At at, typename Unit<BF>::v8 (&q)[N]) {
+  const uint8_t* p = a.q + (row * a.qs + head * a.qh) * kv::size_of(a.q_type);
+  const float sign = a.scale < 0.0f ? -1.0f : 1.0f;
+  if (a.q_type == OSMOS_F32) q_steps<BF, N, OSMOS_F32>(p, a.dim, in, sign, at, q);
+  else if (a.q_type == OSMOS_F16) q_steps<BF, N, OSMOS_F16>(p, a.dim, in, sign, at, q);
+  else q_steps<BF, N, OSMOS_BF16>(p, a.dim, in, sign, at, q);
 }
 
 __device__ inline void put4(const Args& a, uint64_t at, f32x4 y) {
@@ -111,12 +121,14 @@ __device__ inline float finite_max(float m) { return m == -__builtin_inff() ? 0.
 // scores and outputs are computed transposed, S^T = K Q^T and O^T = V^T P^T, on v_mfma_f32_16x16x32 with up to 16 of a kv
 // head's query heads as columns: then a lane holds one query head's scores (of 8 keys of a tile of 32), its maximum, sum
 // and scaling are the lane's own, and the accumulator's layout of P^T is the B operand's of the second product but for the
-// order of the keys, which the V rows' order takes up. K goes straight from memory into the A operand's registers (a lane 16 bytes of
-// one key's row); V passes through the wave's own LDS tile, as its columns are wanted: written as it lies (16-byte pieces
-// rotated by row so that the transposing reads meet no bank twice), read by ds_read_tr.
+// order of the keys, which the V rows' order takes up. K goes straight from memory into the A operand's registers (a lane
+// 16 bytes of one key's row); V passes through the wave's own LDS tile, as its columns are wanted: written as it lies
+// (16-byte pieces turned by row so that the transposing reads meet no bank twice), read by ds_read_tr.
 // a workgroup is 4 waves over one chunk of a sequence's keys for one kv head; wave w takes the tiles w, w + 4, ..: no
 // barrier until the waves' results are joined. the next tile's rows are loaded while this one is worked on, and the page
-// ids of the one after.
+// ids of the one after. with pages of 16 tokens or more (WIDE) half a tile lies in one page, so that its place is the
+// wave's and not a lane's: scalar loads and arithmetic, where smaller pages take some 60 vector instructions a tile.
+// no load is conditional: a place that is masked reads a row that exists and its score and value are then replaced.
 template <bool F8, int D> struct TokenTile {
   static constexpr int kSize = F8 ? 1 : 2;
   static constexpr int kRow = D * kSize;                        // bytes of a V row in LDS
@@ -138,61 +150,68 @@ __device__ inline int keys_of(const Seq& q, uint32_t window) {
   return q.rows < 1 || n < 0 ? 0 : n;
 }
 
+// the sum of x over this lane and those below it
+__device__ inline uint32_t wave_scan(uint32_t x) {
+#define OSM_ADD_DPP(ctrl, rows) x += (uint32_t) __builtin_amdgcn_update_dpp(0, (int) x, ctrl, rows, 0xF, false)
+  OSM_ADD_DPP(0x111, 0xF);  // row_shr 1, 2, 4, 8
+  OSM_ADD_DPP(0x112, 0xF);
+  OSM_ADD_DPP(0x114, 0xF);
+  OSM_ADD_DPP(0x118, 0xF);
+  OSM_ADD_DPP(0x142, 0xA);  // row_bcast 15, 31
+  OSM_ADD_DPP(0x143, 0xC);
+#undef OSM_ADD_DPP
+  return x;
+}
+__device__ inline int lane_of(int x, int lane) { return __builtin_amdgcn_readlane(x, lane); }
+
 // the step's work cut into chunks of one length, so that `want` of them hold all its keys (at least kLeast keys each, whole
 // 128s: a tile for each wave): workgroup `index` takes chunk c of sequence s's n. every workgroup reads all lengths, 64 a
 // round, and finds its place by their running sum, as no one else knows them; at most want + n_seq chunks.
-constexpr uint32_t kLeast = 256;
+constexpr uint32_t kLeast = 384;
 struct Work {
   uint32_t s, c, n, chunk;
+  Seq seq;
 };
 __device__ inline bool find_work(const Step& st, uint32_t page, uint32_t window, uint32_t want, uint32_t index, Work& w) {
   const uint32_t lane = threadIdx.x & 63;
-  auto keys_at = [&](uint32_t s, bool& row) {
-    row = false;
-    if (s >= st.n_seq) return 0;
-    const Seq q = sequence(st, s, page);
-    row = q.rows >= 1;
-    return keys_of(q, window);
-  };
-  uint64_t total = 0;
-  bool row0 = false;
-  int keys0 = 0;
-  for (uint32_t s = 0; s < st.n_seq; s += 64) {
-    bool row;
-    const int k = keys_at(s + lane, row);
-    if (s == 0) row0 = row, keys0 = k;
-    total += (uint32_t) k;
+  Seq none, q;
+  none.row0 = none.rows = none.len = none.end = 0, none.table = st.table;
+  uint32_t total = 0;  // in tiles of 32
+  q = lane < st.n_seq ? sequence(st, lane, page) : none;
+  for (uint32_t s = 0;;) {
+    total += (uint32_t) lane_of((int) wave_scan(((uint32_t) keys_of(q, window) + 31) / 32), 63);
+    if ((s += 64) >= st.n_seq) break;
+    q = s + lane < st.n_seq ? sequence(st, s + lane, page) : none;
   }
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) total += __shfl_xor(total, o);
-  const uint64_t even = (total + want - 1) / want;
-  w.chunk = even < kLeast ? kLeast : (uint32_t) ((even + 127) / 128 * 128);
+  const uint32_t even = total / want + 1;
+  w.chunk = even * 32 <= kLeast ? kLeast : (even + 3) / 4 * 128;
   uint32_t before = 0;
   for (uint32_t s = 0; s < st.n_seq; s += 64) {
-    bool row = row0;
-    int k = keys0;
-    if (s) k = keys_at(s + lane, row);
-    const uint32_t n = !row ? 0 : k <= (int) w.chunk ? 1 : ((uint32_t) k + w.chunk - 1) / w.chunk;
-    uint32_t x = n;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-      const uint32_t y = __shfl_up(x, o);
-      if ((int) lane >= o) x += y;
-    }
-    const uint64_t past = __ballot(before + x > index);
+    if (st.n_seq > 64) q = s + lane < st.n_seq ? sequence(st, s + lane, page) : none;
+    const int k = keys_of(q, window);
+    const uint32_t n = q.rows < 1 ? 0 : k <= (int) w.chunk ? 1 : ((uint32_t) k + w.chunk - 1) / w.chunk, x = before + wave_scan(n);
+    const uint64_t past = __ballot(x > index);
     if (past) {
       const int at = __builtin_ctzll(past);
       w.s = s + (uint32_t) at;
-      w.n = (uint32_t) __builtin_amdgcn_readlane((int) n, at);
-      w.c = index - (before + (uint32_t) __builtin_amdgcn_readlane((int) x, at) - w.n);
+      w.n = (uint32_t) lane_of((int) n, at);
+      w.c = index - ((uint32_t) lane_of((int) x, at) - w.n);
+      w.seq.row0 = lane_of(q.row0, at), w.seq.rows = lane_of(q.rows, at), w.seq.len = lane_of(q.len, at), w.seq.end = lane_of(q.end, at);
+      w.seq.table = (const int32_t*) ((uint64_t) (uint32_t) lane_of((int) ((uint64_t) q.table >> 32), at) << 32 |
+                                      (uint32_t) lane_of((int) (uint64_t) q.table, at));
       return true;
     }
-    before += (uint32_t) __builtin_amdgcn_readlane((int) x, 63);
+    before = (uint32_t) lane_of((int) x, 63);
   }
   return false;
 }
 
-template <bool BF, bool F8, int D>
+// a word of a table at a place that is the whole wave's
+__device__ inline int uniform_word(const int32_t* p) {
+  return *(const __attribute__((address_space(4))) int32_t*) (uint64_t) p;
+}
+
+template <bool BF, bool F8, int D, bool WIDE>
 __global__ __launch_bounds__(256, D > 128 ? 1 : 2) void token_kernel(Args a, Kv kv, Step st, uint32_t want, uint32_t tiles,
                                                                    uint32_t* __restrict__ cut, float* __restrict__ part) {
   typedef Unit<BF> U;
@@ -201,7 +220,8 @@ __global__ __launch_bounds__(256, D > 128 ? 1 : 2) void token_kernel(Args a, Kv 
   constexpr int kSteps = D / 32, kDims = D / 16;
   __shared__ __attribute__((aligned(16))) uint8_t lds[4][T::kLds];
   __shared__ float ml[4][2][16];
-  const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x / 64, r = lane & 15, quad = lane / 16;
+  const uint32_t lane = threadIdx.x & 63, wave = (uint32_t) __builtin_amdgcn_readfirstlane((int) threadIdx.x / 64);
+  const uint32_t r = lane & 15, quad = lane / 16;
   uint32_t b = blockIdx.x;
   const uint32_t mt = b % tiles;
   b /= tiles;
@@ -210,71 +230,87 @@ __global__ __launch_bounds__(256, D > 128 ? 1 : 2) void token_kernel(Args a, Kv 
   Work work;
   if (!find_work(st, kv.page, a.window, want, b, work)) return;
   const uint32_t s = work.s;
-  const Seq seq = sequence(st, s, kv.page);
+  const Seq seq = work.seq;
   const int begin = first_key(seq, a.window), from = (begin & ~31) + (int) (work.c * work.chunk);
   const int to = seq.end - from > (int) work.chunk ? from + (int) work.chunk : seq.end;
   if (cut && work.c == 0 && g == 0 && mt == 0 && threadIdx.x == 0) cut[2 * s] = b, cut[2 * s + 1] = work.n;
   const uint32_t row = (uint32_t) (seq.row0 + seq.rows - 1);
   const uint32_t heads = a.group - mt * 16 < 16 ? a.group - mt * 16 : 16, head0 = g * a.group + mt * 16;
 
+  // the rows of a tile that a lane loads are 16 i + r, their 16-byte pieces 4 p + quad
+  const uint32_t dim_bytes = a.dim * T::kSize, shift = 31 - __builtin_clz(kv.page);
+  const uint64_t page_bytes = (uint64_t) kv.heads * kv.page * dim_bytes, head_at = (uint64_t) g * kv.page * dim_bytes;
+  uint32_t piece[T::kPieces];
+#pragma unroll
+  for (int p = 0; p < T::kPieces; p++) {
+    const uint32_t d = 64 * p + 16 * quad;
+    piece[p] = (WIDE ? r * dim_bytes : 0) + (d < dim_bytes ? d : 0);
+  }
+  int id[2];
+  auto ids = [&](int j0) {
+#pragma unroll
+    for (int i = 0; i < 2; i++) {
+      const int j = j0 + 16 * i + (WIDE ? 0 : (int) r), last = to - 1;
+      const int32_t* at = seq.table + ((uint32_t) (j < last ? j : last) >> shift);
+      id[i] = WIDE ? uniform_word(at) : gload<int>(at);
+    }
+  };
+  u32x4 kr[2][T::kPieces], vr[2][T::kPieces];
+  bool page_in[2];
+  auto load = [&](int j0) {
+#pragma unroll
+    for (int i = 0; i < 2; i++) {
+      page_in[i] = (uint32_t) id[i] < kv.pages;
+      const uint32_t slot = (uint32_t) (j0 + 16 * i + (WIDE ? 0 : (int) r)) & (kv.page - 1);
+      const uint64_t at = (page_in[i] ? (uint32_t) id[i] : 0u) * page_bytes + head_at + slot * dim_bytes;
+      const uint8_t *k = kv.k + at, *v = kv.v + at;
+#pragma unroll
+      for (int p = 0; p < T::kPieces; p++) kr[i][p] = gload<u32x4>(k + piece[p]);
+#pragma unroll
+      for (int p = 0; p < T::kPieces; p++) vr[i][p] = gload<u32x4>(v + piece[p]);
+    }
+  };
+
+  const int first = from + 32 * (int) wave;
+  if (first < to) ids(first);
+
   // Q^T as the B operand: column lane % 16, 8 dims a lane of each step's 32; of 8-bit keys a lane loads 16 dims at once,
   // so that two steps share 64 dims
   v8 q[kSteps];
-#pragma unroll
-  for (int i = 0; i < kSteps; i++) {
-    const uint32_t d = F8 ? (uint32_t) (64 * (i / 2) + 16 * quad + 8 * (i % 2)) : (uint32_t) (32 * i + 8 * quad);
-    q[i] = v8{};
-    if (r < heads && d < a.dim) q[i] = q8<BF>(a, row * a.qs + (head0 + r) * a.qh + d);
-  }
-  const float unit = a.scale * kLog2E * (F8 && kv.scale ? kv.scale[g] : 1.0f);
+  load_q<BF, kSteps>(a, row, head0 + (r < heads ? r : 0), r < heads, [&](int i) {
+    return F8 ? (uint32_t) (64 * (i / 2) + 16 * quad + 8 * (i % 2)) : (uint32_t) (32 * i + 8 * quad);
+  }, q);
+  const float unit = fabsf(a.scale) * kLog2E * (F8 && kv.scale ? kv.scale[g] : 1.0f);
 
   f32x4 o[kDims];
 #pragma unroll
   for (int i = 0; i < kDims; i++) o[i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
   float m = -__builtin_inff(), l = 0.0f;
 
-  const uint32_t dim_bytes = a.dim * T::kSize;
-  // the two rows of a tile that a lane loads: its page ids (-1: none) and, from them, its rows' places
-  const uint32_t shift = 31 - __builtin_clz(kv.page);
-  auto ids = [&](int j0, int (&id)[2]) {
-#pragma unroll
-    for (int i = 0; i < 2; i++) {
-      const int j = j0 + 16 * i + (int) r;
-      id[i] = j < to && j >= begin ? seq.table[(uint32_t) j >> shift] : -1;
-    }
-  };
-  u32x4 kr[2][T::kPieces], vr[2][T::kPieces];
-  bool in[2];
-  auto load = [&](int j0, const int (&id)[2]) {
-#pragma unroll
-    for (int i = 0; i < 2; i++) {
-      in[i] = (uint32_t) id[i] < kv.pages;
-      const uint32_t slot = (uint32_t) (j0 + 16 * i + (int) r) & (kv.page - 1);
-      const uint64_t at = (((uint64_t) (in[i] ? (uint32_t) id[i] : 0u) * kv.heads + g) * kv.page + slot) * dim_bytes;
-#pragma unroll
-      for (int p = 0; p < T::kPieces; p++) {
-        const uint32_t d = 64 * p + 16 * quad;
-        kr[i][p] = vr[i][p] = u32x4{0, 0, 0, 0};
-        if (in[i] && d < dim_bytes) {
-          kr[i][p] = gload<u32x4>(kv.k + at + d);
-          vr[i][p] = gload<u32x4>(kv.v + at + d);
-        }
-      }
-    }
-  };
-
   uint8_t* tile = lds[wave];
-  int id[2];
-  const int first = from + 32 * (int) wave;
   if (first < to) {
-    ids(first, id);
-    load(first, id);
-    ids(first + 128, id);
+    load(first);
+    ids(first + 128);
   }
   for (int j0 = first; j0 < to; j0 += 128) {
-    // V's rows into LDS (zeros for keys that are masked: what lies there has no influence)
-    const uint32_t low = (uint32_t) __ballot(in[0]) & 0xFFFF, high = (uint32_t) __ballot(in[1]) & 0xFFFF;
-    const uint32_t live = low | high << 16;
+    // the tile's keys that are there, a bit each
+    uint32_t live = 0xFFFFFFFFu;
+    if (WIDE) {
+      if (!page_in[0]) live &= 0xFFFF0000u;
+      if (!page_in[1]) live &= 0x0000FFFFu;
+    } else {
+      live = ((uint32_t) __ballot(page_in[0]) & 0xFFFFu) | (uint32_t) __ballot(page_in[1]) << 16;
+    }
+    if (j0 + 32 > to) live &= (1u << (to - j0)) - 1;
+    if (j0 < begin) live &= 0xFFFFFFFFu << (begin - j0);
+    if (live != 0xFFFFFFFFu) {  // (zeros for the others' values: what lies there has no influence)
+#pragma unroll
+      for (int i = 0; i < 2; i++)
+        if (!(live >> (16 * i + r) & 1)) {
+#pragma unroll
+          for (int p = 0; p < T::kPieces; p++) vr[i][p] = u32x4{0, 0, 0, 0};
+        }
+    }
 #pragma unroll
     for (int i = 0; i < 2; i++)
 #pragma unroll
@@ -284,6 +320,11 @@ __global__ __launch_bounds__(256, D > 128 ? 1 : 2) void token_kernel(Args a, Kv 
 #pragma unroll
     for (int i = 0; i < 2; i++) {
       x[i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+      if (a.dim < D) {  // (the piece read in place of one past the dims)
+#pragma unroll
+        for (int p = 0; p < T::kPieces; p++)
+          if (64 * p + 16 * quad >= dim_bytes) kr[i][p] = u32x4{0, 0, 0, 0};
+      }
 #pragma unroll
       for (int k = 0; k < kSteps; k++) {
         v8 ka;
@@ -293,14 +334,10 @@ __global__ __launch_bounds__(256, D > 128 ? 1 : 2) void token_kernel(Args a, Kv 
       }
     }
     if (j0 + 128 < to) {
-      load(j0 + 128, id);
-      ids(j0 + 256, id);
+      load(j0 + 128);
+      ids(j0 + 256);
     }
     __builtin_amdgcn_sched_barrier(0);  // (the loads go out before the softmax)
-#pragma unroll
-    for (int i = 0; i < 2; i++)
-#pragma unroll
-      for (int j = 0; j < 4; j++) x[i][j] *= unit;
     if (live != 0xFFFFFFFFu) {
 #pragma unroll
       for (int i = 0; i < 2; i++)
@@ -309,22 +346,24 @@ __global__ __launch_bounds__(256, D > 128 ? 1 : 2) void token_kernel(Args a, Kv 
           if (!(live >> (16 * i + 4 * quad + j) & 1)) x[i][j] = -__builtin_inff();
     }
     float top = fmaxf(fmaxf(fmaxf(x[0][0], x[0][1]), fmaxf(x[0][2], x[0][3])), fmaxf(fmaxf(x[1][0], x[1][1]), fmaxf(x[1][2], x[1][3])));
-    top = fmaxf(m, max_rows(top));
-    const float base = finite_max(top), fade = __builtin_amdgcn_exp2f(m - base);
-    m = top;
+    top = fmaxf(m, max_rows(top) * unit);
+    const float base = finite_max(top);
+    if (__any(top > m)) {  // (seldom, once the greatest scores have been met)
+      const float fade = __builtin_amdgcn_exp2f(m - base);
+      m = top;
+      l *= fade;
+#pragma unroll
+      for (int t = 0; t < kDims; t++) o[t] *= fade;
+    }
     v8 p;
-    float sum = 0.0f;
 #pragma unroll
     for (int i = 0; i < 2; i++)
 #pragma unroll
       for (int j = 0; j < 4; j++) {
-        const float e = __builtin_amdgcn_exp2f(x[i][j] - base);
-        sum += e;
+        const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(x[i][j], unit, -base));
+        l += e;
         p[4 * i + j] = (typename U::e) e;
       }
-    l = __builtin_fmaf(l, fade, sum);
-#pragma unroll
-    for (int t = 0; t < kDims; t++) o[t] *= fade;
     // O^T: V^T's columns of keys 4 quad + 0 .. 3 and 16 + 4 quad + 0 .. 3, as P^T's lanes hold them
 #pragma unroll
     for (int t = 0; t < kDims; t++) {
@@ -336,9 +375,9 @@ __global__ __launch_bounds__(256, D > 128 ? 1 : 2) void token_kernel(Args a, Kv 
         va = from_f8<BF>(u32x2{(uint32_t) w[0], (uint32_t) w[1]});
       } else {
         typedef short s16x4 __attribute__((ext_vector_type(4)));
-        const int key = 4 * (int) quad + (int) (r / 4), piece = 2 * t + (int) (r & 3) / 2, part8 = 8 * (r & 1);
-        const s16x4 w0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*) (tile + T::at(key, piece) + part8));
-        const s16x4 w1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*) (tile + T::at(key + 16, piece) + part8));
+        const int key = 4 * (int) quad + (int) (r / 4), at = 2 * t + (int) (r & 3) / 2, part8 = 8 * (r & 1);
+        const s16x4 w0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*) (tile + T::at(key, at) + part8));
+        const s16x4 w1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*) (tile + T::at(key + 16, at) + part8));
         va = __builtin_bit_cast(v8, __builtin_shufflevector(w0, w1, 0, 1, 2, 3, 4, 5, 6, 7));
       }
       o[t] = U::mfma16(va, p, o[t]);
@@ -422,7 +461,7 @@ __global__ __launch_bounds__(256) void join_kernel(Args a, Step st, uint32_t pag
 
 // how a token step is launched: the chunks that the sequences are cut into for each kv head and 16 of its query heads, and
 // the workspace: where each sequence's chunks begin and how many they are, then the chunks' results
-constexpr uint32_t kWant = 1024;
+constexpr uint32_t kWant = 512;
 struct Cut {
   uint32_t want, most, tiles, dim;  // most: chunks there can be
   bool split;                       // whether a sequence can have more than one
@@ -448,7 +487,8 @@ template <bool BF, bool F8>
 bool run_token(const Args& a, const Kv& k, const Step& st, const Cut& c, uint8_t* workspace, hipStream_t stream) {
   const uint64_t blocks = (uint64_t) c.most * k.heads * c.tiles, rows = (uint64_t) st.n_seq * a.heads;
   if (blocks > 0x7FFFFFFFull || rows > 0x7FFFFFFFull) return false;
-  auto* kernel = c.dim == 64 ? token_kernel<BF, F8, 64> : c.dim == 128 ? token_kernel<BF, F8, 128> : token_kernel<BF, F8, 256>;
+  auto* kernel = k.page >= 16 ? (c.dim == 64 ? token_kernel<BF, F8, 64, true> : c.dim == 128 ? token_kernel<BF, F8, 128, true> : token_kernel<BF, F8, 256, true>)
+                              : (c.dim == 64 ? token_kernel<BF, F8, 64, false> : c.dim == 128 ? token_kernel<BF, F8, 128, false> : token_kernel<BF, F8, 256, false>);
   uint32_t* cut = c.split ? (uint32_t*) workspace : nullptr;
   float* part = (float*) (workspace + c.head);
   kernel<<<(uint32_t) blocks, 256, 0, stream>>>(a, k, st, c.want, c.tiles, cut, part);
