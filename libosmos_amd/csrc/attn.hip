@@ -10,7 +10,6 @@ namespace attn {
 using kv::Seq;
 using kv::Step;
 using kv::sequence;
-using kv::sequence_of;
 
 struct Args {
   const uint8_t* q;
@@ -31,6 +30,8 @@ struct Kv {
 
 // ---- the two 16-bit types the products are taken in ----
 typedef kv::f32x4 f32x4;
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef kv::u32x2 u32x2;
 typedef kv::u32x4 u32x4;
 typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
@@ -40,14 +41,18 @@ template <bool BF> struct Unit;
 template <> struct Unit<false> {
   typedef _Float16 e;
   typedef kv::f16x8 v8;
+  typedef _Float16 v4 __attribute__((ext_vector_type(4)));
   static __device__ inline f32x4 mfma16(v8 a, v8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
+  static __device__ inline f32x16 mfma32(v8 a, v8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
   static __device__ inline f16x2 f8_low(uint32_t w) { return __builtin_amdgcn_cvt_scalef32_pk_f16_fp8((int) w, 1.0f, false); }
   static __device__ inline f16x2 f8_high(uint32_t w) { return __builtin_amdgcn_cvt_scalef32_pk_f16_fp8((int) w, 1.0f, true); }
 };
 template <> struct Unit<true> {
   typedef __bf16 e;
   typedef kv::bf16x8 v8;
+  typedef __bf16 v4 __attribute__((ext_vector_type(4)));
   static __device__ inline f32x4 mfma16(v8 a, v8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
+  static __device__ inline f32x16 mfma32(v8 a, v8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
   static __device__ inline bf16x2 f8_low(uint32_t w) { return __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((int) w, 1.0f, false); }
   static __device__ inline bf16x2 f8_high(uint32_t w) { return __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((int) w, 1.0f, true); }
 };
@@ -374,7 +379,6 @@ __global__ __launch_bounds__(256, D > 128 ? 1 : 2) void token_kernel(Args a, Kv 
         const auto w = __builtin_amdgcn_ds_read_tr8_b64_v2i32((__attribute__((address_space(3))) i32x2*) (tile + T::at(key, t) + 8 * (r & 1)));
         va = from_f8<BF>(u32x2{(uint32_t) w[0], (uint32_t) w[1]});
       } else {
-        typedef short s16x4 __attribute__((ext_vector_type(4)));
         const int key = 4 * (int) quad + (int) (r / 4), at = 2 * t + (int) (r & 3) / 2, part8 = 8 * (r & 1);
         const s16x4 w0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*) (tile + T::at(key, at) + part8));
         const s16x4 w1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*) (tile + T::at(key + 16, at) + part8));
@@ -503,76 +507,312 @@ bool run_token(const Args& a, const Kv& k, const Step& st, const Cut& c, uint8_t
 // whether the products are taken in bf16
 __host__ __device__ inline bool in_bf16(uint32_t kv_type, uint32_t q_type) { return kv_type == OSMOS_BF16 || (kv_type == OSMOS_F8 && q_type == OSMOS_BF16); }
 
-__device__ inline float value(uint32_t type, const uint8_t* p, uint64_t i) {
-  if (type == OSMOS_F32) return ((const float*) p)[i];
-  if (type == OSMOS_F16) return (float) ((const _Float16*) p)[i];
-  if (type == OSMOS_BF16) return (float) ((const __bf16*) p)[i];
-  return __builtin_amdgcn_cvt_f32_fp8(p[i], 0);
+// ---- rows of prompts (osmos_attn_prompt, osmos_attn_chunk) ----
+// transposed as above, on v_mfma_f32_32x32x16: a wave holds 32 query rows as columns, a lane one of them (lane % 32) with
+// half the keys of a tile (by lane / 32), so that a row's maximum takes one exchange between two lanes and its scaling none, and P^T is the
+// second product's B operand as it comes out of the first. a query row is a (token, head) pair of one kv head, the heads
+// of a token next to one another: heads that share keys share their loads, a tile of rows covers few tokens (less work
+// lost at the causal edge), and a step of few tokens still fills the rows. a workgroup is W waves of rows over tiles of 64
+// keys, K and V in LDS twice (one tile worked on while the next, loaded into registers meanwhile, is written), one barrier
+// a tile. pieces of 16 bytes turned by row so that neither K's row reads nor V's transposing reads meet a bank twice.
+enum Source { kPacked, kPages, kPagesF8 };
+
+template <int D> struct RowsTile {
+  static constexpr int kKeys = D > 128 ? 32 : 64, kRow = 2 * D, kBytes = kKeys * kRow;
+  static __device__ inline int k_at(int row, int c) { return row * kRow + ((c ^ (D % 128 ? row >> 1 & 7 : row & 15)) * 16); }
+  static __device__ inline int v_at(int row, int c) { return row * kRow + ((c ^ (4 * (D % 128 ? row >> 1 & 1 : row & 3))) * 16); }
+};
+
+__device__ inline float max_halves(float x) {
+  auto r = __builtin_amdgcn_permlane32_swap(__float_as_int(x), __float_as_int(x), false, false);
+  return fmaxf(__int_as_float(r[0]), __int_as_float(r[1]));
+}
+__device__ inline float sum_halves(float x) {
+  auto r = __builtin_amdgcn_permlane32_swap(__float_as_int(x), __float_as_int(x), false, false);
+  return __int_as_float(r[0]) + __int_as_float(r[1]);
 }
 
-// a wave a row and head: 64 keys a round, a key a lane for the scores, a dim a lane (in turns of 64) for the output
-__global__ __launch_bounds__(64) void row_kernel(Args a, Kv kv, Step st) {
-  __shared__ float qv[OSMOS_ATTN_MAX_DIM];
-  const uint32_t t = blockIdx.x, h = blockIdx.y, lane = threadIdx.x, g = h / a.group;
-  const int s = sequence_of(st, (int) t);
-  if (s < 0) return;
-  const Seq seq = sequence(st, (uint32_t) s, kv.page);
-  if ((int) t < seq.row0 || (int) t >= seq.row0 + seq.rows) return;
-  const int pos = seq.len - (seq.row0 + seq.rows - (int) t);
-  const int end = pos + 1 < seq.end ? pos + 1 : seq.end;
-  const int begin = a.window && pos + 1 > (int) a.window ? pos + 1 - (int) a.window : 0;
-  const bool bf = in_bf16(kv.type, a.q_type);
-  for (uint32_t d = lane; d < a.dim; d += 64) {
-    const float x = value(a.q_type, a.q, t * a.qs + h * a.qh + d);
-    qv[d] = bf ? (float) (__bf16) x : (float) (_Float16) x;
+// tile `index` of the step's tiles of `rows` query rows (the last ones first: they see the most keys): its sequence and its
+// place among that sequence's
+__device__ inline bool find_rows(const Step& st, uint32_t page, uint32_t group, uint32_t rows, uint32_t index, Seq& seq, uint32_t& tile) {
+  const uint32_t lane = threadIdx.x & 63;
+  Seq none, q;
+  none.row0 = none.rows = none.len = none.end = 0, none.table = st.table;
+  auto tiles = [&](const Seq& x) { return (uint32_t) (((uint64_t) (uint32_t) x.rows * group + rows - 1) / rows); };
+  uint32_t total = 0;
+  q = lane < st.n_seq ? sequence(st, lane, page) : none;
+  for (uint32_t s = 0;;) {
+    total += (uint32_t) lane_of((int) wave_scan(tiles(q)), 63);
+    if ((s += 64) >= st.n_seq) break;
+    q = s + lane < st.n_seq ? sequence(st, s + lane, page) : none;
   }
-  __syncthreads();
-  const float ks = kv.scale ? kv.scale[g] : 1.0f, vs = kv.scale ? kv.scale[kv.heads + g] : 1.0f;
-  float m = -__builtin_inff(), l = 0.0f, o[4] = {};
-  for (int j0 = begin; j0 < end; j0 += 64) {
-    const int j = j0 + (int) lane;
-    bool in = j < end;
-    uint64_t kat = 0, vat = 0;
-    if (in) {
-      if (kv.page) {
-        const uint32_t id = (uint32_t) seq.table[(uint32_t) j / kv.page];
-        in = id < kv.pages;
-        kat = vat = (((uint64_t) id * kv.heads + g) * kv.page + (uint32_t) j % kv.page) * a.dim;
+  if (index >= total) return false;
+  index = total - 1 - index;
+  uint32_t before = 0;
+  for (uint32_t s = 0; s < st.n_seq; s += 64) {
+    if (st.n_seq > 64) q = s + lane < st.n_seq ? sequence(st, s + lane, page) : none;
+    const uint32_t n = tiles(q), x = before + wave_scan(n);
+    const uint64_t past = __ballot(x > index);
+    if (past) {
+      const int at = __builtin_ctzll(past);
+      tile = index - ((uint32_t) lane_of((int) x, at) - (uint32_t) lane_of((int) n, at));
+      seq.row0 = lane_of(q.row0, at), seq.rows = lane_of(q.rows, at), seq.len = lane_of(q.len, at), seq.end = lane_of(q.end, at);
+      seq.table = (const int32_t*) ((uint64_t) (uint32_t) lane_of((int) ((uint64_t) q.table >> 32), at) << 32 |
+                                    (uint32_t) lane_of((int) (uint64_t) q.table, at));
+      return true;
+    }
+    before = (uint32_t) lane_of((int) x, 63);
+  }
+  return false;
+}
+
+// whether one of 8 16-bit values is an infinity or NaN
+template <bool BF>
+__device__ inline bool not_finite(u32x4 w) {
+  constexpr uint32_t e = BF ? 0x7F80u : 0x7C00u;
+  bool bad = false;
+#pragma unroll
+  for (int i = 0; i < 4; i++) bad = bad || (w[i] & e) == e || (w[i] >> 16 & e) == e;
+  return bad;
+}
+
+template <bool BF, int SRC, int D, int W>
+__global__ __launch_bounds__(64 * W, D > 128 ? 1 : 2) void rows_kernel(Args a, Kv kv, Step st) {
+  typedef Unit<BF> U;
+  typedef typename U::v8 v8;
+  typedef RowsTile<D> T;
+  constexpr int kThreads = 64 * W, kRows = 32 * W, kSteps = D / 16, kDims = D / 32, kKeys = T::kKeys, kParts = kKeys / 32;
+  constexpr int kPieces = SRC == kPagesF8 ? kKeys * D / 16 : kKeys * D / 8;  // 16-byte pieces of a tile's keys in memory
+  constexpr int kEach = (kPieces + kThreads - 1) / kThreads, kPer = kPieces / kKeys;
+  __shared__ __attribute__((aligned(16))) uint8_t lds[2][2][T::kBytes];
+  const uint32_t lane = threadIdx.x & 63, wave = (uint32_t) __builtin_amdgcn_readfirstlane((int) threadIdx.x / 64);
+  const uint32_t half = lane / 32, col = lane & 31;
+  const uint32_t g = blockIdx.x % kv.heads;
+  Seq seq;
+  uint32_t tile;
+  if (!find_rows(st, SRC == kPacked ? 0 : kv.page, a.group, kRows, blockIdx.x / kv.heads, seq, tile)) return;
+
+  // the rows: the workgroup's, the wave's, the lane's, and the positions of their tokens
+  const uint32_t all = (uint32_t) seq.rows * a.group, row0 = tile * kRows, last = all - 1 < row0 + kRows - 1 ? all - 1 : row0 + kRows - 1;
+  const int base = seq.len - seq.rows;
+  const int pos_lo = base + (int) (row0 / a.group), pos_hi = base + (int) (last / a.group);
+  const uint32_t wrow = row0 + 32 * wave, wlast = last < wrow + 31 ? last : wrow + 31;
+  const bool idle = wrow > last;
+  const int wpos_lo = base + (int) (wrow / a.group), wpos_hi = base + (int) (wlast / a.group);
+  const uint32_t row = wrow + col, token = row / a.group, head = g * a.group + row % a.group;
+  const bool in = row < all;
+  const int pos = base + (int) token;
+  const int window = a.window ? (int) a.window : 0x7FFFFFFF;
+  const int from = a.window && pos_lo >= window ? (pos_lo - window + 1) & ~(kKeys - 1) : 0;
+  const int to = pos_hi + 1 < seq.end ? pos_hi + 1 : seq.end;
+
+  // a thread's pieces of a tile's keys: rows kthread / kPer + .., loaded a tile ahead, their page ids two
+  const uint32_t size = SRC == kPagesF8 ? 1 : 2, dim_bytes = a.dim * size, shift = SRC == kPacked ? 0 : 31 - __builtin_clz(kv.page);
+  const uint64_t page_bytes = (uint64_t) kv.heads * kv.page * dim_bytes, head_at = (uint64_t) g * kv.page * dim_bytes;
+  u32x4 kr[kEach], vr[kEach];
+  int id[kEach], live_id = 0;
+  bool there[kEach];
+  uint64_t live_next = 0;
+  auto key_row = [&](int n) { return (int) ((threadIdx.x + n * kThreads) / kPer); };
+  auto piece = [&](int n) { return (threadIdx.x + n * kThreads) % kPer; };
+  auto clamp_key = [&](int j) { return j < to ? j : to - 1; };
+  auto ids = [&](int j0) {
+    if constexpr (SRC != kPacked) {
+#pragma unroll
+      for (int n = 0; n < kEach; n++) id[n] = gload<int>(seq.table + ((uint32_t) clamp_key(j0 + (key_row(n) & (kKeys - 1))) >> shift));
+      live_id = gload<int>(seq.table + ((uint32_t) clamp_key(j0 + (int) (lane & (kKeys - 1))) >> shift));
+    }
+  };
+  auto load = [&](int j0) {
+    live_next = __ballot(((int) lane >= kKeys || j0 + (int) lane < to) && (SRC == kPacked || (uint32_t) live_id < kv.pages));
+#pragma unroll
+    for (int n = 0; n < kEach; n++) {
+      const int j = clamp_key(j0 + (key_row(n) & (kKeys - 1)));
+      const uint32_t at = piece(n) * 16 < dim_bytes ? piece(n) * 16 : 0;
+      if constexpr (SRC == kPacked) {
+        kr[n] = gload<u32x4>(kv.k + ((uint64_t) (seq.row0 + j) * kv.ks + g * kv.kh) * 2 + at);
+        vr[n] = gload<u32x4>(kv.v + ((uint64_t) (seq.row0 + j) * kv.vs + g * kv.vh) * 2 + at);
       } else {
-        kat = (uint64_t) (seq.row0 + j) * kv.ks + g * kv.kh, vat = (uint64_t) (seq.row0 + j) * kv.vs + g * kv.vh;
+        there[n] = (uint32_t) id[n] < kv.pages;
+        const uint64_t p = (there[n] ? (uint32_t) id[n] : 0u) * page_bytes + head_at + ((uint32_t) j & (kv.page - 1)) * dim_bytes + at;
+        kr[n] = gload<u32x4>(kv.k + p);
+        vr[n] = gload<u32x4>(kv.v + p);
       }
     }
-    float x = 0.0f;
-    if (in)
-      for (uint32_t d = 0; d < a.dim; d++) x = __builtin_fmaf(qv[d], value(kv.type, kv.k, kat + d), x);
-    x = in ? x * (a.scale * ks) : -__builtin_inff();
-    float top = x;
-    for (int o2 = 1; o2 < 64; o2 <<= 1) top = fmaxf(top, __shfl_xor(top, o2));
-    top = fmaxf(top, m);
-    if (top == -__builtin_inff()) continue;
-    const float p = in ? expf(x - top) : 0.0f, c = expf(m - top);
-    float sum = p;
-    for (int o2 = 1; o2 < 64; o2 <<= 1) sum += __shfl_xor(sum, o2);
-    l = l * c + sum, m = top;
-    for (int i = 0; i < 4; i++) o[i] *= c;
-    for (int i = 0; i < 64; i++) {
-      if (!__shfl((int) in, i)) continue;
-      const float pi = __shfl(p, i);
-      const uint64_t at = ((uint64_t) (uint32_t) __shfl((int) (vat >> 32), i) << 32) | (uint32_t) __shfl((int) vat, i);
-      for (int e = 0; e < 4; e++)
-        if (lane + 64 * e < a.dim) o[e] = __builtin_fmaf(pi, value(kv.type, kv.v, at + lane + 64 * e), o[e]);
+  };
+  // the loaded tile into LDS. values of keys that are not there are zeros (masked, they have no influence); whether, in a
+  // tile that some rows see in part, a value is not finite
+  auto store = [&](int buf, uint64_t live, bool partial) {
+    bool bad = false;
+    uint8_t *k = lds[buf][0], *v = lds[buf][1];
+#pragma unroll
+    for (int n = 0; n < kEach; n++) {
+      if (kPieces % kThreads && threadIdx.x + n * kThreads >= kPieces) break;
+      const int r = key_row(n);
+      const uint32_t c = piece(n);
+      if (live != ~0ull && !(live >> r & 1)) vr[n] = u32x4{0, 0, 0, 0};
+      if (a.dim < D && c * 16 >= dim_bytes) kr[n] = vr[n] = u32x4{0, 0, 0, 0};
+      if constexpr (SRC == kPagesF8) {
+#pragma unroll
+        for (int i = 0; i < 2; i++) {
+          const u32x4 kw = __builtin_bit_cast(u32x4, from_f8<BF>(u32x2{kr[n][2 * i], kr[n][2 * i + 1]}));
+          const u32x4 vw = __builtin_bit_cast(u32x4, from_f8<BF>(u32x2{vr[n][2 * i], vr[n][2 * i + 1]}));
+          *(u32x4*) (k + T::k_at(r, 2 * c + i)) = kw;
+          *(u32x4*) (v + T::v_at(r, 2 * c + i)) = vw;
+          if (partial) bad = bad || not_finite<BF>(vw);
+        }
+      } else {
+        *(u32x4*) (k + T::k_at(r, c)) = kr[n];
+        *(u32x4*) (v + T::v_at(r, c)) = vr[n];
+        if (partial) bad = bad || not_finite<BF>(vr[n]);
+      }
+    }
+    if (partial) return __syncthreads_or(bad) != 0;
+    __syncthreads();
+    return false;
+  };
+  auto partial = [&](int j0) { return j0 + kKeys - 1 > pos_lo || j0 <= pos_hi - window; };
+
+  if (from < to) ids(from);
+  v8 q[kSteps];
+  load_q<BF, kSteps>(a, (uint64_t) seq.row0 + (in ? token : 0), in ? head : 0, in, [&](int i) { return (uint32_t) (16 * i + 8 * half); }, q);
+  const float unit = fabsf(a.scale) * kLog2E * (SRC == kPagesF8 && kv.scale ? kv.scale[g] : 1.0f);
+  f32x16 o[kDims];
+#pragma unroll
+  for (int i = 0; i < kDims; i++) o[i] = f32x16{};
+  float m = -__builtin_inff(), l = 0.0f;
+
+  uint64_t live = 0;
+  bool bad = false;
+  if (from < to) {
+    load(from);
+    ids(from + kKeys);
+    live = live_next;
+    bad = store(0, live, partial(from));
+  }
+  for (int j0 = from, buf = 0; j0 < to; j0 += kKeys, buf ^= 1) {
+    const bool more = j0 + kKeys < to;
+    if (more) {
+      load(j0 + kKeys);
+      ids(j0 + 2 * kKeys);
+    }
+    const uint8_t *kt = lds[buf][0], *vt = lds[buf][1];
+    if (!idle && j0 <= wpos_hi && (!a.window || j0 + kKeys - 1 > wpos_lo - window)) {
+      f32x16 x[kParts];
+#pragma unroll
+      for (int t = 0; t < kParts; t++) {
+        x[t] = f32x16{};
+#pragma unroll
+        for (int i = 0; i < kSteps; i++) x[t] = U::mfma32(*(const v8*) (kt + T::k_at(32 * t + (int) col, 2 * i + (int) half)), q[i], x[t]);
+      }
+      const bool masked = live != ~0ull || j0 + kKeys - 1 > wpos_lo || (a.window && j0 <= wpos_hi - window);
+      if (masked) {
+        const int hi = pos - j0, lo = a.window && pos >= window ? pos - window - j0 : -1;  // keys lo + 1 .. hi of the tile
+        const uint64_t mine = live >> (4 * half);
+#pragma unroll
+        for (int t = 0; t < kParts; t++)
+#pragma unroll
+          for (int i = 0; i < 16; i++) {
+            const int key = 32 * t + 8 * (i / 4) + i % 4, at = key + 4 * (int) half;
+            if (at > hi || at <= lo || !(mine >> key & 1)) x[t][i] = -__builtin_inff();
+          }
+      }
+      float top = x[0][0];
+#pragma unroll
+      for (int t = 0; t < kParts; t++)
+#pragma unroll
+        for (int i = 0; i < 16; i++) top = fmaxf(top, x[t][i]);
+      top = fmaxf(m, max_halves(top) * unit);
+      const float sub = finite_max(top);
+      if (__any(top > m)) {
+        const float fade = __builtin_amdgcn_exp2f(m - sub);
+        m = top;
+        l *= fade;
+#pragma unroll
+        for (int i = 0; i < kDims; i++) o[i] *= fade;
+      }
+      v8 p[2 * kParts];
+#pragma unroll
+      for (int t = 0; t < kParts; t++)
+#pragma unroll
+        for (int i = 0; i < 16; i++) {
+          const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(x[t][i], unit, -sub));
+          l += e;
+          p[2 * t + i / 8][i % 8] = (typename U::e) e;
+        }
+      if (!(masked && bad)) {
+        // V^T's columns of keys 16 u + 4 half + 0 .. 3 and 8 more on, as P^T's lanes hold them
+        const int r = (int) (4 * half + (lane & 15) / 4), dims = (int) (16 * (lane >> 4 & 1) + 4 * (lane & 3));
+#pragma unroll
+        for (int u = 0; u < 2 * kParts; u++)
+#pragma unroll
+          for (int i = 0; i < kDims; i++) {
+            const uint8_t* at = vt + T::v_at(16 * u + r, 4 * i + dims / 8) + dims % 8 * 2;
+            const s16x4 w0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*) at);
+            const s16x4 w1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*) (at + 8 * T::kRow));
+            o[i] = U::mfma32(__builtin_bit_cast(v8, __builtin_shufflevector(w0, w1, 0, 1, 2, 3, 4, 5, 6, 7)), p[u], o[i]);
+          }
+      } else {
+        // a value that is not finite must not reach rows that its key is masked for (0 times it is NaN): key by key, the
+        // probability made again from the scores' own operands
+#pragma clang loop unroll(disable)
+        for (int j = 0; j < kKeys; j++) {
+          float e = 0.0f;
+#pragma unroll
+          for (int i = 0; i < kSteps; i++) {
+            const v8 kw = *(const v8*) (kt + T::k_at(j, 2 * i + (int) half));
+#pragma unroll
+            for (int n = 0; n < 8; n++) e = __builtin_fmaf((float) kw[n], (float) q[i][n], e);
+          }
+          e = __builtin_amdgcn_exp2f(__builtin_fmaf(sum_halves(e), unit, -sub));
+          const bool sees = (live >> j & 1) && j <= pos - j0 && (!a.window || j > pos - window - j0);
+          e = (float) (typename U::e) e;
+#pragma unroll
+          for (int i = 0; i < kDims; i++)
+#pragma unroll
+            for (int n = 0; n < 4; n++) {
+              const typename U::v4 w = *(const typename U::v4*) (vt + T::v_at(j, 4 * i + n) + 8 * half);
+#pragma unroll
+              for (int d = 0; d < 4; d++) {
+                const float y = __builtin_fmaf(e, (float) w[d], o[i][4 * n + d]);
+                o[i][4 * n + d] = sees ? y : o[i][4 * n + d];
+              }
+            }
+        }
+      }
+    }
+    if (more) {
+      live = live_next;
+      bad = store(buf ^ 1, live, partial(j0 + kKeys));
     }
   }
-  for (int e = 0; e < 4; e++) {
-    const uint32_t d = lane + 64 * e;
-    if (d >= a.dim) break;
-    const float y = l > 0.0f ? o[e] * vs / l : l == 0.0f ? 0.0f : l;
-    const uint64_t at = t * a.os + h * a.oh + d;
-    if (a.out_type == OSMOS_F32) ((float*) a.out)[at] = y;
-    else if (a.out_type == OSMOS_F16) ((_Float16*) a.out)[at] = (_Float16) y;
-    else ((__bf16*) a.out)[at] = (__bf16) y;
-  }
-  if (a.lse && lane == 0) a.lse[(uint64_t) t * a.heads + h] = m + logf(l);
+
+  if (!in) return;
+  l = sum_halves(l);
+  const float inv = l == 0.0f ? 0.0f : (SRC == kPagesF8 && kv.scale ? kv.scale[kv.heads + g] : 1.0f) / l;
+  const uint64_t at = ((uint64_t) seq.row0 + token) * a.os + head * a.oh;
+#pragma unroll
+  for (int i = 0; i < kDims; i++)
+#pragma unroll
+    for (int n = 0; n < 4; n++) {
+      const uint32_t d = 32 * i + 8 * n + 4 * half;
+      if (d < a.dim) put4(a, at + d, f32x4{o[i][4 * n], o[i][4 * n + 1], o[i][4 * n + 2], o[i][4 * n + 3]} * inv);
+    }
+  if (a.lse && half == 0) a.lse[((uint64_t) seq.row0 + token) * a.heads + head] = (m + log2f(l)) * kLn2;
+}
+
+template <bool BF, int SRC>
+bool run_rows(const Args& a, const Kv& k, const OsmosKvStep* step, hipStream_t stream) {
+  constexpr int W = 8, WD = 4;
+  const uint32_t rows = a.dim <= 128 ? 32 * W : 32 * WD;
+  const uint64_t tiles = (uint64_t) step->n_tok * a.group / rows + step->n_seq, blocks = tiles * k.heads;
+  if (blocks > 0x7FFFFFFFull || (uint64_t) step->n_tok * a.group > 0x7FFFFFFFull) return false;
+  const Step st = kv::step_of(step);
+  if (a.dim <= 64) rows_kernel<BF, SRC, 64, W><<<(uint32_t) blocks, 64 * W, 0, stream>>>(a, k, st);
+  else if (a.dim <= 128) rows_kernel<BF, SRC, 128, W><<<(uint32_t) blocks, 64 * W, 0, stream>>>(a, k, st);
+  else if (a.dim <= 192) rows_kernel<BF, SRC, 192, WD><<<(uint32_t) blocks, 64 * WD, 0, stream>>>(a, k, st);
+  else rows_kernel<BF, SRC, 256, WD><<<(uint32_t) blocks, 64 * WD, 0, stream>>>(a, k, st);
+  return hipGetLastError() == hipSuccess;
 }
 
 inline bool row_type(uint32_t t) { return t == OSMOS_F32 || t == OSMOS_F16 || t == OSMOS_BF16; }
@@ -597,11 +837,6 @@ inline Kv pages_of(const OsmosKv* kv, uint32_t layer) {
             kv->scale ? kv->scale + 2ull * layer * kv->heads : nullptr};
 }
 
-bool run_rows(const OsmosAttn* a, const Kv& k, uint32_t dim, const OsmosKvStep* step, void* stream) {
-  row_kernel<<<dim3(step->n_tok, a->heads), 64, 0, (hipStream_t) stream>>>(args_of(a, k.heads, dim), k, kv::step_of(step));
-  return hipGetLastError() == hipSuccess;
-}
-
 }  // namespace attn
 }  // namespace osm
 
@@ -622,14 +857,19 @@ extern "C" OSM_API bool osmos_attn_prompt(const OsmosAttn* a, const OsmosKvRows*
   if (!attn::args_ok(a, r->heads, r->dim) || !kv::step_ok(step, false)) return false;
   const attn::Kv k{(const uint8_t*) r->k, (const uint8_t*) r->v, r->k_stride, r->k_head, r->v_stride, r->v_head, r->type,
                    0, 0, r->heads, nullptr};
-  return attn::run_rows(a, k, r->dim, step, stream);
+  const attn::Args args = attn::args_of(a, r->heads, r->dim);
+  return r->type == OSMOS_BF16 ? attn::run_rows<true, attn::kPacked>(args, k, step, (hipStream_t) stream)
+                               : attn::run_rows<false, attn::kPacked>(args, k, step, (hipStream_t) stream);
 }
 
 extern "C" OSM_API bool osmos_attn_chunk(const OsmosAttn* a, const OsmosKv* kv, uint32_t layer, const OsmosKvStep* step,
                                          void* workspace, uint64_t workspace_bytes, void* stream) {
   (void) workspace, (void) workspace_bytes;
   if (!kv::cache_ok(kv) || layer >= kv->layers || !attn::args_ok(a, kv->heads, kv->dim) || !kv::step_ok(step, true)) return false;
-  return attn::run_rows(a, attn::pages_of(kv, layer), kv->dim, step, stream);
+  const bool bf = attn::in_bf16(kv->type, a->q_type), f8 = kv->type == OSMOS_F8;
+  auto* run = bf ? (f8 ? attn::run_rows<true, attn::kPagesF8> : attn::run_rows<true, attn::kPages>)
+                 : (f8 ? attn::run_rows<false, attn::kPagesF8> : attn::run_rows<false, attn::kPages>);
+  return run(attn::args_of(a, kv->heads, kv->dim), attn::pages_of(kv, layer), step, (hipStream_t) stream);
 }
 
 extern "C" OSM_API bool osmos_attn_token(const OsmosAttn* a, const OsmosKv* kv, uint32_t layer, const OsmosKvStep* step,
