@@ -2,6 +2,8 @@
 //
 // a row's output is sum_j p_j v_j / sum_j p_j with p_j = exp(scale q k_j - m), m the greatest score, in one pass: the
 // running m and sum, the sum and output scaled by exp(m_old - m_new) where m grows.
+#include <type_traits>
+
 #include "kvcache.h"
 
 namespace osm {
@@ -566,13 +568,17 @@ __device__ inline bool find_rows(const Step& st, uint32_t page, uint32_t group, 
   return false;
 }
 
-// whether one of 8 16-bit values is an infinity or NaN
+// zeros for the infinities and NaN among 8 16-bit values; whether there were any
 template <bool BF>
-__device__ inline bool not_finite(u32x4 w) {
+__device__ inline bool take_finite(u32x4& w) {
   constexpr uint32_t e = BF ? 0x7F80u : 0x7C00u;
   bool bad = false;
 #pragma unroll
-  for (int i = 0; i < 4; i++) bad = bad || (w[i] & e) == e || (w[i] >> 16 & e) == e;
+  for (int i = 0; i < 4; i++) {
+    const bool low = (w[i] & e) == e, high = (w[i] >> 16 & e) == e;
+    w[i] &= (low ? 0u : 0xFFFFu) | (high ? 0u : 0xFFFF0000u);
+    bad = bad || low || high;
+  }
   return bad;
 }
 
@@ -640,11 +646,14 @@ __global__ __launch_bounds__(64 * W, D > 128 ? 1 : 2) void rows_kernel(Args a, K
       }
     }
   };
-  // the loaded tile into LDS. values of keys that are not there are zeros (masked, they have no influence); whether, in a
-  // tile that some rows see in part, a value is not finite
-  auto store = [&](int buf, uint64_t live, bool partial) {
-    bool bad = false;
+  auto partial = [&](int j0) { return j0 + kKeys - 1 > pos_lo || j0 <= pos_hi - window; };
+  // the loaded tile into LDS. values of keys that are not there are zeros: masked, they have no influence. in a tile that
+  // some of the rows see in part, so are infinities and NaN, as 0 times them would reach the rows that do not see them:
+  // those that do get them at the end
+  bool bad = false;
+  auto store = [&](int buf, int j0, uint64_t live) {
     uint8_t *k = lds[buf][0], *v = lds[buf][1];
+    const bool part = partial(j0);
 #pragma unroll
     for (int n = 0; n < kEach; n++) {
       if (kPieces % kThreads && threadIdx.x + n * kThreads >= kPieces) break;
@@ -656,22 +665,19 @@ __global__ __launch_bounds__(64 * W, D > 128 ? 1 : 2) void rows_kernel(Args a, K
 #pragma unroll
         for (int i = 0; i < 2; i++) {
           const u32x4 kw = __builtin_bit_cast(u32x4, from_f8<BF>(u32x2{kr[n][2 * i], kr[n][2 * i + 1]}));
-          const u32x4 vw = __builtin_bit_cast(u32x4, from_f8<BF>(u32x2{vr[n][2 * i], vr[n][2 * i + 1]}));
+          u32x4 vw = __builtin_bit_cast(u32x4, from_f8<BF>(u32x2{vr[n][2 * i], vr[n][2 * i + 1]}));
+          if (part && take_finite<BF>(vw)) bad = true;
           *(u32x4*) (k + T::k_at(r, 2 * c + i)) = kw;
           *(u32x4*) (v + T::v_at(r, 2 * c + i)) = vw;
-          if (partial) bad = bad || not_finite<BF>(vw);
         }
       } else {
+        if (part && take_finite<BF>(vr[n])) bad = true;
         *(u32x4*) (k + T::k_at(r, c)) = kr[n];
         *(u32x4*) (v + T::v_at(r, c)) = vr[n];
-        if (partial) bad = bad || not_finite<BF>(vr[n]);
       }
     }
-    if (partial) return __syncthreads_or(bad) != 0;
     __syncthreads();
-    return false;
   };
-  auto partial = [&](int j0) { return j0 + kKeys - 1 > pos_lo || j0 <= pos_hi - window; };
 
   if (from < to) ids(from);
   v8 q[kSteps];
@@ -683,14 +689,15 @@ __global__ __launch_bounds__(64 * W, D > 128 ? 1 : 2) void rows_kernel(Args a, K
   float m = -__builtin_inff(), l = 0.0f;
 
   uint64_t live = 0;
-  bool bad = false;
   if (from < to) {
     load(from);
     ids(from + kKeys);
     live = live_next;
-    bad = store(0, live, partial(from));
+    store(0, from, live);
   }
-  for (int j0 = from, buf = 0; j0 < to; j0 += kKeys, buf ^= 1) {
+  // one tile, from the buffer that the next one is not written to (a constant: it goes into the LDS reads' offsets)
+  auto step = [&](int j0, auto buffer) {
+    constexpr int buf = decltype(buffer)::value;
     const bool more = j0 + kKeys < to;
     if (more) {
       load(j0 + kKeys);
@@ -707,15 +714,25 @@ __global__ __launch_bounds__(64 * W, D > 128 ? 1 : 2) void rows_kernel(Args a, K
       }
       const bool masked = live != ~0ull || j0 + kKeys - 1 > wpos_lo || (a.window && j0 <= wpos_hi - window);
       if (masked) {
-        const int hi = pos - j0, lo = a.window && pos >= window ? pos - window - j0 : -1;  // keys lo + 1 .. hi of the tile
-        const uint64_t mine = live >> (4 * half);
+        // the row's keys are lo + 1 .. hi of the tile (less the half's 4, so that the lane's keys are constants)
+        const int hi = pos - j0 - 4 * (int) half, lo = a.window && pos >= window ? pos - window - j0 - 4 * (int) half : -5;
 #pragma unroll
         for (int t = 0; t < kParts; t++)
 #pragma unroll
           for (int i = 0; i < 16; i++) {
-            const int key = 32 * t + 8 * (i / 4) + i % 4, at = key + 4 * (int) half;
-            if (at > hi || at <= lo || !(mine >> key & 1)) x[t][i] = -__builtin_inff();
+            const int key = 32 * t + 8 * (i / 4) + i % 4;
+            if (key > hi || key <= lo) x[t][i] = -__builtin_inff();
           }
+        if (live != ~0ull) {
+          const uint64_t mine = live >> (4 * half);
+#pragma unroll
+          for (int t = 0; t < kParts; t++) {
+            const uint32_t bits = (uint32_t) (mine >> (32 * t));
+#pragma unroll
+            for (int i = 0; i < 16; i++)
+              if (!(bits >> (8 * (i / 4) + i % 4) & 1)) x[t][i] = -__builtin_inff();
+          }
+        }
       }
       float top = x[0][0];
 #pragma unroll
@@ -740,53 +757,63 @@ __global__ __launch_bounds__(64 * W, D > 128 ? 1 : 2) void rows_kernel(Args a, K
           l += e;
           p[2 * t + i / 8][i % 8] = (typename U::e) e;
         }
-      if (!(masked && bad)) {
-        // V^T's columns of keys 16 u + 4 half + 0 .. 3 and 8 more on, as P^T's lanes hold them
-        const int r = (int) (4 * half + (lane & 15) / 4), dims = (int) (16 * (lane >> 4 & 1) + 4 * (lane & 3));
+      // V^T's columns of keys 16 u + 4 half + 0 .. 3 and 8 more on, as P^T's lanes hold them
+      const int r = (int) (4 * half + (lane & 15) / 4), dims = (int) (16 * (lane >> 4 & 1) + 4 * (lane & 3));
 #pragma unroll
-        for (int u = 0; u < 2 * kParts; u++)
+      for (int u = 0; u < 2 * kParts; u++)
 #pragma unroll
-          for (int i = 0; i < kDims; i++) {
-            const uint8_t* at = vt + T::v_at(16 * u + r, 4 * i + dims / 8) + dims % 8 * 2;
-            const s16x4 w0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*) at);
-            const s16x4 w1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*) (at + 8 * T::kRow));
-            o[i] = U::mfma32(__builtin_bit_cast(v8, __builtin_shufflevector(w0, w1, 0, 1, 2, 3, 4, 5, 6, 7)), p[u], o[i]);
+        for (int i = 0; i < kDims; i++) {
+          const uint8_t* at = vt + T::v_at(16 * u + r, 4 * i + dims / 8) + dims % 8 * 2;
+          const s16x4 w0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*) at);
+          const s16x4 w1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*) (at + 8 * T::kRow));
+          o[i] = U::mfma32(__builtin_bit_cast(v8, __builtin_shufflevector(w0, w1, 0, 1, 2, 3, 4, 5, 6, 7)), p[u], o[i]);
+        }
+    }
+    if (more) {
+      live = live_next;
+      store(buf ^ 1, j0 + kKeys, live);
+    }
+  };
+  for (int j0 = from; j0 < to; j0 += 2 * kKeys) {
+    step(j0, std::integral_constant<int, 0>());
+    if (j0 + kKeys < to) step(j0 + kKeys, std::integral_constant<int, 1>());
+  }
+
+  if (__syncthreads_or(bad)) {
+    // seldom: the infinities and NaN left out above, added to the rows that see their keys
+    for (int t = from; t < to; t += kKeys)
+      if (partial(t))
+        for (int j = t; j < (t + kKeys < to ? t + kKeys : to); j++) {
+          uint64_t at;
+          if constexpr (SRC == kPacked) {
+            at = ((uint64_t) (seq.row0 + j) * kv.vs + g * kv.vh) * 2;
+          } else {
+            const uint32_t page = (uint32_t) seq.table[(uint32_t) j >> shift];
+            if (page >= kv.pages) continue;
+            at = page * page_bytes + head_at + ((uint32_t) j & (kv.page - 1)) * dim_bytes;
           }
-      } else {
-        // a value that is not finite must not reach rows that its key is masked for (0 times it is NaN): key by key, the
-        // probability made again from the scores' own operands
-#pragma clang loop unroll(disable)
-        for (int j = 0; j < kKeys; j++) {
-          float e = 0.0f;
-#pragma unroll
-          for (int i = 0; i < kSteps; i++) {
-            const v8 kw = *(const v8*) (kt + T::k_at(j, 2 * i + (int) half));
-#pragma unroll
-            for (int n = 0; n < 8; n++) e = __builtin_fmaf((float) kw[n], (float) q[i][n], e);
-          }
-          e = __builtin_amdgcn_exp2f(__builtin_fmaf(sum_halves(e), unit, -sub));
-          const bool sees = (live >> j & 1) && j <= pos - j0 && (!a.window || j > pos - window - j0);
-          e = (float) (typename U::e) e;
+          if (j > pos || j <= pos - window) continue;
 #pragma unroll
           for (int i = 0; i < kDims; i++)
 #pragma unroll
             for (int n = 0; n < 4; n++) {
-              const typename U::v4 w = *(const typename U::v4*) (vt + T::v_at(j, 4 * i + n) + 8 * half);
-#pragma unroll
-              for (int d = 0; d < 4; d++) {
-                const float y = __builtin_fmaf(e, (float) w[d], o[i][4 * n + d]);
-                o[i][4 * n + d] = sees ? y : o[i][4 * n + d];
+              const uint32_t d = 32 * i + 8 * n + 4 * half;
+              if (d >= a.dim) continue;
+              f32x4 w;
+              if constexpr (SRC == kPagesF8) {
+                const uint32_t x = gload<uint32_t>(kv.v + at + d);
+                const auto low = U::f8_low(x), high = U::f8_high(x);
+                w = f32x4{(float) low[0], (float) low[1], (float) high[0], (float) high[1]};
+              } else {
+                const typename U::v4 x = gload<typename U::v4>(kv.v + at + d * 2);
+                w = f32x4{(float) x[0], (float) x[1], (float) x[2], (float) x[3]};
               }
+#pragma unroll
+              for (int e = 0; e < 4; e++)
+                if (!(fabsf(w[e]) < __builtin_inff())) o[i][4 * n + e] += w[e];
             }
         }
-      }
-    }
-    if (more) {
-      live = live_next;
-      bad = store(buf ^ 1, live, partial(j0 + kKeys));
-    }
   }
-
   if (!in) return;
   l = sum_halves(l);
   const float inv = l == 0.0f ? 0.0f : (SRC == kPagesF8 && kv.scale ? kv.scale[kv.heads + g] : 1.0f) / l;
