@@ -582,6 +582,19 @@ __device__ inline bool take_finite(u32x4& w) {
   return bad;
 }
 
+// the scheduler's order for N products of R LDS reads each: the reads four products ahead
+template <int N, int R>
+__device__ inline void feed() {
+  constexpr int kAhead = 4;
+  __builtin_amdgcn_sched_group_barrier(0x100, kAhead * R, 0);
+#pragma unroll
+  for (int i = 0; i < N - kAhead; i++) {
+    __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+    __builtin_amdgcn_sched_group_barrier(0x100, R, 0);
+  }
+  __builtin_amdgcn_sched_group_barrier(0x008, kAhead, 0);
+}
+
 template <bool BF, int SRC, int D, int W>
 __global__ __launch_bounds__(64 * W, D > 128 ? 1 : 2) void rows_kernel(Args a, Kv kv, Step st) {
   typedef Unit<BF> U;
@@ -616,6 +629,7 @@ __global__ __launch_bounds__(64 * W, D > 128 ? 1 : 2) void rows_kernel(Args a, K
   const uint32_t size = SRC == kPagesF8 ? 1 : 2, dim_bytes = a.dim * size, shift = SRC == kPacked ? 0 : 31 - __builtin_clz(kv.page);
   const uint64_t page_bytes = (uint64_t) kv.heads * kv.page * dim_bytes, head_at = (uint64_t) g * kv.page * dim_bytes;
   u32x4 kr[kEach], vr[kEach];
+  const uint8_t *kp[kEach], *vp[kEach];  // packed rows: the pieces' places
   int id[kEach], live_id = 0;
   bool there[kEach];
   uint64_t live_next = 0;
@@ -636,8 +650,14 @@ __global__ __launch_bounds__(64 * W, D > 128 ? 1 : 2) void rows_kernel(Args a, K
       const int j = clamp_key(j0 + (key_row(n) & (kKeys - 1)));
       const uint32_t at = piece(n) * 16 < dim_bytes ? piece(n) * 16 : 0;
       if constexpr (SRC == kPacked) {
-        kr[n] = gload<u32x4>(kv.k + ((uint64_t) (seq.row0 + j) * kv.ks + g * kv.kh) * 2 + at);
-        vr[n] = gload<u32x4>(kv.v + ((uint64_t) (seq.row0 + j) * kv.vs + g * kv.vh) * 2 + at);
+        if (j0 == from || j0 + kKeys > to) {
+          kp[n] = kv.k + ((uint64_t) (seq.row0 + j) * kv.ks + g * kv.kh) * 2 + at;
+          vp[n] = kv.v + ((uint64_t) (seq.row0 + j) * kv.vs + g * kv.vh) * 2 + at;
+        } else {
+          kp[n] += kv.ks * (2 * kKeys), vp[n] += kv.vs * (2 * kKeys);
+        }
+        kr[n] = gload<u32x4>(kp[n]);
+        vr[n] = gload<u32x4>(vp[n]);
       } else {
         there[n] = (uint32_t) id[n] < kv.pages;
         const uint64_t p = (there[n] ? (uint32_t) id[n] : 0u) * page_bytes + head_at + ((uint32_t) j & (kv.page - 1)) * dim_bytes + at;
@@ -707,11 +727,12 @@ __global__ __launch_bounds__(64 * W, D > 128 ? 1 : 2) void rows_kernel(Args a, K
     if (!idle && j0 <= wpos_hi && (!a.window || j0 + kKeys - 1 > wpos_lo - window)) {
       f32x16 x[kParts];
 #pragma unroll
-      for (int t = 0; t < kParts; t++) {
-        x[t] = f32x16{};
+      for (int t = 0; t < kParts; t++) x[t] = f32x16{};
 #pragma unroll
-        for (int i = 0; i < kSteps; i++) x[t] = U::mfma32(*(const v8*) (kt + T::k_at(32 * t + (int) col, 2 * i + (int) half)), q[i], x[t]);
-      }
+      for (int i = 0; i < kSteps; i++)
+#pragma unroll
+        for (int t = 0; t < kParts; t++) x[t] = U::mfma32(*(const v8*) (kt + T::k_at(32 * t + (int) col, 2 * i + (int) half)), q[i], x[t]);
+      feed<kSteps * kParts, 1>();
       const bool masked = live != ~0ull || j0 + kKeys - 1 > wpos_lo || (a.window && j0 <= wpos_hi - window);
       if (masked) {
         // the row's keys are lo + 1 .. hi of the tile (less the half's 4, so that the lane's keys are constants)
@@ -768,6 +789,7 @@ __global__ __launch_bounds__(64 * W, D > 128 ? 1 : 2) void rows_kernel(Args a, K
           const s16x4 w1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*) (at + 8 * T::kRow));
           o[i] = U::mfma32(__builtin_bit_cast(v8, __builtin_shufflevector(w0, w1, 0, 1, 2, 3, 4, 5, 6, 7)), p[u], o[i]);
         }
+      feed<2 * kParts * kDims, 2>();
     }
     if (more) {
       live = live_next;
