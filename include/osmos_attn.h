@@ -27,6 +27,7 @@ extern "C" {
 #define OSMOS_BF16 30u
 #define OSMOS_F8 0x200u  /* e4m3, saturating at 448; no GGUF id */
 #define OSMOS_ATTN_MAX_DIM 256u
+#define OSMOS_ATTN_MAX_STRIDE (1u << 24) /* values between two packed rows of keys or values */
 #define OSMOS_KV_MAX_PAGE 4096u
 #define OSMOS_KV_MAX_REQUESTS 1024u
 

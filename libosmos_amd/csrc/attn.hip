@@ -72,7 +72,8 @@ __device__ inline typename Unit<BF>::v8 from_f8(u32x2 w) {
 }
 
 // a lane's values of a query head as the B operand of N steps, 8 dims each from at(i) on, in the products' type (an F32 q's
-// rounded once), negated for a negative scale; zeros where `in` is false or past the dims
+// rounded once), negated for a negative scale; zeros where `in` is false, past the
+// dims and for a scale of 0
 template <bool BF, int N, uint32_t T, class At>
 __device__ inline void q_steps(const uint8_t* p, uint32_t dim, bool in, float sign, At at, typename Unit<BF>::v8 (&q)[N]) {
   float x[N][8];
@@ -88,7 +89,7 @@ __device__ inline void q_steps(const uint8_t* p, uint32_t dim, bool in, float si
 template <bool BF, int N, class At>
 __device__ inline void load_q(const Args& a, uint64_t row, uint32_t head, bool in, At at, typename Unit<BF>::v8 (&q)[N]) {
   const uint8_t* p = a.q + (row * a.qs + head * a.qh) * kv::size_of(a.q_type);
-  const float sign = a.scale < 0.0f ? -1.0f : 1.0f;
+  const float sign = a.scale < 0.0f ? -1.0f : a.scale == 0.0f ? 0.0f : 1.0f;
   if (a.q_type == OSMOS_F32) q_steps<BF, N, OSMOS_F32>(p, a.dim, in, sign, at, q);
   else if (a.q_type == OSMOS_F16) q_steps<BF, N, OSMOS_F16>(p, a.dim, in, sign, at, q);
   else q_steps<BF, N, OSMOS_BF16>(p, a.dim, in, sign, at, q);
@@ -121,6 +122,8 @@ __device__ inline float sum_rows(float x) {
 }
 
 constexpr float kLog2E = 1.44269504088896341f, kLn2 = 0.693147180559945309f;
+// what a score is multiplied with (its sign is in q; of a scale of 0 q is zeros, as -infinity times 0 would be NaN)
+__device__ inline float unit_of(const Args& a) { return a.scale == 0.0f ? 1.0f : fabsf(a.scale) * kLog2E; }
 // a maximum as what is subtracted: of nothing (-infinity), zero, so that exp2 of the difference is 0 and not NaN
 __device__ inline float finite_max(float m) { return m == -__builtin_inff() ? 0.0f : m; }
 
@@ -287,7 +290,7 @@ __global__ __launch_bounds__(256, D > 128 ? 1 : 2) void token_kernel(Args a, Kv 
   load_q<BF, kSteps>(a, row, head0 + (r < heads ? r : 0), r < heads, [&](int i) {
     return F8 ? (uint32_t) (64 * (i / 2) + 16 * quad + 8 * (i % 2)) : (uint32_t) (32 * i + 8 * quad);
   }, q);
-  const float unit = fabsf(a.scale) * kLog2E * (F8 && kv.scale ? kv.scale[g] : 1.0f);
+  const float unit = unit_of(a) * (F8 && kv.scale ? kv.scale[g] : 1.0f);
 
   f32x4 o[kDims];
 #pragma unroll
@@ -514,10 +517,18 @@ __host__ __device__ inline bool in_bf16(uint32_t kv_type, uint32_t q_type) { ret
 // half the keys of a tile (by lane / 32), so that a row's maximum takes one exchange between two lanes and its scaling none, and P^T is the
 // second product's B operand as it comes out of the first. a query row is a (token, head) pair of one kv head, the heads
 // of a token next to one another: heads that share keys share their loads, a tile of rows covers few tokens (less work
-// lost at the causal edge), and a step of few tokens still fills the rows. a workgroup is W waves of rows over tiles of 64
-// keys, K and V in LDS twice (one tile worked on while the next, loaded into registers meanwhile, is written), one barrier
-// a tile. pieces of 16 bytes turned by row so that neither K's row reads nor V's transposing reads meet a bank twice.
+// lost at the causal edge), and a step of few tokens still fills the rows.
+// a workgroup is W waves of rows over tiles of 64 keys, K and V in LDS twice, pieces of 16 bytes turned by row so that
+// neither K's row reads nor V's transposing reads meet a bank twice. a tile is two phases of a wave: its scores' products, the
+// writing of loaded keys and values into LDS and the last tile's output products (matrix units), then its softmax (vector
+// units). of 8 waves, two a SIMD, the second four run one phase behind the first, so that one of a SIMD's two waves
+// is on the matrix units while the other is on the vector units: in step, each would wait for the other's kind (the phases
+// then took 97 % of the time one after another). a barrier ends each phase.
 enum Source { kPacked, kPages, kPagesF8 };
+
+// a row's scores are taken against its running maximum as it was until one is past it by more than this (in powers of two):
+// probabilities to 2^8 cost no accuracy in either type, and most tiles then leave the output and the sum unscaled
+constexpr float kSlack = 8.0f;
 
 template <int D> struct RowsTile {
   static constexpr int kKeys = D > 128 ? 32 : 64, kRow = 2 * D, kBytes = kKeys * kRow;
@@ -568,29 +579,38 @@ __device__ inline bool find_rows(const Step& st, uint32_t page, uint32_t group, 
   return false;
 }
 
-// zeros for the infinities and NaN among 8 16-bit values; whether there were any
-template <bool BF>
+// zeros for the infinities and NaN among 16 bytes of values (e4m3 has NaN alone); whether there were any
+template <bool BF, bool F8>
 __device__ inline bool take_finite(u32x4& w) {
-  constexpr uint32_t e = BF ? 0x7F80u : 0x7C00u;
+  constexpr int bits = F8 ? 8 : 16;
+  constexpr uint32_t e = F8 ? 0x7Fu : BF ? 0x7F80u : 0x7C00u;
   bool bad = false;
 #pragma unroll
   for (int i = 0; i < 4; i++) {
-    const bool low = (w[i] & e) == e, high = (w[i] >> 16 & e) == e;
-    w[i] &= (low ? 0u : 0xFFFFu) | (high ? 0u : 0xFFFF0000u);
-    bad = bad || low || high;
+    uint32_t keep = 0xFFFFFFFFu;
+#pragma unroll
+    for (int b = 0; b < 32; b += bits)
+      if ((w[i] >> b & e) == e) keep &= ~(((1u << bits) - 1) << b), bad = true;
+    w[i] &= keep;
   }
   return bad;
 }
 
-// the scheduler's order for N products of R LDS reads each: the reads four products ahead
-template <int N, int R>
+// the scheduler's order for a block of N scores' products (an LDS read each) and M outputs' (two each), the reads four
+// products ahead
+template <int N, int M>
 __device__ inline void feed() {
   constexpr int kAhead = 4;
-  __builtin_amdgcn_sched_group_barrier(0x100, kAhead * R, 0);
+  __builtin_amdgcn_sched_group_barrier(0x100, kAhead, 0);
 #pragma unroll
   for (int i = 0; i < N - kAhead; i++) {
     __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
-    __builtin_amdgcn_sched_group_barrier(0x100, R, 0);
+    __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+  }
+#pragma unroll
+  for (int i = 0; i < M; i++) {
+    __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+    __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
   }
   __builtin_amdgcn_sched_group_barrier(0x008, kAhead, 0);
 }
@@ -603,7 +623,9 @@ __global__ __launch_bounds__(64 * W, D > 128 ? 1 : 2) void rows_kernel(Args a, K
   constexpr int kThreads = 64 * W, kRows = 32 * W, kSteps = D / 16, kDims = D / 32, kKeys = T::kKeys, kParts = kKeys / 32;
   constexpr int kPieces = SRC == kPagesF8 ? kKeys * D / 16 : kKeys * D / 8;  // 16-byte pieces of a tile's keys in memory
   constexpr int kEach = (kPieces + kThreads - 1) / kThreads, kPer = kPieces / kKeys;
-  __shared__ __attribute__((aligned(16))) uint8_t lds[2][2][T::kBytes];
+  __shared__ __attribute__((aligned(16))) uint8_t lds[2][2][T::kBytes];  // [keys, values][tile & 1]
+  typedef std::integral_constant<int, 0> Even;
+  typedef std::integral_constant<int, 1> Odd;
   const uint32_t lane = threadIdx.x & 63, wave = (uint32_t) __builtin_amdgcn_readfirstlane((int) threadIdx.x / 64);
   const uint32_t half = lane / 32, col = lane & 31;
   const uint32_t g = blockIdx.x % kv.heads;
@@ -616,7 +638,6 @@ __global__ __launch_bounds__(64 * W, D > 128 ? 1 : 2) void rows_kernel(Args a, K
   const int base = seq.len - seq.rows;
   const int pos_lo = base + (int) (row0 / a.group), pos_hi = base + (int) (last / a.group);
   const uint32_t wrow = row0 + 32 * wave, wlast = last < wrow + 31 ? last : wrow + 31;
-  const bool idle = wrow > last;
   const int wpos_lo = base + (int) (wrow / a.group), wpos_hi = base + (int) (wlast / a.group);
   const uint32_t row = wrow + col, token = row / a.group, head = g * a.group + row % a.group;
   const bool in = row < all;
@@ -625,180 +646,232 @@ __global__ __launch_bounds__(64 * W, D > 128 ? 1 : 2) void rows_kernel(Args a, K
   const int from = a.window && pos_lo >= window ? (pos_lo - window + 1) & ~(kKeys - 1) : 0;
   const int to = pos_hi + 1 < seq.end ? pos_hi + 1 : seq.end;
 
-  // a thread's pieces of a tile's keys: rows kthread / kPer + .., loaded a tile ahead, their page ids two
+  // a thread's 16-byte pieces of a tile: of rows key_row(i). stage s writes the keys of tile s + 1 and the values of tile s
+  // into LDS, loaded into registers a tile's time before; page ids are loaded one stage ahead of that. past the last tile
+  // the last is loaded and written again, which no one reads: the products' phase has no conditions in it
   const uint32_t size = SRC == kPagesF8 ? 1 : 2, dim_bytes = a.dim * size, shift = SRC == kPacked ? 0 : 31 - __builtin_clz(kv.page);
   const uint64_t page_bytes = (uint64_t) kv.heads * kv.page * dim_bytes, head_at = (uint64_t) g * kv.page * dim_bytes;
+  const int n = from < to ? (to - from + kKeys - 1) / kKeys : 0;
+  const bool late = W == 8 && wave >= 4;
   u32x4 kr[kEach], vr[kEach];
-  const uint8_t *kp[kEach], *vp[kEach];  // packed rows: the pieces' places
-  int id[kEach], live_id = 0;
-  bool there[kEach];
-  uint64_t live_next = 0;
-  auto key_row = [&](int n) { return (int) ((threadIdx.x + n * kThreads) / kPer); };
-  auto piece = [&](int n) { return (threadIdx.x + n * kThreads) % kPer; };
-  auto clamp_key = [&](int j) { return j < to ? j : to - 1; };
-  auto ids = [&](int j0) {
+  int kid[kEach], vid[kEach], live_id = 0;
+  uint64_t live_old = 0, live = 0, live_new = 0;  // of tiles s - 1, s and s + 1: the keys that are there, a bit each
+  auto key_row = [&](int i) __attribute__((always_inline)) { return (int) ((threadIdx.x + i * kThreads) / kPer) & (kKeys - 1); };
+  auto piece = [&](int i) __attribute__((always_inline)) { return (threadIdx.x + i * kThreads) % kPer; };
+  auto start = [&](int t) __attribute__((always_inline)) { return from + (t < n ? t : n - 1) * kKeys; };
+  auto clamp_key = [&](int j) __attribute__((always_inline)) { return j < to ? j : to - 1; };
+  auto ids = [&](int t) __attribute__((always_inline)) {
     if constexpr (SRC != kPacked) {
 #pragma unroll
-      for (int n = 0; n < kEach; n++) id[n] = gload<int>(seq.table + ((uint32_t) clamp_key(j0 + (key_row(n) & (kKeys - 1))) >> shift));
-      live_id = gload<int>(seq.table + ((uint32_t) clamp_key(j0 + (int) (lane & (kKeys - 1))) >> shift));
+      for (int i = 0; i < kEach; i++) vid[i] = kid[i], kid[i] = gload<int>(seq.table + ((uint32_t) clamp_key(start(t) + key_row(i)) >> shift));
+      live_id = gload<int>(seq.table + ((uint32_t) clamp_key(start(t) + (int) (lane & (kKeys - 1))) >> shift));
     }
   };
-  auto load = [&](int j0) {
-    live_next = __ballot(((int) lane >= kKeys || j0 + (int) lane < to) && (SRC == kPacked || (uint32_t) live_id < kv.pages));
+  // packed rows: where tiles of keys and of values lie, the next of each to be loaded
+  const uint8_t *kplace = kv.k + ((uint64_t) (seq.row0 + from) * kv.ks + g * kv.kh) * 2, *vplace = kv.v + ((uint64_t) (seq.row0 + from) * kv.vs + g * kv.vh) * 2;
+  auto load = [&](int t, const uint8_t*& plane, uint32_t stride, const int (&id)[kEach], u32x4 (&to_regs)[kEach]) __attribute__((always_inline)) {
+    const int j0 = start(t);
 #pragma unroll
-    for (int n = 0; n < kEach; n++) {
-      const int j = clamp_key(j0 + (key_row(n) & (kKeys - 1)));
-      const uint32_t at = piece(n) * 16 < dim_bytes ? piece(n) * 16 : 0;
-      if constexpr (SRC == kPacked) {
-        if (j0 == from || j0 + kKeys > to) {
-          kp[n] = kv.k + ((uint64_t) (seq.row0 + j) * kv.ks + g * kv.kh) * 2 + at;
-          vp[n] = kv.v + ((uint64_t) (seq.row0 + j) * kv.vs + g * kv.vh) * 2 + at;
-        } else {
-          kp[n] += kv.ks * (2 * kKeys), vp[n] += kv.vs * (2 * kKeys);
-        }
-        kr[n] = gload<u32x4>(kp[n]);
-        vr[n] = gload<u32x4>(vp[n]);
+    for (int i = 0; i < kEach; i++) {
+      const uint32_t d = piece(i) * 16 < dim_bytes ? piece(i) * 16 : 0;
+      if constexpr (SRC == kPacked) {  // (a place that is the wave's, and the lane's from there)
+        to_regs[i] = gload<u32x4>(plane + ((uint32_t) (clamp_key(j0 + key_row(i)) - j0) * (stride * 2) + d));
       } else {
-        there[n] = (uint32_t) id[n] < kv.pages;
-        const uint64_t p = (there[n] ? (uint32_t) id[n] : 0u) * page_bytes + head_at + ((uint32_t) j & (kv.page - 1)) * dim_bytes + at;
-        kr[n] = gload<u32x4>(kv.k + p);
-        vr[n] = gload<u32x4>(kv.v + p);
+        const uint32_t page = (uint32_t) id[i] < kv.pages ? (uint32_t) id[i] : 0u, slot = (uint32_t) clamp_key(j0 + key_row(i)) & (kv.page - 1);
+        to_regs[i] = gload<u32x4>(plane + (page * page_bytes + head_at + slot * dim_bytes + d));
+      }
+    }
+    if (SRC == kPacked && t + 1 < n) plane += (uint64_t) stride * (2 * kKeys);
+  };
+  if constexpr (SRC != kPacked) kplace = kv.k, vplace = kv.v;
+  auto there = [&](int t) __attribute__((always_inline)) {
+    return __ballot(((int) lane >= kKeys || start(t) + (int) lane < to) && (SRC == kPacked || (uint32_t) live_id < kv.pages));
+  };
+  auto load_stage = [&](int s) __attribute__((always_inline)) {
+    live_old = live, live = live_new, live_new = there(s + 1);
+    load(s + 1, kplace, (uint32_t) kv.ks, kid, kr);
+    load(s, vplace, (uint32_t) kv.vs, vid, vr);
+    ids(s + 2);
+  };
+  // what must not reach LDS: keys' pieces past the dims (q is zeros there, but 0 times an infinity would be NaN); values of
+  // keys that are not there (masked, they have no influence); and in a tile that some of the rows see in part infinities and
+  // NaN, as 0 times them would reach the rows that do not see them: those that do get them at the end
+  auto partial = [&](int j0) __attribute__((always_inline)) { return j0 + kKeys - 1 > pos_lo || j0 <= pos_hi - window; };
+  bool bad = false;
+  auto mend_stage = [&](int s) __attribute__((always_inline)) {
+    if (a.dim < D) {
+      asm volatile("");  // (a branch: selects would wait for the loads here, in every tile)
+#pragma unroll
+      for (int i = 0; i < kEach; i++)
+        if (piece(i) * 16 >= dim_bytes) kr[i] = u32x4{0, 0, 0, 0};
+    }
+    const bool part = partial(start(s));
+    if (part || live != ~0ull) {
+      asm volatile("");
+#pragma unroll
+      for (int i = 0; i < kEach; i++) {
+        if (!(live >> key_row(i) & 1)) vr[i] = u32x4{0, 0, 0, 0};
+        if (part && take_finite<BF, SRC == kPagesF8>(vr[i])) bad = true;
       }
     }
   };
-  auto partial = [&](int j0) { return j0 + kKeys - 1 > pos_lo || j0 <= pos_hi - window; };
-  // the loaded tile into LDS. values of keys that are not there are zeros: masked, they have no influence. in a tile that
-  // some of the rows see in part, so are infinities and NaN, as 0 times them would reach the rows that do not see them:
-  // those that do get them at the end
-  bool bad = false;
-  auto store = [&](int buf, int j0, uint64_t live) {
-    uint8_t *k = lds[buf][0], *v = lds[buf][1];
-    const bool part = partial(j0);
+  auto write = [&](uint8_t* to_tile, bool values, const u32x4 (&regs)[kEach]) __attribute__((always_inline)) {
 #pragma unroll
-    for (int n = 0; n < kEach; n++) {
-      if (kPieces % kThreads && threadIdx.x + n * kThreads >= kPieces) break;
-      const int r = key_row(n);
-      const uint32_t c = piece(n);
-      if (live != ~0ull && !(live >> r & 1)) vr[n] = u32x4{0, 0, 0, 0};
-      if (a.dim < D && c * 16 >= dim_bytes) kr[n] = vr[n] = u32x4{0, 0, 0, 0};
+    for (int i = 0; i < kEach; i++) {
+      if (kPieces % kThreads && threadIdx.x + i * kThreads >= kPieces) break;
+      const int r = key_row(i), c = (int) piece(i);
       if constexpr (SRC == kPagesF8) {
 #pragma unroll
-        for (int i = 0; i < 2; i++) {
-          const u32x4 kw = __builtin_bit_cast(u32x4, from_f8<BF>(u32x2{kr[n][2 * i], kr[n][2 * i + 1]}));
-          u32x4 vw = __builtin_bit_cast(u32x4, from_f8<BF>(u32x2{vr[n][2 * i], vr[n][2 * i + 1]}));
-          if (part && take_finite<BF>(vw)) bad = true;
-          *(u32x4*) (k + T::k_at(r, 2 * c + i)) = kw;
-          *(u32x4*) (v + T::v_at(r, 2 * c + i)) = vw;
-        }
+        for (int w = 0; w < 2; w++)
+          *(u32x4*) (to_tile + (values ? T::v_at(r, 2 * c + w) : T::k_at(r, 2 * c + w))) = __builtin_bit_cast(u32x4, from_f8<BF>(u32x2{regs[i][2 * w], regs[i][2 * w + 1]}));
       } else {
-        if (part && take_finite<BF>(vr[n])) bad = true;
-        *(u32x4*) (k + T::k_at(r, c)) = kr[n];
-        *(u32x4*) (v + T::v_at(r, c)) = vr[n];
+        *(u32x4*) (to_tile + (values ? T::v_at(r, c) : T::k_at(r, c))) = regs[i];
       }
     }
-    __syncthreads();
+  };
+  // the end of a phase: LDS writes done and seen; loads from memory stay in flight
+  auto meet = [&]() __attribute__((always_inline)) {
+    __builtin_amdgcn_sched_barrier(0);  // (no instruction into the other phase: a softmax among the products keeps both waves waiting)
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
+    __builtin_amdgcn_s_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
+    __builtin_amdgcn_sched_barrier(0);
   };
 
-  if (from < to) ids(from);
+  if (n) {
+    ids(0);
+    live_new = there(0);
+    load(0, kplace, (uint32_t) kv.ks, kid, kr);
+    ids(1);
+  }
   v8 q[kSteps];
   load_q<BF, kSteps>(a, (uint64_t) seq.row0 + (in ? token : 0), in ? head : 0, in, [&](int i) { return (uint32_t) (16 * i + 8 * half); }, q);
-  const float unit = fabsf(a.scale) * kLog2E * (SRC == kPagesF8 && kv.scale ? kv.scale[g] : 1.0f);
-  f32x16 o[kDims];
+  const float unit = unit_of(a) * (SRC == kPagesF8 && kv.scale ? kv.scale[g] : 1.0f);
+  f32x16 o[kDims], x[kParts];
 #pragma unroll
   for (int i = 0; i < kDims; i++) o[i] = f32x16{};
+  v8 p[2 * kParts];
   float m = -__builtin_inff(), l = 0.0f;
 
-  uint64_t live = 0;
-  if (from < to) {
-    load(from);
-    ids(from + kKeys);
-    live = live_next;
-    store(0, from, live);
-  }
-  // one tile, from the buffer that the next one is not written to (a constant: it goes into the LDS reads' offsets)
-  auto step = [&](int j0, auto buffer) {
-    constexpr int buf = decltype(buffer)::value;
-    const bool more = j0 + kKeys < to;
-    if (more) {
-      load(j0 + kKeys);
-      ids(j0 + 2 * kKeys);
-    }
-    const uint8_t *kt = lds[buf][0], *vt = lds[buf][1];
-    if (!idle && j0 <= wpos_hi && (!a.window || j0 + kKeys - 1 > wpos_lo - window)) {
-      f32x16 x[kParts];
+  // a lane's places in a tile's keys and values: all of them by one exclusive or and one addition from the first (D a power
+  // of two), made anew for each tile, as there are no registers to keep them in
+  const int vrow = (int) (4 * half + (lane & 15) / 4), vdims = (int) (16 * (lane >> 4 & 1) + 4 * (lane & 3));
+  const uint32_t kfirst = (uint32_t) T::k_at((int) col, (int) half), vfirst = (uint32_t) (T::v_at(vrow, vdims / 8) + vdims % 8 * 2);
+  auto scores = [&](const uint8_t* kt) __attribute__((always_inline)) {
+    uint32_t at0 = kfirst;
+    asm volatile("" : "+v"(at0));
 #pragma unroll
-      for (int t = 0; t < kParts; t++) x[t] = f32x16{};
+    for (int i = 0; i < kParts; i++) x[i] = f32x16{};
 #pragma unroll
-      for (int i = 0; i < kSteps; i++)
+    for (int i = 0; i < kSteps; i++)
 #pragma unroll
-        for (int t = 0; t < kParts; t++) x[t] = U::mfma32(*(const v8*) (kt + T::k_at(32 * t + (int) col, 2 * i + (int) half)), q[i], x[t]);
-      feed<kSteps * kParts, 1>();
-      const bool masked = live != ~0ull || j0 + kKeys - 1 > wpos_lo || (a.window && j0 <= wpos_hi - window);
-      if (masked) {
-        // the row's keys are lo + 1 .. hi of the tile (less the half's 4, so that the lane's keys are constants)
-        const int hi = pos - j0 - 4 * (int) half, lo = a.window && pos >= window ? pos - window - j0 - 4 * (int) half : -5;
-#pragma unroll
-        for (int t = 0; t < kParts; t++)
-#pragma unroll
-          for (int i = 0; i < 16; i++) {
-            const int key = 32 * t + 8 * (i / 4) + i % 4;
-            if (key > hi || key <= lo) x[t][i] = -__builtin_inff();
-          }
-        if (live != ~0ull) {
-          const uint64_t mine = live >> (4 * half);
-#pragma unroll
-          for (int t = 0; t < kParts; t++) {
-            const uint32_t bits = (uint32_t) (mine >> (32 * t));
-#pragma unroll
-            for (int i = 0; i < 16; i++)
-              if (!(bits >> (8 * (i / 4) + i % 4) & 1)) x[t][i] = -__builtin_inff();
-          }
-        }
+      for (int k = 0; k < kParts; k++) {
+        const uint32_t at = (D & (D - 1)) == 0 ? (at0 ^ (uint32_t) (32 * i)) + (uint32_t) (32 * k * T::kRow) : (uint32_t) T::k_at(32 * k + (int) col, 2 * i + (int) half);
+        x[k] = U::mfma32(*(const v8*) (kt + at), q[i], x[k]);
       }
-      float top = x[0][0];
+  };
+  auto outputs = [&](const uint8_t* vt) __attribute__((always_inline)) {
+    // V^T's columns of keys 16 u + 4 half + 0 .. 3 and 8 more on, as P^T's lanes hold them
+    uint32_t at0 = vfirst;
+    asm volatile("" : "+v"(at0));
 #pragma unroll
-      for (int t = 0; t < kParts; t++)
+    for (int u = 0; u < 2 * kParts; u++)
 #pragma unroll
-        for (int i = 0; i < 16; i++) top = fmaxf(top, x[t][i]);
-      top = fmaxf(m, max_halves(top) * unit);
-      const float sub = finite_max(top);
-      if (__any(top > m)) {
-        const float fade = __builtin_amdgcn_exp2f(m - sub);
-        m = top;
-        l *= fade;
-#pragma unroll
-        for (int i = 0; i < kDims; i++) o[i] *= fade;
+      for (int i = 0; i < kDims; i++) {
+        const uint32_t at = (D & (D - 1)) == 0 ? (at0 ^ (uint32_t) (64 * i)) + (uint32_t) (16 * u * T::kRow) : (uint32_t) (T::v_at(16 * u + vrow, 4 * i + vdims / 8) + vdims % 8 * 2);
+        const s16x4 w0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*) (vt + at));
+        const s16x4 w1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*) (vt + at + 8 * T::kRow));
+        o[i] = U::mfma32(__builtin_bit_cast(v8, __builtin_shufflevector(w0, w1, 0, 1, 2, 3, 4, 5, 6, 7)), p[u], o[i]);
       }
-      v8 p[2 * kParts];
+  };
+  auto softmax = [&](int t) __attribute__((always_inline)) {
+    const int j0 = start(t);
+    if (live_old != ~0ull || j0 + kKeys - 1 > wpos_lo || (a.window && j0 <= wpos_hi - window)) {
+      // the row's keys are lo + 1 .. hi of the tile (less the half's 4, so that the lane's keys are constants)
+      const int hi = pos - j0 - 4 * (int) half, lo = a.window && pos >= window ? pos - window - j0 - 4 * (int) half : -5;
+      const uint64_t mine = live_old >> (4 * half);
 #pragma unroll
-      for (int t = 0; t < kParts; t++)
+      for (int k = 0; k < kParts; k++) {
+        const uint32_t bits = (uint32_t) (mine >> (32 * k));
 #pragma unroll
         for (int i = 0; i < 16; i++) {
-          const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(x[t][i], unit, -sub));
-          l += e;
-          p[2 * t + i / 8][i % 8] = (typename U::e) e;
+          const int key = 32 * k + 8 * (i / 4) + i % 4;
+          if (key > hi || key <= lo || !(bits >> (key & 31) & 1)) x[k][i] = -__builtin_inff();
         }
-      // V^T's columns of keys 16 u + 4 half + 0 .. 3 and 8 more on, as P^T's lanes hold them
-      const int r = (int) (4 * half + (lane & 15) / 4), dims = (int) (16 * (lane >> 4 & 1) + 4 * (lane & 3));
-#pragma unroll
-      for (int u = 0; u < 2 * kParts; u++)
-#pragma unroll
-        for (int i = 0; i < kDims; i++) {
-          const uint8_t* at = vt + T::v_at(16 * u + r, 4 * i + dims / 8) + dims % 8 * 2;
-          const s16x4 w0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*) at);
-          const s16x4 w1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*) (at + 8 * T::kRow));
-          o[i] = U::mfma32(__builtin_bit_cast(v8, __builtin_shufflevector(w0, w1, 0, 1, 2, 3, 4, 5, 6, 7)), p[u], o[i]);
-        }
-      feed<2 * kParts * kDims, 2>();
+      }
     }
-    if (more) {
-      live = live_next;
-      store(buf ^ 1, j0 + kKeys, live);
+    float top = x[0][0];
+#pragma unroll
+    for (int k = 0; k < kParts; k++)
+#pragma unroll
+      for (int i = 0; i < 16; i++) top = fmaxf(top, x[k][i]);
+    top = max_halves(top) * unit;
+    if (__any(top > m + kSlack)) {
+      const float next = fmaxf(m, top), fade = __builtin_amdgcn_exp2f(m - finite_max(next));
+      m = next;
+      l *= fade;
+#pragma unroll
+      for (int i = 0; i < kDims; i++) o[i] *= fade;
     }
+    const float sub = finite_max(m);
+#pragma unroll
+    for (int k = 0; k < kParts; k++)
+#pragma unroll
+      for (int i = 0; i < 16; i++) {
+        const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(x[k][i], unit, -sub));
+        l += e;
+        p[2 * k + i / 8][i % 8] = (typename U::e) e;
+      }
   };
-  for (int j0 = from; j0 < to; j0 += 2 * kKeys) {
-    step(j0, std::integral_constant<int, 0>());
-    if (j0 + kKeys < to) step(j0 + kKeys, std::integral_constant<int, 1>());
+  // the products' phase after tile t's softmax: the next tile's scores, tile t's outputs, the next stage
+  auto products = [&](int t, auto buf) __attribute__((always_inline)) {
+    constexpr int b = decltype(buf)::value;
+    scores(lds[0][1 - b]);
+    outputs(lds[1][b]);
+    feed<kSteps * kParts, 2 * kParts * kDims>();
+    mend_stage(t + 1);
+    write(lds[0][b], false, kr);
+    write(lds[1][1 - b], true, vr);
+    load_stage(t + 2);
+  };
+
+  if (n) {
+    if (a.dim < D) {
+#pragma unroll
+      for (int i = 0; i < kEach; i++)
+        if (piece(i) * 16 >= dim_bytes) kr[i] = u32x4{0, 0, 0, 0};
+    }
+    write(lds[0][0], false, kr);
+    load_stage(0);
+    meet();
+    if (late) meet();
+    mend_stage(0);
+    scores(lds[0][0]);
+    write(lds[0][1], false, kr);
+    write(lds[1][0], true, vr);
+    load_stage(1);
+    meet();
+    int t = 0;
+    for (; t + 2 < n; t += 2) {
+      softmax(t);
+      meet();
+      products(t, Even());
+      meet();
+      softmax(t + 1);
+      meet();
+      products(t + 1, Odd());
+      meet();
+    }
+    softmax(t);
+    if (t + 1 < n) {
+      meet();
+      products(t, Even());
+      meet();
+      softmax(++t);
+    }
+    meet();
+    outputs(lds[1][t & 1]);
+    if (!late) meet();
   }
 
   if (__syncthreads_or(bad)) {
@@ -903,6 +976,7 @@ extern "C" OSM_API bool osmos_attn_prompt(const OsmosAttn* a, const OsmosKvRows*
   if (!r || !r->k || !r->v || !r->heads || r->heads > 4096 || (r->type != OSMOS_F16 && r->type != OSMOS_BF16)) return false;
   if (!r->dim || r->dim > OSMOS_ATTN_MAX_DIM || r->dim % 16 || (uintptr_t) r->k % 16 || (uintptr_t) r->v % 16) return false;
   if (r->k_stride % 8 || r->k_head % 8 || r->v_stride % 8 || r->v_head % 8) return false;
+  if (r->k_stride > OSMOS_ATTN_MAX_STRIDE || r->v_stride > OSMOS_ATTN_MAX_STRIDE) return false;
   if (!attn::args_ok(a, r->heads, r->dim) || !kv::step_ok(step, false)) return false;
   const attn::Kv k{(const uint8_t*) r->k, (const uint8_t*) r->v, r->k_stride, r->k_head, r->v_stride, r->v_head, r->type,
                    0, 0, r->heads, nullptr};
