@@ -518,12 +518,13 @@ __host__ __device__ inline bool in_bf16(uint32_t kv_type, uint32_t q_type) { ret
 // second product's B operand as it comes out of the first. a query row is a (token, head) pair of one kv head, the heads
 // of a token next to one another: heads that share keys share their loads, a tile of rows covers few tokens (less work
 // lost at the causal edge), and a step of few tokens still fills the rows.
-// a workgroup is W waves of rows over tiles of 64 keys, K and V in LDS twice, pieces of 16 bytes turned by row so that
-// neither K's row reads nor V's transposing reads meet a bank twice. a tile is two phases of a wave: its scores' products, the
-// writing of loaded keys and values into LDS and the last tile's output products (matrix units), then its softmax (vector
-// units). of 8 waves, two a SIMD, the second four run one phase behind the first, so that one of a SIMD's two waves
-// is on the matrix units while the other is on the vector units: in step, each would wait for the other's kind (the phases
-// then took 97 % of the time one after another). a barrier ends each phase.
+// a workgroup is 4 waves of rows over tiles of 32 keys, K and V in LDS twice, pieces of 16 bytes turned by row so that
+// neither K's row reads nor V's transposing reads meet a bank twice; one barrier a tile, between the products of one tile (its
+// scores', the last tile's outputs') and the next's, so that the waves of a SIMD, of two workgroups, are on the matrix and
+// the vector units at different times. measured against it for a prompt of 8192 (32 heads of 128 on 8): 8 waves and tiles of 64
+// keys 5 % faster with the second four waves held one phase behind the first, the same without; but prompts of 1 to 2111 tokens
+// 11 % slower, chunks over 8-bit pages 22 %, one of 77 tokens 60 %.
+constexpr int kKeys = 32, kRowWaves = 4, kRows = 32 * kRowWaves;
 enum Source { kPacked, kPages, kPagesF8 };
 
 // a row's scores are taken against its running maximum as it was until one is past it by more than this (in powers of two):
@@ -531,7 +532,7 @@ enum Source { kPacked, kPages, kPagesF8 };
 constexpr float kSlack = 8.0f;
 
 template <int D> struct RowsTile {
-  static constexpr int kKeys = D > 128 ? 32 : 64, kRow = 2 * D, kBytes = kKeys * kRow;
+  static constexpr int kRow = 2 * D, kBytes = kKeys * kRow;
   static __device__ inline int k_at(int row, int c) { return row * kRow + ((c ^ (D % 128 ? row >> 1 & 7 : row & 15)) * 16); }
   static __device__ inline int v_at(int row, int c) { return row * kRow + ((c ^ (4 * (D % 128 ? row >> 1 & 1 : row & 3))) * 16); }
 };
@@ -545,17 +546,42 @@ __device__ inline float sum_halves(float x) {
   return __int_as_float(r[0]) + __int_as_float(r[1]);
 }
 
-// tile `index` of the step's tiles of `rows` query rows (the last ones first: they see the most keys): its sequence and its
-// place among that sequence's
-__device__ inline bool find_rows(const Step& st, uint32_t page, uint32_t group, uint32_t rows, uint32_t index, Seq& seq, uint32_t& tile) {
+// tile `index` of the step's tiles of kRows query rows: its sequence and its place there. every workgroup finds its own. up to
+// 64 sequences (a lane each) in the order of the places, the last places of all sequences first: they see the most keys, and
+// what starts late should be short. more sequences from the last to the first, by their running sums
+__device__ inline bool find_rows(const Step& st, uint32_t page, uint32_t group, uint32_t index, Seq& seq, uint32_t& tile) {
   const uint32_t lane = threadIdx.x & 63;
   Seq none, q;
   none.row0 = none.rows = none.len = none.end = 0, none.table = st.table;
-  auto tiles = [&](const Seq& x) { return (uint32_t) (((uint64_t) (uint32_t) x.rows * group + rows - 1) / rows); };
-  uint32_t total = 0;
+  auto tiles = [&](const Seq& x) { return (uint32_t) (((uint64_t) (uint32_t) x.rows * group + kRows - 1) / kRows); };
+  auto sum = [&](uint32_t x) { return (uint32_t) lane_of((int) wave_scan(x), 63); };
+  auto take = [&](int at) {
+    seq.row0 = lane_of(q.row0, at), seq.rows = lane_of(q.rows, at), seq.len = lane_of(q.len, at), seq.end = lane_of(q.end, at);
+    seq.table = (const int32_t*) ((uint64_t) (uint32_t) lane_of((int) ((uint64_t) q.table >> 32), at) << 32 |
+                                  (uint32_t) lane_of((int) (uint64_t) q.table, at));
+  };
   q = lane < st.n_seq ? sequence(st, lane, page) : none;
+  if (st.n_seq <= 64) {
+    const uint32_t n = tiles(q);
+    if (index >= sum(n)) return false;
+    // the greatest place that more than `index` tiles lie at or after
+    auto after = [&](uint32_t place) { return sum(n > place ? n - place : 0); };
+    uint32_t low = 0, high = 1;
+    while (after(high) > index) low = high, high *= 2;
+    while (high - low > 1) {
+      const uint32_t mid = (low + high) / 2;
+      if (after(mid) > index) low = mid;
+      else high = mid;
+    }
+    tile = low;
+    uint64_t has = __ballot(n > low);
+    for (uint32_t turn = index - after(low + 1); turn; turn--) has &= has - 1;
+    take(__builtin_ctzll(has));
+    return true;
+  }
+  uint32_t total = 0;
   for (uint32_t s = 0;;) {
-    total += (uint32_t) lane_of((int) wave_scan(tiles(q)), 63);
+    total += sum(tiles(q));
     if ((s += 64) >= st.n_seq) break;
     q = s + lane < st.n_seq ? sequence(st, s + lane, page) : none;
   }
@@ -563,15 +589,13 @@ __device__ inline bool find_rows(const Step& st, uint32_t page, uint32_t group, 
   index = total - 1 - index;
   uint32_t before = 0;
   for (uint32_t s = 0; s < st.n_seq; s += 64) {
-    if (st.n_seq > 64) q = s + lane < st.n_seq ? sequence(st, s + lane, page) : none;
+    q = s + lane < st.n_seq ? sequence(st, s + lane, page) : none;
     const uint32_t n = tiles(q), x = before + wave_scan(n);
     const uint64_t past = __ballot(x > index);
     if (past) {
       const int at = __builtin_ctzll(past);
       tile = index - ((uint32_t) lane_of((int) x, at) - (uint32_t) lane_of((int) n, at));
-      seq.row0 = lane_of(q.row0, at), seq.rows = lane_of(q.rows, at), seq.len = lane_of(q.len, at), seq.end = lane_of(q.end, at);
-      seq.table = (const int32_t*) ((uint64_t) (uint32_t) lane_of((int) ((uint64_t) q.table >> 32), at) << 32 |
-                                    (uint32_t) lane_of((int) (uint64_t) q.table, at));
+      take(at);
       return true;
     }
     before = (uint32_t) lane_of((int) x, 63);
@@ -615,12 +639,13 @@ __device__ inline void feed() {
   __builtin_amdgcn_sched_group_barrier(0x008, kAhead, 0);
 }
 
-template <bool BF, int SRC, int D, int W>
-__global__ __launch_bounds__(64 * W, D > 128 ? 1 : 2) void rows_kernel(Args a, Kv kv, Step st) {
+template <bool BF, int SRC, int D>
+__global__ __launch_bounds__(64 * kRowWaves, D > 128 ? 1 : 2) void rows_kernel(Args a, Kv kv, Step st, uint32_t parts,
+                                                                               float* __restrict__ part) {
   typedef Unit<BF> U;
   typedef typename U::v8 v8;
   typedef RowsTile<D> T;
-  constexpr int kThreads = 64 * W, kRows = 32 * W, kSteps = D / 16, kDims = D / 32, kKeys = T::kKeys, kParts = kKeys / 32;
+  constexpr int kThreads = 64 * kRowWaves, kSteps = D / 16, kDims = D / 32;
   constexpr int kPieces = SRC == kPagesF8 ? kKeys * D / 16 : kKeys * D / 8;  // 16-byte pieces of a tile's keys in memory
   constexpr int kEach = (kPieces + kThreads - 1) / kThreads, kPer = kPieces / kKeys;
   __shared__ __attribute__((aligned(16))) uint8_t lds[2][2][T::kBytes];  // [keys, values][tile & 1]
@@ -628,10 +653,10 @@ __global__ __launch_bounds__(64 * W, D > 128 ? 1 : 2) void rows_kernel(Args a, K
   typedef std::integral_constant<int, 1> Odd;
   const uint32_t lane = threadIdx.x & 63, wave = (uint32_t) __builtin_amdgcn_readfirstlane((int) threadIdx.x / 64);
   const uint32_t half = lane / 32, col = lane & 31;
-  const uint32_t g = blockIdx.x % kv.heads;
+  const uint32_t g = blockIdx.x % kv.heads, part_of = blockIdx.x / kv.heads % parts, index = blockIdx.x / kv.heads / parts;
   Seq seq;
   uint32_t tile;
-  if (!find_rows(st, SRC == kPacked ? 0 : kv.page, a.group, kRows, blockIdx.x / kv.heads, seq, tile)) return;
+  if (!find_rows(st, SRC == kPacked ? 0 : kv.page, a.group, index, seq, tile)) return;
 
   // the rows: the workgroup's, the wave's, the lane's, and the positions of their tokens
   const uint32_t all = (uint32_t) seq.rows * a.group, row0 = tile * kRows, last = all - 1 < row0 + kRows - 1 ? all - 1 : row0 + kRows - 1;
@@ -643,8 +668,13 @@ __global__ __launch_bounds__(64 * W, D > 128 ? 1 : 2) void rows_kernel(Args a, K
   const bool in = row < all;
   const int pos = base + (int) token;
   const int window = a.window ? (int) a.window : 0x7FFFFFFF;
-  const int from = a.window && pos_lo >= window ? (pos_lo - window + 1) & ~(kKeys - 1) : 0;
-  const int to = pos_hi + 1 < seq.end ? pos_hi + 1 : seq.end;
+  int from = a.window && pos_lo >= window ? (pos_lo - window + 1) & ~(kKeys - 1) : 0;
+  int to = pos_hi + 1 < seq.end ? pos_hi + 1 : seq.end;
+  if (parts > 1 && from < to) {  // (its part of the keys, in whole tiles)
+    const int each = ((to - from + kKeys - 1) / kKeys + (int) parts - 1) / (int) parts * kKeys;
+    from += (int) part_of * each;
+    to = to - from > each ? from + each : to;
+  }
 
   // a thread's 16-byte pieces of a tile: of rows key_row(i). stage s writes the keys of tile s + 1 and the values of tile s
   // into LDS, loaded into registers a tile's time before; page ids are loaded one stage ahead of that. past the last tile
@@ -652,10 +682,9 @@ __global__ __launch_bounds__(64 * W, D > 128 ? 1 : 2) void rows_kernel(Args a, K
   const uint32_t size = SRC == kPagesF8 ? 1 : 2, dim_bytes = a.dim * size, shift = SRC == kPacked ? 0 : 31 - __builtin_clz(kv.page);
   const uint64_t page_bytes = (uint64_t) kv.heads * kv.page * dim_bytes, head_at = (uint64_t) g * kv.page * dim_bytes;
   const int n = from < to ? (to - from + kKeys - 1) / kKeys : 0;
-  const bool late = W == 8 && wave >= 4;
   u32x4 kr[kEach], vr[kEach];
   int kid[kEach], vid[kEach], live_id = 0;
-  uint64_t live_old = 0, live = 0, live_new = 0;  // of tiles s - 1, s and s + 1: the keys that are there, a bit each
+  uint32_t live_old = 0, live = 0, live_new = 0;  // of tiles s - 1, s and s + 1: the keys that are there, a bit each
   auto key_row = [&](int i) __attribute__((always_inline)) { return (int) ((threadIdx.x + i * kThreads) / kPer) & (kKeys - 1); };
   auto piece = [&](int i) __attribute__((always_inline)) { return (threadIdx.x + i * kThreads) % kPer; };
   auto start = [&](int t) __attribute__((always_inline)) { return from + (t < n ? t : n - 1) * kKeys; };
@@ -685,7 +714,7 @@ __global__ __launch_bounds__(64 * W, D > 128 ? 1 : 2) void rows_kernel(Args a, K
   };
   if constexpr (SRC != kPacked) kplace = kv.k, vplace = kv.v;
   auto there = [&](int t) __attribute__((always_inline)) {
-    return __ballot(((int) lane >= kKeys || start(t) + (int) lane < to) && (SRC == kPacked || (uint32_t) live_id < kv.pages));
+    return (uint32_t) __ballot(start(t) + (int) (lane & (kKeys - 1)) < to && (SRC == kPacked || (uint32_t) live_id < kv.pages));
   };
   auto load_stage = [&](int s) __attribute__((always_inline)) {
     live_old = live, live = live_new, live_new = there(s + 1);
@@ -706,7 +735,7 @@ __global__ __launch_bounds__(64 * W, D > 128 ? 1 : 2) void rows_kernel(Args a, K
         if (piece(i) * 16 >= dim_bytes) kr[i] = u32x4{0, 0, 0, 0};
     }
     const bool part = partial(start(s));
-    if (part || live != ~0ull) {
+    if (part || live != ~0u) {
       asm volatile("");
 #pragma unroll
       for (int i = 0; i < kEach; i++) {
@@ -729,13 +758,11 @@ __global__ __launch_bounds__(64 * W, D > 128 ? 1 : 2) void rows_kernel(Args a, K
       }
     }
   };
-  // the end of a phase: LDS writes done and seen; loads from memory stay in flight
+  // the end of a tile's products: LDS writes done and seen; loads from memory stay in flight
   auto meet = [&]() __attribute__((always_inline)) {
-    __builtin_amdgcn_sched_barrier(0);  // (no instruction into the other phase: a softmax among the products keeps both waves waiting)
     __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
     __builtin_amdgcn_s_barrier();
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
-    __builtin_amdgcn_sched_barrier(0);
   };
 
   if (n) {
@@ -747,10 +774,10 @@ __global__ __launch_bounds__(64 * W, D > 128 ? 1 : 2) void rows_kernel(Args a, K
   v8 q[kSteps];
   load_q<BF, kSteps>(a, (uint64_t) seq.row0 + (in ? token : 0), in ? head : 0, in, [&](int i) { return (uint32_t) (16 * i + 8 * half); }, q);
   const float unit = unit_of(a) * (SRC == kPagesF8 && kv.scale ? kv.scale[g] : 1.0f);
-  f32x16 o[kDims], x[kParts];
+  f32x16 o[kDims], x;
 #pragma unroll
   for (int i = 0; i < kDims; i++) o[i] = f32x16{};
-  v8 p[2 * kParts];
+  v8 p[2];
   float m = -__builtin_inff(), l = 0.0f;
 
   // a lane's places in a tile's keys and values: all of them by one exclusive or and one addition from the first (D a power
@@ -760,22 +787,19 @@ __global__ __launch_bounds__(64 * W, D > 128 ? 1 : 2) void rows_kernel(Args a, K
   auto scores = [&](const uint8_t* kt) __attribute__((always_inline)) {
     uint32_t at0 = kfirst;
     asm volatile("" : "+v"(at0));
+    x = f32x16{};
 #pragma unroll
-    for (int i = 0; i < kParts; i++) x[i] = f32x16{};
-#pragma unroll
-    for (int i = 0; i < kSteps; i++)
-#pragma unroll
-      for (int k = 0; k < kParts; k++) {
-        const uint32_t at = (D & (D - 1)) == 0 ? (at0 ^ (uint32_t) (32 * i)) + (uint32_t) (32 * k * T::kRow) : (uint32_t) T::k_at(32 * k + (int) col, 2 * i + (int) half);
-        x[k] = U::mfma32(*(const v8*) (kt + at), q[i], x[k]);
-      }
+    for (int i = 0; i < kSteps; i++) {
+      const uint32_t at = (D & (D - 1)) == 0 ? at0 ^ (uint32_t) (32 * i) : (uint32_t) T::k_at((int) col, 2 * i + (int) half);
+      x = U::mfma32(*(const v8*) (kt + at), q[i], x);
+    }
   };
   auto outputs = [&](const uint8_t* vt) __attribute__((always_inline)) {
     // V^T's columns of keys 16 u + 4 half + 0 .. 3 and 8 more on, as P^T's lanes hold them
     uint32_t at0 = vfirst;
     asm volatile("" : "+v"(at0));
 #pragma unroll
-    for (int u = 0; u < 2 * kParts; u++)
+    for (int u = 0; u < 2; u++)
 #pragma unroll
       for (int i = 0; i < kDims; i++) {
         const uint32_t at = (D & (D - 1)) == 0 ? (at0 ^ (uint32_t) (64 * i)) + (uint32_t) (16 * u * T::kRow) : (uint32_t) (T::v_at(16 * u + vrow, 4 * i + vdims / 8) + vdims % 8 * 2);
@@ -786,25 +810,19 @@ __global__ __launch_bounds__(64 * W, D > 128 ? 1 : 2) void rows_kernel(Args a, K
   };
   auto softmax = [&](int t) __attribute__((always_inline)) {
     const int j0 = start(t);
-    if (live_old != ~0ull || j0 + kKeys - 1 > wpos_lo || (a.window && j0 <= wpos_hi - window)) {
+    if (live_old != ~0u || j0 + kKeys - 1 > wpos_lo || (a.window && j0 <= wpos_hi - window)) {
       // the row's keys are lo + 1 .. hi of the tile (less the half's 4, so that the lane's keys are constants)
       const int hi = pos - j0 - 4 * (int) half, lo = a.window && pos >= window ? pos - window - j0 - 4 * (int) half : -5;
-      const uint64_t mine = live_old >> (4 * half);
+      const uint32_t mine = live_old >> (4 * half);
 #pragma unroll
-      for (int k = 0; k < kParts; k++) {
-        const uint32_t bits = (uint32_t) (mine >> (32 * k));
-#pragma unroll
-        for (int i = 0; i < 16; i++) {
-          const int key = 32 * k + 8 * (i / 4) + i % 4;
-          if (key > hi || key <= lo || !(bits >> (key & 31) & 1)) x[k][i] = -__builtin_inff();
-        }
+      for (int i = 0; i < 16; i++) {
+        const int key = 8 * (i / 4) + i % 4;
+        if (key > hi || key <= lo || !(mine >> key & 1)) x[i] = -__builtin_inff();
       }
     }
-    float top = x[0][0];
+    float top = x[0];
 #pragma unroll
-    for (int k = 0; k < kParts; k++)
-#pragma unroll
-      for (int i = 0; i < 16; i++) top = fmaxf(top, x[k][i]);
+    for (int i = 1; i < 16; i++) top = fmaxf(top, x[i]);
     top = max_halves(top) * unit;
     if (__any(top > m + kSlack)) {
       const float next = fmaxf(m, top), fade = __builtin_amdgcn_exp2f(m - finite_max(next));
@@ -815,20 +833,18 @@ __global__ __launch_bounds__(64 * W, D > 128 ? 1 : 2) void rows_kernel(Args a, K
     }
     const float sub = finite_max(m);
 #pragma unroll
-    for (int k = 0; k < kParts; k++)
-#pragma unroll
-      for (int i = 0; i < 16; i++) {
-        const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(x[k][i], unit, -sub));
-        l += e;
-        p[2 * k + i / 8][i % 8] = (typename U::e) e;
-      }
+    for (int i = 0; i < 16; i++) {
+      const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(x[i], unit, -sub));
+      l += e;
+      p[i / 8][i % 8] = (typename U::e) e;
+    }
   };
   // the products' phase after tile t's softmax: the next tile's scores, tile t's outputs, the next stage
   auto products = [&](int t, auto buf) __attribute__((always_inline)) {
     constexpr int b = decltype(buf)::value;
     scores(lds[0][1 - b]);
     outputs(lds[1][b]);
-    feed<kSteps * kParts, 2 * kParts * kDims>();
+    feed<kSteps, 2 * kDims>();
     mend_stage(t + 1);
     write(lds[0][b], false, kr);
     write(lds[1][1 - b], true, vr);
@@ -844,7 +860,6 @@ __global__ __launch_bounds__(64 * W, D > 128 ? 1 : 2) void rows_kernel(Args a, K
     write(lds[0][0], false, kr);
     load_stage(0);
     meet();
-    if (late) meet();
     mend_stage(0);
     scores(lds[0][0]);
     write(lds[0][1], false, kr);
@@ -854,24 +869,19 @@ __global__ __launch_bounds__(64 * W, D > 128 ? 1 : 2) void rows_kernel(Args a, K
     int t = 0;
     for (; t + 2 < n; t += 2) {
       softmax(t);
-      meet();
       products(t, Even());
       meet();
       softmax(t + 1);
-      meet();
       products(t + 1, Odd());
       meet();
     }
     softmax(t);
     if (t + 1 < n) {
-      meet();
       products(t, Even());
       meet();
       softmax(++t);
     }
-    meet();
     outputs(lds[1][t & 1]);
-    if (!late) meet();
   }
 
   if (__syncthreads_or(bad)) {
@@ -911,6 +921,17 @@ __global__ __launch_bounds__(64 * W, D > 128 ? 1 : 2) void rows_kernel(Args a, K
   }
   if (!in) return;
   l = sum_halves(l);
+  if (parts > 1) {
+    float* at = part + ((uint64_t) blockIdx.x * kRows + (row - row0)) * (D + 4);
+    const float v_scale = SRC == kPagesF8 && kv.scale ? kv.scale[kv.heads + g] : 1.0f;
+#pragma unroll
+    for (int i = 0; i < kDims; i++)
+#pragma unroll
+      for (int n = 0; n < 4; n++)
+        *(f32x4*) (at + 32 * i + 8 * n + 4 * half) = f32x4{o[i][4 * n], o[i][4 * n + 1], o[i][4 * n + 2], o[i][4 * n + 3]} * v_scale;
+    if (half == 0) at[D] = m, at[D + 1] = l;
+    return;
+  }
   const float inv = l == 0.0f ? 0.0f : (SRC == kPagesF8 && kv.scale ? kv.scale[kv.heads + g] : 1.0f) / l;
   const uint64_t at = ((uint64_t) seq.row0 + token) * a.os + head * a.oh;
 #pragma unroll
@@ -923,20 +944,80 @@ __global__ __launch_bounds__(64 * W, D > 128 ? 1 : 2) void rows_kernel(Args a, K
   if (a.lse && half == 0) a.lse[((uint64_t) seq.row0 + token) * a.heads + head] = (m + log2f(l)) * kLn2;
 }
 
+// the parts' results of each row joined, in the parts' order: D / 4 lanes (a power of two of them) a row
+template <int D>
+__global__ __launch_bounds__(256) void rows_join_kernel(Args a, Step st, uint32_t page, uint32_t kv_heads, uint32_t parts,
+                                                        const float* __restrict__ part) {
+  constexpr uint32_t kLanes = D <= 64 ? 16 : D <= 128 ? 32 : 64, kEach = 256 / kLanes;
+  uint32_t b = blockIdx.x;
+  const uint32_t piece = b % (kRows / kEach);
+  b /= kRows / kEach;
+  const uint32_t g = b % kv_heads, index = b / kv_heads;
+  Seq seq;
+  uint32_t tile;
+  if (!find_rows(st, page, a.group, index, seq, tile)) return;
+  const uint32_t r = piece * kEach + threadIdx.x / kLanes, d = threadIdx.x % kLanes * 4, row = tile * kRows + r;
+  if (row >= (uint32_t) seq.rows * a.group || d >= a.dim) return;
+  const float* p = part + (((uint64_t) index * parts * kv_heads + g) * kRows + r) * (D + 4);
+  const uint64_t step = (uint64_t) kv_heads * kRows * (D + 4);
+  float m = -__builtin_inff(), l = 0.0f;
+  f32x4 y = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 4
+  for (uint32_t c = 0; c < parts; c++) {
+    const f32x4 o = *(const f32x4*) (p + c * step + d);
+    const float mc = p[c * step + D], lc = p[c * step + D + 1];
+    const float top = fmaxf(m, mc), base = finite_max(top), f = __builtin_amdgcn_exp2f(m - base), fc = __builtin_amdgcn_exp2f(mc - base);
+    y = y * f + o * fc;
+    l = l * f + lc * fc;
+    m = top;
+  }
+  const uint32_t token = (uint32_t) seq.row0 + row / a.group, head = g * a.group + row % a.group;
+  put4(a, (uint64_t) token * a.os + head * a.oh + d, y * (l == 0.0f ? 0.0f : 1.0f / l));
+  if (a.lse && d == 0) a.lse[(uint64_t) token * a.heads + head] = (m + log2f(l)) * kLn2;
+}
+
+// how the rows are launched: tiles there can be, and the parts that each tile's keys are cut into: one, but where the tiles
+// leave compute units without work and the keys are many (a part of 256 keys or more, so that it costs more than its join)
+constexpr uint64_t kFull = 1536, kLeastPart = 256;
+struct RowsCut {
+  uint64_t tiles;
+  uint32_t parts, dim;
+};
+inline RowsCut rows_cut(const OsmosAttn* a, uint32_t kv_heads, uint32_t dim, const OsmosKvStep* st) {
+  RowsCut c;
+  c.tiles = (uint64_t) st->n_tok * (a->heads / kv_heads) / kRows + (st->n_seq < st->n_tok ? st->n_seq : st->n_tok);
+  const uint64_t blocks = c.tiles * kv_heads, longest = st->len ? st->max_len : st->max_tok;
+  uint64_t keys = longest;
+  if (a->window && a->window + (uint64_t) kRows + 31 < keys) keys = a->window + (uint64_t) kRows + 31;
+  uint64_t parts = blocks ? kFull / blocks : 1;
+  if (parts > keys / kLeastPart) parts = keys / kLeastPart;
+  c.parts = (uint32_t) (parts < 1 ? 1 : parts > 64 ? 64 : parts);
+  c.dim = dim <= 64 ? 64 : dim <= 128 ? 128 : dim <= 192 ? 192 : 256;
+  return c;
+}
+inline uint64_t rows_bytes(const RowsCut& c, uint32_t kv_heads) {
+  return c.parts > 1 ? c.tiles * kv_heads * c.parts * kRows * (c.dim + 4) * 4 : 0;
+}
+
 template <bool BF, int SRC>
-bool run_rows(const Args& a, const Kv& k, const OsmosKvStep* step, hipStream_t stream) {
-  constexpr int W = 8, WD = 4;
-  const uint32_t rows = a.dim <= 128 ? 32 * W : 32 * WD;
-  const uint64_t tiles = (uint64_t) step->n_tok * a.group / rows + step->n_seq, blocks = tiles * k.heads;
+bool run_rows(const Args& a, const Kv& k, const OsmosKvStep* step, const RowsCut& c, float* part, hipStream_t stream) {
+  const uint64_t blocks = c.tiles * k.heads * c.parts;
   if (blocks > 0x7FFFFFFFull || (uint64_t) step->n_tok * a.group > 0x7FFFFFFFull) return false;
   const Step st = kv::step_of(step);
-  if (a.dim <= 64) rows_kernel<BF, SRC, 64, W><<<(uint32_t) blocks, 64 * W, 0, stream>>>(a, k, st);
-  else if (a.dim <= 128) rows_kernel<BF, SRC, 128, W><<<(uint32_t) blocks, 64 * W, 0, stream>>>(a, k, st);
-  else if (a.dim <= 192) rows_kernel<BF, SRC, 192, WD><<<(uint32_t) blocks, 64 * WD, 0, stream>>>(a, k, st);
-  else rows_kernel<BF, SRC, 256, WD><<<(uint32_t) blocks, 64 * WD, 0, stream>>>(a, k, st);
+  auto* kernel = c.dim == 64 ? rows_kernel<BF, SRC, 64> : c.dim == 128 ? rows_kernel<BF, SRC, 128> : c.dim == 192 ? rows_kernel<BF, SRC, 192> : rows_kernel<BF, SRC, 256>;
+  kernel<<<(uint32_t) blocks, 64 * kRowWaves, 0, stream>>>(a, k, st, c.parts, part);
+  if (hipGetLastError() != hipSuccess) return false;
+  if (c.parts > 1) {
+    const uint32_t pieces = kRows / (c.dim == 64 ? 16 : c.dim == 128 ? 8 : 4);
+    auto* join = c.dim == 64 ? rows_join_kernel<64> : c.dim == 128 ? rows_join_kernel<128> : c.dim == 192 ? rows_join_kernel<192> : rows_join_kernel<256>;
+    join<<<(uint32_t) (c.tiles * k.heads * pieces), 256, 0, stream>>>(a, st, SRC == kPacked ? 0 : k.page, k.heads, c.parts, part);
+  }
   return hipGetLastError() == hipSuccess;
 }
 
+inline bool room_ok(uint64_t need, const void* workspace, uint64_t bytes) {
+  return !need || (workspace && (uintptr_t) workspace % 256 == 0 && bytes >= need);
+}
 inline bool row_type(uint32_t t) { return t == OSMOS_F32 || t == OSMOS_F16 || t == OSMOS_BF16; }
 inline bool stride_ok(uint64_t stride, uint32_t type) { return stride * kv::size_of(type) % 16 == 0; }
 
@@ -967,12 +1048,14 @@ using namespace osm;
 extern "C" OSM_API uint64_t osmos_attn_workspace(const OsmosAttn* a, uint32_t kv_heads, uint32_t dim,
                                                  const OsmosKvStep* step) {
   if (!a || !a->heads || !kv_heads || a->heads % kv_heads || !dim || dim > OSMOS_ATTN_MAX_DIM || !step) return 0;
-  return step->max_tok == 1 && step->len ? attn::token_bytes(a, attn::cut_of(a, kv_heads, dim, step)) : 0;
+  if (!step->n_seq || !step->n_tok) return 0;
+  const uint64_t rows = attn::rows_bytes(attn::rows_cut(a, kv_heads, dim, step), kv_heads);
+  const uint64_t token = step->max_tok == 1 && step->len ? attn::token_bytes(a, attn::cut_of(a, kv_heads, dim, step)) : 0;
+  return rows > token ? rows : token;
 }
 
 extern "C" OSM_API bool osmos_attn_prompt(const OsmosAttn* a, const OsmosKvRows* r, const OsmosKvStep* step,
                                           void* workspace, uint64_t workspace_bytes, void* stream) {
-  (void) workspace, (void) workspace_bytes;
   if (!r || !r->k || !r->v || !r->heads || r->heads > 4096 || (r->type != OSMOS_F16 && r->type != OSMOS_BF16)) return false;
   if (!r->dim || r->dim > OSMOS_ATTN_MAX_DIM || r->dim % 16 || (uintptr_t) r->k % 16 || (uintptr_t) r->v % 16) return false;
   if (r->k_stride % 8 || r->k_head % 8 || r->v_stride % 8 || r->v_head % 8) return false;
@@ -980,19 +1063,21 @@ extern "C" OSM_API bool osmos_attn_prompt(const OsmosAttn* a, const OsmosKvRows*
   if (!attn::args_ok(a, r->heads, r->dim) || !kv::step_ok(step, false)) return false;
   const attn::Kv k{(const uint8_t*) r->k, (const uint8_t*) r->v, r->k_stride, r->k_head, r->v_stride, r->v_head, r->type,
                    0, 0, r->heads, nullptr};
-  const attn::Args args = attn::args_of(a, r->heads, r->dim);
-  return r->type == OSMOS_BF16 ? attn::run_rows<true, attn::kPacked>(args, k, step, (hipStream_t) stream)
-                               : attn::run_rows<false, attn::kPacked>(args, k, step, (hipStream_t) stream);
+  const attn::RowsCut c = attn::rows_cut(a, r->heads, r->dim, step);
+  if (!attn::room_ok(attn::rows_bytes(c, r->heads), workspace, workspace_bytes)) return false;
+  auto* run = r->type == OSMOS_BF16 ? attn::run_rows<true, attn::kPacked> : attn::run_rows<false, attn::kPacked>;
+  return run(attn::args_of(a, r->heads, r->dim), k, step, c, (float*) workspace, (hipStream_t) stream);
 }
 
 extern "C" OSM_API bool osmos_attn_chunk(const OsmosAttn* a, const OsmosKv* kv, uint32_t layer, const OsmosKvStep* step,
                                          void* workspace, uint64_t workspace_bytes, void* stream) {
-  (void) workspace, (void) workspace_bytes;
   if (!kv::cache_ok(kv) || layer >= kv->layers || !attn::args_ok(a, kv->heads, kv->dim) || !kv::step_ok(step, true)) return false;
   const bool bf = attn::in_bf16(kv->type, a->q_type), f8 = kv->type == OSMOS_F8;
   auto* run = bf ? (f8 ? attn::run_rows<true, attn::kPagesF8> : attn::run_rows<true, attn::kPages>)
                  : (f8 ? attn::run_rows<false, attn::kPagesF8> : attn::run_rows<false, attn::kPages>);
-  return run(attn::args_of(a, kv->heads, kv->dim), attn::pages_of(kv, layer), step, (hipStream_t) stream);
+  const attn::RowsCut c = attn::rows_cut(a, kv->heads, kv->dim, step);
+  if (!attn::room_ok(attn::rows_bytes(c, kv->heads), workspace, workspace_bytes)) return false;
+  return run(attn::args_of(a, kv->heads, kv->dim), attn::pages_of(kv, layer), step, c, (float*) workspace, (hipStream_t) stream);
 }
 
 extern "C" OSM_API bool osmos_attn_token(const OsmosAttn* a, const OsmosKv* kv, uint32_t layer, const OsmosKvStep* step,
@@ -1000,8 +1085,7 @@ extern "C" OSM_API bool osmos_attn_token(const OsmosAttn* a, const OsmosKv* kv, 
   if (!kv::cache_ok(kv) || layer >= kv->layers || !attn::args_ok(a, kv->heads, kv->dim) || !kv::step_ok(step, true)) return false;
   if (step->max_tok != 1) return false;
   const attn::Cut c = attn::cut_of(a, kv->heads, kv->dim, step);
-  const uint64_t need = attn::token_bytes(a, c);
-  if (need && (!workspace || (uintptr_t) workspace % 256 || workspace_bytes < need)) return false;
+  if (!attn::room_ok(attn::token_bytes(a, c), workspace, workspace_bytes)) return false;
   const bool bf = attn::in_bf16(kv->type, a->q_type), f8 = kv->type == OSMOS_F8;
   auto* run = bf ? (f8 ? attn::run_token<true, true> : attn::run_token<true, false>)
                  : (f8 ? attn::run_token<false, true> : attn::run_token<false, false>);
