@@ -1,0 +1,63 @@
+"""A decoder block's attention over quantized projections, for Python callers: the query, key, value and output matrices in
+GGUF row layout (mm_run), the step's keys and values into the paged cache (osmos_kv_append), attention over the cache
+(osmos_attn_token for a step of single tokens, osmos_attn_chunk for prompts). What follows it in a block is
+layer.LaneLayer (the routed experts). Rows are float32 as the library's products have them; buffers are made once a step
+shape and reused; nothing here computes.
+"""
+import ctypes
+
+from . import attn, capi
+
+
+class AttentionLayer:
+    def __init__(self, cache, layer, heads, wq, wk, wv, wo, dim):
+        """cache: attn.KvCache; layer: its layer here; heads: query heads; wq, wk, wv, wo: (GGUF type, uint8 device tensor),
+        rows heads x cache.dim (wq), cache.heads x cache.dim (wk, wv) of dim values, dim rows of heads x cache.dim (wo)"""
+        self.cache, self.layer, self.heads, self.dim = cache, layer, heads, dim
+        self.w, self.wo = ((wq, heads * cache.dim), (wk, cache.heads * cache.dim), (wv, cache.heads * cache.dim)), wo
+        for (t, _), rows in self.w:
+            if not capi.lib().mm_fits(t, rows, dim):
+                raise ValueError("AttentionLayer: mm does not take %d x %d of type %d" % (rows, dim, t))
+        if not capi.lib().mm_fits(wo[0], dim, heads * cache.dim):
+            raise ValueError("AttentionLayer: mm does not take the output matrix")
+        self._made = {}
+
+    def _buffers(self, n):
+        import torch
+        if n not in self._made:
+            hd, rows = self.cache.dim, self.heads + 2 * self.cache.heads
+            tiles = (n + 15) // 16 * 16
+            b = {"qkv": torch.empty((n, rows, hd), device="cuda"), "o": torch.empty((n, self.heads, hd), device="cuda"),
+                 "x16": torch.empty(tiles * self.dim, dtype=torch.float16, device="cuda"),
+                 "o16": torch.empty(tiles * self.heads * hd, dtype=torch.float16, device="cuda"),
+                 "overflow": torch.zeros(1, dtype=torch.int32, device="cuda")}
+            b["q"], b["k"], b["v"] = b["qkv"].split([self.heads, self.cache.heads, self.cache.heads], 1)
+            self._made[n] = b
+        return self._made[n]
+
+    def calls(self, step):
+        """the append and the attention of a step, bound to this layer's buffers of its size (made once a KvStep)"""
+        b = self._buffers(step.n_tok)
+        kind = attn.TokenAttention if step.desc.max_tok == 1 else attn.ChunkAttention
+        return attn.Append(self.cache, self.layer, step, b["k"], b["v"]), kind(self.cache, self.layer, step, b["q"], b["o"])
+
+    def forward(self, x, calls, out, stream=None):
+        """out (n, dim) = the block's attention of x (n, dim), float32, for the step that `calls` were made for"""
+        L, n = capi.lib(), x.shape[0]
+        b, append, attention = self._buffers(n), *calls
+
+        def need(ok, what):
+            if not ok:
+                raise RuntimeError("%s refused" % what)
+        need(L.mm_x16(capi.addr(x), self.dim, n, self.dim, capi.addr(b["x16"]), capi.addr(b["overflow"]), stream), "mm_x16")
+        stride = b["qkv"].stride(0)
+        for ((t, w), rows), y in zip(self.w, (b["q"], b["k"], b["v"])):
+            need(L.mm_run(t, capi.addr(w), rows, self.dim, capi.addr(b["x16"]), n, ctypes.c_void_p(y.data_ptr()), stride,
+                          stream), "mm_run")
+        append.run(stream)
+        attention.run(stream)
+        cols = self.heads * self.cache.dim
+        need(L.mm_x16(capi.addr(b["o"]), cols, n, cols, capi.addr(b["o16"]), capi.addr(b["overflow"]), stream), "mm_x16")
+        need(L.mm_run(self.wo[0], capi.addr(self.wo[1]), self.dim, cols, capi.addr(b["o16"]), n, capi.addr(out), self.dim,
+                      stream), "mm_run")
+        return out

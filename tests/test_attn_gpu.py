@@ -385,3 +385,61 @@ def test_offsets_past_32_bits():
                                torch.float16, torch.float16)
         attn_ref.check(out[:, h], lse[:, h], *want, h)
         attn_ref.check(o2[:, h], l2[:, h], *want, h)
+
+
+@pytest.mark.parametrize("scale", [-0.3, 0.0, 0.5])
+def test_other_scales(scale):
+    """a negative scale and none: the mask and the maximum go by the scaled scores"""
+    from libosmos_amd import attn
+    g, lens = _gen(12), [300, 40]
+    pg = Paged(g, lens, 2, 64, 16, "f16")
+    here = lambda m: torch.ones(m, dtype=torch.bool, device="cuda")  # noqa: E731
+    for token, rows in ((True, [1, 1]), (False, [70, 40])):
+        n = sum(rows)
+        q = _normal(g, n, 4, 64).half()
+        out, lse = torch.empty_like(q), torch.empty((n, 4), device="cuda")
+        step = attn.KvStep(_ints(_starts(rows)), pg.len, pg.table, n_tok=n, max_tok=max(rows), max_len=300)
+        print("scale", scale, token, flush=True)
+        (attn.TokenAttention if token else attn.ChunkAttention)(pg.cache, 1, step, q, out, lse, scale=scale).run()
+        torch.cuda.synchronize()
+        t = 0
+        for s, (r, m) in enumerate(zip(rows, lens)):
+            pos = torch.arange(m - r, m, device="cuda")
+            for h in range(4):
+                k, v = (attn_ref.rows_of_pages(pg.data, None, 1, w, pg.table[s], m, h // 2)[0] for w in (0, 1))
+                want = list(attn_ref.attend(q[t:t + r, h].double() * math.copysign(1.0, scale), k, v, pos, here(m), abs(scale),
+                                            0, torch.float16, torch.float16))
+                attn_ref.check(out[t:t + r, h], lse[t:t + r, h], *want, (scale, token, s, h))
+            t += r
+
+
+@pytest.mark.parametrize("token", [True, False])
+def test_many_sequences(token):
+    """more sequences than a wave has lanes, some without rows, some without tokens; the same bits twice"""
+    from libosmos_amd import attn
+    g = _gen(13)
+    n_seq = 150
+    lens = [(37 * i * i) % 700 + (i % 3 > 0) for i in range(n_seq)]
+    lens[7] = 0
+    rows = [1 if i % 5 else 0 for i in range(n_seq)] if token else [min(lens[i], (11 * i) % 23) for i in range(n_seq)]
+    pg = Paged(g, lens, 2, 64, 16, "bf16", layers=2)
+    n = sum(rows)
+    q = _normal(g, n, 4, 64).bfloat16()
+    step = attn.KvStep(_ints(_starts(rows)), pg.len, pg.table, n_tok=n, max_tok=max(rows), max_len=max(lens))
+    got = []
+    for _ in range(2):
+        out, lse = torch.full_like(q, 7.0), torch.empty((n, 4), device="cuda")
+        print("many", token, flush=True)
+        (attn.TokenAttention if token else attn.ChunkAttention)(pg.cache, 1, step, q, out, lse).run()
+        torch.cuda.synchronize()
+        got.append((out, lse))
+    assert torch.equal(got[0][0], got[1][0]) and torch.equal(got[0][1], got[1][1])
+    t = 0
+    for s, (r, m) in enumerate(zip(rows, lens)):
+        if r:
+            pos = torch.arange(m - r, m, device="cuda")
+            for h in (0, 3):
+                (k, here), (v, _) = (attn_ref.rows_of_pages(pg.data, None, 1, w, pg.table[s], m, h // 2) for w in (0, 1))
+                want = attn_ref.attend(q[t:t + r, h].double(), k, v, pos, here, 0.125, 0, torch.bfloat16, torch.bfloat16)
+                attn_ref.check(out[t:t + r, h], lse[t:t + r, h], *want, (s, h))
+        t += r
