@@ -29,6 +29,7 @@ extern "C" {
 #define OSMOS_ATTN_MAX_DIM 256u
 #define OSMOS_ATTN_MAX_STRIDE (1u << 24) /* values between two packed rows of keys or values */
 #define OSMOS_KV_MAX_PAGE 4096u
+#define OSMOS_KV_MAX_PAGE_VALUES (1u << 28) /* heads x page x dim */
 #define OSMOS_KV_MAX_REQUESTS 1024u
 
 typedef struct OsmosKv
@@ -38,7 +39,8 @@ typedef struct OsmosKv
   uint32_t type;        /* OSMOS_F16, OSMOS_BF16 or OSMOS_F8 */
   uint32_t layers, pages;
   uint32_t page;        /* tokens a page: a power of two up to OSMOS_KV_MAX_PAGE */
-  uint32_t heads, dim;  /* dim: a multiple of 16 up to OSMOS_ATTN_MAX_DIM */
+  uint32_t heads, dim;  /* dim: a multiple of 16 up to OSMOS_ATTN_MAX_DIM; heads x page x dim up to
+                           OSMOS_KV_MAX_PAGE_VALUES */
 } OsmosKv;
 
 typedef struct OsmosKvStep

@@ -1,7 +1,10 @@
 // libosmos MI355X - attention over packed rows and over the paged cache (include/osmos_attn.h).
 //
 // a row's output is sum_j p_j v_j / sum_j p_j with p_j = exp(scale q k_j - m), m the greatest score, in one pass: the
-// running m and sum, the sum and output scaled by exp(m_old - m_new) where m grows.
+// running m and sum, the sum and output scaled by exp(m_old - m_new) where m grows. scores, sums, maxima and outputs are
+// kept in float; the p_j, in 0 .. 1 (of rows of prompts up to 2^8), are rounded to the products' 16-bit type, as the matrix
+// units take no other: an error of the size of a 16-bit output's own rounding and independent of it (a bf16 prompt of 8192
+// is 2.2e-3 off in all, relative, where the output's rounding alone makes 1.6e-3). the sum takes the p_j before that.
 #include <type_traits>
 
 #include "kvcache.h"
@@ -11,6 +14,7 @@ namespace attn {
 
 using kv::Seq;
 using kv::Step;
+using kv::lane_of;
 using kv::sequence;
 
 struct Args {
@@ -139,6 +143,10 @@ __device__ inline float finite_max(float m) { return m == -__builtin_inff() ? 0.
 // ids of the one after. with pages of 16 tokens or more (WIDE) half a tile lies in one page, so that its place is the
 // wave's and not a lane's: scalar loads and arithmetic, where smaller pages take some 60 vector instructions a tile.
 // no load is conditional: a place that is masked reads a row that exists and its score and value are then replaced.
+// bound by memory: one sequence of 131072 tokens (8 kv heads of 128, bf16) 93 us for 537 MB, 5.8 TB/s; 256 of 4096 6.05 TB/s (a
+// streaming read reaches 7.2). a short step is a chain of loads: lengths, page ids, rows, some 1.7 us a tile of a wave's.
+// two tiles in flight a wave instead of one (244 registers) measured the same, three workgroups a compute unit (10 spilled
+// registers) 14 % slower.
 template <bool F8, int D> struct TokenTile {
   static constexpr int kSize = F8 ? 1 : 2;
   static constexpr int kRow = D * kSize;                        // bytes of a V row in LDS
@@ -172,7 +180,6 @@ __device__ inline uint32_t wave_scan(uint32_t x) {
 #undef OSM_ADD_DPP
   return x;
 }
-__device__ inline int lane_of(int x, int lane) { return __builtin_amdgcn_readlane(x, lane); }
 
 // the step's work cut into chunks of one length, so that `want` of them hold all its keys (at least kLeast keys each, whole
 // 128s: a tile for each wave): workgroup `index` takes chunk c of sequence s's n. every workgroup reads all lengths, 64 a
@@ -206,9 +213,7 @@ __device__ inline bool find_work(const Step& st, uint32_t page, uint32_t window,
       w.s = s + (uint32_t) at;
       w.n = (uint32_t) lane_of((int) n, at);
       w.c = index - ((uint32_t) lane_of((int) x, at) - w.n);
-      w.seq.row0 = lane_of(q.row0, at), w.seq.rows = lane_of(q.rows, at), w.seq.len = lane_of(q.len, at), w.seq.end = lane_of(q.end, at);
-      w.seq.table = (const int32_t*) ((uint64_t) (uint32_t) lane_of((int) ((uint64_t) q.table >> 32), at) << 32 |
-                                      (uint32_t) lane_of((int) (uint64_t) q.table, at));
+      w.seq = lane_of(q, at);
       return true;
     }
     before = (uint32_t) lane_of((int) x, 63);
@@ -424,7 +429,8 @@ __global__ __launch_bounds__(256, D > 128 ? 1 : 2) void token_kernel(Args a, Kv 
   }
 }
 
-// the chunks' results of a row and head joined, in the chunks' order: a workgroup D / 4 threads of 4 dims in 256 / (D / 4)
+// the chunks' results of a row and head joined, in the chunks' order (4.4 us after a step of 64 sequences, most of it the
+// launch and two dependent loads): a workgroup D / 4 threads of 4 dims in 256 / (D / 4)
 // groups, each group every so many chunks, then the groups in order
 template <int D>
 __global__ __launch_bounds__(256) void join_kernel(Args a, Step st, uint32_t page,
@@ -468,8 +474,11 @@ __global__ __launch_bounds__(256) void join_kernel(Args a, Step st, uint32_t pag
   if (a.lse && i == 0) a.lse[(uint64_t) row * a.heads + h] = (top + log2f(l)) * kLn2;
 }
 
-// how a token step is launched: the chunks that the sequences are cut into for each kv head and 16 of its query heads, and
-// the workspace: where each sequence's chunks begin and how many they are, then the chunks' results
+// how a token step is launched: the chunks that the sequences are cut into for each kv head and 16 of its query heads (the
+// chip holds 512 of their workgroups; 512 / 768 / 1024 / 2048 wanted measured 99 / 100 / 106 / 112 us for one sequence of 131072 and
+// 44 / 45 / 43 / 50 for 64 of 1 to 8192; chunks of at least 256 / 384 / 512 keys 9.3 / 6.4 / 6.4 us for one of 333, which
+// then needs no join, and 20 / 17 / 17.5 for 24 wide 8-bit ones), and the workspace: where each sequence's chunks begin and
+// how many they are, then the chunks' results
 constexpr uint32_t kWant = 512;
 struct Cut {
   uint32_t want, most, tiles, dim;  // most: chunks there can be
@@ -523,7 +532,9 @@ __host__ __device__ inline bool in_bf16(uint32_t kv_type, uint32_t q_type) { ret
 // scores', the last tile's outputs') and the next's, so that the waves of a SIMD, of two workgroups, are on the matrix and
 // the vector units at different times. measured against it for a prompt of 8192 (32 heads of 128 on 8): 8 waves and tiles of 64
 // keys 5 % faster with the second four waves held one phase behind the first, the same without; but prompts of 1 to 2111 tokens
-// 11 % slower, chunks over 8-bit pages 22 %, one of 77 tokens 60 %.
+// 11 % slower, chunks over 8-bit pages 22 %, one of 77 tokens 60 %. that prompt takes 583 us, 943 TFLOP/s of the causal half,
+// where a library product of 8192 x 8192 x 8192 reaches 1187; the matrix units are busy 40 % of the time and the vector units
+// 50 %, and neither reads further ahead, other orders of the phases nor wave priorities changed it.
 constexpr int kKeys = 32, kRowWaves = 4, kRows = 32 * kRowWaves;
 enum Source { kPacked, kPages, kPagesF8 };
 
@@ -555,11 +566,6 @@ __device__ inline bool find_rows(const Step& st, uint32_t page, uint32_t group, 
   none.row0 = none.rows = none.len = none.end = 0, none.table = st.table;
   auto tiles = [&](const Seq& x) { return (uint32_t) (((uint64_t) (uint32_t) x.rows * group + kRows - 1) / kRows); };
   auto sum = [&](uint32_t x) { return (uint32_t) lane_of((int) wave_scan(x), 63); };
-  auto take = [&](int at) {
-    seq.row0 = lane_of(q.row0, at), seq.rows = lane_of(q.rows, at), seq.len = lane_of(q.len, at), seq.end = lane_of(q.end, at);
-    seq.table = (const int32_t*) ((uint64_t) (uint32_t) lane_of((int) ((uint64_t) q.table >> 32), at) << 32 |
-                                  (uint32_t) lane_of((int) (uint64_t) q.table, at));
-  };
   q = lane < st.n_seq ? sequence(st, lane, page) : none;
   if (st.n_seq <= 64) {
     const uint32_t n = tiles(q);
@@ -576,7 +582,7 @@ __device__ inline bool find_rows(const Step& st, uint32_t page, uint32_t group, 
     tile = low;
     uint64_t has = __ballot(n > low);
     for (uint32_t turn = index - after(low + 1); turn; turn--) has &= has - 1;
-    take(__builtin_ctzll(has));
+    seq = lane_of(q, __builtin_ctzll(has));
     return true;
   }
   uint32_t total = 0;
@@ -595,7 +601,7 @@ __device__ inline bool find_rows(const Step& st, uint32_t page, uint32_t group, 
     if (past) {
       const int at = __builtin_ctzll(past);
       tile = index - ((uint32_t) lane_of((int) x, at) - (uint32_t) lane_of((int) n, at));
-      take(at);
+      seq = lane_of(q, at);
       return true;
     }
     before = (uint32_t) lane_of((int) x, 63);
@@ -977,7 +983,9 @@ __global__ __launch_bounds__(256) void rows_join_kernel(Args a, Step st, uint32_
 }
 
 // how the rows are launched: tiles there can be, and the parts that each tile's keys are cut into: one, but where the tiles
-// leave compute units without work and the keys are many (a part of 256 keys or more, so that it costs more than its join)
+// leave compute units without work and the keys are many (a part of 256 keys or more, so that it costs more than its join).
+// 923 rows of 24 heads over 7109 tokens of 8-bit pages (184 tiles at most): whole 175 us, for 512 / 768 / 1024 / 1536 / 2048
+// workgroups 131 / 114 / 102 / 96 / 105
 constexpr uint64_t kFull = 1536, kLeastPart = 256;
 struct RowsCut {
   uint64_t tiles;

@@ -11,7 +11,6 @@ extern "C" {
 namespace osm {
 namespace kv {
 
-typedef float f32x2 __attribute__((ext_vector_type(2)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
@@ -102,27 +101,47 @@ __device__ inline Seq sequence(const Step& st, uint32_t s, uint32_t page) {
   return q;
 }
 
-// the sequence of row t: the last one that starts at or before it, -1 for none. the whole wave asks for one t: 64 starts
-// a round
-__device__ inline int sequence_of(const Step& st, int t) {
+// lane `at`'s sequence, for the whole wave
+__device__ inline int lane_of(int x, int lane) { return __builtin_amdgcn_readlane(x, lane); }
+__device__ inline Seq lane_of(const Seq& q, int at) {
+  Seq r;
+  r.row0 = lane_of(q.row0, at), r.rows = lane_of(q.rows, at), r.len = lane_of(q.len, at), r.end = lane_of(q.end, at);
+  r.table = (const int32_t*) ((uint64_t) (uint32_t) lane_of((int) ((uint64_t) q.table >> 32), at) << 32 |
+                              (uint32_t) lane_of((int) (uint64_t) q.table, at));
+  return r;
+}
+
+// the sequence of row t, the last one that starts at or before it; false for none. the whole wave asks for one t: up to 64
+// sequences are read whole at once, a lane each, so that no load waits for the search; more by their starts, 64 a round
+__device__ inline bool sequence_of(const Step& st, int t, uint32_t page, Seq& q) {
   const uint32_t lane = threadIdx.x & 63;
+  if (st.n_seq <= 64) {
+    const Seq mine = sequence(st, lane < st.n_seq ? lane : 0, page);
+    const uint64_t at = __ballot(lane < st.n_seq && st.start[lane < st.n_seq ? lane : 0] <= t);
+    if (!at) return false;
+    q = lane_of(mine, 63 - __builtin_clzll(at));
+    return true;
+  }
   uint32_t lo = 0, n = st.n_seq;
   for (;;) {
     const uint32_t by = (n + 63) / 64, i = lane * by;
     const uint64_t at = __ballot(i < n && st.start[lo + (i < n ? i : 0)] <= t);
     const int c = __popcll(at);
-    if (c == 0) return -1;
+    if (c == 0) return false;
     lo += (uint32_t) (c - 1) * by;
     n = by < n - (uint32_t) (c - 1) * by ? by : n - (uint32_t) (c - 1) * by;
-    if (by == 1) return (int) lo;
+    if (by == 1) break;
   }
+  q = sequence(st, lo, page);
+  return true;
 }
 
 inline bool shape_ok(const OsmosKv* kv) {
   if (!kv || (kv->type != OSMOS_F16 && kv->type != OSMOS_BF16 && kv->type != OSMOS_F8)) return false;
   if (!kv->layers || kv->layers > 4096 || !kv->pages || kv->pages > 0x7FFFFFF0u || !kv->heads || kv->heads > 4096) return false;
   if (!kv->page || kv->page > OSMOS_KV_MAX_PAGE || (kv->page & (kv->page - 1))) return false;
-  return kv->dim && kv->dim <= OSMOS_ATTN_MAX_DIM && kv->dim % 16 == 0;
+  return kv->dim && kv->dim <= OSMOS_ATTN_MAX_DIM && kv->dim % 16 == 0 &&
+         (uint64_t) kv->heads * kv->page * kv->dim <= OSMOS_KV_MAX_PAGE_VALUES;
 }
 inline bool cache_ok(const OsmosKv* kv) {
   return shape_ok(kv) && kv->data && (uintptr_t) kv->data % 16 == 0 && (kv->type == OSMOS_F8 || !kv->scale);

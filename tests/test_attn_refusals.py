@@ -36,7 +36,7 @@ def _rows(**o):
 
 
 BAD_KV = [dict(type=0), dict(type=2), dict(layers=0), dict(pages=0), dict(page=0), dict(page=24), dict(page=8192),
-          dict(heads=0), dict(dim=0), dict(dim=24), dict(dim=272)]
+          dict(heads=0), dict(dim=0), dict(dim=24), dict(dim=272), dict(heads=4096, page=4096)]
 BAD_CACHE = BAD_KV + [dict(data=None), dict(data=A + 8), dict(scale=A)]
 BAD_STEP = [dict(start=None), dict(len=None), dict(table=None), dict(n_seq=0), dict(n_tok=0), dict(max_tok=0),
             dict(max_len=0), dict(seqs=1), dict(table_stride=0)]
@@ -90,7 +90,7 @@ def test_attn(L, o):
     assert not L.osmos_attn_prompt(ctypes.byref(_attn(**o)), ctypes.byref(_rows()), ctypes.byref(st), P(A), 1 << 40, None)
 
 
-@pytest.mark.parametrize("o", [dict(k=None), dict(v=A + 4), dict(k_stride=129), dict(v_head=60), dict(type=0), dict(type=0x200),
+@pytest.mark.parametrize("o", [dict(k=None), dict(v=A + 4), dict(k_stride=129), dict(v_head=60), dict(v_stride=1 << 25), dict(type=0), dict(type=0x200),
                                dict(heads=0), dict(dim=20), dict(dim=288)], ids=str)
 def test_rows(L, o):
     st = _step(len=None, table=None, seqs=0, table_stride=0, max_len=0)

@@ -72,6 +72,29 @@ def test_append(src, kind, heads, dim, page, rows, lens):
     assert torch.equal(got.nan_to_num(9.0, 8.0, -8.0), want.nan_to_num(9.0, 8.0, -8.0))
 
 
+def test_append_quotients():
+    """8-bit values are the quotients' own roundings: every float16 value over scales of many sizes, those next to a rounding's
+    edge among them"""
+    from libosmos_amd import attn
+    heads, dim, page = 64, 128, 8
+    bits = torch.arange(65536, device="cuda").to(torch.int32)
+    x = bits.to(torch.int16).view(torch.float16).view(8, heads, dim)
+    scale = torch.empty((1, 2, heads), device="cuda")
+    for seed, (low, high) in enumerate(((0.001, 0.02), (0.5, 1.5), (1e-22, 1e-17), (1e18, 1e21), (-0.3, -0.01))):
+        scale.uniform_(low, high, generator=torch.Generator("cuda").manual_seed(seed))
+        data = torch.zeros((1, 2, 1, heads, page, dim), device="cuda").to(T["f8"])
+        step = attn.KvStep(_ints([0, 8]), _ints([8]), _ints([[0]]), n_tok=8, max_tok=8, max_len=8)
+        k, v = x, x.flip(0).contiguous()
+        print("quotients", low, flush=True)
+        attn.Append(attn.KvCache(data, scale), 0, step, k, v).run()
+        torch.cuda.synchronize()
+        for w, t in enumerate((k, v)):
+            want = (t.float() / scale[0, w][:, None]).clamp(-448, 448).to(T["f8"]).float().transpose(0, 1)
+            got = data[0, w, 0].float()
+            assert torch.equal(torch.isnan(got), torch.isnan(want))
+            assert torch.equal(got.nan_to_num(9.0), want.nan_to_num(9.0)), (low, w)
+
+
 class Model:
     """the pool, one request after another"""
 
