@@ -91,9 +91,10 @@ __device__ inline void q_steps(const uint8_t* p, uint32_t dim, bool in, float si
   }
 }
 template <bool BF, int N, class At>
-__device__ inline void load_q(const Args& a, uint64_t row, uint32_t head, bool in, At at, typename Unit<BF>::v8 (&q)[N]) {
+__device__ inline void load_q(const Args& a, uint64_t row, uint32_t head, bool in, float scale, At at,
+                              typename Unit<BF>::v8 (&q)[N]) {
   const uint8_t* p = a.q + (row * a.qs + head * a.qh) * kv::size_of(a.q_type);
-  const float sign = a.scale < 0.0f ? -1.0f : a.scale == 0.0f ? 0.0f : 1.0f;
+  const float sign = scale < 0.0f ? -1.0f : scale == 0.0f ? 0.0f : 1.0f;
   if (a.q_type == OSMOS_F32) q_steps<BF, N, OSMOS_F32>(p, a.dim, in, sign, at, q);
   else if (a.q_type == OSMOS_F16) q_steps<BF, N, OSMOS_F16>(p, a.dim, in, sign, at, q);
   else q_steps<BF, N, OSMOS_BF16>(p, a.dim, in, sign, at, q);
@@ -127,7 +128,7 @@ __device__ inline float sum_rows(float x) {
 
 constexpr float kLog2E = 1.44269504088896341f, kLn2 = 0.693147180559945309f;
 // what a score is multiplied with (its sign is in q; of a scale of 0 q is zeros, as -infinity times 0 would be NaN)
-__device__ inline float unit_of(const Args& a) { return a.scale == 0.0f ? 1.0f : fabsf(a.scale) * kLog2E; }
+__device__ inline float unit_of(float scale) { return scale == 0.0f ? 1.0f : fabsf(scale) * kLog2E; }
 // a maximum as what is subtracted: of nothing (-infinity), zero, so that exp2 of the difference is 0 and not NaN
 __device__ inline float finite_max(float m) { return m == -__builtin_inff() ? 0.0f : m; }
 
@@ -292,10 +293,10 @@ __global__ __launch_bounds__(256, D > 128 ? 1 : 2) void token_kernel(Args a, Kv 
   // Q^T as the B operand: column lane % 16, 8 dims a lane of each step's 32; of 8-bit keys a lane loads 16 dims at once,
   // so that two steps share 64 dims
   v8 q[kSteps];
-  load_q<BF, kSteps>(a, row, head0 + (r < heads ? r : 0), r < heads, [&](int i) {
+  const float scale = a.scale * (F8 && kv.scale ? kv.scale[g] : 1.0f), unit = unit_of(scale);
+  load_q<BF, kSteps>(a, row, head0 + (r < heads ? r : 0), r < heads, scale, [&](int i) {
     return F8 ? (uint32_t) (64 * (i / 2) + 16 * quad + 8 * (i % 2)) : (uint32_t) (32 * i + 8 * quad);
   }, q);
-  const float unit = unit_of(a) * (F8 && kv.scale ? kv.scale[g] : 1.0f);
 
   f32x4 o[kDims];
 #pragma unroll
@@ -533,8 +534,8 @@ __host__ __device__ inline bool in_bf16(uint32_t kv_type, uint32_t q_type) { ret
 // the vector units at different times. measured against it for a prompt of 8192 (32 heads of 128 on 8): 8 waves and tiles of 64
 // keys 5 % faster with the second four waves held one phase behind the first, the same without; but prompts of 1 to 2111 tokens
 // 11 % slower, chunks over 8-bit pages 22 %, one of 77 tokens 60 %. that prompt takes 583 us, 943 TFLOP/s of the causal half,
-// where a library product of 8192 x 8192 x 8192 reaches 1187; the matrix units are busy 40 % of the time and the vector units
-// 50 %, and neither reads further ahead, other orders of the phases nor wave priorities changed it.
+// where a library product of 8192 x 8192 x 8192 reaches 1187; the matrix units are busy 45 % of the time and the vector units
+// 52 %, and neither reads further ahead, other orders of the phases nor wave priorities changed it.
 constexpr int kKeys = 32, kRowWaves = 4, kRows = 32 * kRowWaves;
 enum Source { kPacked, kPages, kPagesF8 };
 
@@ -778,8 +779,9 @@ __global__ __launch_bounds__(64 * kRowWaves, D > 128 ? 1 : 2) void rows_kernel(A
     ids(1);
   }
   v8 q[kSteps];
-  load_q<BF, kSteps>(a, (uint64_t) seq.row0 + (in ? token : 0), in ? head : 0, in, [&](int i) { return (uint32_t) (16 * i + 8 * half); }, q);
-  const float unit = unit_of(a) * (SRC == kPagesF8 && kv.scale ? kv.scale[g] : 1.0f);
+  const float scale = a.scale * (SRC == kPagesF8 && kv.scale ? kv.scale[g] : 1.0f), unit = unit_of(scale);
+  load_q<BF, kSteps>(a, (uint64_t) seq.row0 + (in ? token : 0), in ? head : 0, in, scale,
+                     [&](int i) { return (uint32_t) (16 * i + 8 * half); }, q);
   f32x16 o[kDims], x;
 #pragma unroll
   for (int i = 0; i < kDims; i++) o[i] = f32x16{};

@@ -443,3 +443,41 @@ def test_many_sequences(token):
                 want = attn_ref.attend(q[t:t + r, h].double(), k, v, pos, here, 0.125, 0, torch.bfloat16, torch.bfloat16)
                 attn_ref.check(out[t:t + r, h], lse[t:t + r, h], *want, (s, h))
         t += r
+
+
+@pytest.mark.parametrize("kind", ["f16", "bf16"])
+def test_signs_of_8_bit_scales(kind):
+    """an 8-bit cache whose scales are negative or zero for some heads, and NaN among its masked bytes"""
+    from libosmos_amd import attn
+    g, lens = _gen(14), [500, 33, 64]
+    pg = Paged(g, lens, 4, 64, 16, "f8")
+    pg.scale[1, 0, 0] *= -1.0   # (keys of head 0)
+    pg.scale[1, 0, 1] = 0.0     # (of head 1: every score 0)
+    pg.scale[1, 1, 2] *= -1.0   # (values of head 2)
+    for token, rows in ((True, [1, 1, 1]), (False, [90, 33, 5])):
+        n = sum(rows)
+        q = _normal(g, n, 8, 64).to(T[kind])
+        out, lse = torch.empty_like(q), torch.empty((n, 8), device="cuda")
+        step = attn.KvStep(_ints(_starts(rows)), pg.len, pg.table, n_tok=n, max_tok=max(rows), max_len=500)
+        print("signs", kind, token, flush=True)
+        (attn.TokenAttention if token else attn.ChunkAttention)(pg.cache, 1, step, q, out, lse).run()
+        torch.cuda.synchronize()
+        t = 0
+        for s, (r, m) in enumerate(zip(rows, lens)):
+            pos = torch.arange(m - r, m, device="cuda")
+            for h in range(8):
+                (k, here), (v, _) = (attn_ref.rows_of_pages(pg.data, pg.scale, 1, w, pg.table[s], m, h // 2) for w in (0, 1))
+                want = attn_ref.attend(q[t:t + r, h].double(), k, v, pos, here, 0.125, 0, T[kind], T[kind])
+                attn_ref.check(out[t:t + r, h], lse[t:t + r, h], *want, (token, s, h))
+            t += r
+    bad = 300  # a value's byte of NaN that only some rows of a tile see
+    pg.data.view(torch.uint8)[1, 1, pg.table[0, bad // 16], :, bad % 16, ::5] = 0x7F
+    rows = [220, 0, 0]
+    q = _normal(g, 220, 8, 64).to(T[kind])
+    out = torch.empty_like(q)
+    step = attn.KvStep(_ints(_starts(rows)), pg.len, pg.table, n_tok=220, max_tok=220, max_len=500)
+    attn.ChunkAttention(pg.cache, 1, step, q, out).run()
+    torch.cuda.synchronize()
+    sees = torch.arange(280, 500, device="cuda") >= bad
+    assert torch.isnan(out[sees][..., ::5]).all() and torch.isfinite(out[~sees]).all()
+    assert torch.isfinite(out[sees][..., 1::5]).all()
