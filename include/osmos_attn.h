@@ -99,7 +99,8 @@ bool osmos_attn_prompt(const OsmosAttn *a, const OsmosKvRows *kv, const OsmosKvS
 /* rows over the cache (the step's own among its tokens: osmos_kv_append goes first) */
 bool osmos_attn_chunk(const OsmosAttn *a, const OsmosKv *kv, uint32_t layer, const OsmosKvStep *step, void *workspace,
                       uint64_t workspace_bytes, void *stream);
-/* osmos_attn_chunk where every sequence brings one row or none (max_tok 1): the cache read once, split over its length */
+/* osmos_attn_chunk where every sequence brings one row or none (max_tok 1): the cache read once, split over its length.
+   refused: n_seq sequences of max_len tokens, or of what a table row holds, past 2^32 tiles of 32 tokens */
 bool osmos_attn_token(const OsmosAttn *a, const OsmosKv *kv, uint32_t layer, const OsmosKvStep *step, void *workspace,
                       uint64_t workspace_bytes, void *stream);
 

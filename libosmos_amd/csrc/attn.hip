@@ -1094,6 +1094,9 @@ extern "C" OSM_API bool osmos_attn_token(const OsmosAttn* a, const OsmosKv* kv, 
                                          void* workspace, uint64_t workspace_bytes, void* stream) {
   if (!kv::cache_ok(kv) || layer >= kv->layers || !attn::args_ok(a, kv->heads, kv->dim) || !kv::step_ok(step, true)) return false;
   if (step->max_tok != 1) return false;
+  // (a step's tiles are counted in 32 bits)
+  const uint64_t room = (uint64_t) step->table_stride * kv->page, longest = room < step->max_len ? room : step->max_len;
+  if (step->n_seq * (longest / 32 + 1) > 0xFFFFFFFFull) return false;
   const attn::Cut c = attn::cut_of(a, kv->heads, kv->dim, step);
   if (!attn::room_ok(attn::token_bytes(a, c), workspace, workspace_bytes)) return false;
   const bool bf = attn::in_bf16(kv->type, a->q_type), f8 = kv->type == OSMOS_F8;

@@ -117,3 +117,9 @@ def test_others(L):
         assert not L.osmos_kv_fork(kv, good, P(A), P(A), n, None, None)
         assert not L.osmos_kv_free(kv, good, P(A), n, None)
     assert not L.osmos_kv_copy(kv, P(A), P(A), 0, None)
+
+
+def test_token_tiles(L):
+    """a step whose tiles of 32 keys would pass 32 bits, by its bounds and by its tables' room"""
+    assert not _token(L, step=_step(n_seq=66, seqs=66, max_len=0x7FFF0000, table_stride=1 << 27))
+    assert not _token(L, step=_step(n_seq=1 << 20, seqs=1 << 20, max_len=0x7FFF0000, table_stride=1 << 13))
