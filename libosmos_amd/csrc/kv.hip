@@ -39,9 +39,8 @@ __global__ __launch_bounds__(64 * kAppendRows) void append_kernel(const uint8_t*
   const uint32_t t = blockIdx.x * kAppendRows + threadIdx.x / 64, lane = threadIdx.x & 63;
   if (t >= st.n_tok) return;
   const uint32_t half = heads * dim / 8, pieces = 2 * half, per = dim / 8;
-  uint8_t* to = nullptr;
-  for (uint32_t c0 = lane; c0 < pieces; c0 += 256) {
-    float x[4][8];
+  float x[4][8];
+  auto load = [&](uint32_t c0) __attribute__((always_inline)) {
 #pragma unroll
     for (int i = 0; i < 4; i++) {
       const uint32_t c = c0 + 64 * i;
@@ -49,15 +48,17 @@ __global__ __launch_bounds__(64 * kAppendRows) void append_kernel(const uint8_t*
       const uint32_t at = c < half ? c : c - half;
       load8<SRC>(c < half ? k + ((uint64_t) t * ks + at * 8ull) * size_of(SRC) : v + ((uint64_t) t * vs + at * 8ull) * size_of(SRC), x[i]);
     }
-    if (!to) {
-      Seq q;
-      if (!sequence_of(st, (int) t, page, q)) return;
-      const int pos = q.len - (q.row0 + q.rows - (int) t);
-      if ((int) t < q.row0 || (int) t >= q.row0 + q.rows || pos < 0 || pos >= q.end) return;
-      const uint32_t id = (uint32_t) gload<int>(q.table + (uint32_t) pos / page);
-      if (id >= pages) return;
-      to = data + ((uint64_t) id * heads * page + ((uint32_t) pos & (page - 1))) * dim * size_of(DST);
-    }
+  };
+  load(lane);
+  // (every lane takes part in the search, those of a short row that have no piece too)
+  Seq q;
+  if (!sequence_of(st, (int) t, page, q)) return;
+  const int pos = q.len - (q.row0 + q.rows - (int) t);
+  if ((int) t < q.row0 || (int) t >= q.row0 + q.rows || pos < 0 || pos >= q.end) return;
+  const uint32_t id = (uint32_t) gload<int>(q.table + (uint32_t) pos / page);
+  if (id >= pages) return;
+  uint8_t* to = data + ((uint64_t) id * heads * page + ((uint32_t) pos & (page - 1))) * dim * size_of(DST);
+  for (uint32_t c0 = lane; c0 < pieces;) {
 #pragma unroll
     for (int i = 0; i < 4; i++) {
       const uint32_t c = c0 + 64 * i;
@@ -69,6 +70,7 @@ __global__ __launch_bounds__(64 * kAppendRows) void append_kernel(const uint8_t*
       }
       store8<DST>(to + (second ? plane : 0) + ((uint64_t) h * page * dim + d * 8) * size_of(DST), x[i]);
     }
+    if ((c0 += 256) < pieces) load(c0);
   }
 }
 

@@ -112,7 +112,8 @@ __device__ inline Seq lane_of(const Seq& q, int at) {
 }
 
 // the sequence of row t, the last one that starts at or before it; false for none. the whole wave asks for one t: up to 64
-// sequences are read whole at once, a lane each, so that no load waits for the search; more by their starts, 64 a round
+// sequences are read whole at once, a lane each, so that no load waits for the search; more by their starts, 64 a round. all 64
+// lanes have to be active: one that is not hides its sequence
 __device__ inline bool sequence_of(const Step& st, int t, uint32_t page, Seq& q) {
   const uint32_t lane = threadIdx.x & 63;
   if (st.n_seq <= 64) {
