@@ -53,6 +53,8 @@ typedef struct OsmosKvStep
   uint32_t max_tok;     /* no sequence brings more rows */
   uint32_t max_len;     /* no sequence has more tokens: later keys are left out */
   uint32_t seqs, table_stride;
+  const int32_t *live;  /* n_seq, or NULL: 0 for a sequence that takes no part in this step (osmos_kv_grow's `done`, as its
+                           tokens are not in len): its rows are not written, and see no key */
 } OsmosKvStep;
 
 /* the bytes of a cache's data; 0 for a shape or type out of range */
@@ -93,7 +95,7 @@ typedef struct OsmosKvRows
 /* the most device memory (256-byte aligned) that an attention call over the step needs as its workspace, 0 for none; a
    workspace is written before it is read, and calls that share one are ordered on one stream */
 uint64_t osmos_attn_workspace(const OsmosAttn *a, uint32_t kv_heads, uint32_t dim, const OsmosKvStep *step);
-/* whole prompts: row t's keys are its sequence's rows up to t (step->len, table, seq unused: NULL) */
+/* whole prompts: row t's keys are its sequence's rows up to t (step->len, table, seq, live unused: NULL) */
 bool osmos_attn_prompt(const OsmosAttn *a, const OsmosKvRows *kv, const OsmosKvStep *step, void *workspace,
                        uint64_t workspace_bytes, void *stream);
 /* rows over the cache (the step's own among its tokens: osmos_kv_append goes first) */
@@ -108,7 +110,8 @@ bool osmos_attn_token(const OsmosAttn *a, const OsmosKv *kv, uint32_t layer, con
    OsmosKvStep, a table row's ids past its pages -1. the operations take request lists of up to
    OSMOS_KV_MAX_REQUESTS sequences in device memory and act in stream order with no host round trip; their outcome is
    fixed by the lists' order. `done` (n, may be NULL): 1 for a request carried out, 0 for a refused one, which changes
-   nothing. */
+   nothing. a step queued behind osmos_kv_grow takes its `done` as OsmosKvStep's live: without it a refused sequence's
+   rows would be written over the last tokens it has, in pages that others may hold too. */
 typedef struct OsmosKvPool
 {
   int32_t *ref;         /* pages, 16-byte aligned */

@@ -91,6 +91,7 @@ class KvPool:
                    torch.full((seqs, width), -1, dtype=torch.int32, device="cuda"))
 
     def grow(self, seq, add, done=None, stream=None):
+        """add[i] more tokens for seq[i]; done[i] 0: refused. a step queued behind it takes `done` as its `live`"""
         if add.numel() != seq.numel() or (done is not None and done.numel() != seq.numel()):
             raise ValueError("KvPool.grow: seq, add and done have one entry a request")
         if not capi.lib().osmos_kv_grow(self._kv, self._pool, capi.addr(_ints(seq, "seq")), capi.addr(_ints(add, "add")),
@@ -116,21 +117,26 @@ class KvPool:
 
 class KvStep:
     """The rows of one step (OsmosKvStep): start (sequences + 1), len and table as the pool's, seq the step's sequences'
-    places in them (None: in order). n_tok rows in all; no sequence brings more than max_tok, none is longer than max_len."""
+    places in them (None: in order). n_tok rows in all; no sequence brings more than max_tok, none is longer than max_len.
+    live (None: all): 0 for a sequence that takes no part, KvPool.grow's `done` where the step follows it unread: its rows are
+    not appended and attend to nothing."""
 
-    def __init__(self, start, len=None, table=None, *, n_tok, max_tok, max_len=0, seq=None):
-        self.start, self.len, self.table, self.seq = start, len, table, seq
-        for t, name in ((start, "start"), (len, "len"), (table, "table"), (seq, "seq")):
+    def __init__(self, start, len=None, table=None, *, n_tok, max_tok, max_len=0, seq=None, live=None):
+        self.start, self.len, self.table, self.seq, self.live = start, len, table, seq, live
+        for t, name in ((start, "start"), (len, "len"), (table, "table"), (seq, "seq"), (live, "live")):
             if t is not None:
                 _ints(t, name)
         if seq is not None and seq.numel() != start.numel() - 1:
             raise ValueError("KvStep: seq has an entry a sequence of the step")
+        if live is not None and live.numel() != start.numel() - 1:
+            raise ValueError("KvStep: live has an entry a sequence of the step")
         if table is not None and (table.dim() != 2 or len is None or table.shape[0] != len.numel()):
             raise ValueError("KvStep: table has a row a sequence of len")
         at = lambda t: None if t is None else t.data_ptr()  # noqa: E731
         self.n_tok = n_tok
         self.desc = capi.OsmosKvStep(at(start), at(len), at(table), at(seq), start.numel() - 1, n_tok, max_tok, max_len,
-                                     0 if table is None else table.shape[0], 0 if table is None else table.shape[1])
+                                     0 if table is None else table.shape[0], 0 if table is None else table.shape[1],
+                                     at(live))
 
 
 class _Call:

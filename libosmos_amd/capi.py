@@ -99,7 +99,7 @@ class OsmosKv(ctypes.Structure):
 
 class OsmosKvStep(ctypes.Structure):
     _fields_ = [("start", P), ("len", P), ("table", P), ("seq", P), ("n_seq", U32), ("n_tok", U32), ("max_tok", U32),
-                ("max_len", U32), ("seqs", U32), ("table_stride", U32)]
+                ("max_len", U32), ("seqs", U32), ("table_stride", U32), ("live", P)]
 
 
 class OsmosAttn(ctypes.Structure):

@@ -67,13 +67,13 @@ __device__ inline void store8(void* p, const float (&x)[8]) {
 
 // a step's tables with their bounds
 struct Step {
-  const int32_t *start, *len, *table, *seq;
+  const int32_t *start, *len, *table, *seq, *live;
   uint32_t n_seq, n_tok, max_len, seqs, width;  // width: table_stride
 };
 
 struct Seq {
   int row0, rows;        // its rows in the step
-  int len;               // its tokens, the rows' among them
+  int len;               // its tokens, the rows' among them (none where it takes no part in the step)
   int end;               // the tokens that may be read: len within the table's room and max_len
   const int32_t* table;  // its pages (paged only)
 };
@@ -94,7 +94,8 @@ __device__ inline Seq sequence(const Step& st, uint32_t s, uint32_t page) {
       return q;
     }
     const uint64_t room = (uint64_t) st.width * page;
-    q.len = clampi(st.len[id], 0, 0x7FFFFFFF);
+    const bool live = !st.live || st.live[s];
+    q.len = live ? clampi(st.len[id], 0, 0x7FFFFFFF) : 0;
     q.end = clampi(q.len, 0, room < st.max_len ? (int) room : (int) st.max_len);
     q.table = st.table + (uint64_t) id * st.width;
   }
@@ -156,7 +157,7 @@ inline bool step_ok(const OsmosKvStep* st, bool paged) {
          st->max_len <= 0x7FFF0000u;
 }
 inline Step step_of(const OsmosKvStep* st) {
-  return Step{st->start, st->len, st->table, st->seq, st->n_seq, st->n_tok, st->max_len, st->seqs, st->table_stride};
+  return Step{st->start, st->len, st->table, st->seq, st->live, st->n_seq, st->n_tok, st->max_len, st->seqs, st->table_stride};
 }
 
 }  // namespace kv
