@@ -2,9 +2,12 @@
 //
 // a row's output is sum_j p_j v_j / sum_j p_j with p_j = exp(scale q k_j - m), m the greatest score, in one pass: the
 // running m and sum, the sum and output scaled by exp(m_old - m_new) where m grows. scores, sums, maxima and outputs are
-// kept in float; the p_j, in 0 .. 1 (of rows of prompts up to 2^8), are rounded to the products' 16-bit type, as the matrix
-// units take no other: an error of the size of a 16-bit output's own rounding and independent of it (a bf16 prompt of 8192
-// is 2.2e-3 off in all, relative, where the output's rounding alone makes 1.6e-3). the sum takes the p_j before that.
+// kept in float; the p_j are rounded to the products' 16-bit type, as the matrix units take no other: an error of the size of a
+// 16-bit output's own rounding and independent of it (a bf16 prompt of 8192 is 2.2e-3 off in all, relative, where the
+// output's rounding alone makes 1.6e-3). the sum takes the p_j before that. f16 has no values between 0 and 2^-24, and
+// thousands of keys of less weight than that count together: its p_j are taken 2^lift times as large, up to 2^15, by a running m
+// that is the greatest score less the lift (in powers of two), and the factor leaves sum and output at the end. a tile's p_j are
+// summed before they join the running sum, which one by one would not notice those below 2^-24 of it.
 #include <type_traits>
 
 #include "kvcache.h"
@@ -48,6 +51,7 @@ template <> struct Unit<false> {
   typedef _Float16 e;
   typedef kv::f16x8 v8;
   typedef _Float16 v4 __attribute__((ext_vector_type(4)));
+  static constexpr int kLift = 15;  // p_j up to 2 to this
   static __device__ inline f32x4 mfma16(v8 a, v8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
   static __device__ inline f32x16 mfma32(v8 a, v8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
   static __device__ inline f16x2 f8_low(uint32_t w) { return __builtin_amdgcn_cvt_scalef32_pk_f16_fp8((int) w, 1.0f, false); }
@@ -57,6 +61,7 @@ template <> struct Unit<true> {
   typedef __bf16 e;
   typedef kv::bf16x8 v8;
   typedef __bf16 v4 __attribute__((ext_vector_type(4)));
+  static constexpr int kLift = 0;
   static __device__ inline f32x4 mfma16(v8 a, v8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
   static __device__ inline f32x16 mfma32(v8 a, v8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
   static __device__ inline bf16x2 f8_low(uint32_t w) { return __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((int) w, 1.0f, false); }
@@ -362,7 +367,7 @@ __global__ __launch_bounds__(256, D > 128 ? 1 : 2) void token_kernel(Args a, Kv 
           if (!(live >> (16 * i + 4 * quad + j) & 1)) x[i][j] = -__builtin_inff();
     }
     float top = fmaxf(fmaxf(fmaxf(x[0][0], x[0][1]), fmaxf(x[0][2], x[0][3])), fmaxf(fmaxf(x[1][0], x[1][1]), fmaxf(x[1][2], x[1][3])));
-    top = fmaxf(m, max_rows(top) * unit);
+    top = fmaxf(m, __builtin_fmaf(max_rows(top), unit, -(float) U::kLift));
     const float base = finite_max(top);
     if (__any(top > m)) {  // (seldom, once the greatest scores have been met)
       const float fade = __builtin_amdgcn_exp2f(m - base);
@@ -372,14 +377,16 @@ __global__ __launch_bounds__(256, D > 128 ? 1 : 2) void token_kernel(Args a, Kv 
       for (int t = 0; t < kDims; t++) o[t] *= fade;
     }
     v8 p;
+    float sum = 0.0f;
 #pragma unroll
     for (int i = 0; i < 2; i++)
 #pragma unroll
       for (int j = 0; j < 4; j++) {
         const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(x[i][j], unit, -base));
-        l += e;
+        sum = i + j ? sum + e : e;
         p[4 * i + j] = (typename U::e) e;
       }
+    l += sum;
     // O^T: V^T's columns of keys 4 quad + 0 .. 3 and 16 + 4 quad + 0 .. 3, as P^T's lanes hold them
 #pragma unroll
     for (int t = 0; t < kDims; t++) {
@@ -400,11 +407,13 @@ __global__ __launch_bounds__(256, D > 128 ? 1 : 2) void token_kernel(Args a, Kv 
   }
 
   // the waves' results joined: each scaled to the greatest maximum, then summed in the waves' order
-  l = sum_rows(l);
+  constexpr float kDown = 1.0f / (1 << U::kLift);
+  m += (float) U::kLift;
+  l = sum_rows(l) * kDown;
   if (quad == 0) ml[wave][0][r] = m, ml[wave][1][r] = l;
   __syncthreads();
   float top = fmaxf(fmaxf(ml[0][0][r], ml[1][0][r]), fmaxf(ml[2][0][r], ml[3][0][r]));
-  const float base = finite_max(top), mine = __builtin_amdgcn_exp2f(m - base);
+  const float base = finite_max(top), mine = __builtin_amdgcn_exp2f(m - base) * kDown;
   float* out = (float*) lds[wave];
 #pragma unroll
   for (int t = 0; t < kDims; t++) *(f32x4*) (out + r * (D + 4) + 16 * t + 4 * quad) = o[t] * mine;
@@ -540,8 +549,9 @@ constexpr int kKeys = 32, kRowWaves = 4, kRows = 32 * kRowWaves;
 enum Source { kPacked, kPages, kPagesF8 };
 
 // a row's scores are taken against its running maximum as it was until one is past it by more than this (in powers of two):
-// probabilities to 2^8 cost no accuracy in either type, and most tiles then leave the output and the sum unscaled
-constexpr float kSlack = 8.0f;
+// probabilities to 2^8 (in f16, lifted by the rest, to 2^15) cost no accuracy in either type, and most tiles then leave the output
+// and the sum unscaled
+constexpr int kSlack = 8;
 
 template <int D> struct RowsTile {
   static constexpr int kRow = 2 * D, kBytes = kKeys * kRow;
@@ -653,6 +663,7 @@ __global__ __launch_bounds__(64 * kRowWaves, D > 128 ? 1 : 2) void rows_kernel(A
   typedef typename U::v8 v8;
   typedef RowsTile<D> T;
   constexpr int kThreads = 64 * kRowWaves, kSteps = D / 16, kDims = D / 32;
+  constexpr int kLift = BF ? 0 : U::kLift - kSlack;
   constexpr int kPieces = SRC == kPagesF8 ? kKeys * D / 16 : kKeys * D / 8;  // 16-byte pieces of a tile's keys in memory
   constexpr int kEach = (kPieces + kThreads - 1) / kThreads, kPer = kPieces / kKeys;
   __shared__ __attribute__((aligned(16))) uint8_t lds[2][2][T::kBytes];  // [keys, values][tile & 1]
@@ -831,8 +842,8 @@ __global__ __launch_bounds__(64 * kRowWaves, D > 128 ? 1 : 2) void rows_kernel(A
     float top = x[0];
 #pragma unroll
     for (int i = 1; i < 16; i++) top = fmaxf(top, x[i]);
-    top = max_halves(top) * unit;
-    if (__any(top > m + kSlack)) {
+    top = __builtin_fmaf(max_halves(top), unit, -(float) kLift);
+    if (__any(top > m + (float) kSlack)) {
       const float next = fmaxf(m, top), fade = __builtin_amdgcn_exp2f(m - finite_max(next));
       m = next;
       l *= fade;
@@ -840,12 +851,14 @@ __global__ __launch_bounds__(64 * kRowWaves, D > 128 ? 1 : 2) void rows_kernel(A
       for (int i = 0; i < kDims; i++) o[i] *= fade;
     }
     const float sub = finite_max(m);
+    float sum = 0.0f;
 #pragma unroll
     for (int i = 0; i < 16; i++) {
       const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(x[i], unit, -sub));
-      l += e;
+      sum = i ? sum + e : e;
       p[i / 8][i % 8] = (typename U::e) e;
     }
+    l += sum;
   };
   // the products' phase after tile t's softmax: the next tile's scores, tile t's outputs, the next stage
   auto products = [&](int t, auto buf) __attribute__((always_inline)) {
@@ -928,10 +941,12 @@ __global__ __launch_bounds__(64 * kRowWaves, D > 128 ? 1 : 2) void rows_kernel(A
         }
   }
   if (!in) return;
-  l = sum_halves(l);
+  constexpr float kDown = 1.0f / (1 << kLift);
+  const float v_scale = (SRC == kPagesF8 && kv.scale ? kv.scale[kv.heads + g] : 1.0f) * kDown;
+  m += (float) kLift;
+  l = sum_halves(l) * kDown;
   if (parts > 1) {
     float* at = part + ((uint64_t) blockIdx.x * kRows + (row - row0)) * (D + 4);
-    const float v_scale = SRC == kPagesF8 && kv.scale ? kv.scale[kv.heads + g] : 1.0f;
 #pragma unroll
     for (int i = 0; i < kDims; i++)
 #pragma unroll
@@ -940,7 +955,7 @@ __global__ __launch_bounds__(64 * kRowWaves, D > 128 ? 1 : 2) void rows_kernel(A
     if (half == 0) at[D] = m, at[D + 1] = l;
     return;
   }
-  const float inv = l == 0.0f ? 0.0f : (SRC == kPagesF8 && kv.scale ? kv.scale[kv.heads + g] : 1.0f) / l;
+  const float inv = l == 0.0f ? 0.0f : v_scale / l;
   const uint64_t at = ((uint64_t) seq.row0 + token) * a.os + head * a.oh;
 #pragma unroll
   for (int i = 0; i < kDims; i++)
