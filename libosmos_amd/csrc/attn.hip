@@ -10,6 +10,7 @@
 // summed before they join the running sum, which one by one would not notice those below 2^-24 of it.
 #include <type_traits>
 
+#include "attnhost.h"
 #include "kvcache.h"
 
 namespace osm {
@@ -187,10 +188,8 @@ __device__ inline uint32_t wave_scan(uint32_t x) {
   return x;
 }
 
-// the step's work cut into chunks of one length, so that `want` of them hold all its keys (at least kLeast keys each, whole
-// 128s: a tile for each wave): workgroup `index` takes chunk c of sequence s's n. every workgroup reads all lengths, 64 a
-// round, and finds its place by their running sum, as no one else knows them; at most want + n_seq chunks.
-constexpr uint32_t kLeast = 384;
+// the step's work cut into chunks (chunk_keys): workgroup `index` takes chunk c of sequence s's n. every workgroup reads all
+// lengths, 64 a round, and finds its place by their running sum, as no one else knows them; at most want + n_seq chunks.
 struct Work {
   uint32_t s, c, n, chunk;
   Seq seq;
@@ -206,13 +205,12 @@ __device__ inline bool find_work(const Step& st, uint32_t page, uint32_t window,
     if ((s += 64) >= st.n_seq) break;
     q = s + lane < st.n_seq ? sequence(st, s + lane, page) : none;
   }
-  const uint32_t even = total / want + 1;
-  w.chunk = even * 32 <= kLeast ? kLeast : (even + 3) / 4 * 128;
+  w.chunk = chunk_keys(total, want);
   uint32_t before = 0;
   for (uint32_t s = 0; s < st.n_seq; s += 64) {
     if (st.n_seq > 64) q = s + lane < st.n_seq ? sequence(st, s + lane, page) : none;
     const int k = keys_of(q, window);
-    const uint32_t n = q.rows < 1 ? 0 : k <= (int) w.chunk ? 1 : ((uint32_t) k + w.chunk - 1) / w.chunk, x = before + wave_scan(n);
+    const uint32_t n = q.rows < 1 ? 0 : chunks_of(k, w.chunk), x = before + wave_scan(n);
     const uint64_t past = __ballot(x > index);
     if (past) {
       const int at = __builtin_ctzll(past);
@@ -482,33 +480,6 @@ __global__ __launch_bounds__(256) void join_kernel(Args a, Step st, uint32_t pag
   }
   if (4 * i < a.dim) put4(a, row * a.os + h * a.oh + 4 * i, y * (l == 0.0f ? 0.0f : 1.0f / l));
   if (a.lse && i == 0) a.lse[(uint64_t) row * a.heads + h] = (top + log2f(l)) * kLn2;
-}
-
-// how a token step is launched: the chunks that the sequences are cut into for each kv head and 16 of its query heads (the
-// chip holds 512 of their workgroups; 512 / 768 / 1024 / 2048 wanted measured 99 / 100 / 106 / 112 us for one sequence of 131072 and
-// 44 / 45 / 43 / 50 for 64 of 1 to 8192; chunks of at least 256 / 384 / 512 keys 9.3 / 6.4 / 6.4 us for one of 333, which
-// then needs no join, and 20 / 17 / 17.5 for 24 wide 8-bit ones), and the workspace: where each sequence's chunks begin and
-// how many they are, then the chunks' results
-constexpr uint32_t kWant = 512;
-struct Cut {
-  uint32_t want, most, tiles, dim;  // most: chunks there can be
-  bool split;                       // whether a sequence can have more than one
-  uint64_t head;                    // the workspace's bytes before the results
-};
-inline Cut cut_of(const OsmosAttn* a, uint32_t kv_heads, uint32_t dim, const OsmosKvStep* st) {
-  Cut c;
-  c.tiles = (a->heads / kv_heads + 15) / 16;
-  c.dim = dim <= 64 ? 64 : dim <= 128 ? 128 : 256;
-  c.want = kWant / (kv_heads * c.tiles) ? kWant / (kv_heads * c.tiles) : 1;
-  const uint64_t keys = a->window && a->window + 31ull < st->max_len ? a->window + 31ull : st->max_len;
-  c.split = keys > kLeast;
-  const uint64_t each = st->n_seq * ((keys + kLeast - 1) / kLeast), even = (uint64_t) c.want + st->n_seq;
-  c.most = (uint32_t) (each < even ? each : even);
-  c.head = (st->n_seq * 8ull + 255) / 256 * 256;
-  return c;
-}
-inline uint64_t token_bytes(const OsmosAttn* a, const Cut& c) {
-  return c.split ? c.head + (uint64_t) c.most * a->heads * (c.dim + 4) * 4 : 0;
 }
 
 template <bool BF, bool F8>
