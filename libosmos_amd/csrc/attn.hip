@@ -10,7 +10,6 @@
 // summed before they join the running sum, which one by one would not notice those below 2^-24 of it.
 #include <type_traits>
 
-#include "attnhost.h"
 #include "kvcache.h"
 
 namespace osm {
@@ -484,17 +483,16 @@ __global__ __launch_bounds__(256) void join_kernel(Args a, Step st, uint32_t pag
 
 template <bool BF, bool F8>
 bool run_token(const Args& a, const Kv& k, const Step& st, const Cut& c, uint8_t* workspace, hipStream_t stream) {
-  const uint64_t blocks = (uint64_t) c.most * k.heads * c.tiles, rows = (uint64_t) st.n_seq * a.heads;
-  if (blocks > 0x7FFFFFFFull || rows > 0x7FFFFFFFull) return false;
+  const uint32_t blocks = c.most * k.heads * c.tiles;
   auto* kernel = k.page >= 16 ? (c.dim == 64 ? token_kernel<BF, F8, 64, true> : c.dim == 128 ? token_kernel<BF, F8, 128, true> : token_kernel<BF, F8, 256, true>)
                               : (c.dim == 64 ? token_kernel<BF, F8, 64, false> : c.dim == 128 ? token_kernel<BF, F8, 128, false> : token_kernel<BF, F8, 256, false>);
   uint32_t* cut = c.split ? (uint32_t*) workspace : nullptr;
   float* part = (float*) (workspace + c.head);
-  kernel<<<(uint32_t) blocks, 256, 0, stream>>>(a, k, st, c.want, c.tiles, cut, part);
+  kernel<<<blocks, 256, 0, stream>>>(a, k, st, c.want, c.tiles, cut, part);
   if (hipGetLastError() != hipSuccess) return false;
   if (c.split) {
     auto* join = c.dim == 64 ? join_kernel<64> : c.dim == 128 ? join_kernel<128> : join_kernel<256>;
-    join<<<(uint32_t) rows, 256, 0, stream>>>(a, st, k.page, cut, part);
+    join<<<st.n_seq * a.heads, 256, 0, stream>>>(a, st, k.page, cut, part);
   }
   return hipGetLastError() == hipSuccess;
 }
@@ -516,7 +514,8 @@ __host__ __device__ inline bool in_bf16(uint32_t kv_type, uint32_t q_type) { ret
 // 11 % slower, chunks over 8-bit pages 22 %, one of 77 tokens 60 %. that prompt takes 583 us, 943 TFLOP/s of the causal half,
 // where a library product of 8192 x 8192 x 8192 reaches 1187; the matrix units are busy 45 % of the time and the vector units
 // 52 %, and neither reads further ahead, other orders of the phases nor wave priorities changed it.
-constexpr int kKeys = 32, kRowWaves = 4, kRows = 32 * kRowWaves;
+constexpr int kKeys = 32, kRowWaves = 4;
+static_assert(kRows == 32 * kRowWaves);
 enum Source { kPacked, kPages, kPagesF8 };
 
 // a row's scores are taken against its running maximum as it was until one is past it by more than this (in powers of two):
@@ -970,38 +969,11 @@ __global__ __launch_bounds__(256) void rows_join_kernel(Args a, Step st, uint32_
   if (a.lse && d == 0) a.lse[(uint64_t) token * a.heads + head] = (m + log2f(l)) * kLn2;
 }
 
-// how the rows are launched: tiles there can be, and the parts that each tile's keys are cut into: one, but where the tiles
-// leave compute units without work and the keys are many (a part of 256 keys or more, so that it costs more than its join).
-// 923 rows of 24 heads over 7109 tokens of 8-bit pages (184 tiles at most): whole 175 us, for 512 / 768 / 1024 / 1536 / 2048
-// workgroups 131 / 114 / 102 / 96 / 105
-constexpr uint64_t kFull = 1536, kLeastPart = 256;
-struct RowsCut {
-  uint64_t tiles;
-  uint32_t parts, dim;
-};
-inline RowsCut rows_cut(const OsmosAttn* a, uint32_t kv_heads, uint32_t dim, const OsmosKvStep* st) {
-  RowsCut c;
-  c.tiles = (uint64_t) st->n_tok * (a->heads / kv_heads) / kRows + (st->n_seq < st->n_tok ? st->n_seq : st->n_tok);
-  const uint64_t blocks = c.tiles * kv_heads, longest = st->len ? st->max_len : st->max_tok;
-  uint64_t keys = longest;
-  if (a->window && a->window + (uint64_t) kRows + 31 < keys) keys = a->window + (uint64_t) kRows + 31;
-  uint64_t parts = blocks ? kFull / blocks : 1;
-  if (parts > keys / kLeastPart) parts = keys / kLeastPart;
-  c.parts = (uint32_t) (parts < 1 ? 1 : parts > 64 ? 64 : parts);
-  c.dim = dim <= 64 ? 64 : dim <= 128 ? 128 : dim <= 192 ? 192 : 256;
-  return c;
-}
-inline uint64_t rows_bytes(const RowsCut& c, uint32_t kv_heads) {
-  return c.parts > 1 ? c.tiles * kv_heads * c.parts * kRows * (c.dim + 4) * 4 : 0;
-}
-
 template <bool BF, int SRC>
 bool run_rows(const Args& a, const Kv& k, const OsmosKvStep* step, const RowsCut& c, float* part, hipStream_t stream) {
-  const uint64_t blocks = c.tiles * k.heads * c.parts;
-  if (blocks > 0x7FFFFFFFull || (uint64_t) step->n_tok * a.group > 0x7FFFFFFFull) return false;
   const Step st = kv::step_of(step);
   auto* kernel = c.dim == 64 ? rows_kernel<BF, SRC, 64> : c.dim == 128 ? rows_kernel<BF, SRC, 128> : c.dim == 192 ? rows_kernel<BF, SRC, 192> : rows_kernel<BF, SRC, 256>;
-  kernel<<<(uint32_t) blocks, 64 * kRowWaves, 0, stream>>>(a, k, st, c.parts, part);
+  kernel<<<(uint32_t) (c.tiles * k.heads * c.parts), 64 * kRowWaves, 0, stream>>>(a, k, st, c.parts, part);
   if (hipGetLastError() != hipSuccess) return false;
   if (c.parts > 1) {
     const uint32_t pieces = kRows / (c.dim == 64 ? 16 : c.dim == 128 ? 8 : 4);
@@ -1011,20 +983,6 @@ bool run_rows(const Args& a, const Kv& k, const OsmosKvStep* step, const RowsCut
   return hipGetLastError() == hipSuccess;
 }
 
-inline bool room_ok(uint64_t need, const void* workspace, uint64_t bytes) {
-  return !need || (workspace && (uintptr_t) workspace % 256 == 0 && bytes >= need);
-}
-inline bool row_type(uint32_t t) { return t == OSMOS_F32 || t == OSMOS_F16 || t == OSMOS_BF16; }
-inline bool stride_ok(uint64_t stride, uint32_t type) { return stride * kv::size_of(type) % 16 == 0; }
-
-inline bool args_ok(const OsmosAttn* a, uint32_t kv_heads, uint32_t dim) {
-  if (!a || !a->q || !a->out || (uintptr_t) a->q % 16 || (uintptr_t) a->out % 16) return false;
-  if (!row_type(a->q_type) || !row_type(a->out_type) || !a->heads || a->heads > 4096 || a->heads % kv_heads) return false;
-  if (!stride_ok(a->q_stride, a->q_type) || !stride_ok(a->q_head, a->q_type) || !stride_ok(a->out_stride, a->out_type) ||
-      !stride_ok(a->out_head, a->out_type))
-    return false;
-  return a->window <= 0x7FFFFFFFu && a->scale == a->scale && dim;
-}
 inline Args args_of(const OsmosAttn* a, uint32_t kv_heads, uint32_t dim) {
   return Args{(const uint8_t*) a->q, (uint8_t*) a->out, a->lse, a->q_stride, a->q_head, a->out_stride, a->out_head,
               a->q_type, a->out_type, a->heads, a->heads / kv_heads, a->window, dim, a->scale};
@@ -1052,42 +1010,30 @@ extern "C" OSM_API uint64_t osmos_attn_workspace(const OsmosAttn* a, uint32_t kv
 
 extern "C" OSM_API bool osmos_attn_prompt(const OsmosAttn* a, const OsmosKvRows* r, const OsmosKvStep* step,
                                           void* workspace, uint64_t workspace_bytes, void* stream) {
-  if (!r || !r->k || !r->v || !r->heads || r->heads > 4096 || (r->type != OSMOS_F16 && r->type != OSMOS_BF16)) return false;
-  if (!r->dim || r->dim > OSMOS_ATTN_MAX_DIM || r->dim % 16 || (uintptr_t) r->k % 16 || (uintptr_t) r->v % 16) return false;
-  if (r->k_stride % 8 || r->k_head % 8 || r->v_stride % 8 || r->v_head % 8) return false;
-  if (r->k_stride > OSMOS_ATTN_MAX_STRIDE || r->v_stride > OSMOS_ATTN_MAX_STRIDE) return false;
-  if (!attn::args_ok(a, r->heads, r->dim) || !kv::step_ok(step, false)) return false;
+  if (!attn::prompt_ok(a, r, step, workspace, workspace_bytes)) return false;
   const attn::Kv k{(const uint8_t*) r->k, (const uint8_t*) r->v, r->k_stride, r->k_head, r->v_stride, r->v_head, r->type,
                    0, 0, r->heads, nullptr};
-  const attn::RowsCut c = attn::rows_cut(a, r->heads, r->dim, step);
-  if (!attn::room_ok(attn::rows_bytes(c, r->heads), workspace, workspace_bytes)) return false;
   auto* run = r->type == OSMOS_BF16 ? attn::run_rows<true, attn::kPacked> : attn::run_rows<false, attn::kPacked>;
-  return run(attn::args_of(a, r->heads, r->dim), k, step, c, (float*) workspace, (hipStream_t) stream);
+  return run(attn::args_of(a, r->heads, r->dim), k, step, attn::rows_cut(a, r->heads, r->dim, step), (float*) workspace,
+             (hipStream_t) stream);
 }
 
 extern "C" OSM_API bool osmos_attn_chunk(const OsmosAttn* a, const OsmosKv* kv, uint32_t layer, const OsmosKvStep* step,
                                          void* workspace, uint64_t workspace_bytes, void* stream) {
-  if (!kv::cache_ok(kv) || layer >= kv->layers || !attn::args_ok(a, kv->heads, kv->dim) || !kv::step_ok(step, true)) return false;
+  if (!attn::chunk_ok(a, kv, layer, step, workspace, workspace_bytes)) return false;
   const bool bf = attn::in_bf16(kv->type, a->q_type), f8 = kv->type == OSMOS_F8;
   auto* run = bf ? (f8 ? attn::run_rows<true, attn::kPagesF8> : attn::run_rows<true, attn::kPages>)
                  : (f8 ? attn::run_rows<false, attn::kPagesF8> : attn::run_rows<false, attn::kPages>);
-  const attn::RowsCut c = attn::rows_cut(a, kv->heads, kv->dim, step);
-  if (!attn::room_ok(attn::rows_bytes(c, kv->heads), workspace, workspace_bytes)) return false;
-  return run(attn::args_of(a, kv->heads, kv->dim), attn::pages_of(kv, layer), step, c, (float*) workspace, (hipStream_t) stream);
+  return run(attn::args_of(a, kv->heads, kv->dim), attn::pages_of(kv, layer), step, attn::rows_cut(a, kv->heads, kv->dim, step),
+             (float*) workspace, (hipStream_t) stream);
 }
 
 extern "C" OSM_API bool osmos_attn_token(const OsmosAttn* a, const OsmosKv* kv, uint32_t layer, const OsmosKvStep* step,
                                          void* workspace, uint64_t workspace_bytes, void* stream) {
-  if (!kv::cache_ok(kv) || layer >= kv->layers || !attn::args_ok(a, kv->heads, kv->dim) || !kv::step_ok(step, true)) return false;
-  if (step->max_tok != 1) return false;
-  // (a step's tiles are counted in 32 bits)
-  const uint64_t room = (uint64_t) step->table_stride * kv->page, longest = room < step->max_len ? room : step->max_len;
-  if (step->n_seq * (longest / 32 + 1) > 0xFFFFFFFFull) return false;
-  const attn::Cut c = attn::cut_of(a, kv->heads, kv->dim, step);
-  if (!attn::room_ok(attn::token_bytes(a, c), workspace, workspace_bytes)) return false;
+  if (!attn::token_ok(a, kv, layer, step, workspace, workspace_bytes)) return false;
   const bool bf = attn::in_bf16(kv->type, a->q_type), f8 = kv->type == OSMOS_F8;
   auto* run = bf ? (f8 ? attn::run_token<true, true> : attn::run_token<true, false>)
                  : (f8 ? attn::run_token<false, true> : attn::run_token<false, false>);
-  return run(attn::args_of(a, kv->heads, kv->dim), attn::pages_of(kv, layer), kv::step_of(step), c, (uint8_t*) workspace,
-             (hipStream_t) stream);
+  return run(attn::args_of(a, kv->heads, kv->dim), attn::pages_of(kv, layer), kv::step_of(step),
+             attn::cut_of(a, kv->heads, kv->dim, step), (uint8_t*) workspace, (hipStream_t) stream);
 }

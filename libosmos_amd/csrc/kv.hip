@@ -337,18 +337,10 @@ __global__ __launch_bounds__(256) void move_kernel(Pool p, uint8_t* data, uint64
 
 constexpr uint32_t kCopyGrid = 4096;
 
-inline uint64_t page_bytes(const OsmosKv* kv) { return (uint64_t) kv->heads * kv->page * kv->dim * size_of(kv->type); }
-inline uint64_t plane_bytes(const OsmosKv* kv) { return page_bytes(kv) * kv->pages; }
 inline uint32_t parts_of(const OsmosKv* kv) { return (uint32_t) ((page_bytes(kv) + kPart - 1) / kPart); }
 inline uint32_t copy_grid(const OsmosKv* kv, uint64_t pairs) {
   const uint64_t n = pairs * 2 * kv->layers * parts_of(kv);
   return (uint32_t) (n < kCopyGrid ? n : kCopyGrid);
-}
-// scratch: three lists of whole 16-page pieces, then the copy list and the counts
-inline uint64_t list_ints(const OsmosKv* kv) { return (kv->pages + 15ull) / 16 * 16; }
-inline bool pool_ok(const OsmosKv* kv, const OsmosKvPool* p) {
-  return cache_ok(kv) && p && p->ref && (uintptr_t) p->ref % 16 == 0 && p->len && p->table && p->scratch &&
-         (uintptr_t) p->scratch % 16 == 0 && p->seqs && p->seqs <= 0x7FFFFFFFu && p->table_stride;
 }
 inline Pool pool_of(const OsmosKv* kv, const OsmosKvPool* p) {
   return Pool{p->ref, p->len, p->table, kv->pages, kv->page, p->seqs, p->table_stride};
@@ -370,11 +362,7 @@ extern "C" OSM_API uint64_t osmos_kv_bytes(const OsmosKv* kv) {
 
 extern "C" OSM_API bool osmos_kv_append(const OsmosKv* kv, uint32_t layer, const OsmosKvStep* step, uint32_t type,
                                         const void* k, uint64_t k_stride, const void* v, uint64_t v_stride, void* stream) {
-  if (!kv::cache_ok(kv) || layer >= kv->layers || !kv::step_ok(step, true) || !k || !v) return false;
-  if (type != OSMOS_F32 && type != OSMOS_F16 && type != OSMOS_BF16) return false;
-  const uint64_t row = (uint64_t) kv->heads * kv->dim, size = kv::size_of(type);
-  if ((uintptr_t) k % 16 || (uintptr_t) v % 16 || k_stride * size % 16 || v_stride * size % 16) return false;
-  if (step->n_tok > 1 && (k_stride < row || v_stride < row)) return false;
+  if (!kv::append_ok(kv, layer, step, type, k, k_stride, v, v_stride)) return false;
   const uint64_t plane = kv::plane_bytes(kv);
   auto* kernel = type == OSMOS_F32 ? kv::append_to<OSMOS_F32>(kv->type) : type == OSMOS_F16 ? kv::append_to<OSMOS_F16>(kv->type) : kv::append_to<OSMOS_BF16>(kv->type);
   kernel<<<(step->n_tok + kv::kAppendRows - 1) / kv::kAppendRows, 64 * kv::kAppendRows, 0, (hipStream_t) stream>>>(
@@ -389,7 +377,7 @@ extern "C" OSM_API uint64_t osmos_kv_scratch(const OsmosKv* kv) {
 
 extern "C" OSM_API bool osmos_kv_grow(const OsmosKv* kv, const OsmosKvPool* pool, const int32_t* seq, const int32_t* add,
                                       uint32_t n, int32_t* done, void* stream) {
-  if (!kv::pool_ok(kv, pool) || !seq || !add || !n || n > OSMOS_KV_MAX_REQUESTS) return false;
+  if (!kv::requests_ok(kv, pool, seq, add, n)) return false;
   int32_t* list = (int32_t*) pool->scratch;
   int2* copies = (int2*) (list + 3 * kv::list_ints(kv));
   kv::grow_kernel<<<1, kv::kPoolThreads, 0, (hipStream_t) stream>>>(kv::pool_of(kv, pool), seq, add, n, list, copies, done);
@@ -402,14 +390,14 @@ extern "C" OSM_API bool osmos_kv_grow(const OsmosKv* kv, const OsmosKvPool* pool
 
 extern "C" OSM_API bool osmos_kv_fork(const OsmosKv* kv, const OsmosKvPool* pool, const int32_t* from, const int32_t* to,
                                       uint32_t n, int32_t* done, void* stream) {
-  if (!kv::pool_ok(kv, pool) || !from || !to || !n || n > OSMOS_KV_MAX_REQUESTS) return false;
+  if (!kv::requests_ok(kv, pool, from, to, n)) return false;
   kv::fork_kernel<<<n, 256, 0, (hipStream_t) stream>>>(kv::pool_of(kv, pool), from, to, n, done);
   return hipGetLastError() == hipSuccess;
 }
 
 extern "C" OSM_API bool osmos_kv_free(const OsmosKv* kv, const OsmosKvPool* pool, const int32_t* seq, uint32_t n,
                                       void* stream) {
-  if (!kv::pool_ok(kv, pool) || !seq || !n || n > OSMOS_KV_MAX_REQUESTS) return false;
+  if (!kv::requests_ok(kv, pool, seq, seq, n)) return false;
   kv::free_kernel<<<n, 256, 0, (hipStream_t) stream>>>(kv::pool_of(kv, pool), seq);
   return hipGetLastError() == hipSuccess;
 }
@@ -427,7 +415,7 @@ extern "C" OSM_API bool osmos_kv_compact(const OsmosKv* kv, const OsmosKvPool* p
 }
 
 extern "C" OSM_API bool osmos_kv_copy(const OsmosKv* kv, const int32_t* from, const int32_t* to, uint32_t n, void* stream) {
-  if (!kv::cache_ok(kv) || !from || !to || !n) return false;
+  if (!kv::copy_ok(kv, from, to, n)) return false;
   kv::copy_kernel<<<kv::copy_grid(kv, n), 256, 0, (hipStream_t) stream>>>(
       (uint8_t*) kv->data, kv::page_bytes(kv), kv::plane_bytes(kv), 2 * kv->layers, kv::parts_of(kv), kv->pages, from, to, 1, n);
   return hipGetLastError() == hipSuccess;

@@ -2,11 +2,8 @@
 // the cache's and the callers' types, and a step's sequences as the device memory says they are, clamped so that no table
 // leads a kernel out of its buffers.
 #pragma once
+#include "attnhost.h"
 #include "common.h"
-
-extern "C" {
-#include "../../include/osmos_attn.h"
-}
 
 namespace osm {
 namespace kv {
@@ -16,8 +13,6 @@ typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
-
-__host__ __device__ constexpr uint32_t size_of(uint32_t type) { return type == OSMOS_F32 ? 4 : type == OSMOS_F8 ? 1 : 2; }
 
 // 8 consecutive values as floats
 template <uint32_t T>
@@ -138,24 +133,6 @@ __device__ inline bool sequence_of(const Step& st, int t, uint32_t page, Seq& q)
   return true;
 }
 
-inline bool shape_ok(const OsmosKv* kv) {
-  if (!kv || (kv->type != OSMOS_F16 && kv->type != OSMOS_BF16 && kv->type != OSMOS_F8)) return false;
-  if (!kv->layers || kv->layers > 4096 || !kv->pages || kv->pages > 0x7FFFFFF0u || !kv->heads || kv->heads > 4096) return false;
-  if (!kv->page || kv->page > OSMOS_KV_MAX_PAGE || (kv->page & (kv->page - 1))) return false;
-  return kv->dim && kv->dim <= OSMOS_ATTN_MAX_DIM && kv->dim % 16 == 0 &&
-         (uint64_t) kv->heads * kv->page * kv->dim <= OSMOS_KV_MAX_PAGE_VALUES;
-}
-inline bool cache_ok(const OsmosKv* kv) {
-  return shape_ok(kv) && kv->data && (uintptr_t) kv->data % 16 == 0 && (kv->type == OSMOS_F8 || !kv->scale);
-}
-inline bool step_ok(const OsmosKvStep* st, bool paged) {
-  if (!st || !st->start || !st->n_seq || st->n_seq > 0x100000u || !st->n_tok || st->n_tok > 0x7FFFFFFFu || !st->max_tok ||
-      st->max_tok > 0x7FFFFFFFu)
-    return false;
-  if (!paged) return true;
-  return st->len && st->table && st->table_stride && st->seqs && (st->seq || st->n_seq <= st->seqs) && st->max_len &&
-         st->max_len <= 0x7FFF0000u;
-}
 inline Step step_of(const OsmosKvStep* st) {
   return Step{st->start, st->len, st->table, st->seq, st->live, st->n_seq, st->n_tok, st->max_len, st->seqs, st->table_stride};
 }
