@@ -9,6 +9,10 @@ import ctypes
 from . import attn, capi
 
 
+class _Calls(tuple):
+    """a step's (append, attention), with the layer and the buffers that they were made for"""
+
+
 class AttentionLayer:
     def __init__(self, cache, layer, heads, wq, wk, wv, wo, dim):
         """cache: attn.KvCache; layer: its layer here; heads: query heads; wq, wk, wv, wo: (GGUF type, uint8 device tensor),
@@ -39,12 +43,22 @@ class AttentionLayer:
         """the append and the attention of a step, bound to this layer's buffers of its size (made once a KvStep)"""
         b = self._buffers(step.n_tok)
         kind = attn.TokenAttention if step.desc.max_tok == 1 else attn.ChunkAttention
-        return attn.Append(self.cache, self.layer, step, b["k"], b["v"]), kind(self.cache, self.layer, step, b["q"], b["o"])
+        calls = _Calls((attn.Append(self.cache, self.layer, step, b["k"], b["v"]),
+                        kind(self.cache, self.layer, step, b["q"], b["o"])))
+        calls.owner, calls.buffers, calls.n = self, b, step.n_tok
+        return calls
 
     def forward(self, x, calls, out, stream=None):
-        """out (n, dim) = the block's attention of x (n, dim), float32, for the step that `calls` were made for"""
-        L, n = capi.lib(), x.shape[0]
-        b, append, attention = self._buffers(n), *calls
+        """out (n, dim) = the block's attention of x (n, dim), contiguous float32, for the step that `calls` were made for"""
+        import torch
+        if getattr(calls, "owner", None) is not self:
+            raise ValueError("AttentionLayer.forward: calls of another layer")
+        for t, name in ((x, "x"), (out, "out")):
+            if t.dtype != torch.float32 or not t.is_contiguous() or not t.is_cuda:
+                raise TypeError("AttentionLayer.forward: %s is a contiguous float32 device tensor" % name)
+            if tuple(t.shape) != (calls.n, self.dim):
+                raise ValueError("AttentionLayer.forward: %s is (rows of the step, dim)" % name)
+        L, n, b, (append, attention) = capi.lib(), calls.n, calls.buffers, calls
 
         def need(ok, what):
             if not ok:

@@ -1,0 +1,48 @@
+"""AttentionLayer's steps and their buffers (libosmos_amd.block): a step runs on the rows and buffers that its calls were made for."""
+import pytest
+
+pytestmark = pytest.mark.gpu
+
+torch = pytest.importorskip("torch")
+
+from tests.test_block_gpu import DIM, HD, HEADS, KV, PAGE, _ints, _weights  # noqa: E402
+
+
+def _layer(pages=60, seqs=2):
+    from libosmos_amd import attn
+    from libosmos_amd.block import AttentionLayer
+    w = [_weights(r, c, i)[0] for i, (r, c) in enumerate(((HEADS * HD, DIM), (KV * HD, DIM), (KV * HD, DIM), (DIM, HEADS * HD)))]
+    cache = attn.KvCache.empty(torch.float16, 1, pages, KV, PAGE, HD)
+    pool = attn.KvPool.empty(cache, seqs, 40 * PAGE)
+    return cache, pool, AttentionLayer(cache, 0, HEADS, *w, DIM)
+
+
+def _step(pool, rows):
+    from libosmos_amd import attn
+    starts = [sum(rows[:i]) for i in range(len(rows) + 1)]
+    return attn.KvStep(_ints(starts), pool.len, pool.table, n_tok=sum(rows), max_tok=max(rows), max_len=40 * PAGE)
+
+
+def test_rows_of_another_step_are_refused():
+    cache, pool, layer = _layer()
+    pool.grow(_ints([0, 1]), _ints([3, 1]))
+    calls = layer.calls(_step(pool, [3, 1]))
+    layer.calls(_step(pool, [1, 1]))
+    x, out = (torch.zeros((4, DIM), device="cuda") for _ in range(2))
+    torch.cuda.synchronize()
+    before = cache.data.clone()
+    wide = torch.zeros((4, 2 * DIM), device="cuda")
+    bad = [(x[:2], out[:2]), (x[:2], out), (x, out[:3]), (x.half(), out), (x, out.half()), (x.double(), out), (wide[:, :DIM], out),
+           (x, wide[:, :DIM]), (x.T.contiguous().T, out), (x.cpu(), out), (x.view(2, 2 * DIM), out), (x.view(-1), out)]
+    for a, b in bad:
+        print("refused", tuple(a.shape), a.dtype, tuple(b.shape), b.dtype, flush=True)
+        with pytest.raises((TypeError, ValueError)):
+            layer.forward(a, calls, b)
+    other = _layer()[2]
+    with pytest.raises(ValueError):
+        other.forward(x, calls, out)
+    torch.cuda.synchronize()
+    assert torch.equal(cache.data, before)
+    layer.forward(x, calls, out)
+    torch.cuda.synchronize()
+    assert (out == 0).all()
