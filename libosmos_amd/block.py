@@ -16,7 +16,10 @@ class _Calls(tuple):
 class AttentionLayer:
     def __init__(self, cache, layer, heads, wq, wk, wv, wo, dim):
         """cache: attn.KvCache; layer: its layer here; heads: query heads; wq, wk, wv, wo: (GGUF type, uint8 device tensor),
-        rows heads x cache.dim (wq), cache.heads x cache.dim (wk, wv) of dim values, dim rows of heads x cache.dim (wo)"""
+        rows heads x cache.dim (wq), cache.heads x cache.dim (wk, wv) of dim values, dim rows of heads x cache.dim (wo).
+        overflow: an int32 device value, set to 1 by a step whose x or attention rows are past f16's range (they become
+        infinities in the products) and left so for the caller to read and clear"""
+        import torch
         self.cache, self.layer, self.heads, self.dim = cache, layer, heads, dim
         self.w, self.wo = ((wq, heads * cache.dim), (wk, cache.heads * cache.dim), (wv, cache.heads * cache.dim)), wo
         for (t, _), rows in self.w:
@@ -24,6 +27,7 @@ class AttentionLayer:
                 raise ValueError("AttentionLayer: mm does not take %d x %d of type %d" % (rows, dim, t))
         if not capi.lib().mm_fits(wo[0], dim, heads * cache.dim):
             raise ValueError("AttentionLayer: mm does not take the output matrix")
+        self.overflow = torch.zeros(1, dtype=torch.int32, device="cuda")
         self._made = {}
 
     def _buffers(self, n):
@@ -31,10 +35,10 @@ class AttentionLayer:
         if n not in self._made:
             hd, rows = self.cache.dim, self.heads + 2 * self.cache.heads
             tiles = (n + 15) // 16 * 16
-            b = {"qkv": torch.empty((n, rows, hd), device="cuda"), "o": torch.empty((n, self.heads, hd), device="cuda"),
+            # (o zeros: a row that belongs to no sequence of the step is not written)
+            b = {"qkv": torch.empty((n, rows, hd), device="cuda"), "o": torch.zeros((n, self.heads, hd), device="cuda"),
                  "x16": torch.empty(tiles * self.dim, dtype=torch.float16, device="cuda"),
-                 "o16": torch.empty(tiles * self.heads * hd, dtype=torch.float16, device="cuda"),
-                 "overflow": torch.zeros(1, dtype=torch.int32, device="cuda")}
+                 "o16": torch.empty(tiles * self.heads * hd, dtype=torch.float16, device="cuda")}
             b["q"], b["k"], b["v"] = b["qkv"].split([self.heads, self.cache.heads, self.cache.heads], 1)
             self._made[n] = b
         return self._made[n]
@@ -63,7 +67,7 @@ class AttentionLayer:
         def need(ok, what):
             if not ok:
                 raise RuntimeError("%s refused" % what)
-        need(L.mm_x16(capi.addr(x), self.dim, n, self.dim, capi.addr(b["x16"]), capi.addr(b["overflow"]), stream), "mm_x16")
+        need(L.mm_x16(capi.addr(x), self.dim, n, self.dim, capi.addr(b["x16"]), capi.addr(self.overflow), stream), "mm_x16")
         stride = b["qkv"].stride(0)
         for ((t, w), rows), y in zip(self.w, (b["q"], b["k"], b["v"])):
             need(L.mm_run(t, capi.addr(w), rows, self.dim, capi.addr(b["x16"]), n, ctypes.c_void_p(y.data_ptr()), stride,
@@ -71,7 +75,7 @@ class AttentionLayer:
         append.run(stream)
         attention.run(stream)
         cols = self.heads * self.cache.dim
-        need(L.mm_x16(capi.addr(b["o"]), cols, n, cols, capi.addr(b["o16"]), capi.addr(b["overflow"]), stream), "mm_x16")
+        need(L.mm_x16(capi.addr(b["o"]), cols, n, cols, capi.addr(b["o16"]), capi.addr(self.overflow), stream), "mm_x16")
         need(L.mm_run(self.wo[0], capi.addr(self.wo[1]), self.dim, cols, capi.addr(b["o16"]), n, capi.addr(out), self.dim,
                       stream), "mm_run")
         return out

@@ -46,3 +46,35 @@ def test_rows_of_another_step_are_refused():
     layer.forward(x, calls, out)
     torch.cuda.synchronize()
     assert (out == 0).all()
+
+
+def test_overflow_is_reported():
+    """layer.overflow: 0 while every row fits f16, 1 once one does not, until the caller clears it"""
+    cache, pool, layer = _layer()
+    pool.grow(_ints([0, 1]), _ints([2, 2]))
+    calls = layer.calls(_step(pool, [2, 2]))
+    out = torch.empty((4, DIM), device="cuda")
+    for value, want in ((1.0, 0), (65504.0, 0), (65510.0, 1), (1.0, 1)):
+        x = torch.zeros((4, DIM), device="cuda")
+        x[2, 7] = value
+        layer.forward(x, calls, out)
+        torch.cuda.synchronize()
+        assert layer.overflow.tolist() == [want], value
+    layer.overflow.zero_()
+    layer.forward(x, calls, out)
+    torch.cuda.synchronize()
+    assert layer.overflow.tolist() == [0]
+
+
+def test_rows_of_no_sequence_stay_finite():
+    """rows that a step's sequences leave out (a batch padded to one size) reach neither the cache nor the overflow flag"""
+    from libosmos_amd import attn
+    cache, pool, layer = _layer()
+    pool.grow(_ints([0, 1]), _ints([1, 1]))
+    junk = torch.full((1 << 20,), float("inf"), device="cuda")  # (what new buffers may be made of)
+    del junk
+    step = attn.KvStep(_ints([0, 1, 2]), pool.len, pool.table, n_tok=16, max_tok=1, max_len=40 * PAGE)
+    x, out = torch.randn((16, DIM), device="cuda"), torch.empty((16, DIM), device="cuda")
+    layer.forward(x, layer.calls(step), out)
+    torch.cuda.synchronize()
+    assert layer.overflow.tolist() == [0] and torch.isfinite(out).all()
