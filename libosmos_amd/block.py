@@ -1,8 +1,9 @@
 """A decoder block's attention over quantized projections, for Python callers: the query, key, value and output matrices in
 GGUF row layout (mm_run), the step's keys and values into the paged cache (osmos_kv_append), attention over the cache
 (osmos_attn_token for a step of single tokens, osmos_attn_chunk for prompts). What follows it in a block is
-layer.LaneLayer (the routed experts). Rows are float32 as the library's products have them; buffers are made once a step
-shape and reused; nothing here computes.
+layer.LaneLayer (the routed experts). Rows are float32 as the library's products have them; a layer keeps one set of buffers, of
+its longest step, that all its steps use: they are ordered on one stream, and a second stream takes a layer object of its
+own. Nothing here computes.
 """
 import ctypes
 
@@ -28,23 +29,26 @@ class AttentionLayer:
         if not capi.lib().mm_fits(wo[0], dim, heads * cache.dim):
             raise ValueError("AttentionLayer: mm does not take the output matrix")
         self.overflow = torch.zeros(1, dtype=torch.int32, device="cuda")
-        self._made = {}
+        self._made, self._rows = {}, 0
 
     def _buffers(self, n):
+        """a step's rows of the one set of buffers, which the longest step so far made"""
         import torch
-        if n not in self._made:
-            hd, rows = self.cache.dim, self.heads + 2 * self.cache.heads
+        hd, kv = self.cache.dim, self.cache.heads
+        if n > self._rows:
             tiles = (n + 15) // 16 * 16
             # (o zeros: a row that belongs to no sequence of the step is not written)
-            b = {"qkv": torch.empty((n, rows, hd), device="cuda"), "o": torch.zeros((n, self.heads, hd), device="cuda"),
-                 "x16": torch.empty(tiles * self.dim, dtype=torch.float16, device="cuda"),
-                 "o16": torch.empty(tiles * self.heads * hd, dtype=torch.float16, device="cuda")}
-            b["q"], b["k"], b["v"] = b["qkv"].split([self.heads, self.cache.heads, self.cache.heads], 1)
-            self._made[n] = b
-        return self._made[n]
+            self._made = {"qkv": torch.empty((n, self.heads + 2 * kv, hd), device="cuda"),
+                          "o": torch.zeros((n, self.heads, hd), device="cuda"),
+                          "x16": torch.empty(tiles * self.dim, dtype=torch.float16, device="cuda"),
+                          "o16": torch.empty(tiles * self.heads * hd, dtype=torch.float16, device="cuda")}
+            self._rows = n
+        b = dict(self._made, o=self._made["o"][:n])
+        b["q"], b["k"], b["v"] = b["qkv"][:n].split([self.heads, kv, kv], 1)
+        return b
 
     def calls(self, step):
-        """the append and the attention of a step, bound to this layer's buffers of its size (made once a KvStep)"""
+        """the append and the attention of a step, bound to its rows of this layer's buffers (made once a KvStep)"""
         b = self._buffers(step.n_tok)
         kind = attn.TokenAttention if step.desc.max_tok == 1 else attn.ChunkAttention
         calls = _Calls((attn.Append(self.cache, self.layer, step, b["k"], b["v"]),

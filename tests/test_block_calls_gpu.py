@@ -78,3 +78,41 @@ def test_rows_of_no_sequence_stay_finite():
     layer.forward(x, layer.calls(step), out)
     torch.cuda.synchronize()
     assert layer.overflow.tolist() == [0] and torch.isfinite(out).all()
+
+
+def test_one_set_of_buffers():
+    """prompts of many lengths: the layer keeps the buffers of the longest, and calls made before and after it run right on their own"""
+    cache, pool, layer = _layer(pages=200, seqs=1)
+    pool.grow(_ints([0]), _ints([640]))
+    cache.data.copy_(torch.randn(cache.data.shape, device="cuda"))
+    a_row = (HEADS + 2 * KV + HEADS) * HD * 4 + (DIM + HEADS * HD) * 2
+    first, outs = layer.calls(_step(pool, [3])), {}
+    x = torch.randn((640, DIM), device="cuda")
+    torch.cuda.synchronize()
+    start = torch.cuda.memory_allocated()
+    for n in range(1, 641, 9):
+        layer.calls(_step(pool, [n]))
+    kept = torch.cuda.memory_allocated() - start
+    assert kept <= 1.1 * 656 * a_row + (1 << 20), "%d bytes kept where one set of 640 rows is %d" % (kept, 640 * a_row)
+
+    def run(calls, n):
+        out = torch.full((n, DIM), float("nan"), device="cuda")
+        layer.forward(x[:n], calls, out)
+        torch.cuda.synchronize()
+        return out
+    late = {n: layer.calls(_step(pool, [n])) for n in (3, 640, 17)}
+    alone = {n: _layer_like(layer, cache) for n in (3, 640, 17)}
+    for n in (3, 640, 17, 3):
+        other = torch.full((n, DIM), float("nan"), device="cuda")
+        alone[n].forward(x[:n], alone[n].calls(_step(pool, [n])), other)
+        torch.cuda.synchronize()
+        outs[n] = other
+        assert torch.equal(run(late[n], n), other), n
+    alone[3].forward(x[:3], alone[3].calls(_step(pool, [3])), outs[3])  # (the tokens of the last step again)
+    torch.cuda.synchronize()
+    assert torch.equal(run(first, 3), outs[3])
+
+
+def _layer_like(layer, cache):
+    from libosmos_amd.block import AttentionLayer
+    return AttentionLayer(cache, 0, HEADS, *[w for w, _ in layer.w], layer.wo, DIM)
