@@ -56,8 +56,10 @@ class AttentionLayer:
         calls.owner, calls.buffers, calls.n = self, b, step.n_tok
         return calls
 
-    def forward(self, x, calls, out, stream=None):
-        """out (n, dim) = the block's attention of x (n, dim), contiguous float32, for the step that `calls` were made for"""
+    def forward(self, x, calls, out, stream=None, between=None):
+        """out (n, dim) = the block's attention of x (n, dim), contiguous float32, for the step that `calls` were made for.
+        between(q, k, v, stream): queues on the stream what the model does to the projections' rows, in place, before the keys
+        and values go into the cache (rotary positions, norms, biases): float32 views (n, heads, cache.dim)"""
         import torch
         if getattr(calls, "owner", None) is not self:
             raise ValueError("AttentionLayer.forward: calls of another layer")
@@ -76,6 +78,8 @@ class AttentionLayer:
         for ((t, w), rows), y in zip(self.w, (b["q"], b["k"], b["v"])):
             need(L.mm_run(t, capi.addr(w), rows, self.dim, capi.addr(b["x16"]), n, ctypes.c_void_p(y.data_ptr()), stride,
                           stream), "mm_run")
+        if between:
+            between(b["q"], b["k"], b["v"], stream)
         append.run(stream)
         attention.run(stream)
         cols = self.heads * self.cache.dim

@@ -116,3 +116,51 @@ def test_one_set_of_buffers():
 def _layer_like(layer, cache):
     from libosmos_amd.block import AttentionLayer
     return AttentionLayer(cache, 0, HEADS, *[w for w, _ in layer.w], layer.wo, DIM)
+
+
+def _rotate(x, pos):
+    """rotary positions: pairs (i, i + HD / 2) turned by pos 10000^(-2 i / HD), in place"""
+    half = x.shape[-1] // 2
+    angle = pos[:, None].double() * 10000.0 ** (-2.0 * torch.arange(half, device="cuda").double() / x.shape[-1])
+    c, s = angle.cos()[:, None].to(x.dtype), angle.sin()[:, None].to(x.dtype)
+    a, b = x[..., :half].clone(), x[..., half:].clone()
+    x[..., :half], x[..., half:] = a * c - b * s, a * s + b * c
+
+
+@pytest.mark.parametrize("rows", [1, 40])
+def test_positions_between_projections_and_cache(rows):
+    """a step with rotary positions on its queries and keys: the cache holds the turned keys, and the outputs are those of the same
+    rows turned and attended call by call"""
+    from libosmos_amd import attn
+    cache, pool, layer = _layer(seqs=2)
+    cache.data.copy_(torch.randn(cache.data.shape, device="cuda"))
+    pool.grow(_ints([0, 1]), _ints([77, 300]))
+    step = _step(pool, [rows, rows])
+    n = 2 * rows
+    pos = torch.cat([torch.arange(m - rows, m, device="cuda") for m in (77, 300)])
+    x, plain, out = torch.randn((n, DIM), device="cuda"), torch.empty((n, DIM), device="cuda"), torch.empty((n, DIM), device="cuda")
+    calls = layer.calls(step)
+    before = cache.data.clone()
+    layer.forward(x, calls, plain)
+    torch.cuda.synchronize()
+    # the projections' rows as the plain step left them
+    q, k, v = (calls.buffers[w].clone() for w in "qkv")
+    cache.data.copy_(before)
+    seen = []
+
+    def between(q, k, v, stream):
+        seen.append((tuple(q.shape), tuple(k.shape), tuple(v.shape), stream))
+        _rotate(q, pos), _rotate(k, pos)
+    layer.forward(x, calls, out, between=between)
+    torch.cuda.synchronize()
+    assert seen == [((n, HEADS, HD), (n, KV, HD), (n, KV, HD), None)]
+    _rotate(q, pos), _rotate(k, pos)
+    got = cache.data.clone()
+    cache.data.copy_(before)
+    o = torch.empty((n, HEADS, HD), device="cuda")
+    attn.Append(cache, 0, step, k, v).run()
+    (attn.TokenAttention if rows == 1 else attn.ChunkAttention)(cache, 0, step, q, o).run()
+    torch.cuda.synchronize()
+    assert torch.equal(got, cache.data) and not torch.equal(got, before)
+    assert torch.equal(calls.buffers["o"], o)
+    assert torch.isfinite(out).all() and not torch.equal(out, plain)
