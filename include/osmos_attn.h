@@ -62,7 +62,7 @@ uint64_t osmos_kv_bytes(const OsmosKv *kv);
 
 /* the step's rows into the pages: k and v n_tok rows of heads x dim values of `type` (F32, F16 or BF16; row t at
    k + t k_stride values, 16-byte aligned rows), each value rounded once to the cache's type (nearest, ties to even;
-   F8: of value / scale, saturating; NaN stays NaN). */
+   F8: the float quotient value / scale, saturating; NaN stays NaN). */
 bool osmos_kv_append(const OsmosKv *kv, uint32_t layer, const OsmosKvStep *step, uint32_t type, const void *k,
                      uint64_t k_stride, const void *v, uint64_t v_stride, void *stream);
 
@@ -71,7 +71,8 @@ bool osmos_kv_append(const OsmosKv *kv, uint32_t layer, const OsmosKvStep *step,
    last `window` of them. a row that sees none gets zeros. lse (may be NULL): n_tok x heads, the logarithm of the
    row's sum of exp(scale q k), -infinity for a row that sees none. what is masked has no influence, infinities and NaN
    among it. q and out F32, F16 or BF16. products on the matrix units in the keys' type (F8: q's, F16 for F32), sums
-   and softmax in F32: an F32 q and the probabilities are rounded to that type first. */
+   and softmax in F32: an F32 q and the probabilities (times a power of two in F16) are rounded to that type first, a q past
+   F16's range to an infinity. */
 typedef struct OsmosAttn
 {
   const void *q;
@@ -101,7 +102,8 @@ bool osmos_attn_prompt(const OsmosAttn *a, const OsmosKvRows *kv, const OsmosKvS
 /* rows over the cache (the step's own among its tokens: osmos_kv_append goes first) */
 bool osmos_attn_chunk(const OsmosAttn *a, const OsmosKv *kv, uint32_t layer, const OsmosKvStep *step, void *workspace,
                       uint64_t workspace_bytes, void *stream);
-/* osmos_attn_chunk where every sequence brings one row or none (max_tok 1): the cache read once, split over its length.
+/* osmos_attn_chunk where every sequence brings one row or none (max_tok 1): the cache read once for each 16 query heads of a kv
+   head, split over its length.
    refused: n_seq sequences of max_len tokens, or of what a table row holds, past 2^32 tiles of 32 tokens */
 bool osmos_attn_token(const OsmosAttn *a, const OsmosKv *kv, uint32_t layer, const OsmosKvStep *step, void *workspace,
                       uint64_t workspace_bytes, void *stream);

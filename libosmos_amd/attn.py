@@ -2,6 +2,11 @@
 are the memory, each call one call of the C ABI on the given stream. The objects bind a call to its buffers once - a
 serving program makes them with its buffers and runs them every step, eagerly or under graph capture; nothing here
 computes.
+
+Streams: a call is queued on the hipStream_t given as `stream`, on the null stream for None - never on torch's current stream by
+itself, so that inside torch.cuda.stream(s) s.cuda_stream is passed. What a call or a pool allocates (workspaces, scratch) comes from
+torch's allocator for the stream current when the object is made and lives as long as the object: keep that until the work that
+it queued elsewhere is done. Calls that share an object run in order on one stream.
 """
 import ctypes
 

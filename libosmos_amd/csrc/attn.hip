@@ -149,7 +149,7 @@ __device__ inline float finite_max(float m) { return m == -__builtin_inff() ? 0.
 // ids of the one after. with pages of 16 tokens or more (WIDE) half a tile lies in one page, so that its place is the
 // wave's and not a lane's: scalar loads and arithmetic, where smaller pages take some 60 vector instructions a tile.
 // no load is conditional: a place that is masked reads a row that exists and its score and value are then replaced.
-// bound by memory: one sequence of 131072 tokens (8 kv heads of 128, bf16) 93 us for 537 MB, 5.8 TB/s; 256 of 4096 6.05 TB/s (a
+// bound by memory: one sequence of 131072 tokens (8 kv heads of 128, bf16) 93 us for 537 MB, 5.8 TB/s (a
 // streaming read reaches 7.2). a short step is a chain of loads: lengths, page ids, rows, some 1.7 us a tile of a wave's.
 // two tiles in flight a wave instead of one (244 registers) measured the same, three workgroups a compute unit (10 spilled
 // registers) 14 % slower.

@@ -66,11 +66,13 @@ constexpr uint32_t chunk_keys(uint32_t total, uint32_t want) {
 // the chunks of a sequence of k keys
 constexpr uint32_t chunks_of(int k, uint32_t chunk) { return (uint32_t) k <= chunk ? 1 : ((uint32_t) k + chunk - 1) / chunk; }
 
-// how a token step is launched: the chunks that the sequences are cut into for each kv head and 16 of its query heads (the
-// chip holds 512 of their workgroups; 512 / 768 / 1024 / 2048 wanted measured 99 / 100 / 106 / 112 us for one sequence of 131072 and
-// 44 / 45 / 43 / 50 for 64 of 1 to 8192; chunks of at least 256 / 384 / 512 keys 9.3 / 6.4 / 6.4 us for one of 333, which
-// then needs no join, and 20 / 17 / 17.5 for 24 wide 8-bit ones), and the workspace: where each sequence's chunks begin and
-// how many they are, then the chunks' results
+// how a token step is launched: the chunks that the sequences are cut into for each kv head and 16 of its query heads, and the
+// workspace: where each sequence's chunks begin and how many they are, then the chunks' results. 512 workgroups are what the
+// chip holds of the instances for 16-bit heads of 128 and 8-bit ones of 256, two a compute unit (16-bit 256: one, 8-bit 128:
+// three, heads of 64: four or five). 512 / 768 / 1024 / 2048 wanted measured 99 / 100 / 106 / 112 us for one sequence of 131072
+// and 44 / 45 / 43 / 50 for 64 of 1 to 8192, both 16-bit heads of 128; the other instances take the same number unmeasured. chunks
+// of at least 256 / 384 / 512 keys 9.3 / 6.4 / 6.4 us for one of 333, which then needs no join, and 20 / 17 / 17.5 for 24 8-bit
+// ones of heads of 256
 constexpr uint32_t kWant = 512;
 struct Cut {
   uint32_t want, most, tiles, dim;  // most: chunks there can be
@@ -98,7 +100,7 @@ constexpr int kRows = 128;  // query rows a workgroup of rows_kernel
 // how the rows are launched: tiles there can be, and the parts that each tile's keys are cut into: one, but where the tiles
 // leave compute units without work and the keys are many (a part of 256 keys or more, so that it costs more than its join).
 // 923 rows of 24 heads over 7109 tokens of 8-bit pages (184 tiles at most): whole 175 us, for 512 / 768 / 1024 / 1536 / 2048
-// workgroups 131 / 114 / 102 / 96 / 105
+// workgroups 131 / 114 / 102 / 96 / 105; other head sizes and page types take the same number unmeasured
 constexpr uint64_t kFull = 1536, kLeastPart = 256;
 struct RowsCut {
   uint64_t tiles;

@@ -7,13 +7,15 @@ namespace kv {
 
 // ---- append. a wave a row: its lanes take the row's 8-value pieces of k and v in turn, the loads of four in flight while
 // the row's sequence and page are looked up (start, len and table are a chain of dependent loads, the rows themselves are
-// not). 48 rows of 2 x 8 x 128 floats: 3.3 us, the launch and that chain; 8256 rows of 2 x 4 x 128 bf16 into 8 bits: 10.0 us
+// not). 48 rows of 2 x 8 x 128 floats: 3.7 us, the launch and that chain; 8256 rows of 2 x 4 x 128 bf16 into 8 bits: 9.2 us
 // for 25 MB, the same chain in every wave of the one round that the chip holds ----
 constexpr int kAppendRows = 4;  // rows (waves) a workgroup
 
 // x / f, each quotient rounded to nearest as a division's, for what is then saturated at 448: by f's reciprocal r, rounded to
-// nearest, and q + r (x - f q), exact in its remainder (Markstein's theorem). values past 1000 f, infinities among them, are
-// taken as that. three instructions a value where a division is some twelve: 8256 rows of 2 x 4 x 128 10.7 -> 10.0 us
+// nearest, and q + r (x - f q), exact in its remainder (Markstein's theorem; q may be more than one step off, which it does not
+// cover: on the host every mantissa of f with the seven x around each of e4m3's edges and 1.5e9 random pairs gave the division's
+// bits). values past 1000 f, infinities among them, are taken as that. three instructions a value where a division is some
+// twelve: 8256 rows of 2 x 4 x 128 10.7 -> 10.0 us
 __device__ inline void divide8(float (&x)[8], float f) {
   const float size = fabsf(f);
   if (size > 0x1p-60f && size < 0x1p60f) {
