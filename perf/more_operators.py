@@ -7,7 +7,8 @@ operator, in its plain form (elementary torch operations in float32; angles, and
 choice's border, in float64) or, with `own`, through libosmos_amd.rows; exact() is the same from the definition in float64.
 
 Notation: a norm's rows are n x dim. Tiles are mm's: token t's column c at (t / 16) 16 dim + (c / 16) 256 + (t % 16) 16 + c % 16,
-zeros up to a whole tile of tokens. Codes are the lane's: 32 values a scale, scale = largest / 127. A rotary pair is (i, i + rot / 2)
+zeros up to a whole tile of tokens. A row's tokens are chosen from in the order of their logits, the greatest first, the lower
+index first among equals. Codes are the lane's: 32 values a scale, scale = largest / 127. A rotary pair is (i, i + rot / 2)
 in the half layout, (2 i, 2 i + 1) with `pairs`; what follows the first rot values of a head stays as it is. A step's rows,
 lengths, tables and cache are those of perf/operators.py.
 """
@@ -388,13 +389,13 @@ def _sample(s):
     keep &= w >= s["min_p"].double()[:, None]
     keep[:, 0] = True
     keep &= ~greedy | (rank == 0)
-    w = torch.zeros_like(w).scatter_(1, order, w * keep)  # back in the tokens' order
+    w = w * keep
     c = w.cumsum(1)
     total = c[:, -1:]
-    token = (c <= s["u"].double()[:, None] * total).sum(1, keepdim=True)
-    prob = w.gather(1, token) / total
+    at = (c <= s["u"].double()[:, None] * total).sum(1, keepdim=True)  # the first whose running sum passes u of the whole
+    token, prob = order.gather(1, at), w.gather(1, at) / total
     out = token[:, 0].to(torch.int32), prob[:, 0].float(), keep.sum(1).to(torch.int32)
-    return out + ((w / total).float(),) if s["case"]["probs"] else out
+    return out + (torch.zeros_like(w).scatter_(1, order, w / total).float(),) if s["case"]["probs"] else out
 
 
 # ---------------------------------------------------------------- the same from the definition, in 64 bits
@@ -494,9 +495,7 @@ def _exact_sample(s, case):
         some = (w >= m * w[0]) & ((before < p) | (p >= 1))
         some[0] = True
         kept, w = kept[some], w[some] / w[some].sum()
-        back = torch.argsort(kept)
-        at = int((w[back].cumsum(0) <= u).sum().clamp(max=len(w) - 1))
-        probs.append(float(w[back][at]))
+        probs.append(float(w[int((w.cumsum(0) <= u).sum().clamp(max=len(w) - 1))]))
         all_probs[i, kept] = w
     out = None, torch.tensor(probs, dtype=torch.float64, device="cuda"), None
     return out + (all_probs,) if case["probs"] else out
