@@ -14,6 +14,7 @@
 #include "osmos/gpu/q8.h"
 #include "osmos/gpu/quant.h"
 #include "osmos_attn.h"
+#include "osmos_rows.h"
 
 #define OSMOS_LANE_MAX_PAIRS 4096 /* osmos_lane_tables' most (token, expert) pairs a step */
 

@@ -133,6 +133,42 @@ SIGS.update({
 })
 
 
+# include/osmos_rows.h
+
+class OsmosNorm(ctypes.Structure):
+    _fields_ = [("x", P), ("add", P), ("sum", P), ("weight", P), ("out", P), ("x16", P), ("overflow", P), ("codes", P),
+                ("scales", P), ("x_stride", U64), ("add_stride", U64), ("sum_stride", U64), ("out_stride", U64), ("type", U32),
+                ("weight_type", U32), ("out_type", U32), ("n", U32), ("dim", U32), ("eps", F32), ("offset", F32)]
+
+
+class OsmosRopeScaling(ctypes.Structure):
+    _fields_ = [("kind", U32), ("base", ctypes.c_double), ("factor", ctypes.c_double), ("context", ctypes.c_double),
+                ("low", ctypes.c_double), ("high", ctypes.c_double)]
+
+
+class OsmosRope(ctypes.Structure):
+    _fields_ = [("turns", P), ("q_weight", P), ("k_weight", P), ("q", P), ("k", P), ("q_out", P), ("k_out", P), ("q_stride", U64),
+                ("q_head", U64), ("k_stride", U64), ("k_head", U64), ("q_out_stride", U64), ("q_out_head", U64),
+                ("k_out_stride", U64), ("k_out_head", U64), ("type", U32), ("out_type", U32), ("heads", U32), ("kv_heads", U32),
+                ("n", U32), ("dim", U32), ("rot", U32), ("layout", U32), ("scale", F32), ("eps", F32), ("offset", F32)]
+
+
+class OsmosSample(ctypes.Structure):
+    _fields_ = [("logits", P), ("u", P), ("temperature", P), ("top_p", P), ("min_p", P), ("top_k", P), ("token", P), ("prob", P),
+                ("kept", P), ("probs", P), ("stride", U64), ("type", U32), ("n", U32), ("vocab", U32)]
+
+
+_RO, _SA = ctypes.POINTER(OsmosRope), ctypes.POINTER(OsmosSample)
+SIGS.update({
+    "osmos_norm": (B, [ctypes.POINTER(OsmosNorm), P]),
+    "osmos_rope_turns": (B, [ctypes.POINTER(OsmosRopeScaling), U32, ctypes.POINTER(ctypes.c_double), ctypes.POINTER(F32)]),
+    "osmos_rope": (B, [_RO, P, P]),
+    "osmos_rope_append": (B, [_RO, _KV, U32, _ST, P, U64, U64, P]),
+    "osmos_sample_workspace": (U64, [_SA]),
+    "osmos_sample": (B, [_SA, P, U64, P]),
+})
+
+
 # include/osmos/gpu/quant.h
 QUANT_Q5_K = 13
 QUANT_Q5_KR = 0x100 | QUANT_Q5_K

@@ -11,27 +11,6 @@ namespace kv {
 // for 25 MB, the same chain in every wave of the one round that the chip holds ----
 constexpr int kAppendRows = 4;  // rows (waves) a workgroup
 
-// x / f, each quotient rounded to nearest as a division's, for what is then saturated at 448: by f's reciprocal r, rounded to
-// nearest, and q + r (x - f q), exact in its remainder (Markstein's theorem; q may be more than one step off, which it does not
-// cover: on the host every mantissa of f with the seven x around each of e4m3's edges and 1.5e9 random pairs gave the division's
-// bits). values past 1000 f, infinities among them, are taken as that. three instructions a value where a division is some
-// twelve: 8256 rows of 2 x 4 x 128 10.7 -> 10.0 us
-__device__ inline void divide8(float (&x)[8], float f) {
-  const float size = fabsf(f);
-  if (size > 0x1p-60f && size < 0x1p60f) {
-    const float r = __fdiv_rn(1.0f, f), most = 1000.0f * size;
-#pragma unroll
-    for (int j = 0; j < 8; j++) {
-      const float y = __builtin_amdgcn_fmed3f(x[j], -most, most), q = y * r;
-      const float z = __builtin_fmaf(__builtin_fmaf(-q, f, y), r, q);
-      x[j] = x[j] != x[j] ? x[j] : z;
-    }
-  } else {
-#pragma unroll
-    for (int j = 0; j < 8; j++) x[j] = __fdiv_rn(x[j], f);
-  }
-}
-
 template <uint32_t SRC, uint32_t DST>
 __global__ __launch_bounds__(64 * kAppendRows) void append_kernel(const uint8_t* __restrict__ k, uint64_t ks,
                                                                   const uint8_t* __restrict__ v, uint64_t vs, Step st,

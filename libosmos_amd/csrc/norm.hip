@@ -1,0 +1,217 @@
+// libosmos MI355X - osmos_norm (include/osmos_rows.h): the residual's addition, the root-mean-square norm and the forms that the
+// products read, in one pass over the rows.
+#include "rowshost.h"
+#include "common.h"
+#include "x16.h"
+
+namespace osm {
+namespace rows {
+
+// 16 bytes of values as floats, at any address that their type allows
+template <uint32_t T> constexpr int per() { return T == OSMOS_F32 ? 4 : 8; }
+typedef float f32x4_u __attribute__((ext_vector_type(4), aligned(4)));
+typedef _Float16 f16x4_u __attribute__((ext_vector_type(4), aligned(2)));
+typedef __bf16 bf16x4_u __attribute__((ext_vector_type(4), aligned(2)));
+
+template <int N>
+__device__ inline void load(uint32_t type, const void* p, uint64_t at, float* x) {
+#pragma unroll
+  for (int i = 0; i < N; i += 4) {
+    if (type == OSMOS_F32) {
+      const f32x4_u v = gload<f32x4_u>((const float*) p + at + i);
+      x[i] = v[0], x[i + 1] = v[1], x[i + 2] = v[2], x[i + 3] = v[3];
+    } else if (type == OSMOS_F16) {
+      const f16x4_u v = gload<f16x4_u>((const _Float16*) p + at + i);
+      x[i] = (float) v[0], x[i + 1] = (float) v[1], x[i + 2] = (float) v[2], x[i + 3] = (float) v[3];
+    } else {
+      const bf16x4_u v = gload<bf16x4_u>((const __bf16*) p + at + i);
+      x[i] = (float) v[0], x[i + 1] = (float) v[1], x[i + 2] = (float) v[2], x[i + 3] = (float) v[3];
+    }
+  }
+}
+template <int N>
+__device__ inline void store(uint32_t type, void* p, uint64_t at, const float* x) {
+#pragma unroll
+  for (int i = 0; i < N; i += 4) {
+    if (type == OSMOS_F32) *(f32x4_u*) ((float*) p + at + i) = f32x4_u{x[i], x[i + 1], x[i + 2], x[i + 3]};
+    else if (type == OSMOS_F16)
+      *(f16x4_u*) ((_Float16*) p + at + i) = f16x4_u{(_Float16) x[i], (_Float16) x[i + 1], (_Float16) x[i + 2], (_Float16) x[i + 3]};
+    else
+      *(bf16x4_u*) ((__bf16*) p + at + i) = bf16x4_u{(__bf16) x[i], (__bf16) x[i + 1], (__bf16) x[i + 2], (__bf16) x[i + 3]};
+  }
+}
+__device__ inline float load1(uint32_t type, const void* p, uint64_t at) {
+  return type == OSMOS_F32 ? ((const float*) p)[at] : type == OSMOS_F16 ? (float) ((const _Float16*) p)[at] : (float) ((const __bf16*) p)[at];
+}
+__device__ inline void store1(uint32_t type, void* p, uint64_t at, float x) {
+  if (type == OSMOS_F32) ((float*) p)[at] = x;
+  else if (type == OSMOS_F16) ((_Float16*) p)[at] = (_Float16) x;
+  else ((__bf16*) p)[at] = (__bf16) x;
+}
+// the first `left` of N values (all of them but in a row's last, partial piece: TAIL, whether rows have one)
+template <int N, bool TAIL>
+__device__ inline void load_part(uint32_t type, const void* p, uint64_t at, uint32_t left, float* x) {
+  if (!TAIL || left >= N) return load<N>(type, p, at, x);
+#pragma unroll
+  for (int i = 0; i < N; i++) x[i] = (uint32_t) i < left ? load1(type, p, at + i) : 0.0f;
+}
+template <int N, bool TAIL>
+__device__ inline void store_part(uint32_t type, void* p, uint64_t at, uint32_t left, const float* x) {
+  if (!TAIL || left >= N) return store<N>(type, p, at, x);
+#pragma unroll
+  for (int i = 0; i < N; i++)
+    if ((uint32_t) i < left) store1(type, p, at + i, x[i]);
+}
+
+// 1 / sqrt(a) for a >= 0, within a few units of float64: the hardware's estimate (2^-26 or better) and two of Newton's steps
+__device__ inline double rsqrt64(double a) {
+  const double e = __builtin_amdgcn_rsq(a);
+  double y = e;
+#pragma unroll
+  for (int i = 0; i < 2; i++) y = __builtin_fma(y * 0.5, __builtin_fma(-a * y, y, 1.0), y);
+  return a > 0.0 && a < __builtin_inf() ? y : e;
+}
+
+struct NormArgs {
+  const void *x, *add;  // (sum may be either: no restrict)
+  void* sum;
+  const void* weight;
+  void* out;
+  _Float16* x16;
+  int32_t* overflow;
+  int8_t* codes;
+  float* scales;
+  uint64_t x_stride, add_stride, sum_stride, out_stride;
+  uint32_t weight_type, out_type, n, dim;
+  float eps, offset;
+  double part;      // 1 / dim
+  uint32_t waves;   // a row's; 1: each wave of the workgroup a row of its own
+};
+
+// a row's values stay in registers between the sum of their squares and their stores: K pieces of 16 bytes a thread
+template <uint32_t T, int K, bool TAIL>
+__global__ __launch_bounds__(1024) void norm_kernel(NormArgs a) {
+  constexpr int N = per<T>();
+  __shared__ double sums[16];
+  const uint32_t lanes = a.waves * 64, wave = threadIdx.x / 64;
+  const uint32_t t = a.waves > 1 ? blockIdx.x : blockIdx.x * (blockDim.x / 64) + wave;
+  const uint32_t at = a.waves > 1 ? threadIdx.x : threadIdx.x & 63;
+  const uint32_t pieces = (a.dim + N - 1) / N;
+  const bool live = t < a.n;  // (a row past the last: of a tile's rest, or none)
+  float s[K][N];
+  double ss = 0.0;
+  if (live) {
+#pragma unroll
+    for (int k = 0; k < K; k++) {
+      const uint32_t c = at + k * lanes;
+      if (c < pieces) load_part<N, TAIL>(T, a.x, t * a.x_stride + c * N, a.dim - c * N, s[k]);
+      else
+#pragma unroll
+        for (int i = 0; i < N; i++) s[k][i] = 0.0f;
+    }
+    if (a.add)
+#pragma unroll
+      for (int k = 0; k < K; k++) {
+        const uint32_t c = at + k * lanes;
+        float d[N];
+        if (c < pieces) {
+          load_part<N, TAIL>(T, a.add, t * a.add_stride + c * N, a.dim - c * N, d);
+#pragma unroll
+          for (int i = 0; i < N; i++) s[k][i] = __fadd_rn(s[k][i], d[i]);
+        }
+      }
+#pragma unroll
+    for (int k = 0; k < K; k++) {
+      const uint32_t c = at + k * lanes;
+      if (a.sum && c < pieces) store_part<N, TAIL>(T, a.sum, t * a.sum_stride + c * N, a.dim - c * N, s[k]);
+#pragma unroll
+      for (int i = 0; i < N; i++) ss = __builtin_fma((double) s[k][i], (double) s[k][i], ss);
+    }
+  }
+  if (!a.out && !a.x16 && !a.codes) return;
+#pragma unroll
+  for (int o = 32; o; o >>= 1) ss += __shfl_xor(ss, o);
+  if (a.waves > 1) {
+    if (at % 64 == 0) sums[wave] = ss;
+    __syncthreads();
+    ss = 0.0;
+    for (uint32_t w = 0; w < a.waves; w++) ss += sums[w];
+  }
+  const float r = (float) rsqrt64(__builtin_fma(ss, a.part, (double) a.eps));
+  bool over = false;
+#pragma unroll
+  for (int k = 0; k < K; k++) {
+    const uint32_t c = at + k * lanes;
+    if (c >= pieces) break;
+    float y[N];
+    if (!live) {
+      if (!a.x16 || t >= (a.n + 15) / 16 * 16) break;
+#pragma unroll
+      for (int i = 0; i < N; i++) y[i] = 0.0f;
+    } else {
+      float w[N];
+      if (a.weight) load_part<N, TAIL>(a.weight_type, a.weight, c * N, a.dim - c * N, w);
+#pragma unroll
+      for (int i = 0; i < N; i++)
+        y[i] = a.weight ? __fmul_rn(__fmul_rn(s[k][i], r), __fadd_rn(w[i], a.offset))
+                        : __fmul_rn(__fmul_rn(s[k][i], r), __fadd_rn(1.0f, a.offset));
+      if (a.out) store_part<N, TAIL>(a.out_type, a.out, t * a.out_stride + c * N, a.dim - c * N, y);
+      if (a.codes) {
+        float am = 0.0f;
+#pragma unroll
+        for (int i = 0; i < N; i++) am = fmaxf(am, fabsf(y[i]));
+        am = fmaxf(am, xor_lane(am, 1));
+        am = fmaxf(am, xor_lane(am, 2));
+        if (N == 4) am = fmaxf(am, xor_lane(am, 4));
+        const float inv = am > 0.0f ? __fdiv_rn(127.0f, am) : 0.0f;
+        uint32_t* q = (uint32_t*) (a.codes + (uint64_t) t * a.dim + c * N);
+#pragma unroll
+        for (int i = 0; i < N; i += 4) {
+          uint32_t v = 0;
+#pragma unroll
+          for (int j = 0; j < 4; j++) v |= ((uint32_t) (int) rintf(__fmul_rn(y[i + j], inv)) & 0xFF) << (8 * j);
+          q[i / 4] = v;
+        }
+        if (c % (32 / N) == 0) a.scales[(uint64_t) t * (a.dim / 32) + c / (32 / N)] = __fdiv_rn(am, 127.0f);
+      }
+    }
+    if (a.x16) {
+      _Float16 h[N];
+#pragma unroll
+      for (int i = 0; i < N; i++) h[i] = x16_round(y[i], over);
+      __builtin_memcpy(__builtin_assume_aligned(a.x16 + x16_at(t, c * N, a.dim), 2 * N), h, 2 * N);
+    }
+  }
+  if (over) *a.overflow = 1;
+}
+
+template <uint32_t T, bool TAIL>
+auto norm_of(uint32_t k) {
+  return k <= 1 ? norm_kernel<T, 1, TAIL> : k <= 2 ? norm_kernel<T, 2, TAIL> : k <= 4 ? norm_kernel<T, 4, TAIL>
+         : k <= 8 ? norm_kernel<T, 8, TAIL> : norm_kernel<T, 64 / per<T>(), TAIL>;
+}
+
+template <uint32_t T>
+bool norm_launch(const OsmosNorm* a, hipStream_t s) {
+  const uint32_t pieces = (a->dim + per<T>() - 1) / per<T>(), rows = a->x16 ? (a->n + 15) / 16 * 16 : a->n;
+  NormArgs b = {a->x, a->add, a->sum, a->weight, a->out, (_Float16*) a->x16, a->overflow, a->codes, a->scales, a->x_stride, a->add_stride,
+                a->sum_stride, a->out_stride, a->weight_type, a->out_type, a->n, a->dim, a->eps, a->offset, 1.0 / a->dim, 0};
+  const uint32_t waves = (pieces + 255) / 256;
+  b.waves = waves > 16 ? 16 : waves;
+  const uint32_t k = (pieces + b.waves * 64 - 1) / (b.waves * 64);
+  auto* kernel = a->dim % per<T>() ? norm_of<T, true>(k) : norm_of<T, false>(k);
+  if (b.waves > 1) kernel<<<rows, b.waves * 64, 0, s>>>(b);
+  else kernel<<<(rows + 3) / 4, 256, 0, s>>>(b);
+  return hipGetLastError() == hipSuccess;
+}
+
+}  // namespace rows
+}  // namespace osm
+
+using namespace osm;
+
+extern "C" OSM_API bool osmos_norm(const OsmosNorm* a, void* stream) {
+  if (!rows::norm_ok(a)) return false;
+  return a->type == OSMOS_F32 ? rows::norm_launch<OSMOS_F32>(a, (hipStream_t) stream)
+         : a->type == OSMOS_F16 ? rows::norm_launch<OSMOS_F16>(a, (hipStream_t) stream) : rows::norm_launch<OSMOS_BF16>(a, (hipStream_t) stream);
+}
