@@ -101,7 +101,9 @@ inline bool turns_of(const OsmosRopeScaling* s, uint32_t rot, double* turns, flo
 }
 
 inline bool sample_ok(const OsmosSample* a) {
-  if (!a || !a->n || a->n > 0x7FFFFFu || !a->vocab || a->vocab > OSMOS_SAMPLE_MAX_VOCAB || !kv::row_type(a->type)) return false;
+  if (!a || !a->n || a->n > 0x7FFFFFu || !a->vocab || a->vocab > OSMOS_SAMPLE_MAX_VOCAB || !kv::row_type(a->type) ||
+      (uint64_t) a->n * a->vocab > 1ull << 40)
+    return false;
   if (!rows_ok(a->logits, a->type, a->stride, a->n, a->vocab) || !a->u || !a->token) return false;
   const void* words[] = {a->u, a->temperature, a->top_p, a->min_p, a->top_k, a->token, a->prob, a->kept, a->probs};
   for (const void* p : words)

@@ -1,9 +1,14 @@
 // libosmos MI355X - osmos_sample (include/osmos_rows.h): one token for each row of logits.
 //
-// tokens are put into bins of their logits, 23 an octave of weight: y = logit x 23 log2(e) / T, bin floor(y), its weight
-// 2^(y / 23). a bin's weights are summed as whole numbers of 2^-42 of its lower edge's weight, so that the sums do not depend on
-// their order; a prefix of the tokens' order is whole bins and then some of one bin's tokens, which are found by their logits'
-// bits and indexes, 1024 parts of what is left at a time.
+// tokens are put into bins of their logits, 23 an octave of weight: y = logit x 23 log2(e) / T, bin rint(y), its weight
+// 2^(y / 23). a bin's weights are summed as whole numbers of 2^-42 of its middle's weight, so that the sums do not depend on
+// their order; a prefix of the tokens' order is whole bins and then some of one bin's tokens, which are found by their places: their
+// logits' bits and indexes.
+//
+// a row is cut into slices: scan_kernel makes each slice's bins, plan_kernel adds a row's up and finds the bins that the limits and
+// the token lie in, list_kernel lists these bins' tokens, draw_kernel chooses among them. bins are whole numbers of y, so that slices
+// agree on them without knowing the row's maximum; a slice keeps the 1024 below its own. a short row is one kernel, its tokens in
+// registers.
 #include "rowshost.h"
 #include "common.h"
 
@@ -13,32 +18,57 @@ namespace rows {
 constexpr int kSampleThreads = 1024, kSampleWaves = kSampleThreads / 64;
 constexpr int kBins = 1024;           // 44.5 octaves below the greatest weight: what is further down is in no bin
 constexpr double kOctave = 23.0;
-constexpr double kOne = 4398046511104.0;  // 2^42: 2^20 tokens of up to 2^(1 / 23) stay under 2^63
+constexpr double kOne = 4398046511104.0;  // 2^42: 2^20 tokens of up to 2^(1 / 46) stay under 2^63
+constexpr uint32_t kList = 2048;      // tokens that are looked at in LDS; more are looked for in the row each time
+constexpr uint32_t kFew = 1024;       // a top_k up to this needs the weights of its own tokens alone: they are listed
+constexpr int kSlots = 8, kParts = kBins / kSlots;  // bins that are looked into at once, parts of each
+constexpr uint32_t kCrowd = 64;       // tokens of a part that are compared with one another
 
-// a logit as the order takes it
+// a logit as the order takes it: +infinity as the type's greatest value (a NaN stays one, and is greater than nothing)
+template <uint32_t T> constexpr float kGreatest = T == OSMOS_F32 ? 3.40282346638528860e38f : T == OSMOS_F16 ? 65504.0f : 3.38953138925153547e38f;
+template <uint32_t T>
+__device__ inline float ordered(float x) {
+  return x > kGreatest<T> ? kGreatest<T> : x;
+}
 template <uint32_t T>
 __device__ inline float logit_at(const void* p, uint64_t i) {
-  float x;
-  if constexpr (T == OSMOS_F32) x = gload<float>((const float*) p + i);
-  else if constexpr (T == OSMOS_F16) x = (float) gload<_Float16>((const _Float16*) p + i);
-  else x = (float) gload<__bf16>((const __bf16*) p + i);
-  return x != x ? -__builtin_inff() : fminf(x, 3.402823466e38f);
+  if constexpr (T == OSMOS_F32) return ordered<T>(gload<float>((const float*) p + i));
+  else if constexpr (T == OSMOS_F16) return ordered<T>((float) gload<_Float16>((const _Float16*) p + i));
+  else return ordered<T>((float) gload<__bf16>((const __bf16*) p + i));
 }
-// (the greatest first, the lower index first among equals)
-__device__ inline uint64_t place(float x, uint32_t i) {
-  const uint32_t b = __float_as_uint(x + 0.0f);  // (-0 is 0)
-  return (uint64_t) (b & 0x80000000u ? b : ~b & 0x7FFFFFFFu) << 32 | i;
-}
+// a token's place in the order (the greatest logit first, the lower index first among equals): the logit's bits, without those
+// that are zero in all of type T's, above `bits` of its index
+template <uint32_t T> constexpr int kDrop = T == OSMOS_F32 ? 0 : T == OSMOS_F16 ? 13 : 16;
+template <uint32_t T>
+struct Order {
+  int bits;
+  __device__ inline uint64_t place(float x, uint32_t i) const {
+    const uint32_t b = __float_as_uint(x + 0.0f);  // (-0 is 0)
+    return (uint64_t) ((b & 0x80000000u ? b : ~b & 0x7FFFFFFFu) >> kDrop<T>) << bits | i;
+  }
+  __device__ inline float logit(uint64_t place) const {
+    const uint32_t k = (uint32_t) (place >> bits) << kDrop<T>;
+    return __uint_as_float(k & 0x80000000u ? k : (~k & 0x7FFFFFFFu) >> kDrop<T> << kDrop<T>);
+  }
+  __device__ inline uint32_t index(uint64_t place) const { return (uint32_t) place & ((1u << bits) - 1); }
+};
 
-// 2^(f / 23) for 0 <= f < 1, within 2^-47
+// 2^(f / 23) for -1/2 <= f <= 1/2, within 2^-45 (its series to the fifth power)
 __device__ inline double part_weight(double f) {
-  const double x = f * (0.69314718055994530942 / kOctave);
-  double r = __builtin_fma(x, 1.0 / 720, 1.0 / 120);
-  r = __builtin_fma(x, r, 1.0 / 24);
-  r = __builtin_fma(x, r, 1.0 / 6);
-  r = __builtin_fma(x, r, 0.5);
-  r = __builtin_fma(x, r, 1.0);
-  return __builtin_fma(x, r, 1.0);
+  constexpr double c = 0.69314718055994530942 / kOctave;
+  double k5 = c * c * c * c * c / 120, k4 = c * c * c * c / 24, k3 = c * c * c / 6, k2 = c * c / 2, k1 = c;
+#if __HIP_DEVICE_COMPILE__
+  asm("" : "+s"(k5), "+s"(k4), "+s"(k3), "+s"(k2), "+s"(k1));  // (in scalar registers: one instruction a step)
+#endif
+  double r = __builtin_fma(f, k5, k4);
+  r = __builtin_fma(f, r, k3);
+  r = __builtin_fma(f, r, k2);
+  r = __builtin_fma(f, r, k1);
+  return __builtin_fma(f, r, 1.0);
+}
+// the same as a whole number of 2^-42 (added to 2^52, whose last bit is 1)
+__device__ inline uint64_t whole_weight(double f) {
+  return (uint64_t) __double_as_longlong(__builtin_fma(part_weight(f), kOne, 4503599627370496.0)) - 0x4330000000000000ull;
 }
 __device__ inline uint64_t whole(double x) { return (uint64_t) __builtin_rint(x); }
 
@@ -50,6 +80,27 @@ struct SampleArgs {
   float *prob, *probs;
   uint64_t stride;
   uint32_t n, vocab;
+  uint32_t slices, slice;  // a row's, and a slice's tokens
+  int bits;                // of a token's index
+  uint8_t *parts, *plans, *cuts;  // the workspace: each slice's Part, each row's RowPlan and Drawn
+  __device__ inline float heat(uint32_t t) const { return temperature ? temperature[t] : 1.0f; }
+  __device__ inline int32_t k(uint32_t t) const { return top_k ? top_k[t] : 0; }
+};
+// whether a row's bins need no weights: those of a few listed tokens do
+__device__ inline bool few(int32_t k) { return k > 0 && (uint32_t) k <= kFew; }
+
+// what is known of a slice
+struct Part {
+  uint64_t first;  // the place of its first token; ~0: none
+  double top;      // its first bin
+  uint32_t valid, used;  // tokens that can be chosen; bins from the first on that are not empty
+  uint64_t mass[kBins];  // (unused for a few)
+  uint32_t count[kBins];
+};
+// what a row was drawn from, for its probabilities
+struct Drawn {
+  uint64_t last;  // the last kept place; ~0: all
+  double by, top, least_y, share;  // least_y: what a kept token's y is at least; share 0: the row's one token is `last`, or none
 };
 
 struct Sum {
@@ -57,59 +108,470 @@ struct Sum {
   uint64_t m;  // their weights
 };
 
-struct SampleLds {
-  uint32_t count[kBins];
-  uint64_t mass[kBins];
-  uint64_t before[kBins + 1];  // the bins' prefix sums, of kOne the greatest bin's edge
+// a row's limits and the bins that they and its token lie in
+struct Plan {
+  double by, top, part, draw, edge;  // Scale; top_p and u in their ranges; min_p as a y
+  uint64_t first, all;      // the first token's place, the bins' weights
+  uint32_t valid, listed;   // tokens that can be chosen, that are listed (more than kList: those past it are not)
+  uint32_t k;               // top_k where it limits, or 0; k_bin kBins: among tokens of no weight
+  int k_bin, m_bin;         // kBins: none
+  int done, small, by_p, slots;  // done: the row's token is given already; small: all bins up to slot_bin[0] are listed; slots 0: too many
+  int from[4], to[4];       // the listed bins, by logit from low to high
+  float low[4], high[4];
+  int slot_bin[kSlots];
+  uint32_t slot_ahead[kSlots];
+  uint64_t slot_before[kSlots];
+};
+// a row's bins' prefix sums: weights (of kOne the first bin's middle) and tokens
+struct Prefix {
+  uint64_t before[kBins + 1];
   uint32_t ahead[kBins + 1];
-  double scale[kBins];         // a bin's weight by the first's
-  uint32_t part_n[kBins];
-  uint64_t part_m[kBins];
-  Sum wave[kSampleWaves];
-  uint64_t word[kSampleWaves], found[4];
+};
+struct RowPlan {
+  Plan plan;
+  Prefix prefix;
+  uint64_t list[kList];
 };
 
-__device__ inline uint64_t shfl64(uint64_t v, int lane) {
-  return (uint64_t) (uint32_t) __shfl((int) (v >> 32), lane) << 32 | (uint32_t) __shfl((int) v, lane);
+struct ScanLds {
+  uint64_t mass[kBins];
+  uint32_t count[kBins];
+  Sum wave[kSampleWaves];
+  uint64_t word[kSampleWaves];
+};
+struct PlanLds {
+  Plan plan;
+  Prefix prefix;
+  Sum wave[kSampleWaves];
+  uint64_t word[kSampleWaves];
+  uint32_t at[8];
+};
+struct DrawLds {
+  uint64_t part_m[kBins], part_lo[kBins], part_hi[kBins];
+  uint32_t part_n[kBins], filled[kBins];
+  uint64_t sorted[kList], weight[kList];
+  Sum wave[kSampleWaves];
+  uint64_t word[kSampleWaves], found[4], lo[kSlots], hi[kSlots], last_m;
+  uint32_t at, crowded, last_n;
+};
+struct WholeLds : PlanLds {
+  union {
+    ScanLds scan;
+    DrawLds draw;
+  };
+  uint64_t list[kList];
+};
+
+// lanes' values by DPP: row_shr 1, 2, 4, 8, then lane 15 of a row to the next and 31 to the upper half; `none` where there is no
+// such lane
+template <int STEP>
+__device__ inline uint32_t from_below(uint32_t x, uint32_t none) {
+  constexpr int ctrl = STEP < 4 ? 0x110 + (1 << STEP) : STEP == 4 ? 0x142 : 0x143;
+  constexpr int rows = STEP < 4 ? 0xF : STEP == 4 ? 0xA : 0xC;
+  return (uint32_t) __builtin_amdgcn_update_dpp((int) none, (int) x, ctrl, rows, 0xF, false);
+}
+template <int STEP>
+__device__ inline uint64_t from_below(uint64_t x, uint64_t none) {
+  return (uint64_t) from_below<STEP>((uint32_t) (x >> 32), (uint32_t) (none >> 32)) << 32 | from_below<STEP>((uint32_t) x, (uint32_t) none);
+}
+template <int STEP = 0>
+__device__ inline Sum wave_sums(Sum x) {  // inclusive
+  x.n += from_below<STEP>(x.n, 0u), x.m += from_below<STEP>(x.m, (uint64_t) 0);
+  if constexpr (STEP < 5) return wave_sums<STEP + 1>(x);
+  else return x;
+}
+template <int STEP = 0>
+__device__ inline uint64_t wave_least(uint64_t x) {  // lane 63: of all
+  const uint64_t y = from_below<STEP>(x, ~0ull);
+  x = y < x ? y : x;
+  if constexpr (STEP < 5) return wave_least<STEP + 1>(x);
+  else return x;
 }
 // inclusive sums over the workgroup's threads in their order
-__device__ inline Sum scan_sum(Sum x, SampleLds& l) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x / 64;
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    const uint32_t n = (uint32_t) __shfl_up((int) x.n, o);
-    const uint64_t m = (uint64_t) (uint32_t) __shfl_up((int) (x.m >> 32), o) << 32 | (uint32_t) __shfl_up((int) x.m, o);
-    if (lane >= o) x.n += n, x.m += m;
+template <typename L>
+__device__ inline Sum scan_sum(Sum x, L& l) {
+  const int wave = threadIdx.x / 64;
+  x = wave_sums(x);
+  __syncthreads();
+  if ((threadIdx.x & 63) == 63) l.wave[wave] = x;
+  __syncthreads();
+  Sum w = {(threadIdx.x & 63) < kSampleWaves ? l.wave[threadIdx.x & 15].n : 0, (threadIdx.x & 63) < kSampleWaves ? l.wave[threadIdx.x & 15].m : 0};
+  w = wave_sums(w);
+  if (wave) {
+    x.n += (uint32_t) __builtin_amdgcn_readlane((int) w.n, wave - 1);
+    x.m += (uint64_t) (uint32_t) __builtin_amdgcn_readlane((int) (w.m >> 32), wave - 1) << 32 | (uint32_t) __builtin_amdgcn_readlane((int) w.m, wave - 1);
   }
-  __syncthreads();
-  if (lane == 63) l.wave[wave] = x;
-  __syncthreads();
-  for (int w = 0; w < wave; w++) x.n += l.wave[w].n, x.m += l.wave[w].m;
   return x;
 }
-__device__ inline uint64_t least(uint64_t x, SampleLds& l) {
-#pragma unroll
-  for (int o = 32; o; o >>= 1) {
-    const uint64_t y = shfl64(x, (threadIdx.x & 63) ^ o);
-    x = y < x ? y : x;
-  }
+template <typename L>
+__device__ inline Sum total(Sum x, L& l) {
+  x = wave_sums(x);
   __syncthreads();
-  if (threadIdx.x % 64 == 0) l.word[threadIdx.x / 64] = x;
+  if ((threadIdx.x & 63) == 63) l.wave[threadIdx.x / 64] = x;
+  __syncthreads();
+  x = {0, 0};
+#pragma unroll
+  for (int w = 0; w < kSampleWaves; w++) x.n += l.wave[w].n, x.m += l.wave[w].m;
+  return x;
+}
+template <typename L>
+__device__ inline uint64_t least(uint64_t x, L& l) {
+  x = wave_least(x);
+  __syncthreads();
+  if ((threadIdx.x & 63) == 63) l.word[threadIdx.x / 64] = x;
   __syncthreads();
   x = l.word[0];
+#pragma unroll
   for (int w = 1; w < kSampleWaves; w++) x = l.word[w] < x ? l.word[w] : x;
   return x;
 }
 
 // where a row's logits lie on the bins' scale
 struct Scale {
-  double by, top;  // bins a unit of logit; the first bin's floor
+  double by, top;  // bins a unit of logit; the first bin
   __device__ inline double y(float x) const { return (double) x * by; }
-  __device__ inline int bin(double floor) const {  // kBins: none
-    const double b = top - floor;
+  __device__ inline int bin(double middle) const {  // kBins: none
+    const double b = top - middle;
     return b < kBins ? (int) b : kBins;
   }
+  __device__ inline int bin_of(float x) const { return bin(__builtin_rint(y(x))); }
 };
+__device__ inline double bins_a_unit(float temperature) { return kOctave * 1.4426950408889634074 / (double) temperature; }
+
+// 16 bytes of logits at any address that their type allows, as they are (past the end: -infinity)
+template <uint32_t T> constexpr uint32_t kPer = T == OSMOS_F32 ? 4 : 8;
+typedef float f32x4_u __attribute__((ext_vector_type(4), aligned(4)));
+typedef _Float16 f16x8_u __attribute__((ext_vector_type(8), aligned(2)));
+typedef __bf16 bf16x8_u __attribute__((ext_vector_type(8), aligned(2)));
+template <uint32_t T>
+__device__ inline void logits_at(const void* p, uint32_t i, uint32_t end, float (&x)[kPer<T>]) {
+  if (i + kPer<T> <= end) {
+    if constexpr (T == OSMOS_F32) {
+      const f32x4_u v = gload<f32x4_u>((const float*) p + i);
+#pragma unroll
+      for (int j = 0; j < 4; j++) x[j] = v[j];
+    } else if constexpr (T == OSMOS_F16) {
+      const f16x8_u v = gload<f16x8_u>((const _Float16*) p + i);
+#pragma unroll
+      for (int j = 0; j < 8; j++) x[j] = (float) v[j];
+    } else {
+      const bf16x8_u v = gload<bf16x8_u>((const __bf16*) p + i);
+#pragma unroll
+      for (int j = 0; j < 8; j++) x[j] = (float) v[j];
+    }
+  } else {
+#pragma unroll
+    for (uint32_t j = 0; j < kPer<T>; j++) x[j] = i + j < end ? logit_at<T>(p, i + j) : -__builtin_inff();
+  }
+}
+
+// tokens begin .. end - 1 of a row, P pieces a thread and round (the rounds' loads in flight together)
+template <uint32_t T, int P>
+struct Tokens {
+  const void* p;
+  uint32_t begin, end;
+  static constexpr uint32_t kRound = kSampleThreads * kPer<T> * P;
+  float x[P][kPer<T>];
+  __device__ inline void load(uint32_t at) {
+#pragma unroll
+    for (int k = 0; k < P; k++) logits_at<T>(p, at + (k * kSampleThreads + threadIdx.x) * kPer<T>, end, x[k]);
+  }
+  template <typename F>
+  __device__ inline void loaded(uint32_t at, F f) const {
+#pragma unroll
+    for (int k = 0; k < P; k++)
+#pragma unroll
+      for (uint32_t j = 0; j < kPer<T>; j++) f(x[k][j], at + (k * kSampleThreads + threadIdx.x) * kPer<T> + j);
+  }
+  // those from low to high
+  template <typename F>
+  __device__ inline void loaded_between(uint32_t at, const Plan& p, F f) const {
+    const float l0 = p.low[0], h0 = p.high[0], l1 = p.low[1], h1 = p.high[1], l2 = p.low[2], h2 = p.high[2], l3 = p.low[3], h3 = p.high[3];
+    const int spans = l3 <= h3 ? 4 : l2 <= h2 ? 3 : l1 <= h1 ? 2 : 1;
+    auto test = [&](auto in) __attribute__((always_inline)) {
+#pragma unroll
+      for (int k = 0; k < P; k++)
+#pragma unroll
+        for (uint32_t j = 0; j < kPer<T>; j++)
+          if (in(x[k][j])) f(x[k][j], at + (k * kSampleThreads + threadIdx.x) * kPer<T> + j);
+    };
+    if (spans == 1) test([&](float v) { return v >= l0 && v <= h0; });
+    else if (spans == 2) test([&](float v) { return (v >= l0 && v <= h0) || (v >= l1 && v <= h1); });
+    else test([&](float v) { return (v >= l0 && v <= h0) || (v >= l1 && v <= h1) || (v >= l2 && v <= h2) || (v >= l3 && v <= h3); });
+  }
+  // in ascending order of a thread's own tokens
+  template <typename F>
+  __device__ inline void each(F f) {
+    for (uint32_t at = begin; at < end; at += kRound) {
+      load(at);
+      loaded(at, f);
+    }
+  }
+};
+
+// the tokens that a row's choice can hang on: the listed ones where the list holds them, or all
+template <uint32_t T>
+struct Near {
+  Tokens<T, 2> row;
+  const Order<T>& order;
+  const uint64_t* list;
+  uint32_t n;
+  template <typename F>
+  __device__ inline void each(F f) {
+    if (n <= kList)
+      for (uint32_t i = threadIdx.x; i < n; i += kSampleThreads) f(order.logit(list[i]), order.index(list[i]));
+    else
+      row.each([&](float x, uint32_t i) {
+        x = ordered<T>(x);
+        if (x > -__builtin_inff()) f(x, i);
+      });
+  }
+};
+
+// a slice's first place and, but for a greedy row, its bins (into l.count and, unless k is small, l.mass): its tokens are one round
+template <uint32_t T, typename R, typename L>
+__device__ inline void scan_slice(R& row, const Order<T>& order, float temperature, int32_t k, L& l, uint64_t& first, double& top, uint32_t& valid) {
+  row.load(row.begin);
+  l.mass[threadIdx.x] = 0, l.count[threadIdx.x] = 0;
+  float best = -__builtin_inff();
+  uint32_t at = 0;
+  row.loaded(row.begin, [&](float x, uint32_t i) {
+    x = ordered<T>(x);
+    if (x > best) best = x, at = i;
+  });
+  first = least(best > -__builtin_inff() ? order.place(best, at) : ~0ull, l);
+  top = 0.0, valid = 0;
+  if (first == ~0ull || !(temperature > 0.0f)) return;
+  Scale sc = {bins_a_unit(temperature), 0.0};
+  sc.top = top = __builtin_rint(sc.y(order.logit(first)));
+  const bool counts = few(k);
+  auto add = [&](float x, bool mass) __attribute__((always_inline)) {
+    x = ordered<T>(x);
+    const double y = sc.y(x), middle = __builtin_rint(y), b = sc.top - middle;
+    if (b < kBins) {
+      const int i = (int) b;
+      atomicAdd(&l.count[i], 1u);
+      if (mass) atomicAdd((unsigned long long*) &l.mass[i], (unsigned long long) whole_weight(y - middle));
+    } else {
+      valid += x > -__builtin_inff();
+    }
+  };
+  if (counts) row.loaded(row.begin, [&](float x, uint32_t) { add(x, false); });
+  else row.loaded(row.begin, [&](float x, uint32_t) { add(x, true); });
+  __syncthreads();
+  valid = total(Sum{valid + l.count[threadIdx.x], 0}, l).n;
+}
+
+constexpr int kPieces = 4;  // 16 bytes of a slice a thread
+template <uint32_t T>
+__global__ __launch_bounds__(kSampleThreads) void scan_kernel(SampleArgs a) {
+  __shared__ ScanLds l;
+  const uint32_t t = blockIdx.x / a.slices, s = blockIdx.x - t * a.slices, begin = s * a.slice;
+  const uint32_t end = begin + a.slice < a.vocab ? begin + a.slice : a.vocab;
+  Tokens<T, kPieces> row = {(const uint8_t*) a.logits + t * a.stride * kv::size_of(T), begin, end};
+  Part* part = (Part*) a.parts + blockIdx.x;
+  const Order<T> order = {a.bits};
+  uint64_t first;
+  double top;
+  uint32_t valid;
+  scan_slice<T>(row, order, a.heat(t), a.k(t), l, first, top, valid);
+  const uint32_t n = valid ? l.count[threadIdx.x] : 0;
+  const uint32_t used = ~(uint32_t) least(~(uint64_t) (n ? threadIdx.x + 1 : 0), l);
+  if (threadIdx.x < used) {
+    part->count[threadIdx.x] = n;
+    if (!few(a.k(t))) part->mass[threadIdx.x] = l.mass[threadIdx.x];
+  }
+  if (threadIdx.x == 0) part->first = first, part->top = top, part->valid = valid, part->used = used;
+}
+
+// a bin's weight by the first's
+__device__ inline double bin_scale(int b) { return exp2(-(double) b / kOctave); }
+// the weight that the first top_p of m's reach, and the one that the drawn token's sum reaches
+__device__ inline uint64_t p_goal(const Plan& p, uint64_t m) {
+  const double g = __builtin_ceil((double) m * p.part);
+  return g > 1.0 ? (uint64_t) g < m ? (uint64_t) g : m : 1;
+}
+__device__ inline uint64_t u_goal(const Plan& p, uint64_t m) {
+  const uint64_t g = (uint64_t) __builtin_floor((double) m * p.draw) + 1;
+  return g < m ? g : m;
+}
+
+// a row's plan from its bins (thread i bin i's sums): what is written is there for all threads when it returns
+template <uint32_t T>
+__device__ inline void make_plan(const SampleArgs& a, uint32_t t, const Order<T>& order, PlanLds& l, uint64_t first, double top, uint32_t valid, Sum bin) {
+  const uint32_t tid = threadIdx.x;
+  const float temperature = a.heat(t), top_p = a.top_p ? a.top_p[t] : 1.0f, min_p = a.min_p ? a.min_p[t] : 0.0f, u = a.u[t];
+  const int32_t k = a.k(t);
+  const Scale sc = {bins_a_unit(temperature), top};
+  Plan& p = l.plan;
+  if (first == ~0ull || !(temperature > 0.0f)) {
+    const bool none = first == ~0ull;
+    if (tid == 0) {
+      a.token[t] = none ? -1 : (int32_t) order.index(first);
+      if (a.prob) a.prob[t] = none ? 0.0f : 1.0f;
+      if (a.kept) a.kept[t] = none ? 0 : 1;
+      if (a.probs) ((Drawn*) a.cuts)[t] = Drawn{first, 0.0, 0.0, 0.0, 0.0};
+      p.done = 1;
+    }
+    __syncthreads();
+    return;
+  }
+  const bool small = few(k);
+  if (tid < 8) l.at[tid] = 0;
+  const Sum sum = scan_sum(Sum{bin.n, small ? 0 : whole((double) bin.m * bin_scale(tid))}, l);
+  l.prefix.ahead[tid + 1] = sum.n, l.prefix.before[tid + 1] = sum.m;
+  if (tid == 0) l.prefix.ahead[0] = 0, l.prefix.before[0] = 0;
+  __syncthreads();
+  const uint32_t* ahead = l.prefix.ahead;
+  const uint64_t *before = l.prefix.before, all = before[kBins];
+  const uint32_t limit = k > 0 && (uint32_t) k < valid ? k : 0;
+  const bool by_k = limit && limit <= ahead[kBins], by_p = top_p < 1.0f;
+  const double edge = sc.y(order.logit(first)) + (min_p > 0.0f ? kOctave * log2((double) (min_p < 1.0f ? min_p : 1.0f)) : 0.0);
+  const int m_bin = min_p > 0.0f ? sc.bin(__builtin_rint(edge)) : kBins;
+  if (tid == 0) {
+    p.by = sc.by, p.top = top, p.part = top_p > 0.0f ? top_p : 0.0f, p.draw = u > 0.0f ? u < 1.0f ? u : 0.99999994f : 0.0f, p.edge = edge;
+    p.first = first, p.all = all, p.valid = valid, p.listed = 0, p.k = limit, p.m_bin = m_bin;
+    p.done = 0, p.small = small, p.by_p = by_p;
+  }
+  if (by_k && ahead[tid + 1] >= limit && ahead[tid] < limit) l.at[0] = tid;
+  __syncthreads();
+  const int k_bin = by_k ? (int) l.at[0] : kBins;
+  int from[4], to[4];
+  if (small) {
+    from[0] = 0, to[0] = by_k ? k_bin : kBins - 1;
+#pragma unroll
+    for (int i = 1; i < 4; i++) from[i] = to[i] = kBins;
+  } else {
+    auto holds = [&](uint64_t goal) { return before[tid + 1] >= goal && before[tid] < goal; };
+    uint64_t least_m = all, most_m = all;
+    if (by_k) least_m = before[k_bin] + 1, most_m = before[k_bin + 1];
+    if (by_p) {
+      if (holds(p_goal(p, least_m))) l.at[1] = tid;
+      if (holds(p_goal(p, most_m))) l.at[2] = tid;
+      __syncthreads();
+      least_m = before[l.at[1]] + 1, most_m = before[l.at[2] + 1];
+    }
+    if (m_bin < kBins) {
+      const uint64_t lo = before[m_bin] > 1 ? before[m_bin] : 1, hi = before[m_bin + 1];
+      least_m = lo < least_m ? lo : least_m, most_m = hi < most_m ? hi : most_m;
+    }
+    if (holds(u_goal(p, least_m))) l.at[3] = tid;
+    if (holds(u_goal(p, most_m))) l.at[4] = tid;
+    __syncthreads();
+    from[0] = (int) l.at[3], to[0] = (int) l.at[4];
+    from[1] = by_p ? (int) l.at[1] : kBins, to[1] = by_p ? (int) l.at[2] : kBins;
+    from[2] = to[2] = k_bin;
+    from[3] = to[3] = m_bin;
+    // (a span within another is not looked for twice; those that are left come first)
+    int n = 1;
+#pragma unroll
+    for (int i = 1; i < 4; i++) {
+      bool in = from[i] >= kBins;
+      for (int j = 0; j < n; j++) in = in || (from[i] >= from[j] && to[i] <= to[j]);
+      const int f = from[i], g = to[i];
+      from[i] = to[i] = kBins;
+      if (!in) from[n] = f, to[n] = g, n++;
+    }
+  }
+  if (tid < 4) {
+    const int i = tid;
+    const double lo = (top - to[i] - 0.5) / sc.by, hi = (top - from[i] + 0.5) / sc.by;
+    const float fl = (float) (lo - 1e-6 * fabs(lo)), fh = (float) (hi + 1e-6 * fabs(hi));
+    p.from[i] = from[i], p.to[i] = to[i];
+    p.low[i] = from[i] >= kBins ? __builtin_inff() : fl == fl ? fl : -__builtin_inff();
+    p.high[i] = from[i] >= kBins ? -__builtin_inff() : fh < kGreatest<T> ? fh : __builtin_inff();
+  }
+  if (tid == 0) {
+    p.k_bin = k_bin;
+    int n = 0;
+    bool fits = !small;
+    for (int i = 0; i < 4 && fits; i++)
+      for (int b = from[i]; b <= to[i] && b < kBins && fits; b++) {
+        bool there = false;
+        for (int j = 0; j < n; j++) there = there || p.slot_bin[j] == b;
+        if (there) continue;
+        fits = n < kSlots;
+        if (fits) p.slot_bin[n] = b, p.slot_ahead[n] = ahead[b], p.slot_before[n] = before[b], n++;
+      }
+    p.slots = fits ? n : 0;
+  }
+  __syncthreads();
+}
+
+template <uint32_t T>
+__global__ __launch_bounds__(kSampleThreads) void plan_kernel(SampleArgs a) {
+  __shared__ PlanLds l;
+  const uint32_t t = blockIdx.x, tid = threadIdx.x, lane = tid & 63;
+  const Part* parts = (const Part*) a.parts + (uint64_t) t * a.slices;
+  const bool small = few(a.k(t));
+  // a lane a slice (64 of them a round), then a thread a bin
+  uint64_t first = ~0ull;
+  double top = -__builtin_inf();
+  uint32_t valid = 0;
+  for (uint32_t s = lane; s < a.slices; s += 64) {
+    const uint64_t f = parts[s].first;
+    if (f != ~0ull) top = fmax(top, parts[s].top), valid += parts[s].valid;
+    first = f < first ? f : first;
+  }
+#pragma unroll
+  for (int o = 32; o; o >>= 1) {
+    const uint64_t f = (uint64_t) (uint32_t) __shfl_xor((int) (first >> 32), o) << 32 | (uint32_t) __shfl_xor((int) first, o);
+    first = f < first ? f : first;
+    top = fmax(top, __shfl_xor(top, o));
+    valid += (uint32_t) __shfl_xor((int) valid, o);
+  }
+  Sum bin = {0, 0};
+#pragma unroll 4
+  for (uint32_t s = 0; s < a.slices; s++) {
+    const double by = top - parts[s].top;
+    const uint32_t j = by < kBins ? tid - (uint32_t) by : ~0u;
+    if (parts[s].first != ~0ull && j < parts[s].used) {
+      bin.n += parts[s].count[j];
+      if (!small) bin.m += parts[s].mass[j];
+    }
+  }
+  const Order<T> order = {a.bits};
+  make_plan<T>(a, t, order, l, first, top, valid, bin);
+  RowPlan* to = (RowPlan*) a.plans + t;
+  if (tid < sizeof(Plan) / 4) ((uint32_t*) &to->plan)[tid] = ((const uint32_t*) &l.plan)[tid];
+  if (l.plan.done) return;
+  to->prefix.before[tid + 1] = l.prefix.before[tid + 1], to->prefix.ahead[tid + 1] = l.prefix.ahead[tid + 1];
+  if (tid == 0) to->prefix.before[0] = 0, to->prefix.ahead[0] = 0;
+}
+
+// a token of the plan's bins
+template <uint32_t T>
+__device__ inline bool planned(const Plan& p, float x) {
+  const int b = Scale{p.by, p.top}.bin_of(ordered<T>(x));
+  return b < kBins && ((b >= p.from[0] && b <= p.to[0]) || (b >= p.from[1] && b <= p.to[1]) || (b >= p.from[2] && b <= p.to[2]) ||
+                       (b >= p.from[3] && b <= p.to[3]));
+}
+
+template <uint32_t T>
+__global__ __launch_bounds__(kSampleThreads) void list_kernel(SampleArgs a) {
+  __shared__ uint64_t list[kList];
+  __shared__ uint32_t listed, start;
+  const uint32_t t = blockIdx.x / a.slices, s = blockIdx.x - t * a.slices, begin = s * a.slice;
+  const uint32_t end = begin + a.slice < a.vocab ? begin + a.slice : a.vocab;
+  RowPlan* row_plan = (RowPlan*) a.plans + t;
+  const Plan& p = row_plan->plan;
+  Tokens<T, kPieces> row = {(const uint8_t*) a.logits + t * a.stride * kv::size_of(T), begin, end};
+  row.load(begin);
+  if (p.done) return;
+  const Order<T> order = {a.bits};
+  if (threadIdx.x == 0) listed = 0;
+  __syncthreads();
+  row.loaded_between(begin, p, [&](float x, uint32_t i) {
+    if (!planned<T>(p, x)) return;
+    const uint32_t at = atomicAdd(&listed, 1u);
+    if (at < kList) list[at] = order.place(ordered<T>(x), i);
+  });
+  __syncthreads();
+  if (threadIdx.x == 0 && listed) start = atomicAdd(&row_plan->plan.listed, listed);
+  __syncthreads();
+  for (uint32_t i = threadIdx.x; i < listed && i < kList; i += kSampleThreads)
+    if (start + i < kList) row_plan->list[start + i] = list[i];
+}
 
 struct Cut {
   uint64_t place;  // the last token
@@ -117,180 +579,351 @@ struct Cut {
   uint64_t m;      // their weights
 };
 
-template <uint32_t T>
-struct Row {
-  const void* p;
-  uint32_t vocab;
-  template <typename F>
-  __device__ inline void each(F f) const {
-    for (uint32_t i = threadIdx.x; i < vocab; i += kSampleThreads) {
-      const float x = logit_at<T>(p, i);
-      if (x > -__builtin_inff()) f(x, i);
-    }
-  }
-};
-
-// the first token of bin b with at least `rank` tokens of the bin up to it (MASS: with at least `goal` of weight up to it)
-template <bool MASS, typename R>
-__device__ Cut find(const R& row, const Scale& sc, SampleLds& l, int b, uint32_t rank, uint64_t goal) {
-  const double scale = l.scale[b];
-  const uint64_t before = l.before[b];
+// the first token of bin b with at least `rank` tokens of the bin up to it (MASS: with at least `goal` of weight up to it): a
+// thousandth of what is left each time
+template <uint32_t T, bool MASS>
+__device__ Cut find(Near<T>& row, const Scale& sc, const Prefix& prefix, DrawLds& l, int b, uint32_t rank, uint64_t goal) {
+  const double scale = bin_scale(b);
+  const uint64_t before = prefix.before[b];
+  const uint32_t tid = threadIdx.x;
   uint64_t lo = ~0ull, hi = ~0ull;  // (hi: the greatest place, inverted)
   row.each([&](float x, uint32_t i) {
-    if (sc.bin(__builtin_floor(sc.y(x))) != b) return;
-    const uint64_t at = place(x, i);
+    if (sc.bin_of(x) != b) return;
+    const uint64_t at = row.order.place(x, i);
     lo = at < lo ? at : lo, hi = ~at < hi ? ~at : hi;
   });
   lo = least(lo, l), hi = ~least(hi, l);
   Sum base = {0, 0};
-  for (;;) {
+  for (int level = 0; level < 6; level++) {  // (a place has 52 bits)
     const int bits = hi > lo ? 64 - __builtin_clzll(hi - lo) : 0, shift = bits > 10 ? bits - 10 : 0;
     __syncthreads();
-    l.part_n[threadIdx.x] = 0, l.part_m[threadIdx.x] = 0;
+    l.part_n[tid] = 0, l.part_m[tid] = 0, l.part_lo[tid] = ~0ull, l.part_hi[tid] = 0;
     __syncthreads();
     row.each([&](float x, uint32_t i) {
-      const double y = sc.y(x), floor = __builtin_floor(y);
-      if (sc.bin(floor) != b) return;
-      const uint64_t at = place(x, i);
+      const double y = sc.y(x), middle = __builtin_rint(y);
+      if (sc.bin(middle) != b) return;
+      const uint64_t at = row.order.place(x, i);
       if (at < lo || at > hi) return;
-      atomicAdd(&l.part_n[(at - lo) >> shift], 1u);
-      atomicAdd((unsigned long long*) &l.part_m[(at - lo) >> shift], (unsigned long long) whole(part_weight(y - floor) * kOne));
+      const uint32_t j = (uint32_t) ((at - lo) >> shift);
+      atomicAdd(&l.part_n[j], 1u);
+      atomicAdd((unsigned long long*) &l.part_m[j], (unsigned long long) whole_weight(y - middle));
+      atomicMin((unsigned long long*) &l.part_lo[j], (unsigned long long) at);
+      atomicMax((unsigned long long*) &l.part_hi[j], (unsigned long long) at);
     });
     __syncthreads();
-    const Sum own = {l.part_n[threadIdx.x], l.part_m[threadIdx.x]};
+    const Sum own = {l.part_n[tid], l.part_m[tid]};
     Sum sum = scan_sum(own, l);
     sum.n += base.n, sum.m += base.m;
     const Sum past = {sum.n - own.n, sum.m - own.m};
     const bool here = MASS ? before + whole((double) sum.m * scale) >= goal && before + whole((double) past.m * scale) < goal
                            : sum.n >= rank && past.n < rank;
-    if (here) l.found[0] = threadIdx.x, l.found[1] = shift ? past.n : sum.n, l.found[2] = shift ? past.m : sum.m;
+    if (here) {
+      const bool one = own.n == 1;
+      l.found[0] = l.part_lo[tid], l.found[1] = one ? l.part_lo[tid] : l.part_hi[tid];
+      l.found[2] = one ? sum.n : past.n, l.found[3] = one ? sum.m : past.m;
+    }
     __syncthreads();
-    base.n = (uint32_t) l.found[1], base.m = l.found[2];
-    lo += l.found[0] << shift;
-    if (!shift) return Cut{lo, l.ahead[b] + base.n, before + whole((double) base.m * scale)};
-    const uint64_t last = lo + (1ull << shift) - 1;
-    hi = last < hi ? last : hi;
+    lo = l.found[0], hi = l.found[1];
+    base.n = (uint32_t) l.found[2], base.m = l.found[3];
+    if (lo >= hi) break;
+  }
+  return Cut{lo, prefix.ahead[b] + base.n, before + whole((double) base.m * scale)};
+}
+
+// bins of more tokens than the list or a part holds, or limits that leave a bound over many bins: one by one, each bin looked
+// through as often as it takes
+template <uint32_t T>
+__device__ __attribute__((noinline)) void draw_slowly(const void* logits, uint32_t vocab, const Order<T>& order, const Plan& p, Prefix& prefix,
+                                                      const uint64_t* list, DrawLds& l, Cut& cut, Cut& d, double& least_y) {
+  const uint32_t tid = threadIdx.x;
+  const Scale sc = {p.by, p.top};
+  Near<T> near = {{logits, 0, vocab}, order, list, p.listed};
+  uint64_t all = p.all;
+  if (p.small) {  // (the bins' weights are not known yet)
+    l.part_m[tid] = 0;
+    __syncthreads();
+    near.each([&](float x, uint32_t) {
+      const double y = sc.y(x), middle = __builtin_rint(y);
+      const int b = sc.bin(middle);
+      if (b < kBins && b <= p.to[0]) atomicAdd((unsigned long long*) &l.part_m[b], (unsigned long long) whole_weight(y - middle));
+    });
+    __syncthreads();
+    const Sum sum = scan_sum(Sum{0, whole((double) l.part_m[tid] * bin_scale(tid))}, l);
+    prefix.before[tid + 1] = sum.m;
+    __syncthreads();
+    all = prefix.before[kBins];
+  }
+  auto by_mass = [&](uint64_t goal) {
+    if (prefix.before[tid + 1] >= goal && prefix.before[tid] < goal) l.at = tid;
+    __syncthreads();
+    const int b = (int) l.at;
+    const Cut c = find<T, true>(near, sc, prefix, l, b, 0, goal);
+    __syncthreads();
+    return c;
+  };
+  cut = Cut{~0ull, p.k ? p.k : p.valid, all};
+  if (p.k_bin < kBins) {
+    cut = find<T, false>(near, sc, prefix, l, p.k_bin, p.k - prefix.ahead[p.k_bin], 0);
+    __syncthreads();
+  }
+  if (p.by_p) cut = by_mass(p_goal(p, cut.m));
+  if (p.m_bin < kBins) {
+    Sum in = {0, 0};
+    near.each([&](float x, uint32_t) {
+      const double y = sc.y(x), middle = __builtin_rint(y);
+      if (y >= p.edge && sc.bin(middle) == p.m_bin) in.n++, in.m += whole_weight(y - middle);
+    });
+    in = total(in, l);
+    in = {prefix.ahead[p.m_bin] + in.n, prefix.before[p.m_bin] + whole((double) in.m * bin_scale(p.m_bin))};
+    if (in.n < cut.n) cut.n = in.n, cut.m = in.m, least_y = p.edge;
+  }
+  d = by_mass(u_goal(p, cut.m));
+}
+
+// the choice among the listed tokens: each one's count and weight up to it. a token's bin (a few: any bin up to the k-th token's;
+// else a slot's bin cut into 128 parts) has its tokens together, and each is compared with the others of its part
+template <uint32_t T>
+__device__ inline void draw(const SampleArgs& a, uint32_t t, const Order<T>& order, const Plan& p, Prefix& prefix, bool loaded, const uint64_t* list,
+                            DrawLds& l) {
+  const uint32_t tid = threadIdx.x, n = p.listed;
+  const void* logits = (const uint8_t*) a.logits + t * a.stride * kv::size_of(T);
+  const Scale sc = {p.by, p.top};
+  const bool small = p.small;
+  if (tid < kSlots) l.lo[tid] = ~0ull, l.hi[tid] = 0;
+  if (tid < 4) l.found[tid] = 0;
+  if (tid == 0) l.crowded = n > kList || (!small && !p.slots), l.at = 0;
+  l.part_n[tid] = 0, l.part_m[tid] = 0, l.filled[tid] = 0;
+  Cut cut = {~0ull, p.k ? p.k : p.valid, p.all}, d;
+  double least_y = -__builtin_inf();
+  uint64_t at[2], weight[2];
+  int bin[2], slot[2];
+  uint32_t part[2];
+  __syncthreads();
+  if (!l.crowded) {
+#pragma unroll
+    for (int j = 0; j < 2; j++) {
+      const uint32_t i = tid + j * kSampleThreads;
+      slot[j] = -1, bin[j] = kBins;
+      if (i >= n) continue;
+      at[j] = list[i];
+      const double y = sc.y(order.logit(at[j])), middle = __builtin_rint(y);
+      weight[j] = whole_weight(y - middle);
+      bin[j] = sc.bin(middle);
+      if (small) {
+        slot[j] = 0;
+        continue;
+      }
+#pragma unroll
+      for (int q = 0; q < kSlots; q++) slot[j] = q < p.slots && bin[j] == p.slot_bin[q] ? q : slot[j];
+      if (slot[j] < 0) continue;
+      atomicMin((unsigned long long*) &l.lo[slot[j]], (unsigned long long) at[j]);
+      atomicMax((unsigned long long*) &l.hi[slot[j]], (unsigned long long) at[j]);
+    }
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < 2; j++) {
+      if (slot[j] < 0) continue;
+      part[j] = bin[j];
+      if (!small) {
+        const uint64_t lo = l.lo[slot[j]], span = l.hi[slot[j]] - lo;
+        const int bits = span ? 64 - __builtin_clzll(span) : 0;
+        part[j] = slot[j] * kParts + (uint32_t) ((at[j] - lo) >> (bits > 7 ? bits - 7 : 0));
+      }
+      atomicAdd(&l.part_n[part[j]], 1u);
+      atomicAdd((unsigned long long*) &l.part_m[part[j]], (unsigned long long) weight[j]);
+    }
+    __syncthreads();
+    const Sum own = {l.part_n[tid], small ? whole((double) l.part_m[tid] * bin_scale(tid)) : l.part_m[tid]};
+    const Sum sum = scan_sum(own, l);
+    // (part_lo and part_hi: the parts' sums of weights and counts before them)
+    l.part_lo[tid] = sum.m - own.m, l.part_hi[tid] = sum.n - own.n;
+    if (own.n > kCrowd) l.crowded = 1;
+    if (tid == kSampleThreads - 1) l.last_m = sum.m;
+    __syncthreads();
+  }
+  if (l.crowded) {
+    if (!loaded) {
+      const Prefix& from = ((const RowPlan*) a.plans + t)->prefix;
+      prefix.before[tid] = from.before[tid], prefix.ahead[tid] = from.ahead[tid];
+      if (tid == 0) prefix.before[kBins] = from.before[kBins], prefix.ahead[kBins] = from.ahead[kBins];
+      __syncthreads();
+    }
+    draw_slowly<T>(logits, a.vocab, order, p, prefix, list, l, cut, d, least_y);
+  } else {
+    if (small) cut.m = l.last_m;
+#pragma unroll
+    for (int j = 0; j < 2; j++) {
+      if (slot[j] < 0) continue;
+      const uint32_t i = (uint32_t) l.part_hi[part[j]] + atomicAdd(&l.filled[part[j]], 1u);
+      l.sorted[i] = at[j], l.weight[i] = weight[j];
+    }
+    __syncthreads();
+    if (tid == 0) l.last_n = 0, l.last_m = 0;
+    uint32_t upto_n[2];
+    uint64_t upto_m[2], past_m[2];
+#pragma unroll
+    for (int j = 0; j < 2; j++) {
+      if (slot[j] < 0) continue;
+      const uint32_t q = part[j], start = (uint32_t) l.part_hi[q], count = l.part_n[q], base = slot[j] * kParts;
+      uint32_t less = 0;
+      uint64_t m = 0;
+      for (uint32_t i = start; i < start + count; i++) {
+        const bool first = l.sorted[i] < at[j];
+        less += first, m += first ? l.weight[i] : 0;
+      }
+      const double scale = bin_scale(bin[j]);
+      uint64_t ahead_m = l.part_lo[q];
+      upto_n[j] = start + less + 1;
+      if (!small) {
+        m += ahead_m - l.part_lo[base], ahead_m = p.slot_before[slot[j]];
+        upto_n[j] += p.slot_ahead[slot[j]] - (uint32_t) l.part_hi[base];
+      }
+      upto_m[j] = ahead_m + whole((double) (m + weight[j]) * scale);
+      past_m[j] = ahead_m + whole((double) m * scale);
+    }
+    auto take = [&](auto is) {
+#pragma unroll
+      for (int j = 0; j < 2; j++)
+        if (slot[j] >= 0 && is(j)) l.found[0] = at[j], l.found[1] = upto_n[j], l.found[2] = upto_m[j];
+      __syncthreads();
+      const Cut c = {l.found[0], (uint32_t) l.found[1], l.found[2]};
+      __syncthreads();
+      return c;
+    };
+    if (p.k_bin < kBins) cut = take([&](int j) { return upto_n[j] == p.k; });
+    if (p.by_p) {
+      const uint64_t goal = p_goal(p, cut.m);
+      cut = take([&](int j) { return upto_m[j] >= goal && past_m[j] < goal; });
+    }
+    if (p.m_bin < kBins) {
+      __syncthreads();
+#pragma unroll
+      for (int j = 0; j < 2; j++)
+        if (slot[j] >= 0 && sc.y(order.logit(at[j])) >= p.edge) {
+          atomicMax(&l.last_n, upto_n[j]);
+          atomicMax((unsigned long long*) &l.last_m, (unsigned long long) upto_m[j]);
+        }
+      __syncthreads();
+      uint32_t last_n = l.last_n;
+      uint64_t last_m = l.last_m;
+      if (!small)
+        for (int q = 0; q < p.slots; q++)  // (none of that bin: all before it)
+          if (p.slot_bin[q] == p.m_bin && p.slot_ahead[q] > last_n) last_n = p.slot_ahead[q], last_m = p.slot_before[q];
+      if (last_n < cut.n) cut.n = last_n, cut.m = last_m, least_y = p.edge;
+    }
+    const uint64_t goal = u_goal(p, cut.m);
+    d = take([&](int j) { return upto_m[j] >= goal && past_m[j] < goal; });
+  }
+  const double share = kOne / (double) cut.m;
+  if (tid == 0) {
+    const double y = sc.y(order.logit(d.place)), middle = __builtin_rint(y);
+    a.token[t] = (int32_t) order.index(d.place);
+    if (a.prob) a.prob[t] = (float) (part_weight(y - middle) * bin_scale(sc.bin(middle)) * share);
+    if (a.kept) a.kept[t] = (int32_t) cut.n;
+    if (a.probs) ((Drawn*) a.cuts)[t] = Drawn{cut.place, sc.by, sc.top, least_y, share};
   }
 }
 
 template <uint32_t T>
-__global__ __launch_bounds__(kSampleThreads) void sample_kernel(SampleArgs a) {
-  __shared__ SampleLds l;
-  const uint32_t t = blockIdx.x, tid = threadIdx.x;
-  const Row<T> row = {(const uint8_t*) a.logits + t * a.stride * kv::size_of(T), a.vocab};
-  const float temperature = a.temperature ? a.temperature[t] : 1.0f;
-  uint64_t first = ~0ull;
-  row.each([&](float x, uint32_t i) {
-    const uint64_t at = place(x, i);
-    first = at < first ? at : first;
-  });
-  first = least(first, l);
-  float* probs = a.probs ? a.probs + (uint64_t) t * a.vocab : nullptr;
-  const bool greedy = !(temperature > 0.0f);
-  if (first == ~0ull || greedy) {
-    const bool none = first == ~0ull;
-    if (tid == 0) {
-      a.token[t] = none ? -1 : (int32_t) (uint32_t) first;
-      if (a.prob) a.prob[t] = none ? 0.0f : 1.0f;
-      if (a.kept) a.kept[t] = none ? 0 : 1;
-    }
-    if (probs)
-      for (uint32_t i = tid; i < a.vocab; i += kSampleThreads) probs[i] = !none && i == (uint32_t) first ? 1.0f : 0.0f;
-    return;
-  }
-  const float most = logit_at<T>(row.p, (uint32_t) first);
-  Scale sc;
-  sc.by = kOctave * 1.4426950408889634074 / (double) temperature;
-  sc.top = __builtin_floor(sc.y(most));
-  l.count[tid] = 0, l.mass[tid] = 0;
-  if (tid < 4) l.found[tid] = 0;
-  l.scale[tid] = exp2(-(double) (int) tid / kOctave);
+__global__ __launch_bounds__(kSampleThreads) void draw_kernel(SampleArgs a) {
+  __shared__ DrawLds l;
+  __shared__ Prefix prefix;
+  __shared__ Plan p;
+  const RowPlan* from = (const RowPlan*) a.plans + blockIdx.x;
+  if (threadIdx.x < sizeof(Plan) / 4) ((uint32_t*) &p)[threadIdx.x] = ((const uint32_t*) &from->plan)[threadIdx.x];
   __syncthreads();
-  uint32_t valid = 0;
-  row.each([&](float x, uint32_t i) {
-    const double y = sc.y(x), floor = __builtin_floor(y);
-    const int b = sc.bin(floor);
-    valid++;
-    if (b >= kBins) return;
-    atomicAdd(&l.count[b], 1u);
-    atomicAdd((unsigned long long*) &l.mass[b], (unsigned long long) whole(part_weight(y - floor) * kOne));
+  if (p.done) return;
+  const Order<T> order = {a.bits};
+  draw<T>(a, blockIdx.x, order, p, prefix, false, from->list, l);
+}
+
+// a row of one slice
+template <uint32_t T>
+__global__ __launch_bounds__(kSampleThreads) void sample_kernel(SampleArgs a) {
+  __shared__ WholeLds l;
+  const uint32_t t = blockIdx.x;
+  Tokens<T, kPieces> row = {(const uint8_t*) a.logits + t * a.stride * kv::size_of(T), 0, a.vocab};
+  const Order<T> order = {a.bits};
+  uint64_t first;
+  double top;
+  uint32_t valid;
+  scan_slice<T>(row, order, a.heat(t), a.k(t), l.scan, first, top, valid);
+  Sum bin = {0, 0};
+  if (valid) bin = {l.scan.count[threadIdx.x], l.scan.mass[threadIdx.x]};
+  make_plan<T>(a, t, order, l, first, top, valid, bin);
+  if (l.plan.done) return;
+  row.loaded_between(0, l.plan, [&](float x, uint32_t i) {
+    if (!planned<T>(l.plan, x)) return;
+    const uint32_t at = atomicAdd(&l.plan.listed, 1u);
+    if (at < kList) l.list[at] = order.place(ordered<T>(x), i);
   });
-  {
-    const Sum all = scan_sum(Sum{valid, 0}, l);
-    if (tid == kSampleThreads - 1) l.found[0] = all.n;
-    __syncthreads();
-    valid = (uint32_t) l.found[0];
-    const Sum sum = scan_sum(Sum{l.count[tid], whole((double) l.mass[tid] * l.scale[tid])}, l);
-    l.ahead[tid + 1] = sum.n, l.before[tid + 1] = sum.m;
-    if (tid == 0) l.ahead[0] = 0, l.before[0] = 0;
-    __syncthreads();
-  }
-  Cut cut = {~0ull, valid, l.before[kBins]};
-  auto by_rank = [&](uint32_t rank) {
-    if (rank > l.ahead[kBins]) {  // (among tokens of no weight)
-      cut.n = rank;
-      return;
-    }
-    if (l.ahead[tid + 1] >= rank && l.ahead[tid] < rank) l.found[3] = tid;
-    __syncthreads();
-    const int b = (int) l.found[3];
-    cut = find<false>(row, sc, l, b, rank - l.ahead[b], 0);
-    __syncthreads();
-  };
-  auto by_mass = [&](uint64_t goal) {
-    if (l.before[tid + 1] >= goal && l.before[tid] < goal) l.found[3] = tid;
-    __syncthreads();
-    const int b = (int) l.found[3];
-    const Cut c = find<true>(row, sc, l, b, 0, goal);
-    __syncthreads();
-    return c;
-  };
-  const int32_t k = a.top_k ? a.top_k[t] : 0;
-  if (k > 0 && (uint32_t) k < cut.n) by_rank((uint32_t) k);
-  const float p = a.top_p ? a.top_p[t] : 1.0f;
-  if (p < 1.0f) {
-    const double goal = (double) cut.m * (double) (p > 0.0f ? p : 0.0f);
-    cut = by_mass(goal > 1.0 ? (uint64_t) __builtin_ceil(goal) : 1);
-  }
-  const float min_p = a.min_p ? a.min_p[t] : 0.0f;
-  if (min_p > 0.0f) {
-    const double edge = sc.y(most) + kOctave * log2((double) (min_p < 1.0f ? min_p : 1.0f));
-    const int b = sc.bin(__builtin_floor(edge));
-    if (b < kBins) {
-      uint32_t in = 0;
-      row.each([&](float x, uint32_t i) {
-        const double y = sc.y(x);
-        in += y >= edge && sc.bin(__builtin_floor(y)) == b;
-      });
-      const Sum all = scan_sum(Sum{in, 0}, l);
-      if (tid == kSampleThreads - 1) l.found[0] = all.n;
-      __syncthreads();
-      const uint32_t n = l.ahead[b] + (uint32_t) l.found[0];
-      __syncthreads();
-      if (n < cut.n) by_rank(n ? n : 1);
+  __syncthreads();
+  draw<T>(a, t, order, l.plan, l.prefix, true, l.list, l.draw);
+}
+
+// every token's part of the kept weights
+template <uint32_t T>
+__global__ __launch_bounds__(kSampleThreads) void probs_kernel(SampleArgs a, uint32_t chunks) {
+  __shared__ double scale[kBins];
+  const uint32_t t = blockIdx.x / chunks, end = a.vocab;
+  const Drawn d = ((const Drawn*) a.cuts)[t];
+  const void* p = (const uint8_t*) a.logits + t * a.stride * kv::size_of(T);
+  float* out = a.probs + (uint64_t) t * a.vocab;
+  const Scale sc = {d.by, d.top};
+  const Order<T> order = {a.bits};
+  scale[threadIdx.x] = exp2(-(double) (int) threadIdx.x / kOctave) * d.share;
+  __syncthreads();
+  const uint32_t i = ((blockIdx.x - t * chunks) * kSampleThreads + threadIdx.x) * kPer<T>;
+  if (i < end) {
+    float x[kPer<T>];
+    logits_at<T>(p, i, end, x);
+#pragma unroll
+    for (uint32_t j = 0; j < kPer<T>; j++) {
+      float v = 0.0f;
+      x[j] = ordered<T>(x[j]);
+      if (x[j] > -__builtin_inff() && order.place(x[j], i + j) <= d.last) {
+        if (d.share == 0.0) {
+          v = order.place(x[j], i + j) == d.last ? 1.0f : 0.0f;
+        } else {
+          const double y = sc.y(x[j]), middle = __builtin_rint(y);
+          const int b = sc.bin(middle);
+          if (b < kBins && y >= d.least_y) v = (float) (part_weight(y - middle) * scale[b]);
+        }
+      }
+      if (i + j < end) out[i + j] = v;
     }
   }
-  const float u = a.u[t];
-  uint64_t goal = (uint64_t) __builtin_floor((double) cut.m * (double) (u > 0.0f ? u < 1.0f ? u : 0.99999994f : 0.0f)) + 1;
-  if (goal > cut.m) goal = cut.m;
-  const Cut drawn = by_mass(goal);
-  const uint32_t token = (uint32_t) drawn.place;
-  const double by = 1.0 / ((double) cut.m / kOne);
-  auto share = [&](float x) {
-    const double y = sc.y(x), floor = __builtin_floor(y);
-    const int b = sc.bin(floor);
-    return b < kBins ? (float) (part_weight(y - floor) * l.scale[b] * by) : 0.0f;
-  };
-  if (tid == 0) {
-    a.token[t] = (int32_t) token;
-    if (a.prob) a.prob[t] = share(logit_at<T>(row.p, token));
-    if (a.kept) a.kept[t] = (int32_t) cut.n;
+}
+
+inline int index_bits(uint32_t vocab) { return vocab > 1 ? 32 - __builtin_clz(vocab - 1) : 0; }
+inline uint32_t slice_of(const OsmosSample* a) { return a->type == OSMOS_F32 ? kSampleThreads * 4 * kPieces : kSampleThreads * 8 * kPieces; }
+inline uint32_t slices_of(const OsmosSample* a) { return (a->vocab + slice_of(a) - 1) / slice_of(a); }
+inline uint64_t round256(uint64_t n) { return (n + 255) / 256 * 256; }
+struct SampleRoom {
+  uint64_t parts, plans, cuts;
+};
+inline SampleRoom room_of(const OsmosSample* a) {
+  const uint64_t rows = a->n, slices = slices_of(a);
+  return {slices > 1 ? round256(rows * slices * sizeof(Part)) : 0, slices > 1 ? round256(rows * sizeof(RowPlan)) : 0,
+          a->probs ? round256(rows * sizeof(Drawn)) : 0};
+}
+
+template <uint32_t T>
+bool sample_launch(const SampleArgs& a, hipStream_t s) {
+  if (a.slices > 1) {
+    scan_kernel<T><<<a.n * a.slices, kSampleThreads, 0, s>>>(a);
+    plan_kernel<T><<<a.n, kSampleThreads, 0, s>>>(a);
+    list_kernel<T><<<a.n * a.slices, kSampleThreads, 0, s>>>(a);
+    draw_kernel<T><<<a.n, kSampleThreads, 0, s>>>(a);
+  } else {
+    sample_kernel<T><<<a.n, kSampleThreads, 0, s>>>(a);
   }
-  if (probs)
-    for (uint32_t i = tid; i < a.vocab; i += kSampleThreads) {
-      const float x = logit_at<T>(row.p, i);
-      probs[i] = x > -__builtin_inff() && place(x, i) <= cut.place ? share(x) : 0.0f;
-    }
+  if (a.probs) {
+    const uint32_t each = kSampleThreads * kPer<T>;
+    const uint32_t chunks = (a.vocab + each - 1) / each;
+    probs_kernel<T><<<a.n * chunks, kSampleThreads, 0, s>>>(a, chunks);
+  }
+  return hipGetLastError() == hipSuccess;
 }
 
 }  // namespace rows
@@ -298,13 +931,20 @@ __global__ __launch_bounds__(kSampleThreads) void sample_kernel(SampleArgs a) {
 
 using namespace osm;
 
-extern "C" OSM_API uint64_t osmos_sample_workspace(const OsmosSample* a) { return 0; }
+extern "C" OSM_API uint64_t osmos_sample_workspace(const OsmosSample* a) {
+  if (!rows::sample_ok(a)) return 0;
+  const rows::SampleRoom r = rows::room_of(a);
+  return r.parts + r.plans + r.cuts;
+}
 
 extern "C" OSM_API bool osmos_sample(const OsmosSample* a, void* workspace, uint64_t workspace_bytes, void* stream) {
-  if (!rows::sample_ok(a)) return false;
+  const uint64_t need = osmos_sample_workspace(a);
+  if (!rows::sample_ok(a) || (need && (!workspace || !rows::aligned(workspace, 256) || workspace_bytes < need))) return false;
+  const rows::SampleRoom r = rows::room_of(a);
+  uint8_t* w = (uint8_t*) workspace;
   const rows::SampleArgs b = {a->logits, a->u, a->temperature, a->top_p, a->min_p, a->top_k, a->token, a->kept, a->prob, a->probs, a->stride,
-                              a->n, a->vocab};
-  auto* kernel = a->type == OSMOS_F32 ? rows::sample_kernel<OSMOS_F32> : a->type == OSMOS_F16 ? rows::sample_kernel<OSMOS_F16> : rows::sample_kernel<OSMOS_BF16>;
-  kernel<<<a->n, rows::kSampleThreads, 0, (hipStream_t) stream>>>(b);
-  return hipGetLastError() == hipSuccess;
+                              a->n, a->vocab, rows::slices_of(a), rows::slice_of(a), rows::index_bits(a->vocab), w, w + r.parts,
+                              w + r.parts + r.plans};
+  return a->type == OSMOS_F32 ? rows::sample_launch<OSMOS_F32>(b, (hipStream_t) stream)
+         : a->type == OSMOS_F16 ? rows::sample_launch<OSMOS_F16>(b, (hipStream_t) stream) : rows::sample_launch<OSMOS_BF16>(b, (hipStream_t) stream);
 }
