@@ -9,6 +9,8 @@
 // the token lie in, list_kernel lists these bins' tokens, draw_kernel chooses among them. bins are whole numbers of y, so that slices
 // agree on them without knowing the row's maximum; a slice keeps the 1024 below its own. a short row is one kernel, its tokens in
 // registers.
+#include <type_traits>
+
 #include "rowshost.h"
 #include "common.h"
 
@@ -21,7 +23,6 @@ constexpr double kOctave = 23.0;
 constexpr double kOne = 4398046511104.0;  // 2^42: 2^20 tokens of up to 2^(1 / 46) stay under 2^63
 constexpr uint32_t kList = 2048;      // tokens that are looked at in LDS; more are looked for in the row each time
 constexpr uint32_t kFew = 1024;       // a top_k up to this needs the weights of its own tokens alone: they are listed
-constexpr int kSlots = 8, kParts = kBins / kSlots;  // bins that are looked into at once, parts of each
 constexpr uint32_t kCrowd = 64;       // tokens of a part that are compared with one another
 
 // a logit as the order takes it: +infinity as the type's greatest value (a NaN stays one, and is greater than nothing)
@@ -93,7 +94,7 @@ __device__ inline bool few(int32_t k) { return k > 0 && (uint32_t) k <= kFew; }
 struct Part {
   uint64_t first;  // the place of its first token; ~0: none
   double top;      // its first bin
-  uint32_t valid, used;  // tokens that can be chosen; bins from the first on that are not empty
+  uint32_t valid;  // tokens that can be chosen; 0 for a greedy row too, and then no bins
   uint64_t mass[kBins];  // (unused for a few)
   uint32_t count[kBins];
 };
@@ -115,12 +116,10 @@ struct Plan {
   uint32_t valid, listed;   // tokens that can be chosen, that are listed (more than kList: those past it are not)
   uint32_t k;               // top_k where it limits, or 0; k_bin kBins: among tokens of no weight
   int k_bin, m_bin;         // kBins: none
-  int done, small, by_p, slots;  // done: the row's token is given already; small: all bins up to slot_bin[0] are listed; slots 0: too many
-  int from[4], to[4];       // the listed bins, by logit from low to high
-  float low[4], high[4];
-  int slot_bin[kSlots];
-  uint32_t slot_ahead[kSlots];
-  uint64_t slot_before[kSlots];
+  int done, small, by_p;    // done: the row's token is given already; small: all bins up to to[0] are listed, whatever their weights
+  int split;                // a listed bin's parts, as a power of two
+  int from[4], to[4], slot[4];  // the listed bins, apart from one another (kBins: none); how many are listed before a span's
+  float low[4], high[4];    // these spans' logits, a little wide
 };
 // a row's bins' prefix sums: weights (of kOne the first bin's middle) and tokens
 struct Prefix {
@@ -137,8 +136,14 @@ struct ScanLds {
   uint64_t mass[kBins];
   uint32_t count[kBins];
   Sum wave[kSampleWaves];
-  uint64_t word[kSampleWaves];
+  float greatest[kSampleWaves];
+  uint32_t index;
 };
+constexpr int kValues = 4096;  // bf16: the values of 2^-8 to 2^8 of either sign
+struct ValueLds : ScanLds {
+  uint32_t value[kValues];
+};
+template <uint32_t T> using ScanOf = std::conditional_t<T == OSMOS_BF16, ValueLds, ScanLds>;
 struct PlanLds {
   Plan plan;
   Prefix prefix;
@@ -147,16 +152,17 @@ struct PlanLds {
   uint32_t at[8];
 };
 struct DrawLds {
-  uint64_t part_m[kBins], part_lo[kBins], part_hi[kBins];
-  uint32_t part_n[kBins], filled[kBins];
+  uint64_t part_m[kBins], part_lo[kBins], part_hi[kBins];  // sums of weights; least and greatest places
+  uint32_t part_n[kBins], before_n[kBins], filled[kBins];
   uint64_t sorted[kList], weight[kList];
   Sum wave[kSampleWaves];
-  uint64_t word[kSampleWaves], found[4], lo[kSlots], hi[kSlots], last_m;
-  uint32_t at, crowded, last_n;
+  uint64_t word[kSampleWaves], found[4], sum;
+  uint32_t at, crowded;
 };
+template <uint32_t T>
 struct WholeLds : PlanLds {
   union {
-    ScanLds scan;
+    ScanOf<T> scan;
     DrawLds draw;
   };
   uint64_t list[kList];
@@ -185,6 +191,12 @@ __device__ inline uint64_t wave_least(uint64_t x) {  // lane 63: of all
   const uint64_t y = from_below<STEP>(x, ~0ull);
   x = y < x ? y : x;
   if constexpr (STEP < 5) return wave_least<STEP + 1>(x);
+  else return x;
+}
+template <int STEP = 0>
+__device__ inline float wave_greatest(float x) {  // lane 63: of all
+  x = fmaxf(x, __uint_as_float(from_below<STEP>(__float_as_uint(x), 0xFF800000u)));
+  if constexpr (STEP < 5) return wave_greatest<STEP + 1>(x);
   else return x;
 }
 // inclusive sums over the workgroup's threads in their order
@@ -283,21 +295,28 @@ struct Tokens {
 #pragma unroll
       for (uint32_t j = 0; j < kPer<T>; j++) f(x[k][j], at + (k * kSampleThreads + threadIdx.x) * kPer<T> + j);
   }
-  // those from low to high
+  // those of a plan's spans' logits: most threads have none, so they are read again
   template <typename F>
   __device__ inline void loaded_between(uint32_t at, const Plan& p, F f) const {
     const float l0 = p.low[0], h0 = p.high[0], l1 = p.low[1], h1 = p.high[1], l2 = p.low[2], h2 = p.high[2], l3 = p.low[3], h3 = p.high[3];
     const int spans = l3 <= h3 ? 4 : l2 <= h2 ? 3 : l1 <= h1 ? 2 : 1;
+    uint32_t hits = 0;
     auto test = [&](auto in) __attribute__((always_inline)) {
 #pragma unroll
       for (int k = 0; k < P; k++)
 #pragma unroll
-        for (uint32_t j = 0; j < kPer<T>; j++)
-          if (in(x[k][j])) f(x[k][j], at + (k * kSampleThreads + threadIdx.x) * kPer<T> + j);
+        for (uint32_t j = 0; j < kPer<T>; j++) hits |= in(x[k][j]) ? 1u << (k * kPer<T> + j) : 0;
     };
+    static_assert(P * kPer<T> <= 32);
     if (spans == 1) test([&](float v) { return v >= l0 && v <= h0; });
     else if (spans == 2) test([&](float v) { return (v >= l0 && v <= h0) || (v >= l1 && v <= h1); });
     else test([&](float v) { return (v >= l0 && v <= h0) || (v >= l1 && v <= h1) || (v >= l2 && v <= h2) || (v >= l3 && v <= h3); });
+    while (hits) {
+      const uint32_t h = __builtin_ctz(hits);
+      hits &= hits - 1;
+      const uint32_t i = at + (h / kPer<T> * kSampleThreads + threadIdx.x) * kPer<T> + h % kPer<T>;
+      f(logit_at<T>(this->p, i), i);
+    }
   }
   // in ascending order of a thread's own tokens
   template <typename F>
@@ -328,64 +347,109 @@ struct Near {
   }
 };
 
-// a slice's first place and, but for a greedy row, its bins (into l.count and, unless k is small, l.mass): its tokens are one round
+// a slice's first place and, but for a greedy row, its bins (into l.count and, unless k is small, l.mass): its tokens are one round.
+// bf16's tokens are few values, often: they are counted by value, and each value is put into its bin once
 template <uint32_t T, typename R, typename L>
 __device__ inline void scan_slice(R& row, const Order<T>& order, float temperature, int32_t k, L& l, uint64_t& first, double& top, uint32_t& valid) {
+  const uint32_t tid = threadIdx.x;
+  const float none = -__builtin_inff();
   row.load(row.begin);
-  l.mass[threadIdx.x] = 0, l.count[threadIdx.x] = 0;
-  float best = -__builtin_inff();
-  uint32_t at = 0;
-  row.loaded(row.begin, [&](float x, uint32_t i) {
-    x = ordered<T>(x);
-    if (x > best) best = x, at = i;
-  });
-  first = least(best > -__builtin_inff() ? order.place(best, at) : ~0ull, l);
-  top = 0.0, valid = 0;
-  if (first == ~0ull || !(temperature > 0.0f)) return;
+  l.mass[tid] = 0, l.count[tid] = 0;
+  if constexpr (T == OSMOS_BF16)
+    for (int i = 0; i < kValues; i += kSampleThreads) l.value[i + tid] = 0;
+  if (tid == 0) l.index = ~0u;
+  float best = none;
+  row.loaded(row.begin, [&](float x, uint32_t) { best = fmaxf(best, x); });
+  float most = wave_greatest(best);
+  if ((tid & 63) == 63) l.greatest[tid / 64] = most;
+  __syncthreads();
+  most = l.greatest[0];
+#pragma unroll
+  for (int w = 1; w < kSampleWaves; w++) most = fmaxf(most, l.greatest[w]);
+  most = ordered<T>(most);
+  first = ~0ull, top = 0.0, valid = 0;
+  if (!(most > none)) return;
+  if (ordered<T>(best) == most) {  // (the lowest index among equals)
+    uint32_t at = ~0u;
+    row.loaded(row.begin, [&](float x, uint32_t i) { at = ordered<T>(x) == most && i < at ? i : at; });
+    atomicMin(&l.index, at);
+  }
+  if (!(temperature > 0.0f)) {
+    __syncthreads();
+    first = order.place(most, l.index);
+    return;
+  }
   Scale sc = {bins_a_unit(temperature), 0.0};
-  sc.top = top = __builtin_rint(sc.y(order.logit(first)));
-  const bool counts = few(k);
-  auto add = [&](float x, bool mass) __attribute__((always_inline)) {
+  sc.top = top = __builtin_rint(sc.y(most));
+  auto add = [&](float x, uint32_t n, bool mass) __attribute__((always_inline)) {
     x = ordered<T>(x);
     const double y = sc.y(x), middle = __builtin_rint(y), b = sc.top - middle;
     if (b < kBins) {
       const int i = (int) b;
-      atomicAdd(&l.count[i], 1u);
-      if (mass) atomicAdd((unsigned long long*) &l.mass[i], (unsigned long long) whole_weight(y - middle));
+      atomicAdd(&l.count[i], n);
+      if (mass) atomicAdd((unsigned long long*) &l.mass[i], (unsigned long long) (n * whole_weight(y - middle)));
     } else {
-      valid += x > -__builtin_inff();
+      valid += x > none ? n : 0;
     }
   };
-  if (counts) row.loaded(row.begin, [&](float x, uint32_t) { add(x, false); });
-  else row.loaded(row.begin, [&](float x, uint32_t) { add(x, true); });
+  const bool mass = !few(k);
+  if constexpr (T == OSMOS_BF16) {
+    constexpr uint32_t least_bits = 0x3B80, span = kValues / 2;  // 2^-8; the first and the last of the span stand for what is outside
+    auto value = [](float x) __attribute__((always_inline)) {
+      const uint32_t b = __float_as_uint(x) >> 16 & 0x7FFF;
+      return (b < least_bits ? least_bits : b > least_bits + span - 1 ? least_bits + span - 1 : b) - least_bits;
+    };
+    bool outside = false;
+    row.loaded(row.begin, [&](float x, uint32_t) {
+      const uint32_t v = value(x);
+      if (v - 1 < span - 2) atomicAdd(&l.value[(__float_as_uint(x) >> 31) * span + v], 1u);
+      else outside = true;
+    });
+    if (outside)
+      row.loaded(row.begin, [&](float x, uint32_t) {
+        if (value(x) - 1 >= span - 2) add(x, 1, mass);
+      });
+    __syncthreads();
+    for (uint32_t i = tid; i < kValues; i += kSampleThreads) {
+      const uint32_t n = l.value[i];
+      if (n) add(__uint_as_float(((i % span) + least_bits) << 16 | i / span << 31), n, mass);
+    }
+  } else {
+    if (mass) row.loaded(row.begin, [&](float x, uint32_t) { add(x, 1, true); });
+    else row.loaded(row.begin, [&](float x, uint32_t) { add(x, 1, false); });
+  }
   __syncthreads();
-  valid = total(Sum{valid + l.count[threadIdx.x], 0}, l).n;
+  first = order.place(most, l.index);
+  valid = total(Sum{valid + l.count[tid], 0}, l).n;
 }
 
 constexpr int kPieces = 4;  // 16 bytes of a slice a thread
 template <uint32_t T>
 __global__ __launch_bounds__(kSampleThreads) void scan_kernel(SampleArgs a) {
-  __shared__ ScanLds l;
-  const uint32_t t = blockIdx.x / a.slices, s = blockIdx.x - t * a.slices, begin = s * a.slice;
+  __shared__ ScanOf<T> l;
+  const uint32_t t = blockIdx.x / a.slices, s = blockIdx.x - t * a.slices, begin = s * a.slice, tid = threadIdx.x;
   const uint32_t end = begin + a.slice < a.vocab ? begin + a.slice : a.vocab;
   Tokens<T, kPieces> row = {(const uint8_t*) a.logits + t * a.stride * kv::size_of(T), begin, end};
   Part* part = (Part*) a.parts + blockIdx.x;
   const Order<T> order = {a.bits};
+  const int32_t k = a.k(t);
   uint64_t first;
   double top;
   uint32_t valid;
-  scan_slice<T>(row, order, a.heat(t), a.k(t), l, first, top, valid);
-  const uint32_t n = valid ? l.count[threadIdx.x] : 0;
-  const uint32_t used = ~(uint32_t) least(~(uint64_t) (n ? threadIdx.x + 1 : 0), l);
-  if (threadIdx.x < used) {
-    part->count[threadIdx.x] = n;
-    if (!few(a.k(t))) part->mass[threadIdx.x] = l.mass[threadIdx.x];
+  scan_slice<T>(row, order, a.heat(t), k, l, first, top, valid);
+  if (valid) {
+    part->count[tid] = l.count[tid];
+    if (!few(k)) part->mass[tid] = l.mass[tid];
   }
-  if (threadIdx.x == 0) part->first = first, part->top = top, part->valid = valid, part->used = used;
+  if (tid == 0) part->first = first, part->top = top, part->valid = valid;
 }
 
-// a bin's weight by the first's
-__device__ inline double bin_scale(int b) { return exp2(-(double) b / kOctave); }
+// 2^(-i / 23), and a bin's weight by the first's
+__constant__ double kRoots[23] = {1.0, 0.9703127527497981, 0.9415068381488909, 0.913556091857009, 0.886435126281122, 0.8601193075159503, 0.834584732969052, 0.809808209650156, 0.7857672331050286, 0.7624399669747326, 0.739805223161718, 0.7178424425847253, 0.6965316765050238, 0.6758535684070215, 0.655789336416791, 0.63632075624254, 0.6174301446215323, 0.599100343258425, 0.5813147032404313, 0.5640570699151549, 0.5473117682173594, 0.5310635884313455, 0.5152977723760047};
+__device__ inline double bin_scale(int b) {
+  const int o = b / 23;
+  return ldexp(kRoots[b - 23 * o], -o);
+}
 // the weight that the first top_p of m's reach, and the one that the drawn token's sum reaches
 __device__ inline uint64_t p_goal(const Plan& p, uint64_t m) {
   const double g = __builtin_ceil((double) m * p.part);
@@ -458,49 +522,48 @@ __device__ inline void make_plan(const SampleArgs& a, uint32_t t, const Order<T>
     if (holds(u_goal(p, least_m))) l.at[3] = tid;
     if (holds(u_goal(p, most_m))) l.at[4] = tid;
     __syncthreads();
-    from[0] = (int) l.at[3], to[0] = (int) l.at[4];
-    from[1] = by_p ? (int) l.at[1] : kBins, to[1] = by_p ? (int) l.at[2] : kBins;
-    from[2] = to[2] = k_bin;
-    from[3] = to[3] = m_bin;
-    // (a span within another is not looked for twice; those that are left come first)
-    int n = 1;
+    const int f[4] = {(int) l.at[3], by_p ? (int) l.at[1] : kBins, k_bin, m_bin}, g[4] = {(int) l.at[4], by_p ? (int) l.at[2] : -1, by_k ? k_bin : -1, m_bin < kBins ? m_bin : -1};
+    // (spans that touch are one; in ascending order, those that are left first)
+    uint32_t taken = 0;
 #pragma unroll
-    for (int i = 1; i < 4; i++) {
-      bool in = from[i] >= kBins;
-      for (int j = 0; j < n; j++) in = in || (from[i] >= from[j] && to[i] <= to[j]);
-      const int f = from[i], g = to[i];
-      from[i] = to[i] = kBins;
-      if (!in) from[n] = f, to[n] = g, n++;
+    for (int n = 0; n < 4; n++) {
+      int a0 = kBins, a1 = -1;
+#pragma unroll
+      for (int i = 0; i < 4; i++)
+        if (!(taken >> i & 1) && f[i] < a0) a0 = f[i], a1 = g[i];
+#pragma unroll
+      for (int twice = 0; twice < 3; twice++)
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+          if (f[i] <= a1 + 1 && f[i] >= a0 && !(taken >> i & 1)) taken |= 1u << i, a1 = g[i] > a1 ? g[i] : a1;
+      from[n] = a0, to[n] = a0 < kBins ? a1 : kBins;
     }
   }
   if (tid < 4) {
-    const int i = tid;
-    const double lo = (top - to[i] - 0.5) / sc.by, hi = (top - from[i] + 0.5) / sc.by;
+    const int f = tid == 0 ? from[0] : tid == 1 ? from[1] : tid == 2 ? from[2] : from[3], g = tid == 0 ? to[0] : tid == 1 ? to[1] : tid == 2 ? to[2] : to[3];
+    const double lo = (top - g - 0.5) / sc.by, hi = (top - f + 0.5) / sc.by;
     const float fl = (float) (lo - 1e-6 * fabs(lo)), fh = (float) (hi + 1e-6 * fabs(hi));
-    p.from[i] = from[i], p.to[i] = to[i];
-    p.low[i] = from[i] >= kBins ? __builtin_inff() : fl == fl ? fl : -__builtin_inff();
-    p.high[i] = from[i] >= kBins ? -__builtin_inff() : fh < kGreatest<T> ? fh : __builtin_inff();
-  }
-  if (tid == 0) {
-    p.k_bin = k_bin;
-    int n = 0;
-    bool fits = !small;
-    for (int i = 0; i < 4 && fits; i++)
-      for (int b = from[i]; b <= to[i] && b < kBins && fits; b++) {
-        bool there = false;
-        for (int j = 0; j < n; j++) there = there || p.slot_bin[j] == b;
-        if (there) continue;
-        fits = n < kSlots;
-        if (fits) p.slot_bin[n] = b, p.slot_ahead[n] = ahead[b], p.slot_before[n] = before[b], n++;
-      }
-    p.slots = fits ? n : 0;
+    int slots = 0;
+#pragma unroll
+    for (int i = 0; i < 3; i++) slots += i < (int) tid && from[i] < kBins ? to[i] - from[i] + 1 : 0;
+    p.from[tid] = f, p.to[tid] = g, p.slot[tid] = slots;
+    p.low[tid] = f >= kBins ? __builtin_inff() : fl == fl ? fl : -__builtin_inff();
+    p.high[tid] = f >= kBins ? -__builtin_inff() : fh < kGreatest<T> ? fh : __builtin_inff();
+    if (tid == 3) {
+      slots += f < kBins ? g - f + 1 : 0;
+      p.split = small ? 0 : 10 - (slots > 1 ? 32 - __builtin_clz(slots - 1) : 0);
+      p.k_bin = k_bin;
+    }
   }
   __syncthreads();
 }
 
+constexpr uint32_t kMostSlices = OSMOS_SAMPLE_MAX_VOCAB / (kSampleThreads * 4 * kPieces);
+constexpr int kAtOnce = 8;  // slices whose bins are loaded together
 template <uint32_t T>
 __global__ __launch_bounds__(kSampleThreads) void plan_kernel(SampleArgs a) {
   __shared__ PlanLds l;
+  __shared__ double tops[kMostSlices];  // (every wave writes the same)
   const uint32_t t = blockIdx.x, tid = threadIdx.x, lane = tid & 63;
   const Part* parts = (const Part*) a.parts + (uint64_t) t * a.slices;
   const bool small = few(a.k(t));
@@ -510,9 +573,13 @@ __global__ __launch_bounds__(kSampleThreads) void plan_kernel(SampleArgs a) {
   uint32_t valid = 0;
   for (uint32_t s = lane; s < a.slices; s += 64) {
     const uint64_t f = parts[s].first;
-    if (f != ~0ull) top = fmax(top, parts[s].top), valid += parts[s].valid;
+    const uint32_t v = parts[s].valid;
+    const double own = v ? parts[s].top : -__builtin_inf();
+    tops[s] = own;
+    top = fmax(top, own), valid += v;
     first = f < first ? f : first;
   }
+  __syncthreads();
 #pragma unroll
   for (int o = 32; o; o >>= 1) {
     const uint64_t f = (uint64_t) (uint32_t) __shfl_xor((int) (first >> 32), o) << 32 | (uint32_t) __shfl_xor((int) first, o);
@@ -521,14 +588,22 @@ __global__ __launch_bounds__(kSampleThreads) void plan_kernel(SampleArgs a) {
     valid += (uint32_t) __shfl_xor((int) valid, o);
   }
   Sum bin = {0, 0};
-#pragma unroll 4
-  for (uint32_t s = 0; s < a.slices; s++) {
-    const double by = top - parts[s].top;
-    const uint32_t j = by < kBins ? tid - (uint32_t) by : ~0u;
-    if (parts[s].first != ~0ull && j < parts[s].used) {
-      bin.n += parts[s].count[j];
-      if (!small) bin.m += parts[s].mass[j];
+  for (uint32_t s0 = 0; s0 < a.slices; s0 += kAtOnce) {
+    uint32_t n[kAtOnce];
+    uint64_t m[kAtOnce];
+    bool in[kAtOnce];
+#pragma unroll
+    for (int i = 0; i < kAtOnce; i++) {
+      const uint32_t s = s0 + i < a.slices ? s0 + i : s0;
+      const double by = top - tops[s];  // (a slice of no bins: infinite)
+      in[i] = s0 + i < a.slices && by <= tid;
+      const Part* from = parts + (in[i] ? s : 0);
+      const uint32_t j = in[i] ? tid - (uint32_t) by : 0;
+      n[i] = from->count[j], m[i] = small ? 0 : from->mass[j];
     }
+#pragma unroll
+    for (int i = 0; i < kAtOnce; i++)
+      if (in[i]) bin.n += n[i], bin.m += m[i];
   }
   const Order<T> order = {a.bits};
   make_plan<T>(a, t, order, l, first, top, valid, bin);
@@ -539,12 +614,16 @@ __global__ __launch_bounds__(kSampleThreads) void plan_kernel(SampleArgs a) {
   if (tid == 0) to->prefix.before[0] = 0, to->prefix.ahead[0] = 0;
 }
 
-// a token of the plan's bins
+// a listed bin's number among them; -1: not listed
+__device__ inline int slot_of(const Plan& p, int b) {
+  int slot = -1;
+#pragma unroll
+  for (int i = 0; i < 4; i++) slot = b >= p.from[i] && b <= p.to[i] ? p.slot[i] + b - p.from[i] : slot;
+  return b < kBins ? slot : -1;
+}
 template <uint32_t T>
 __device__ inline bool planned(const Plan& p, float x) {
-  const int b = Scale{p.by, p.top}.bin_of(ordered<T>(x));
-  return b < kBins && ((b >= p.from[0] && b <= p.to[0]) || (b >= p.from[1] && b <= p.to[1]) || (b >= p.from[2] && b <= p.to[2]) ||
-                       (b >= p.from[3] && b <= p.to[3]));
+  return slot_of(p, Scale{p.by, p.top}.bin_of(x)) >= 0;
 }
 
 template <uint32_t T>
@@ -564,7 +643,7 @@ __global__ __launch_bounds__(kSampleThreads) void list_kernel(SampleArgs a) {
   row.loaded_between(begin, p, [&](float x, uint32_t i) {
     if (!planned<T>(p, x)) return;
     const uint32_t at = atomicAdd(&listed, 1u);
-    if (at < kList) list[at] = order.place(ordered<T>(x), i);
+    if (at < kList) list[at] = order.place(x, i);
   });
   __syncthreads();
   if (threadIdx.x == 0 && listed) start = atomicAdd(&row_plan->plan.listed, listed);
@@ -680,22 +759,21 @@ __device__ __attribute__((noinline)) void draw_slowly(const void* logits, uint32
   d = by_mass(u_goal(p, cut.m));
 }
 
-// the choice among the listed tokens: each one's count and weight up to it. a token's bin (a few: any bin up to the k-th token's;
-// else a slot's bin cut into 128 parts) has its tokens together, and each is compared with the others of its part
+// the choice among the listed tokens: each one's count and weight up to it. a token's bin is cut into 2^split parts of places, each
+// part has its tokens together, and each token is compared with the others of its part
 template <uint32_t T>
-__device__ inline void draw(const SampleArgs& a, uint32_t t, const Order<T>& order, const Plan& p, Prefix& prefix, bool loaded, const uint64_t* list,
-                            DrawLds& l) {
+__device__ inline void draw(const SampleArgs& a, uint32_t t, const Order<T>& order, const Plan& p, Prefix& prefix, const uint64_t* list, DrawLds& l) {
   const uint32_t tid = threadIdx.x, n = p.listed;
   const void* logits = (const uint8_t*) a.logits + t * a.stride * kv::size_of(T);
   const Scale sc = {p.by, p.top};
   const bool small = p.small;
-  if (tid < kSlots) l.lo[tid] = ~0ull, l.hi[tid] = 0;
   if (tid < 4) l.found[tid] = 0;
-  if (tid == 0) l.crowded = n > kList || (!small && !p.slots), l.at = 0;
-  l.part_n[tid] = 0, l.part_m[tid] = 0, l.filled[tid] = 0;
+  if (tid == 0) l.crowded = n > kList, l.at = 0;
+  l.part_n[tid] = 0, l.part_m[tid] = 0, l.filled[tid] = 0, l.part_lo[tid] = ~0ull, l.part_hi[tid] = 0;
   Cut cut = {~0ull, p.k ? p.k : p.valid, p.all}, d;
   double least_y = -__builtin_inf();
   uint64_t at[2], weight[2];
+  double y[2];
   int bin[2], slot[2];
   uint32_t part[2];
   __syncthreads();
@@ -703,68 +781,57 @@ __device__ inline void draw(const SampleArgs& a, uint32_t t, const Order<T>& ord
 #pragma unroll
     for (int j = 0; j < 2; j++) {
       const uint32_t i = tid + j * kSampleThreads;
-      slot[j] = -1, bin[j] = kBins;
+      slot[j] = -1;
       if (i >= n) continue;
       at[j] = list[i];
-      const double y = sc.y(order.logit(at[j])), middle = __builtin_rint(y);
-      weight[j] = whole_weight(y - middle);
+      y[j] = sc.y(order.logit(at[j]));
+      const double middle = __builtin_rint(y[j]);
+      weight[j] = whole_weight(y[j] - middle);
       bin[j] = sc.bin(middle);
-      if (small) {
-        slot[j] = 0;
-        continue;
-      }
-#pragma unroll
-      for (int q = 0; q < kSlots; q++) slot[j] = q < p.slots && bin[j] == p.slot_bin[q] ? q : slot[j];
-      if (slot[j] < 0) continue;
-      atomicMin((unsigned long long*) &l.lo[slot[j]], (unsigned long long) at[j]);
-      atomicMax((unsigned long long*) &l.hi[slot[j]], (unsigned long long) at[j]);
+      slot[j] = slot_of(p, bin[j]);
+      if (!p.split || slot[j] < 0) continue;
+      atomicMin((unsigned long long*) &l.part_lo[slot[j]], (unsigned long long) at[j]);
+      atomicMax((unsigned long long*) &l.part_hi[slot[j]], (unsigned long long) at[j]);
     }
     __syncthreads();
 #pragma unroll
     for (int j = 0; j < 2; j++) {
       if (slot[j] < 0) continue;
-      part[j] = bin[j];
-      if (!small) {
-        const uint64_t lo = l.lo[slot[j]], span = l.hi[slot[j]] - lo;
+      part[j] = slot[j] << p.split;
+      if (p.split) {
+        const uint64_t lo = l.part_lo[slot[j]], span = l.part_hi[slot[j]] - lo;
         const int bits = span ? 64 - __builtin_clzll(span) : 0;
-        part[j] = slot[j] * kParts + (uint32_t) ((at[j] - lo) >> (bits > 7 ? bits - 7 : 0));
+        part[j] += (uint32_t) ((at[j] - lo) >> (bits > p.split ? bits - p.split : 0));
       }
       atomicAdd(&l.part_n[part[j]], 1u);
       atomicAdd((unsigned long long*) &l.part_m[part[j]], (unsigned long long) weight[j]);
     }
     __syncthreads();
+    // (a few's bins are its parts, and their weights are not known yet)
     const Sum own = {l.part_n[tid], small ? whole((double) l.part_m[tid] * bin_scale(tid)) : l.part_m[tid]};
     const Sum sum = scan_sum(own, l);
-    // (part_lo and part_hi: the parts' sums of weights and counts before them)
-    l.part_lo[tid] = sum.m - own.m, l.part_hi[tid] = sum.n - own.n;
+    l.part_m[tid] = sum.m - own.m, l.before_n[tid] = sum.n - own.n;  // before the part
     if (own.n > kCrowd) l.crowded = 1;
-    if (tid == kSampleThreads - 1) l.last_m = sum.m;
+    if (tid == kSampleThreads - 1) l.sum = sum.m;
     __syncthreads();
   }
   if (l.crowded) {
-    if (!loaded) {
-      const Prefix& from = ((const RowPlan*) a.plans + t)->prefix;
-      prefix.before[tid] = from.before[tid], prefix.ahead[tid] = from.ahead[tid];
-      if (tid == 0) prefix.before[kBins] = from.before[kBins], prefix.ahead[kBins] = from.ahead[kBins];
-      __syncthreads();
-    }
     draw_slowly<T>(logits, a.vocab, order, p, prefix, list, l, cut, d, least_y);
   } else {
-    if (small) cut.m = l.last_m;
+    if (small) cut.m = l.sum;
 #pragma unroll
     for (int j = 0; j < 2; j++) {
       if (slot[j] < 0) continue;
-      const uint32_t i = (uint32_t) l.part_hi[part[j]] + atomicAdd(&l.filled[part[j]], 1u);
+      const uint32_t i = l.before_n[part[j]] + atomicAdd(&l.filled[part[j]], 1u);
       l.sorted[i] = at[j], l.weight[i] = weight[j];
     }
     __syncthreads();
-    if (tid == 0) l.last_n = 0, l.last_m = 0;
     uint32_t upto_n[2];
     uint64_t upto_m[2], past_m[2];
 #pragma unroll
     for (int j = 0; j < 2; j++) {
       if (slot[j] < 0) continue;
-      const uint32_t q = part[j], start = (uint32_t) l.part_hi[q], count = l.part_n[q], base = slot[j] * kParts;
+      const uint32_t q = part[j], start = l.before_n[q], count = l.part_n[q], base = (uint32_t) slot[j] << p.split;
       uint32_t less = 0;
       uint64_t m = 0;
       for (uint32_t i = start; i < start + count; i++) {
@@ -772,11 +839,11 @@ __device__ inline void draw(const SampleArgs& a, uint32_t t, const Order<T>& ord
         less += first, m += first ? l.weight[i] : 0;
       }
       const double scale = bin_scale(bin[j]);
-      uint64_t ahead_m = l.part_lo[q];
+      uint64_t ahead_m = l.part_m[q];
       upto_n[j] = start + less + 1;
       if (!small) {
-        m += ahead_m - l.part_lo[base], ahead_m = p.slot_before[slot[j]];
-        upto_n[j] += p.slot_ahead[slot[j]] - (uint32_t) l.part_hi[base];
+        m += ahead_m - l.part_m[base], ahead_m = prefix.before[bin[j]];
+        upto_n[j] += prefix.ahead[bin[j]] - l.before_n[base];
       }
       upto_m[j] = ahead_m + whole((double) (m + weight[j]) * scale);
       past_m[j] = ahead_m + whole((double) m * scale);
@@ -796,29 +863,23 @@ __device__ inline void draw(const SampleArgs& a, uint32_t t, const Order<T>& ord
       cut = take([&](int j) { return upto_m[j] >= goal && past_m[j] < goal; });
     }
     if (p.m_bin < kBins) {
-      __syncthreads();
+      // the last listed token of min_p's weight or more; none of that bin: all before it (counts and weights grow together)
+      Sum last = {0, 0};
 #pragma unroll
       for (int j = 0; j < 2; j++)
-        if (slot[j] >= 0 && sc.y(order.logit(at[j])) >= p.edge) {
-          atomicMax(&l.last_n, upto_n[j]);
-          atomicMax((unsigned long long*) &l.last_m, (unsigned long long) upto_m[j]);
-        }
-      __syncthreads();
-      uint32_t last_n = l.last_n;
-      uint64_t last_m = l.last_m;
-      if (!small)
-        for (int q = 0; q < p.slots; q++)  // (none of that bin: all before it)
-          if (p.slot_bin[q] == p.m_bin && p.slot_ahead[q] > last_n) last_n = p.slot_ahead[q], last_m = p.slot_before[q];
-      if (last_n < cut.n) cut.n = last_n, cut.m = last_m, least_y = p.edge;
+        if (slot[j] >= 0 && y[j] >= p.edge && upto_n[j] > last.n) last = {upto_n[j], upto_m[j]};
+      last.m = ~least(~last.m, l), last.n = ~(uint32_t) least((uint64_t) ~last.n, l);
+      if (!small && prefix.ahead[p.m_bin] > last.n) last = {prefix.ahead[p.m_bin], prefix.before[p.m_bin]};
+      if (last.n < cut.n) cut.n = last.n, cut.m = last.m, least_y = p.edge;
     }
     const uint64_t goal = u_goal(p, cut.m);
     d = take([&](int j) { return upto_m[j] >= goal && past_m[j] < goal; });
   }
   const double share = kOne / (double) cut.m;
   if (tid == 0) {
-    const double y = sc.y(order.logit(d.place)), middle = __builtin_rint(y);
+    const double z = sc.y(order.logit(d.place)), middle = __builtin_rint(z);
     a.token[t] = (int32_t) order.index(d.place);
-    if (a.prob) a.prob[t] = (float) (part_weight(y - middle) * bin_scale(sc.bin(middle)) * share);
+    if (a.prob) a.prob[t] = (float) (part_weight(z - middle) * bin_scale(sc.bin(middle)) * share);
     if (a.kept) a.kept[t] = (int32_t) cut.n;
     if (a.probs) ((Drawn*) a.cuts)[t] = Drawn{cut.place, sc.by, sc.top, least_y, share};
   }
@@ -830,17 +891,20 @@ __global__ __launch_bounds__(kSampleThreads) void draw_kernel(SampleArgs a) {
   __shared__ Prefix prefix;
   __shared__ Plan p;
   const RowPlan* from = (const RowPlan*) a.plans + blockIdx.x;
-  if (threadIdx.x < sizeof(Plan) / 4) ((uint32_t*) &p)[threadIdx.x] = ((const uint32_t*) &from->plan)[threadIdx.x];
+  const uint32_t tid = threadIdx.x;
+  if (tid < sizeof(Plan) / 4) ((uint32_t*) &p)[tid] = ((const uint32_t*) &from->plan)[tid];
+  prefix.before[tid] = from->prefix.before[tid], prefix.ahead[tid] = from->prefix.ahead[tid];  // (what a greedy row's plan leaves is not used)
+  if (tid == 0) prefix.before[kBins] = from->prefix.before[kBins], prefix.ahead[kBins] = from->prefix.ahead[kBins];
   __syncthreads();
   if (p.done) return;
   const Order<T> order = {a.bits};
-  draw<T>(a, blockIdx.x, order, p, prefix, false, from->list, l);
+  draw<T>(a, blockIdx.x, order, p, prefix, from->list, l);
 }
 
 // a row of one slice
 template <uint32_t T>
 __global__ __launch_bounds__(kSampleThreads) void sample_kernel(SampleArgs a) {
-  __shared__ WholeLds l;
+  __shared__ WholeLds<T> l;
   const uint32_t t = blockIdx.x;
   Tokens<T, kPieces> row = {(const uint8_t*) a.logits + t * a.stride * kv::size_of(T), 0, a.vocab};
   const Order<T> order = {a.bits};
@@ -855,10 +919,10 @@ __global__ __launch_bounds__(kSampleThreads) void sample_kernel(SampleArgs a) {
   row.loaded_between(0, l.plan, [&](float x, uint32_t i) {
     if (!planned<T>(l.plan, x)) return;
     const uint32_t at = atomicAdd(&l.plan.listed, 1u);
-    if (at < kList) l.list[at] = order.place(ordered<T>(x), i);
+    if (at < kList) l.list[at] = order.place(x, i);
   });
   __syncthreads();
-  draw<T>(a, t, order, l.plan, l.prefix, true, l.list, l.draw);
+  draw<T>(a, t, order, l.plan, l.prefix, l.list, l.draw);
 }
 
 // every token's part of the kept weights
@@ -871,7 +935,7 @@ __global__ __launch_bounds__(kSampleThreads) void probs_kernel(SampleArgs a, uin
   float* out = a.probs + (uint64_t) t * a.vocab;
   const Scale sc = {d.by, d.top};
   const Order<T> order = {a.bits};
-  scale[threadIdx.x] = exp2(-(double) (int) threadIdx.x / kOctave) * d.share;
+  scale[threadIdx.x] = bin_scale((int) threadIdx.x) * d.share;
   __syncthreads();
   const uint32_t i = ((blockIdx.x - t * chunks) * kSampleThreads + threadIdx.x) * kPer<T>;
   if (i < end) {
