@@ -92,7 +92,7 @@ __device__ inline bool few(int32_t k) { return k > 0 && (uint32_t) k <= kFew; }
 
 // what is known of a slice
 struct Part {
-  uint64_t first;  // the place of its first token; ~0: none
+  uint64_t first;  // the place of its first token (its index in a greedy row alone); ~0: none
   double top;      // its first bin
   uint32_t valid;  // tokens that can be chosen; 0 for a greedy row too, and then no bins
   uint64_t mass[kBins];  // (unused for a few)
@@ -112,7 +112,7 @@ struct Sum {
 // a row's limits and the bins that they and its token lie in
 struct Plan {
   double by, top, part, draw, edge;  // Scale; top_p and u in their ranges; min_p as a y
-  uint64_t first, all;      // the first token's place, the bins' weights
+  uint64_t all;             // the bins' weights
   uint32_t valid, listed;   // tokens that can be chosen, that are listed (more than kList: those past it are not)
   uint32_t k;               // top_k where it limits, or 0; k_bin kBins: among tokens of no weight
   int k_bin, m_bin;         // kBins: none
@@ -139,7 +139,7 @@ struct ScanLds {
   float greatest[kSampleWaves];
   uint32_t index;
 };
-constexpr int kValues = 4096;  // bf16: the values of 2^-8 to 2^8 of either sign
+constexpr int kValues = 8192;  // bf16: the values from 2^-24 to 2^8 of either sign
 struct ValueLds : ScanLds {
   uint32_t value[kValues];
 };
@@ -148,13 +148,11 @@ struct PlanLds {
   Plan plan;
   Prefix prefix;
   Sum wave[kSampleWaves];
-  uint64_t word[kSampleWaves];
-  uint32_t at[8];
 };
 struct DrawLds {
   uint64_t part_m[kBins], part_lo[kBins], part_hi[kBins];  // sums of weights; least and greatest places
   uint32_t part_n[kBins], before_n[kBins], filled[kBins];
-  uint64_t sorted[kList], weight[kList];
+  uint64_t sorted[kList], weight[kList];  // a part's tokens together; then in order, and the weights up to each
   Sum wave[kSampleWaves];
   uint64_t word[kSampleWaves], found[4], sum;
   uint32_t at, crowded;
@@ -252,30 +250,32 @@ __device__ inline double bins_a_unit(float temperature) { return kOctave * 1.442
 
 // 16 bytes of logits at any address that their type allows, as they are (past the end: -infinity)
 template <uint32_t T> constexpr uint32_t kPer = T == OSMOS_F32 ? 4 : 8;
-typedef float f32x4_u __attribute__((ext_vector_type(4), aligned(4)));
-typedef _Float16 f16x8_u __attribute__((ext_vector_type(8), aligned(2)));
-typedef __bf16 bf16x8_u __attribute__((ext_vector_type(8), aligned(2)));
+typedef uint32_t u32x4_1 __attribute__((ext_vector_type(4), aligned(1)));
 template <uint32_t T>
-__device__ inline void logits_at(const void* p, uint32_t i, uint32_t end, float (&x)[kPer<T>]) {
-  if (i + kPer<T> <= end) {
-    if constexpr (T == OSMOS_F32) {
-      const f32x4_u v = gload<f32x4_u>((const float*) p + i);
+struct Piece {
+  uint32_t w[4];
+  __device__ inline void load(const void* p, uint32_t i, uint32_t end) {
+    if (i + kPer<T> <= end) {
+      const u32x4_1 v = gload<u32x4_1>((const uint8_t*) p + (uint64_t) i * kv::size_of(T));
 #pragma unroll
-      for (int j = 0; j < 4; j++) x[j] = v[j];
-    } else if constexpr (T == OSMOS_F16) {
-      const f16x8_u v = gload<f16x8_u>((const _Float16*) p + i);
+      for (int j = 0; j < 4; j++) w[j] = v[j];
+    } else if constexpr (T == OSMOS_F32) {
 #pragma unroll
-      for (int j = 0; j < 8; j++) x[j] = (float) v[j];
+      for (uint32_t j = 0; j < 4; j++) w[j] = i + j < end ? gload<uint32_t>((const uint32_t*) p + i + j) : 0xFF800000u;
     } else {
-      const bf16x8_u v = gload<bf16x8_u>((const __bf16*) p + i);
+      constexpr uint32_t none = T == OSMOS_F16 ? 0xFC00u : 0xFF80u;
 #pragma unroll
-      for (int j = 0; j < 8; j++) x[j] = (float) v[j];
+      for (uint32_t j = 0; j < 4; j++)
+        w[j] = (i + 2 * j < end ? (uint32_t) gload<uint16_t>((const uint16_t*) p + i + 2 * j) : none) |
+               (i + 2 * j + 1 < end ? (uint32_t) gload<uint16_t>((const uint16_t*) p + i + 2 * j + 1) : none) << 16;
     }
-  } else {
-#pragma unroll
-    for (uint32_t j = 0; j < kPer<T>; j++) x[j] = i + j < end ? logit_at<T>(p, i + j) : -__builtin_inff();
   }
-}
+  __device__ inline float at(uint32_t j) const {
+    if constexpr (T == OSMOS_F32) return __uint_as_float(w[j]);
+    else if constexpr (T == OSMOS_BF16) return __uint_as_float(j & 1 ? w[j / 2] & 0xFFFF0000u : w[j / 2] << 16);
+    else return __half2float(__ushort_as_half((unsigned short) (w[j / 2] >> 16 * (j & 1))));
+  }
+};
 
 // tokens begin .. end - 1 of a row, P pieces a thread and round (the rounds' loads in flight together)
 template <uint32_t T, int P>
@@ -283,17 +283,17 @@ struct Tokens {
   const void* p;
   uint32_t begin, end;
   static constexpr uint32_t kRound = kSampleThreads * kPer<T> * P;
-  float x[P][kPer<T>];
+  Piece<T> x[P];
   __device__ inline void load(uint32_t at) {
 #pragma unroll
-    for (int k = 0; k < P; k++) logits_at<T>(p, at + (k * kSampleThreads + threadIdx.x) * kPer<T>, end, x[k]);
+    for (int k = 0; k < P; k++) x[k].load(p, at + (k * kSampleThreads + threadIdx.x) * kPer<T>, end);
   }
   template <typename F>
   __device__ inline void loaded(uint32_t at, F f) const {
 #pragma unroll
     for (int k = 0; k < P; k++)
 #pragma unroll
-      for (uint32_t j = 0; j < kPer<T>; j++) f(x[k][j], at + (k * kSampleThreads + threadIdx.x) * kPer<T> + j);
+      for (uint32_t j = 0; j < kPer<T>; j++) f(x[k].at(j), at + (k * kSampleThreads + threadIdx.x) * kPer<T> + j);
   }
   // those of a plan's spans' logits: most threads have none, so they are read again
   template <typename F>
@@ -305,7 +305,7 @@ struct Tokens {
 #pragma unroll
       for (int k = 0; k < P; k++)
 #pragma unroll
-        for (uint32_t j = 0; j < kPer<T>; j++) hits |= in(x[k][j]) ? 1u << (k * kPer<T> + j) : 0;
+        for (uint32_t j = 0; j < kPer<T>; j++) hits |= in(x[k].at(j)) ? 1u << (k * kPer<T> + j) : 0;
     };
     static_assert(P * kPer<T> <= 32);
     if (spans == 1) test([&](float v) { return v >= l0 && v <= h0; });
@@ -348,18 +348,46 @@ struct Near {
 };
 
 // a slice's first place and, but for a greedy row, its bins (into l.count and, unless k is small, l.mass): its tokens are one round.
-// bf16's tokens are few values, often: they are counted by value, and each value is put into its bin once
+// bf16's tokens are few values, often: they are counted by value, two a word, and each value is put into its bin once
 template <uint32_t T, typename R, typename L>
 __device__ inline void scan_slice(R& row, const Order<T>& order, float temperature, int32_t k, L& l, uint64_t& first, double& top, uint32_t& valid) {
+  constexpr uint32_t kLeastBits = 0x3380, kSpan = kValues / 2;  // (2^-24; the first and the last of the span stand for what is outside)
+  constexpr bool by_value = T == OSMOS_BF16;
   const uint32_t tid = threadIdx.x;
   const float none = -__builtin_inff();
+  const bool warm = temperature > 0.0f, mass = !few(k);
   row.load(row.begin);
   l.mass[tid] = 0, l.count[tid] = 0;
-  if constexpr (T == OSMOS_BF16)
-    for (int i = 0; i < kValues; i += kSampleThreads) l.value[i + tid] = 0;
   if (tid == 0) l.index = ~0u;
   float best = none;
-  row.loaded(row.begin, [&](float x, uint32_t) { best = fmaxf(best, x); });
+  if constexpr (by_value) {
+#pragma unroll
+    for (int i = 0; i < kValues; i += kSampleThreads) l.value[i + tid] = 0;
+    __syncthreads();
+#pragma unroll
+    for (uint32_t i = 0; i < sizeof(row.x) / 4; i++) {
+      typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
+      const uint32_t w = row.x[i / 4].w[i % 4], size = w & 0x7FFF7FFFu;
+      u16x2 v = __builtin_bit_cast(u16x2, size);
+      v = __builtin_elementwise_min(__builtin_elementwise_max(v, u16x2{kLeastBits, kLeastBits}), u16x2{kLeastBits + kSpan - 1, kLeastBits + kSpan - 1}) -
+          u16x2{kLeastBits, kLeastBits};
+      const uint32_t at = __builtin_bit_cast(uint32_t, v) << 2 | (w >> 1 & 0x40004000u);  // (4096 values of 4 bytes a sign)
+      atomicAdd((uint32_t*) ((uint8_t*) l.value + (at & 0xFFFF)), 1u);
+      atomicAdd((uint32_t*) ((uint8_t*) l.value + (at >> 16)), 1u);
+    }
+    __syncthreads();
+    if (l.value[0] | l.value[kSpan - 1] | l.value[kSpan] | l.value[kValues - 1]) {  // (what is past the end is in the last)
+      row.loaded(row.begin, [&](float x, uint32_t) { best = fmaxf(best, x); });
+    } else {
+#pragma unroll
+      for (int j = 0; j < kValues / kSampleThreads; j++) {
+        const uint32_t i = tid + j * kSampleThreads;
+        if (l.value[i]) best = fmaxf(best, __uint_as_float((i % kSpan + kLeastBits) << 16 | i / kSpan << 31));
+      }
+    }
+  } else {
+    row.loaded(row.begin, [&](float x, uint32_t) { best = fmaxf(best, x); });
+  }
   float most = wave_greatest(best);
   if ((tid & 63) == 63) l.greatest[tid / 64] = most;
   __syncthreads();
@@ -369,16 +397,15 @@ __device__ inline void scan_slice(R& row, const Order<T>& order, float temperatu
   most = ordered<T>(most);
   first = ~0ull, top = 0.0, valid = 0;
   if (!(most > none)) return;
-  if (ordered<T>(best) == most) {  // (the lowest index among equals)
+  if (!warm) {  // (the lowest index among equals; elsewhere its logit is all that is asked for)
     uint32_t at = ~0u;
     row.loaded(row.begin, [&](float x, uint32_t i) { at = ordered<T>(x) == most && i < at ? i : at; });
-    atomicMin(&l.index, at);
-  }
-  if (!(temperature > 0.0f)) {
+    if (at != ~0u) atomicMin(&l.index, at);
     __syncthreads();
     first = order.place(most, l.index);
     return;
   }
+  first = order.place(most, 0);
   Scale sc = {bins_a_unit(temperature), 0.0};
   sc.top = top = __builtin_rint(sc.y(most));
   auto add = [&](float x, uint32_t n, bool mass) __attribute__((always_inline)) {
@@ -392,34 +419,22 @@ __device__ inline void scan_slice(R& row, const Order<T>& order, float temperatu
       valid += x > none ? n : 0;
     }
   };
-  const bool mass = !few(k);
-  if constexpr (T == OSMOS_BF16) {
-    constexpr uint32_t least_bits = 0x3B80, span = kValues / 2;  // 2^-8; the first and the last of the span stand for what is outside
-    auto value = [](float x) __attribute__((always_inline)) {
-      const uint32_t b = __float_as_uint(x) >> 16 & 0x7FFF;
-      return (b < least_bits ? least_bits : b > least_bits + span - 1 ? least_bits + span - 1 : b) - least_bits;
-    };
-    bool outside = false;
-    row.loaded(row.begin, [&](float x, uint32_t) {
-      const uint32_t v = value(x);
-      if (v - 1 < span - 2) atomicAdd(&l.value[(__float_as_uint(x) >> 31) * span + v], 1u);
-      else outside = true;
-    });
-    if (outside)
+  if constexpr (by_value) {
+    if (l.value[0] | l.value[kSpan - 1] | l.value[kSpan] | l.value[kValues - 1])
       row.loaded(row.begin, [&](float x, uint32_t) {
-        if (value(x) - 1 >= span - 2) add(x, 1, mass);
+        const uint32_t v = (__float_as_uint(x) >> 16 & 0x7FFF) - kLeastBits;
+        if ((int) v < 1 || v >= kSpan - 1) add(x, 1, mass);
       });
-    __syncthreads();
-    for (uint32_t i = tid; i < kValues; i += kSampleThreads) {
-      const uint32_t n = l.value[i];
-      if (n) add(__uint_as_float(((i % span) + least_bits) << 16 | i / span << 31), n, mass);
+#pragma unroll
+    for (int j = 0; j < kValues / kSampleThreads; j++) {
+      const uint32_t i = tid + j * kSampleThreads, n = l.value[i];
+      if (n && i % kSpan && i % kSpan != kSpan - 1) add(__uint_as_float((i % kSpan + kLeastBits) << 16 | i / kSpan << 31), n, mass);
     }
   } else {
     if (mass) row.loaded(row.begin, [&](float x, uint32_t) { add(x, 1, true); });
     else row.loaded(row.begin, [&](float x, uint32_t) { add(x, 1, false); });
   }
   __syncthreads();
-  first = order.place(most, l.index);
   valid = total(Sum{valid + l.count[tid], 0}, l).n;
 }
 
@@ -450,13 +465,13 @@ __device__ inline double bin_scale(int b) {
   const int o = b / 23;
   return ldexp(kRoots[b - 23 * o], -o);
 }
-// the weight that the first top_p of m's reach, and the one that the drawn token's sum reaches
-__device__ inline uint64_t p_goal(const Plan& p, uint64_t m) {
-  const double g = __builtin_ceil((double) m * p.part);
+// the weight that the first `part` of m's reach, and the one that the sum of the token drawn by `u` reaches
+__device__ inline uint64_t p_goal(double part, uint64_t m) {
+  const double g = __builtin_ceil((double) m * part);
   return g > 1.0 ? (uint64_t) g < m ? (uint64_t) g : m : 1;
 }
-__device__ inline uint64_t u_goal(const Plan& p, uint64_t m) {
-  const uint64_t g = (uint64_t) __builtin_floor((double) m * p.draw) + 1;
+__device__ inline uint64_t u_goal(double u, uint64_t m) {
+  const uint64_t g = (uint64_t) __builtin_floor((double) m * u) + 1;
   return g < m ? g : m;
 }
 
@@ -481,49 +496,46 @@ __device__ inline void make_plan(const SampleArgs& a, uint32_t t, const Order<T>
     return;
   }
   const bool small = few(k);
-  if (tid < 8) l.at[tid] = 0;
   const Sum sum = scan_sum(Sum{bin.n, small ? 0 : whole((double) bin.m * bin_scale(tid))}, l);
   l.prefix.ahead[tid + 1] = sum.n, l.prefix.before[tid + 1] = sum.m;
   if (tid == 0) l.prefix.ahead[0] = 0, l.prefix.before[0] = 0;
   __syncthreads();
-  const uint32_t* ahead = l.prefix.ahead;
-  const uint64_t *before = l.prefix.before, all = before[kBins];
-  const uint32_t limit = k > 0 && (uint32_t) k < valid ? k : 0;
-  const bool by_k = limit && limit <= ahead[kBins], by_p = top_p < 1.0f;
-  const double edge = sc.y(order.logit(first)) + (min_p > 0.0f ? kOctave * log2((double) (min_p < 1.0f ? min_p : 1.0f)) : 0.0);
-  const int m_bin = min_p > 0.0f ? sc.bin(__builtin_rint(edge)) : kBins;
-  if (tid == 0) {
-    p.by = sc.by, p.top = top, p.part = top_p > 0.0f ? top_p : 0.0f, p.draw = u > 0.0f ? u < 1.0f ? u : 0.99999994f : 0.0f, p.edge = edge;
-    p.first = first, p.all = all, p.valid = valid, p.listed = 0, p.k = limit, p.m_bin = m_bin;
-    p.done = 0, p.small = small, p.by_p = by_p;
-  }
-  if (by_k && ahead[tid + 1] >= limit && ahead[tid] < limit) l.at[0] = tid;
-  __syncthreads();
-  const int k_bin = by_k ? (int) l.at[0] : kBins;
-  int from[4], to[4];
-  if (small) {
-    from[0] = 0, to[0] = by_k ? k_bin : kBins - 1;
-#pragma unroll
-    for (int i = 1; i < 4; i++) from[i] = to[i] = kBins;
-  } else {
-    auto holds = [&](uint64_t goal) { return before[tid + 1] >= goal && before[tid] < goal; };
-    uint64_t least_m = all, most_m = all;
-    if (by_k) least_m = before[k_bin] + 1, most_m = before[k_bin + 1];
-    if (by_p) {
-      if (holds(p_goal(p, least_m))) l.at[1] = tid;
-      if (holds(p_goal(p, most_m))) l.at[2] = tid;
-      __syncthreads();
-      least_m = before[l.at[1]] + 1, most_m = before[l.at[2] + 1];
+  if (tid < 64) {  // (one wave: the others would only repeat it)
+    const uint32_t* ahead = l.prefix.ahead;
+    const uint64_t *before = l.prefix.before, all = before[kBins];
+    // the bin whose sum reaches `goal`, the ones before it not
+    auto reaches = [&](const auto* sums, auto goal) {
+      const uint64_t a = __ballot(sums[(tid + 1) * 16] >= goal);
+      const int s = a ? __builtin_ctzll(a) : 63;
+      const uint64_t b = __ballot(sums[s * 16 + (tid & 15) + 1] >= goal);
+      return s * 16 + (b ? __builtin_ctzll(b) : 15);
+    };
+    const uint32_t limit = k > 0 && (uint32_t) k < valid ? k : 0;
+    const bool by_k = limit && limit <= ahead[kBins], by_p = top_p < 1.0f;
+    const double edge = sc.y(order.logit(first)) + (min_p > 0.0f ? kOctave * log2((double) (min_p < 1.0f ? min_p : 1.0f)) : 0.0);
+    const int m_bin = min_p > 0.0f ? sc.bin(__builtin_rint(edge)) : kBins;
+    const double part = top_p > 0.0f ? top_p : 0.0f, drawn = u > 0.0f ? u < 1.0f ? u : 0.99999994f : 0.0f;
+    const int k_bin = by_k ? reaches(ahead, limit) : kBins;
+    // the spans of bins that the token, top_p, top_k and min_p lie in
+    int f[4] = {0, kBins, kBins, kBins}, g[4] = {by_k ? k_bin : kBins - 1, -1, -1, -1};
+    if (!small) {
+      uint64_t least_m = all, most_m = all;
+      if (by_k) f[2] = g[2] = k_bin, least_m = before[k_bin] + 1, most_m = before[k_bin + 1];
+      if (by_p) {
+        f[1] = reaches(before, p_goal(part, least_m));
+        g[1] = least_m == most_m ? f[1] : reaches(before, p_goal(part, most_m));
+        least_m = before[f[1]] + 1, most_m = before[g[1] + 1];
+      }
+      if (m_bin < kBins) {
+        f[3] = g[3] = m_bin;
+        const uint64_t lo = before[m_bin] > 1 ? before[m_bin] : 1, hi = before[m_bin + 1];
+        least_m = lo < least_m ? lo : least_m, most_m = hi < most_m ? hi : most_m;
+      }
+      f[0] = reaches(before, u_goal(drawn, least_m));
+      g[0] = least_m == most_m ? f[0] : reaches(before, u_goal(drawn, most_m));
     }
-    if (m_bin < kBins) {
-      const uint64_t lo = before[m_bin] > 1 ? before[m_bin] : 1, hi = before[m_bin + 1];
-      least_m = lo < least_m ? lo : least_m, most_m = hi < most_m ? hi : most_m;
-    }
-    if (holds(u_goal(p, least_m))) l.at[3] = tid;
-    if (holds(u_goal(p, most_m))) l.at[4] = tid;
-    __syncthreads();
-    const int f[4] = {(int) l.at[3], by_p ? (int) l.at[1] : kBins, k_bin, m_bin}, g[4] = {(int) l.at[4], by_p ? (int) l.at[2] : -1, by_k ? k_bin : -1, m_bin < kBins ? m_bin : -1};
     // (spans that touch are one; in ascending order, those that are left first)
+    int from[4], to[4], slots = 0, slot[4];
     uint32_t taken = 0;
 #pragma unroll
     for (int n = 0; n < 4; n++) {
@@ -536,23 +548,22 @@ __device__ inline void make_plan(const SampleArgs& a, uint32_t t, const Order<T>
 #pragma unroll
         for (int i = 0; i < 4; i++)
           if (f[i] <= a1 + 1 && f[i] >= a0 && !(taken >> i & 1)) taken |= 1u << i, a1 = g[i] > a1 ? g[i] : a1;
-      from[n] = a0, to[n] = a0 < kBins ? a1 : kBins;
+      from[n] = a0, to[n] = a0 < kBins ? a1 : kBins, slot[n] = slots;
+      slots += a0 < kBins ? a1 - a0 + 1 : 0;
     }
-  }
-  if (tid < 4) {
-    const int f = tid == 0 ? from[0] : tid == 1 ? from[1] : tid == 2 ? from[2] : from[3], g = tid == 0 ? to[0] : tid == 1 ? to[1] : tid == 2 ? to[2] : to[3];
-    const double lo = (top - g - 0.5) / sc.by, hi = (top - f + 0.5) / sc.by;
-    const float fl = (float) (lo - 1e-6 * fabs(lo)), fh = (float) (hi + 1e-6 * fabs(hi));
-    int slots = 0;
-#pragma unroll
-    for (int i = 0; i < 3; i++) slots += i < (int) tid && from[i] < kBins ? to[i] - from[i] + 1 : 0;
-    p.from[tid] = f, p.to[tid] = g, p.slot[tid] = slots;
-    p.low[tid] = f >= kBins ? __builtin_inff() : fl == fl ? fl : -__builtin_inff();
-    p.high[tid] = f >= kBins ? -__builtin_inff() : fh < kGreatest<T> ? fh : __builtin_inff();
-    if (tid == 3) {
-      slots += f < kBins ? g - f + 1 : 0;
+    if (tid < 4) {
+      const int a0 = tid == 0 ? from[0] : tid == 1 ? from[1] : tid == 2 ? from[2] : from[3], a1 = tid == 0 ? to[0] : tid == 1 ? to[1] : tid == 2 ? to[2] : to[3];
+      const double lo = (top - a1 - 0.5) / sc.by, hi = (top - a0 + 0.5) / sc.by;
+      const float fl = (float) (lo - 1e-6 * fabs(lo)), fh = (float) (hi + 1e-6 * fabs(hi));
+      p.from[tid] = a0, p.to[tid] = a1, p.slot[tid] = tid == 0 ? slot[0] : tid == 1 ? slot[1] : tid == 2 ? slot[2] : slot[3];
+      p.low[tid] = a0 >= kBins ? __builtin_inff() : fl == fl ? fl : -__builtin_inff();
+      p.high[tid] = a0 >= kBins ? -__builtin_inff() : fh < kGreatest<T> ? fh : __builtin_inff();
+    }
+    if (tid == 0) {
+      p.by = sc.by, p.top = top, p.part = part, p.draw = drawn, p.edge = edge;
+      p.all = all, p.valid = valid, p.listed = 0, p.k = limit, p.k_bin = k_bin, p.m_bin = m_bin;
+      p.done = 0, p.small = small, p.by_p = by_p;
       p.split = small ? 0 : 10 - (slots > 1 ? 32 - __builtin_clz(slots - 1) : 0);
-      p.k_bin = k_bin;
     }
   }
   __syncthreads();
@@ -745,7 +756,7 @@ __device__ __attribute__((noinline)) void draw_slowly(const void* logits, uint32
     cut = find<T, false>(near, sc, prefix, l, p.k_bin, p.k - prefix.ahead[p.k_bin], 0);
     __syncthreads();
   }
-  if (p.by_p) cut = by_mass(p_goal(p, cut.m));
+  if (p.by_p) cut = by_mass(p_goal(p.part, cut.m));
   if (p.m_bin < kBins) {
     Sum in = {0, 0};
     near.each([&](float x, uint32_t) {
@@ -756,7 +767,7 @@ __device__ __attribute__((noinline)) void draw_slowly(const void* logits, uint32
     in = {prefix.ahead[p.m_bin] + in.n, prefix.before[p.m_bin] + whole((double) in.m * bin_scale(p.m_bin))};
     if (in.n < cut.n) cut.n = in.n, cut.m = in.m, least_y = p.edge;
   }
-  d = by_mass(u_goal(p, cut.m));
+  d = by_mass(u_goal(p.draw, cut.m));
 }
 
 // the choice among the listed tokens: each one's count and weight up to it. a token's bin is cut into 2^split parts of places, each
@@ -826,54 +837,61 @@ __device__ inline void draw(const SampleArgs& a, uint32_t t, const Order<T>& ord
       l.sorted[i] = at[j], l.weight[i] = weight[j];
     }
     __syncthreads();
-    uint32_t upto_n[2];
-    uint64_t upto_m[2], past_m[2];
+    uint32_t rank[2];
+    uint64_t upto[2];
 #pragma unroll
     for (int j = 0; j < 2; j++) {
       if (slot[j] < 0) continue;
       const uint32_t q = part[j], start = l.before_n[q], count = l.part_n[q], base = (uint32_t) slot[j] << p.split;
       uint32_t less = 0;
-      uint64_t m = 0;
+      uint64_t m = weight[j];
       for (uint32_t i = start; i < start + count; i++) {
         const bool first = l.sorted[i] < at[j];
         less += first, m += first ? l.weight[i] : 0;
       }
-      const double scale = bin_scale(bin[j]);
-      uint64_t ahead_m = l.part_m[q];
-      upto_n[j] = start + less + 1;
-      if (!small) {
-        m += ahead_m - l.part_m[base], ahead_m = prefix.before[bin[j]];
-        upto_n[j] += prefix.ahead[bin[j]] - l.before_n[base];
-      }
-      upto_m[j] = ahead_m + whole((double) (m + weight[j]) * scale);
-      past_m[j] = ahead_m + whole((double) m * scale);
+      rank[j] = start + less;
+      const uint64_t ahead = l.part_m[q];
+      upto[j] = small ? ahead + whole((double) m * bin_scale(bin[j])) : prefix.before[bin[j]] + whole((double) (m + ahead - l.part_m[base]) * bin_scale(bin[j]));
     }
-    auto take = [&](auto is) {
+    __syncthreads();
 #pragma unroll
-      for (int j = 0; j < 2; j++)
-        if (slot[j] >= 0 && is(j)) l.found[0] = at[j], l.found[1] = upto_n[j], l.found[2] = upto_m[j];
-      __syncthreads();
-      const Cut c = {l.found[0], (uint32_t) l.found[1], l.found[2]};
-      __syncthreads();
-      return c;
+    for (int j = 0; j < 2; j++)
+      if (slot[j] >= 0) l.sorted[rank[j]] = at[j], l.weight[rank[j]] = upto[j];
+    __syncthreads();
+    if (tid >= 64) return;
+    // the first of the listed tokens that `is` holds for, as it does for all that follow
+    auto first_of = [&](auto is) {
+      uint32_t lo = 0, left = n;
+      while (left > 1) {
+        const uint32_t step = (left + 63) / 64, i = lo + tid * step + step - 1;
+        const uint64_t a = __ballot(i < lo + left ? is(i) : true);
+        const uint32_t s = a ? __builtin_ctzll(a) : 63;
+        lo += s * step;
+        left = s * step < left ? left - s * step < step ? left - s * step : step : 1;
+      }
+      return lo < n ? lo : n - 1;
     };
-    if (p.k_bin < kBins) cut = take([&](int j) { return upto_n[j] == p.k; });
+    // the i-th listed token as a cut: how many tokens of the row there are up to it
+    auto cut_at = [&](uint32_t i) {
+      const int b = sc.bin_of(order.logit(l.sorted[i]));
+      return Cut{l.sorted[i], small ? i + 1 : prefix.ahead[b] + i - l.before_n[slot_of(p, b) << p.split] + 1, l.weight[i]};
+    };
+    if (p.k_bin < kBins) cut = cut_at(small ? p.k - 1 : l.before_n[slot_of(p, p.k_bin) << p.split] + p.k - prefix.ahead[p.k_bin] - 1);
     if (p.by_p) {
-      const uint64_t goal = p_goal(p, cut.m);
-      cut = take([&](int j) { return upto_m[j] >= goal && past_m[j] < goal; });
+      const uint64_t goal = p_goal(p.part, cut.m);
+      cut = cut_at(first_of([&](uint32_t i) { return l.weight[i] >= goal; }));
     }
     if (p.m_bin < kBins) {
-      // the last listed token of min_p's weight or more; none of that bin: all before it (counts and weights grow together)
-      Sum last = {0, 0};
-#pragma unroll
-      for (int j = 0; j < 2; j++)
-        if (slot[j] >= 0 && y[j] >= p.edge && upto_n[j] > last.n) last = {upto_n[j], upto_m[j]};
-      last.m = ~least(~last.m, l), last.n = ~(uint32_t) least((uint64_t) ~last.n, l);
-      if (!small && prefix.ahead[p.m_bin] > last.n) last = {prefix.ahead[p.m_bin], prefix.before[p.m_bin]};
+      // the last listed token of min_p's weight or more; none of that bin: all before it
+      const uint32_t i = first_of([&](uint32_t i) { return !(sc.y(order.logit(l.sorted[i])) >= p.edge); });
+      const bool all = sc.y(order.logit(l.sorted[i])) >= p.edge;  // (no listed token is less)
+      Cut last = {0, 0, 0};
+      if (all || i) last = cut_at(all ? i : i - 1);
+      if (!small && prefix.ahead[p.m_bin] > last.n) last.n = prefix.ahead[p.m_bin], last.m = prefix.before[p.m_bin];
       if (last.n < cut.n) cut.n = last.n, cut.m = last.m, least_y = p.edge;
     }
-    const uint64_t goal = u_goal(p, cut.m);
-    d = take([&](int j) { return upto_m[j] >= goal && past_m[j] < goal; });
+    const uint64_t goal = u_goal(p.draw, cut.m);
+    d = cut_at(first_of([&](uint32_t i) { return l.weight[i] >= goal; }));
   }
   const double share = kOne / (double) cut.m;
   if (tid == 0) {
@@ -939,17 +957,17 @@ __global__ __launch_bounds__(kSampleThreads) void probs_kernel(SampleArgs a, uin
   __syncthreads();
   const uint32_t i = ((blockIdx.x - t * chunks) * kSampleThreads + threadIdx.x) * kPer<T>;
   if (i < end) {
-    float x[kPer<T>];
-    logits_at<T>(p, i, end, x);
+    Piece<T> piece;
+    piece.load(p, i, end);
 #pragma unroll
     for (uint32_t j = 0; j < kPer<T>; j++) {
       float v = 0.0f;
-      x[j] = ordered<T>(x[j]);
-      if (x[j] > -__builtin_inff() && order.place(x[j], i + j) <= d.last) {
+      const float x = ordered<T>(piece.at(j));
+      if (x > -__builtin_inff() && order.place(x, i + j) <= d.last) {
         if (d.share == 0.0) {
-          v = order.place(x[j], i + j) == d.last ? 1.0f : 0.0f;
+          v = order.place(x, i + j) == d.last ? 1.0f : 0.0f;
         } else {
-          const double y = sc.y(x[j]), middle = __builtin_rint(y);
+          const double y = sc.y(x), middle = __builtin_rint(y);
           const int b = sc.bin(middle);
           if (b < kBins && y >= d.least_y) v = (float) (part_weight(y - middle) * scale[b]);
         }
