@@ -1,7 +1,7 @@
 // libosmos MI355X - osmos_norm (include/osmos_rows.h): the residual's addition, the root-mean-square norm and the forms that the
 // products read, in one pass over the rows.
 #include "rowshost.h"
-#include "common.h"
+#include "lanes.h"
 #include "x16.h"
 
 namespace osm {
@@ -86,6 +86,7 @@ struct NormArgs {
   float eps, offset;
   double part;      // 1 / dim
   uint32_t waves;   // a row's; 1: each wave of the workgroup a row of its own
+  bool tiles;
 };
 
 // a row's values stay in registers between the sum of their squares and their stores: K pieces of 16 bytes a thread
@@ -94,7 +95,9 @@ __global__ __launch_bounds__(1024) void norm_kernel(NormArgs a) {
   constexpr int N = per<T>();
   __shared__ double sums[16];
   const uint32_t lanes = a.waves * 64, wave = threadIdx.x / 64;
-  const uint32_t t = a.waves > 1 ? blockIdx.x : blockIdx.x * (blockDim.x / 64) + wave;
+  uint32_t t = a.waves > 1 ? blockIdx.x : blockIdx.x * (blockDim.x / 64) + wave;
+  // workgroups go to the 8 XCDs in turn: the 16 rows of a tile, whose values lie in the same lines, to one of them
+  if (a.tiles && a.waves > 1 && blockIdx.x < gridDim.x / 128 * 128) t = blockIdx.x / 128 * 128 + blockIdx.x % 8 * 16 + blockIdx.x / 8 % 16;
   const uint32_t at = a.waves > 1 ? threadIdx.x : threadIdx.x & 63;
   const uint32_t pieces = (a.dim + N - 1) / N;
   const bool live = t < a.n;  // (a row past the last: of a tile's rest, or none)
@@ -129,8 +132,17 @@ __global__ __launch_bounds__(1024) void norm_kernel(NormArgs a) {
     }
   }
   if (!a.out && !a.x16 && !a.codes) return;
+  // (the weights are on their way meanwhile, where there is room for them)
+  constexpr bool early = K * N <= 16;
+  float w[early ? K : 1][N];
+  if constexpr (early)
+    if (a.weight && live)
 #pragma unroll
-  for (int o = 32; o; o >>= 1) ss += __shfl_xor(ss, o);
+      for (int k = 0; k < K; k++) {
+        const uint32_t c = at + k * lanes;
+        if (c < pieces) load_part<N, TAIL>(a.weight_type, a.weight, c * N, a.dim - c * N, w[k]);
+      }
+  ss = wave_total(ss);
   if (a.waves > 1) {
     if (at % 64 == 0) sums[wave] = ss;
     __syncthreads();
@@ -149,11 +161,12 @@ __global__ __launch_bounds__(1024) void norm_kernel(NormArgs a) {
 #pragma unroll
       for (int i = 0; i < N; i++) y[i] = 0.0f;
     } else {
-      float w[N];
-      if (a.weight) load_part<N, TAIL>(a.weight_type, a.weight, c * N, a.dim - c * N, w);
+      float(&own)[N] = w[early ? k : 0];
+      if constexpr (!early)
+        if (a.weight) load_part<N, TAIL>(a.weight_type, a.weight, c * N, a.dim - c * N, own);
 #pragma unroll
       for (int i = 0; i < N; i++)
-        y[i] = a.weight ? __fmul_rn(__fmul_rn(s[k][i], r), __fadd_rn(w[i], a.offset))
+        y[i] = a.weight ? __fmul_rn(__fmul_rn(s[k][i], r), __fadd_rn(own[i], a.offset))
                         : __fmul_rn(__fmul_rn(s[k][i], r), __fadd_rn(1.0f, a.offset));
       if (a.out) store_part<N, TAIL>(a.out_type, a.out, t * a.out_stride + c * N, a.dim - c * N, y);
       if (a.codes) {
@@ -195,8 +208,8 @@ template <uint32_t T>
 bool norm_launch(const OsmosNorm* a, hipStream_t s) {
   const uint32_t pieces = (a->dim + per<T>() - 1) / per<T>(), rows = a->x16 ? (a->n + 15) / 16 * 16 : a->n;
   NormArgs b = {a->x, a->add, a->sum, a->weight, a->out, (_Float16*) a->x16, a->overflow, a->codes, a->scales, a->x_stride, a->add_stride,
-                a->sum_stride, a->out_stride, a->weight_type, a->out_type, a->n, a->dim, a->eps, a->offset, 1.0 / a->dim, 0};
-  const uint32_t waves = (pieces + 255) / 256;
+                a->sum_stride, a->out_stride, a->weight_type, a->out_type, a->n, a->dim, a->eps, a->offset, 1.0 / a->dim, 0, a->x16 != nullptr};
+  const uint32_t each = rows <= 512 ? 1 : 4, waves = (pieces + 64 * each - 1) / (64 * each);
   b.waves = waves > 16 ? 16 : waves;
   const uint32_t k = (pieces + b.waves * 64 - 1) / (b.waves * 64);
   auto* kernel = a->dim % per<T>() ? norm_of<T, true>(k) : norm_of<T, false>(k);

@@ -49,11 +49,11 @@ __device__ inline void store8_as(uint32_t type, void* p, const float (&x)[8]) {
   else kv::store8<OSMOS_BF16>(p, x);
 }
 
-constexpr int kRopeWaves = 4, kAhead = 4;  // kAhead: heads a lane holds the loads of
+constexpr int kRopeWaves = 4;
 
 // a wave takes a row, or a part of its heads: `group` lanes a head, 8 values a lane, so that a lane has the same values of all its
-// heads and makes their sines and cosines once. a half layout's other values come from the other lane by LDS
-template <uint32_t IN, uint32_t DST>
+// heads and makes their sines and cosines once; kAhead: heads it holds the loads of. a half layout's other values come from the other lane by LDS
+template <uint32_t IN, uint32_t DST, int kAhead>
 __global__ __launch_bounds__(64 * kRopeWaves) void rope_kernel(RopeArgs a, const int32_t* __restrict__ positions, kv::Step st, Pages pg) {
   __shared__ float lds[kRopeWaves][64 * 8];
   const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x / 64;
@@ -181,6 +181,12 @@ __global__ __launch_bounds__(64 * kRopeWaves) void rope_kernel(RopeArgs a, const
   }
 }
 
+template <uint32_t IN, int AHEAD>
+auto rope_of(uint32_t dst) {
+  return dst == 0 ? rope_kernel<IN, 0u, AHEAD> : dst == OSMOS_F16 ? rope_kernel<IN, OSMOS_F16, AHEAD>
+         : dst == OSMOS_BF16 ? rope_kernel<IN, OSMOS_BF16, AHEAD> : rope_kernel<IN, OSMOS_F8, AHEAD>;
+}
+
 bool rope_launch(const OsmosRope* o, const int32_t* pos, const kv::Step& st, const Pages& pg, uint32_t dst, const void* v, uint64_t v_stride,
                  uint64_t v_head, hipStream_t s) {
   RopeArgs a = {o->turns, o->q_weight, o->k_weight, (const uint8_t*) o->q, (const uint8_t*) o->k, (const uint8_t*) v, (uint8_t*) o->q_out,
@@ -192,11 +198,10 @@ bool rope_launch(const OsmosRope* o, const int32_t* pos, const kv::Step& st, con
   a.parts = 4096 / a.n < 1 ? 1 : 4096 / a.n < rounds ? 4096 / a.n : rounds;
   const uint64_t waves = (uint64_t) a.n * a.parts;
   const uint32_t grid = (uint32_t) ((waves + kRopeWaves - 1) / kRopeWaves);
-#define OSM_ROPE(IN)                                                                                            \
-  (dst == 0 ? rope_kernel<IN, 0u> : dst == OSMOS_F16 ? rope_kernel<IN, OSMOS_F16> : dst == OSMOS_BF16 ? rope_kernel<IN, OSMOS_BF16> \
-                                                                                   : rope_kernel<IN, OSMOS_F8>)
-  auto* kernel = o->type == OSMOS_F32 ? OSM_ROPE(OSMOS_F32) : o->type == OSMOS_F16 ? OSM_ROPE(OSMOS_F16) : OSM_ROPE(OSMOS_BF16);
-#undef OSM_ROPE
+  const bool one = a.parts == rounds;
+  auto* kernel = o->type == OSMOS_F32 ? one ? rope_of<OSMOS_F32, 1>(dst) : rope_of<OSMOS_F32, 4>(dst)
+                 : o->type == OSMOS_F16 ? one ? rope_of<OSMOS_F16, 1>(dst) : rope_of<OSMOS_F16, 4>(dst)
+                                        : one ? rope_of<OSMOS_BF16, 1>(dst) : rope_of<OSMOS_BF16, 4>(dst);
   kernel<<<grid, 64 * kRopeWaves, 0, s>>>(a, pos, st, pg);
   return hipGetLastError() == hipSuccess;
 }

@@ -13,6 +13,7 @@
 
 #include "rowshost.h"
 #include "common.h"
+#include "lanes.h"
 
 namespace osm {
 namespace rows {
@@ -84,8 +85,14 @@ struct SampleArgs {
   uint32_t slices, slice;  // a row's, and a slice's tokens
   int bits;                // of a token's index
   uint8_t *parts, *plans, *cuts;  // the workspace: each slice's Part, each row's RowPlan and Drawn
-  __device__ inline float heat(uint32_t t) const { return temperature ? temperature[t] : 1.0f; }
-  __device__ inline int32_t k(uint32_t t) const { return top_k ? top_k[t] : 0; }
+};
+// what a row asks for
+struct Wish {
+  float temperature, top_p, min_p, u;
+  int32_t k;
+  __device__ inline Wish(const SampleArgs& a, uint32_t t)
+      : temperature(a.temperature ? a.temperature[t] : 1.0f), top_p(a.top_p ? a.top_p[t] : 1.0f), min_p(a.min_p ? a.min_p[t] : 0.0f), u(a.u[t]),
+        k(a.top_k ? a.top_k[t] : 0) {}
 };
 // whether a row's bins need no weights: those of a few listed tokens do
 __device__ inline bool few(int32_t k) { return k > 0 && (uint32_t) k <= kFew; }
@@ -166,18 +173,6 @@ struct WholeLds : PlanLds {
   uint64_t list[kList];
 };
 
-// lanes' values by DPP: row_shr 1, 2, 4, 8, then lane 15 of a row to the next and 31 to the upper half; `none` where there is no
-// such lane
-template <int STEP>
-__device__ inline uint32_t from_below(uint32_t x, uint32_t none) {
-  constexpr int ctrl = STEP < 4 ? 0x110 + (1 << STEP) : STEP == 4 ? 0x142 : 0x143;
-  constexpr int rows = STEP < 4 ? 0xF : STEP == 4 ? 0xA : 0xC;
-  return (uint32_t) __builtin_amdgcn_update_dpp((int) none, (int) x, ctrl, rows, 0xF, false);
-}
-template <int STEP>
-__device__ inline uint64_t from_below(uint64_t x, uint64_t none) {
-  return (uint64_t) from_below<STEP>((uint32_t) (x >> 32), (uint32_t) (none >> 32)) << 32 | from_below<STEP>((uint32_t) x, (uint32_t) none);
-}
 template <int STEP = 0>
 __device__ inline Sum wave_sums(Sum x) {  // inclusive
   x.n += from_below<STEP>(x.n, 0u), x.m += from_below<STEP>(x.m, (uint64_t) 0);
@@ -278,22 +273,22 @@ struct Piece {
 };
 
 // tokens begin .. end - 1 of a row, P pieces a thread and round (the rounds' loads in flight together)
-template <uint32_t T, int P>
+template <uint32_t T, int P, uint32_t N = kSampleThreads>
 struct Tokens {
   const void* p;
   uint32_t begin, end;
-  static constexpr uint32_t kRound = kSampleThreads * kPer<T> * P;
+  static constexpr uint32_t kRound = N * kPer<T> * P;
   Piece<T> x[P];
   __device__ inline void load(uint32_t at) {
 #pragma unroll
-    for (int k = 0; k < P; k++) x[k].load(p, at + (k * kSampleThreads + threadIdx.x) * kPer<T>, end);
+    for (int k = 0; k < P; k++) x[k].load(p, at + (k * N + threadIdx.x) * kPer<T>, end);
   }
   template <typename F>
   __device__ inline void loaded(uint32_t at, F f) const {
 #pragma unroll
     for (int k = 0; k < P; k++)
 #pragma unroll
-      for (uint32_t j = 0; j < kPer<T>; j++) f(x[k].at(j), at + (k * kSampleThreads + threadIdx.x) * kPer<T> + j);
+      for (uint32_t j = 0; j < kPer<T>; j++) f(x[k].at(j), at + (k * N + threadIdx.x) * kPer<T> + j);
   }
   // those of a plan's spans' logits: most threads have none, so they are read again
   template <typename F>
@@ -314,9 +309,15 @@ struct Tokens {
     while (hits) {
       const uint32_t h = __builtin_ctz(hits);
       hits &= hits - 1;
-      const uint32_t i = at + (h / kPer<T> * kSampleThreads + threadIdx.x) * kPer<T> + h % kPer<T>;
+      const uint32_t i = at + (h / kPer<T> * N + threadIdx.x) * kPer<T> + h % kPer<T>;
       f(logit_at<T>(this->p, i), i);
     }
+  }
+  // all, where the first round is loaded: a second one is read again
+  template <typename F>
+  __device__ inline void again(F f) {
+    if (end - begin <= kRound) loaded(begin, f);
+    else each(f);
   }
   // in ascending order of a thread's own tokens
   template <typename F>
@@ -347,7 +348,8 @@ struct Near {
   }
 };
 
-// a slice's first place and, but for a greedy row, its bins (into l.count and, unless k is small, l.mass): its tokens are one round.
+// a slice's first place and, but for a greedy row, its bins (into l.count and, unless k is small, l.mass): its tokens are one round, but
+// for bf16.
 // bf16's tokens are few values, often: they are counted by value, two a word, and each value is put into its bin once
 template <uint32_t T, typename R, typename L>
 __device__ inline void scan_slice(R& row, const Order<T>& order, float temperature, int32_t k, L& l, uint64_t& first, double& top, uint32_t& valid) {
@@ -364,20 +366,24 @@ __device__ inline void scan_slice(R& row, const Order<T>& order, float temperatu
 #pragma unroll
     for (int i = 0; i < kValues; i += kSampleThreads) l.value[i + tid] = 0;
     __syncthreads();
+    for (uint32_t round = row.begin;;) {
 #pragma unroll
-    for (uint32_t i = 0; i < sizeof(row.x) / 4; i++) {
-      typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
-      const uint32_t w = row.x[i / 4].w[i % 4], size = w & 0x7FFF7FFFu;
-      u16x2 v = __builtin_bit_cast(u16x2, size);
-      v = __builtin_elementwise_min(__builtin_elementwise_max(v, u16x2{kLeastBits, kLeastBits}), u16x2{kLeastBits + kSpan - 1, kLeastBits + kSpan - 1}) -
-          u16x2{kLeastBits, kLeastBits};
-      const uint32_t at = __builtin_bit_cast(uint32_t, v) << 2 | (w >> 1 & 0x40004000u);  // (4096 values of 4 bytes a sign)
-      atomicAdd((uint32_t*) ((uint8_t*) l.value + (at & 0xFFFF)), 1u);
-      atomicAdd((uint32_t*) ((uint8_t*) l.value + (at >> 16)), 1u);
+      for (uint32_t i = 0; i < sizeof(row.x) / 4; i++) {
+        typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
+        const uint32_t w = row.x[i / 4].w[i % 4], size = w & 0x7FFF7FFFu;
+        u16x2 v = __builtin_bit_cast(u16x2, size);
+        v = __builtin_elementwise_min(__builtin_elementwise_max(v, u16x2{kLeastBits, kLeastBits}), u16x2{kLeastBits + kSpan - 1, kLeastBits + kSpan - 1}) -
+            u16x2{kLeastBits, kLeastBits};
+        const uint32_t at = __builtin_bit_cast(uint32_t, v) << 2 | (w >> 1 & 0x40004000u);  // (4096 values of 4 bytes a sign)
+        atomicAdd((uint32_t*) ((uint8_t*) l.value + (at & 0xFFFF)), 1u);
+        atomicAdd((uint32_t*) ((uint8_t*) l.value + (at >> 16)), 1u);
+      }
+      if ((round += row.kRound) >= row.end) break;
+      row.load(round);
     }
     __syncthreads();
     if (l.value[0] | l.value[kSpan - 1] | l.value[kSpan] | l.value[kValues - 1]) {  // (what is past the end is in the last)
-      row.loaded(row.begin, [&](float x, uint32_t) { best = fmaxf(best, x); });
+      row.again([&](float x, uint32_t) { best = fmaxf(best, x); });
     } else {
 #pragma unroll
       for (int j = 0; j < kValues / kSampleThreads; j++) {
@@ -399,7 +405,7 @@ __device__ inline void scan_slice(R& row, const Order<T>& order, float temperatu
   if (!(most > none)) return;
   if (!warm) {  // (the lowest index among equals; elsewhere its logit is all that is asked for)
     uint32_t at = ~0u;
-    row.loaded(row.begin, [&](float x, uint32_t i) { at = ordered<T>(x) == most && i < at ? i : at; });
+    row.again([&](float x, uint32_t i) { at = ordered<T>(x) == most && i < at ? i : at; });
     if (at != ~0u) atomicMin(&l.index, at);
     __syncthreads();
     first = order.place(most, l.index);
@@ -421,7 +427,7 @@ __device__ inline void scan_slice(R& row, const Order<T>& order, float temperatu
   };
   if constexpr (by_value) {
     if (l.value[0] | l.value[kSpan - 1] | l.value[kSpan] | l.value[kValues - 1])
-      row.loaded(row.begin, [&](float x, uint32_t) {
+      row.again([&](float x, uint32_t) {
         const uint32_t v = (__float_as_uint(x) >> 16 & 0x7FFF) - kLeastBits;
         if ((int) v < 1 || v >= kSpan - 1) add(x, 1, mass);
       });
@@ -438,20 +444,22 @@ __device__ inline void scan_slice(R& row, const Order<T>& order, float temperatu
   valid = total(Sum{valid + l.count[tid], 0}, l).n;
 }
 
-constexpr int kPieces = 4;  // 16 bytes of a slice a thread
+// 16 bytes of a slice a thread and round, and of a row that is one slice
+constexpr int kPieces = 4;
+template <uint32_t T> constexpr int kRowPieces = T == OSMOS_F32 ? 8 : 4;
 template <uint32_t T>
-__global__ __launch_bounds__(kSampleThreads) void scan_kernel(SampleArgs a) {
+__global__ __launch_bounds__(kSampleThreads, 8) void scan_kernel(SampleArgs a) {
   __shared__ ScanOf<T> l;
   const uint32_t t = blockIdx.x / a.slices, s = blockIdx.x - t * a.slices, begin = s * a.slice, tid = threadIdx.x;
   const uint32_t end = begin + a.slice < a.vocab ? begin + a.slice : a.vocab;
   Tokens<T, kPieces> row = {(const uint8_t*) a.logits + t * a.stride * kv::size_of(T), begin, end};
   Part* part = (Part*) a.parts + blockIdx.x;
   const Order<T> order = {a.bits};
-  const int32_t k = a.k(t);
+  const int32_t k = a.top_k ? a.top_k[t] : 0;
   uint64_t first;
   double top;
   uint32_t valid;
-  scan_slice<T>(row, order, a.heat(t), k, l, first, top, valid);
+  scan_slice<T>(row, order, a.temperature ? a.temperature[t] : 1.0f, k, l, first, top, valid);
   if (valid) {
     part->count[tid] = l.count[tid];
     if (!few(k)) part->mass[tid] = l.mass[tid];
@@ -477,10 +485,11 @@ __device__ inline uint64_t u_goal(double u, uint64_t m) {
 
 // a row's plan from its bins (thread i bin i's sums): what is written is there for all threads when it returns
 template <uint32_t T>
-__device__ inline void make_plan(const SampleArgs& a, uint32_t t, const Order<T>& order, PlanLds& l, uint64_t first, double top, uint32_t valid, Sum bin) {
+__device__ inline void make_plan(const SampleArgs& a, uint32_t t, const Wish& wish, const Order<T>& order, PlanLds& l, uint64_t first, double top,
+                                 uint32_t valid, Sum bin) {
   const uint32_t tid = threadIdx.x;
-  const float temperature = a.heat(t), top_p = a.top_p ? a.top_p[t] : 1.0f, min_p = a.min_p ? a.min_p[t] : 0.0f, u = a.u[t];
-  const int32_t k = a.k(t);
+  const float temperature = wish.temperature, top_p = wish.top_p, min_p = wish.min_p, u = wish.u;
+  const int32_t k = wish.k;
   const Scale sc = {bins_a_unit(temperature), top};
   Plan& p = l.plan;
   if (first == ~0ull || !(temperature > 0.0f)) {
@@ -577,12 +586,24 @@ __global__ __launch_bounds__(kSampleThreads) void plan_kernel(SampleArgs a) {
   __shared__ double tops[kMostSlices];  // (every wave writes the same)
   const uint32_t t = blockIdx.x, tid = threadIdx.x, lane = tid & 63;
   const Part* parts = (const Part*) a.parts + (uint64_t) t * a.slices;
-  const bool small = few(a.k(t));
-  // a lane a slice (64 of them a round), then a thread a bin
+  const Wish wish(a, t);
+  const bool small = few(wish.k);
+  // the slices' bins as they lie, while their tops are on the way (what a slice of no bins holds is left out): then each to its place
+  uint32_t n[kAtOnce];
+  uint64_t m[kAtOnce];
+  auto load = [&](uint32_t s0) {
+#pragma unroll
+    for (int i = 0; i < kAtOnce; i++) {
+      const Part* from = parts + (s0 + i < a.slices ? s0 + i : s0);
+      n[i] = from->count[tid], m[i] = small ? 0 : from->mass[tid];
+    }
+  };
+  load(0);
+  l.prefix.before[tid] = 0, l.prefix.ahead[tid] = 0;
   uint64_t first = ~0ull;
   double top = -__builtin_inf();
   uint32_t valid = 0;
-  for (uint32_t s = lane; s < a.slices; s += 64) {
+  for (uint32_t s = lane; s < a.slices; s += 64) {  // (a lane a slice)
     const uint64_t f = parts[s].first;
     const uint32_t v = parts[s].valid;
     const double own = v ? parts[s].top : -__builtin_inf();
@@ -590,7 +611,6 @@ __global__ __launch_bounds__(kSampleThreads) void plan_kernel(SampleArgs a) {
     top = fmax(top, own), valid += v;
     first = f < first ? f : first;
   }
-  __syncthreads();
 #pragma unroll
   for (int o = 32; o; o >>= 1) {
     const uint64_t f = (uint64_t) (uint32_t) __shfl_xor((int) (first >> 32), o) << 32 | (uint32_t) __shfl_xor((int) first, o);
@@ -598,26 +618,23 @@ __global__ __launch_bounds__(kSampleThreads) void plan_kernel(SampleArgs a) {
     top = fmax(top, __shfl_xor(top, o));
     valid += (uint32_t) __shfl_xor((int) valid, o);
   }
-  Sum bin = {0, 0};
-  for (uint32_t s0 = 0; s0 < a.slices; s0 += kAtOnce) {
-    uint32_t n[kAtOnce];
-    uint64_t m[kAtOnce];
-    bool in[kAtOnce];
+  __syncthreads();
+  for (uint32_t s0 = 0;;) {
 #pragma unroll
     for (int i = 0; i < kAtOnce; i++) {
-      const uint32_t s = s0 + i < a.slices ? s0 + i : s0;
-      const double by = top - tops[s];  // (a slice of no bins: infinite)
-      in[i] = s0 + i < a.slices && by <= tid;
-      const Part* from = parts + (in[i] ? s : 0);
-      const uint32_t j = in[i] ? tid - (uint32_t) by : 0;
-      n[i] = from->count[j], m[i] = small ? 0 : from->mass[j];
+      const double b = s0 + i < a.slices ? top - tops[s0 + i] + (int) tid : kBins;  // (a slice of no bins: infinite)
+      if (b < kBins) {
+        atomicAdd(&l.prefix.ahead[(int) b], n[i]);
+        atomicAdd((unsigned long long*) &l.prefix.before[(int) b], (unsigned long long) m[i]);
+      }
     }
-#pragma unroll
-    for (int i = 0; i < kAtOnce; i++)
-      if (in[i]) bin.n += n[i], bin.m += m[i];
+    if ((s0 += kAtOnce) >= a.slices) break;
+    load(s0);
   }
+  __syncthreads();
+  const Sum bin = {l.prefix.ahead[tid], l.prefix.before[tid]};
   const Order<T> order = {a.bits};
-  make_plan<T>(a, t, order, l, first, top, valid, bin);
+  make_plan<T>(a, t, wish, order, l, first, top, valid, bin);
   RowPlan* to = (RowPlan*) a.plans + t;
   if (tid < sizeof(Plan) / 4) ((uint32_t*) &to->plan)[tid] = ((const uint32_t*) &l.plan)[tid];
   if (l.plan.done) return;
@@ -637,16 +654,18 @@ __device__ inline bool planned(const Plan& p, float x) {
   return slot_of(p, Scale{p.by, p.top}.bin_of(x)) >= 0;
 }
 
+constexpr int kListThreads = 256;
 template <uint32_t T>
-__global__ __launch_bounds__(kSampleThreads) void list_kernel(SampleArgs a) {
+__global__ __launch_bounds__(kListThreads) void list_kernel(SampleArgs a, uint32_t blocks) {
   __shared__ uint64_t list[kList];
   __shared__ uint32_t listed, start;
-  const uint32_t t = blockIdx.x / a.slices, s = blockIdx.x - t * a.slices, begin = s * a.slice;
-  const uint32_t end = begin + a.slice < a.vocab ? begin + a.slice : a.vocab;
+  constexpr uint32_t each = kListThreads * kPer<T> * kPieces;
+  const uint32_t t = blockIdx.x / blocks, begin = (blockIdx.x - t * blocks) * each;
   RowPlan* row_plan = (RowPlan*) a.plans + t;
-  const Plan& p = row_plan->plan;
-  Tokens<T, kPieces> row = {(const uint8_t*) a.logits + t * a.stride * kv::size_of(T), begin, end};
+  Tokens<T, kPieces, kListThreads> row = {(const uint8_t*) a.logits + t * a.stride * kv::size_of(T), begin,
+                                          begin + each < a.vocab ? begin + each : a.vocab};
   row.load(begin);
+  const Plan p = row_plan->plan;
   if (p.done) return;
   const Order<T> order = {a.bits};
   if (threadIdx.x == 0) listed = 0;
@@ -657,9 +676,10 @@ __global__ __launch_bounds__(kSampleThreads) void list_kernel(SampleArgs a) {
     if (at < kList) list[at] = order.place(x, i);
   });
   __syncthreads();
-  if (threadIdx.x == 0 && listed) start = atomicAdd(&row_plan->plan.listed, listed);
+  if (!listed) return;
+  if (threadIdx.x == 0) start = atomicAdd(&row_plan->plan.listed, listed);
   __syncthreads();
-  for (uint32_t i = threadIdx.x; i < listed && i < kList; i += kSampleThreads)
+  for (uint32_t i = threadIdx.x; i < listed && i < kList; i += kListThreads)
     if (start + i < kList) row_plan->list[start + i] = list[i];
 }
 
@@ -771,9 +791,10 @@ __device__ __attribute__((noinline)) void draw_slowly(const void* logits, uint32
 }
 
 // the choice among the listed tokens: each one's count and weight up to it. a token's bin is cut into 2^split parts of places, each
-// part has its tokens together, and each token is compared with the others of its part
+// part has its tokens together, and each token is compared with the others of its part. at: the list's tokens tid and tid + 1024
 template <uint32_t T>
-__device__ inline void draw(const SampleArgs& a, uint32_t t, const Order<T>& order, const Plan& p, Prefix& prefix, const uint64_t* list, DrawLds& l) {
+__device__ inline void draw(const SampleArgs& a, uint32_t t, const Order<T>& order, const Plan& p, Prefix& prefix, const uint64_t* list,
+                            uint64_t (&at)[2], DrawLds& l) {
   const uint32_t tid = threadIdx.x, n = p.listed;
   const void* logits = (const uint8_t*) a.logits + t * a.stride * kv::size_of(T);
   const Scale sc = {p.by, p.top};
@@ -783,7 +804,7 @@ __device__ inline void draw(const SampleArgs& a, uint32_t t, const Order<T>& ord
   l.part_n[tid] = 0, l.part_m[tid] = 0, l.filled[tid] = 0, l.part_lo[tid] = ~0ull, l.part_hi[tid] = 0;
   Cut cut = {~0ull, p.k ? p.k : p.valid, p.all}, d;
   double least_y = -__builtin_inf();
-  uint64_t at[2], weight[2];
+  uint64_t weight[2];
   double y[2];
   int bin[2], slot[2];
   uint32_t part[2];
@@ -794,7 +815,6 @@ __device__ inline void draw(const SampleArgs& a, uint32_t t, const Order<T>& ord
       const uint32_t i = tid + j * kSampleThreads;
       slot[j] = -1;
       if (i >= n) continue;
-      at[j] = list[i];
       y[j] = sc.y(order.logit(at[j]));
       const double middle = __builtin_rint(y[j]);
       weight[j] = whole_weight(y[j] - middle);
@@ -913,10 +933,11 @@ __global__ __launch_bounds__(kSampleThreads) void draw_kernel(SampleArgs a) {
   if (tid < sizeof(Plan) / 4) ((uint32_t*) &p)[tid] = ((const uint32_t*) &from->plan)[tid];
   prefix.before[tid] = from->prefix.before[tid], prefix.ahead[tid] = from->prefix.ahead[tid];  // (what a greedy row's plan leaves is not used)
   if (tid == 0) prefix.before[kBins] = from->prefix.before[kBins], prefix.ahead[kBins] = from->prefix.ahead[kBins];
+  uint64_t at[2] = {from->list[tid], from->list[tid + kSampleThreads]};  // (past the listed ones: not looked at)
   __syncthreads();
   if (p.done) return;
   const Order<T> order = {a.bits};
-  draw<T>(a, blockIdx.x, order, p, prefix, from->list, l);
+  draw<T>(a, blockIdx.x, order, p, prefix, from->list, at, l);
 }
 
 // a row of one slice
@@ -924,15 +945,16 @@ template <uint32_t T>
 __global__ __launch_bounds__(kSampleThreads) void sample_kernel(SampleArgs a) {
   __shared__ WholeLds<T> l;
   const uint32_t t = blockIdx.x;
-  Tokens<T, kPieces> row = {(const uint8_t*) a.logits + t * a.stride * kv::size_of(T), 0, a.vocab};
+  Tokens<T, kRowPieces<T>> row = {(const uint8_t*) a.logits + t * a.stride * kv::size_of(T), 0, a.vocab};
   const Order<T> order = {a.bits};
+  const Wish wish(a, t);
   uint64_t first;
   double top;
   uint32_t valid;
-  scan_slice<T>(row, order, a.heat(t), a.k(t), l.scan, first, top, valid);
+  scan_slice<T>(row, order, wish.temperature, wish.k, l.scan, first, top, valid);
   Sum bin = {0, 0};
   if (valid) bin = {l.scan.count[threadIdx.x], l.scan.mass[threadIdx.x]};
-  make_plan<T>(a, t, order, l, first, top, valid, bin);
+  make_plan<T>(a, t, wish, order, l, first, top, valid, bin);
   if (l.plan.done) return;
   row.loaded_between(0, l.plan, [&](float x, uint32_t i) {
     if (!planned<T>(l.plan, x)) return;
@@ -940,7 +962,8 @@ __global__ __launch_bounds__(kSampleThreads) void sample_kernel(SampleArgs a) {
     if (at < kList) l.list[at] = order.place(x, i);
   });
   __syncthreads();
-  draw<T>(a, t, order, l.plan, l.prefix, l.list, l.draw);
+  uint64_t at[2] = {l.list[threadIdx.x], l.list[threadIdx.x + kSampleThreads]};
+  draw<T>(a, t, order, l.plan, l.prefix, l.list, at, l.draw);
 }
 
 // every token's part of the kept weights
@@ -978,7 +1001,16 @@ __global__ __launch_bounds__(kSampleThreads) void probs_kernel(SampleArgs a, uin
 }
 
 inline int index_bits(uint32_t vocab) { return vocab > 1 ? 32 - __builtin_clz(vocab - 1) : 0; }
-inline uint32_t slice_of(const OsmosSample* a) { return a->type == OSMOS_F32 ? kSampleThreads * 4 * kPieces : kSampleThreads * 8 * kPieces; }
+// a row of up to 32768 tokens is one slice. bf16's slices cost the same whatever they hold (their values are put into bins at the
+// end): as long as there are 512 of them
+inline uint32_t slice_of(const OsmosSample* a) {
+  constexpr uint32_t round = kSampleThreads * kPieces * 4, row = 32768;
+  if (a->vocab <= row) return row;
+  if (a->type == OSMOS_F32) return round;
+  const uint32_t rounds = (a->vocab + row - 1) / row;
+  const uint64_t each = a->type == OSMOS_BF16 ? (uint64_t) a->n * rounds / 512 : 1;
+  return row * (uint32_t) (each < 1 ? 1 : each < rounds ? each : rounds);
+}
 inline uint32_t slices_of(const OsmosSample* a) { return (a->vocab + slice_of(a) - 1) / slice_of(a); }
 inline uint64_t round256(uint64_t n) { return (n + 255) / 256 * 256; }
 struct SampleRoom {
@@ -995,7 +1027,8 @@ bool sample_launch(const SampleArgs& a, hipStream_t s) {
   if (a.slices > 1) {
     scan_kernel<T><<<a.n * a.slices, kSampleThreads, 0, s>>>(a);
     plan_kernel<T><<<a.n, kSampleThreads, 0, s>>>(a);
-    list_kernel<T><<<a.n * a.slices, kSampleThreads, 0, s>>>(a);
+    const uint32_t list_each = kListThreads * kPer<T> * kPieces, blocks = (a.vocab + list_each - 1) / list_each;
+    list_kernel<T><<<a.n * blocks, kListThreads, 0, s>>>(a, blocks);
     draw_kernel<T><<<a.n, kSampleThreads, 0, s>>>(a);
   } else {
     sample_kernel<T><<<a.n, kSampleThreads, 0, s>>>(a);
