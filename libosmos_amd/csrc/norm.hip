@@ -10,34 +10,44 @@ namespace rows {
 // 16 bytes of values as floats, at any address that their type allows
 template <uint32_t T> constexpr int per() { return T == OSMOS_F32 ? 4 : 8; }
 typedef float f32x4_u __attribute__((ext_vector_type(4), aligned(4)));
-typedef _Float16 f16x4_u __attribute__((ext_vector_type(4), aligned(2)));
-typedef __bf16 bf16x4_u __attribute__((ext_vector_type(4), aligned(2)));
+template <int N> struct Halves {
+  typedef _Float16 F __attribute__((ext_vector_type(N), aligned(2)));
+  typedef __bf16 B __attribute__((ext_vector_type(N), aligned(2)));
+};
 
 template <int N>
 __device__ inline void load(uint32_t type, const void* p, uint64_t at, float* x) {
+  if (type == OSMOS_F32) {
 #pragma unroll
-  for (int i = 0; i < N; i += 4) {
-    if (type == OSMOS_F32) {
+    for (int i = 0; i < N; i += 4) {
       const f32x4_u v = gload<f32x4_u>((const float*) p + at + i);
       x[i] = v[0], x[i + 1] = v[1], x[i + 2] = v[2], x[i + 3] = v[3];
-    } else if (type == OSMOS_F16) {
-      const f16x4_u v = gload<f16x4_u>((const _Float16*) p + at + i);
-      x[i] = (float) v[0], x[i + 1] = (float) v[1], x[i + 2] = (float) v[2], x[i + 3] = (float) v[3];
-    } else {
-      const bf16x4_u v = gload<bf16x4_u>((const __bf16*) p + at + i);
-      x[i] = (float) v[0], x[i + 1] = (float) v[1], x[i + 2] = (float) v[2], x[i + 3] = (float) v[3];
     }
+  } else if (type == OSMOS_F16) {
+    const typename Halves<N>::F v = gload<typename Halves<N>::F>((const _Float16*) p + at);
+#pragma unroll
+    for (int i = 0; i < N; i++) x[i] = (float) v[i];
+  } else {
+    const typename Halves<N>::B v = gload<typename Halves<N>::B>((const __bf16*) p + at);
+#pragma unroll
+    for (int i = 0; i < N; i++) x[i] = (float) v[i];
   }
 }
 template <int N>
 __device__ inline void store(uint32_t type, void* p, uint64_t at, const float* x) {
+  if (type == OSMOS_F32) {
 #pragma unroll
-  for (int i = 0; i < N; i += 4) {
-    if (type == OSMOS_F32) *(f32x4_u*) ((float*) p + at + i) = f32x4_u{x[i], x[i + 1], x[i + 2], x[i + 3]};
-    else if (type == OSMOS_F16)
-      *(f16x4_u*) ((_Float16*) p + at + i) = f16x4_u{(_Float16) x[i], (_Float16) x[i + 1], (_Float16) x[i + 2], (_Float16) x[i + 3]};
-    else
-      *(bf16x4_u*) ((__bf16*) p + at + i) = bf16x4_u{(__bf16) x[i], (__bf16) x[i + 1], (__bf16) x[i + 2], (__bf16) x[i + 3]};
+    for (int i = 0; i < N; i += 4) *(f32x4_u*) ((float*) p + at + i) = f32x4_u{x[i], x[i + 1], x[i + 2], x[i + 3]};
+  } else if (type == OSMOS_F16) {
+    typename Halves<N>::F v;
+#pragma unroll
+    for (int i = 0; i < N; i++) v[i] = (_Float16) x[i];
+    *(typename Halves<N>::F*) ((_Float16*) p + at) = v;
+  } else {
+    typename Halves<N>::B v;
+#pragma unroll
+    for (int i = 0; i < N; i++) v[i] = (__bf16) x[i];
+    *(typename Halves<N>::B*) ((__bf16*) p + at) = v;
   }
 }
 __device__ inline float load1(uint32_t type, const void* p, uint64_t at) {
@@ -209,7 +219,8 @@ bool norm_launch(const OsmosNorm* a, hipStream_t s) {
   const uint32_t pieces = (a->dim + per<T>() - 1) / per<T>(), rows = a->x16 ? (a->n + 15) / 16 * 16 : a->n;
   NormArgs b = {a->x, a->add, a->sum, a->weight, a->out, (_Float16*) a->x16, a->overflow, a->codes, a->scales, a->x_stride, a->add_stride,
                 a->sum_stride, a->out_stride, a->weight_type, a->out_type, a->n, a->dim, a->eps, a->offset, 1.0 / a->dim, 0, a->x16 != nullptr};
-  const uint32_t each = rows <= 512 ? 1 : 4, waves = (pieces + 64 * each - 1) / (64 * each);
+  const uint64_t all = (uint64_t) rows * ((pieces + 63) / 64) / 8192;
+  const uint32_t each = all < 1 ? 1 : all < 4 ? (uint32_t) all : 4, waves = (pieces + 64 * each - 1) / (64 * each);
   b.waves = waves > 16 ? 16 : waves;
   const uint32_t k = (pieces + b.waves * 64 - 1) / (b.waves * 64);
   auto* kernel = a->dim % per<T>() ? norm_of<T, true>(k) : norm_of<T, false>(k);

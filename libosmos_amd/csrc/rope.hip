@@ -62,7 +62,7 @@ __global__ __launch_bounds__(64 * kRopeWaves) void rope_kernel(RopeArgs a, const
   const uint32_t g = lane & (a.group - 1), first = lane / a.group, each = 64 / a.group;
   const uint32_t turned = a.heads + a.kv_heads, all = turned + (DST ? a.kv_heads : 0);
   const bool active = g * 8 < a.dim;
-  float x[kAhead][8];
+  float x[kAhead][8], scale[kAhead];
   auto load = [&](uint32_t h0) __attribute__((always_inline)) {
 #pragma unroll
     for (int i = 0; i < kAhead; i++) {
@@ -72,6 +72,7 @@ __global__ __launch_bounds__(64 * kRopeWaves) void rope_kernel(RopeArgs a, const
         for (int j = 0; j < 8; j++) x[i][j] = 0.0f;
         continue;
       }
+      if (DST == OSMOS_F8 && pg.scale && h >= a.heads) scale[i] = pg.scale[h - a.heads];  // (keys', then values')
       const uint8_t* p = h < a.heads ? a.q + (t * a.q_stride + h * a.q_head) * kv::size_of(IN)
                          : h < turned ? a.k + (t * a.k_stride + (h - a.heads) * a.k_head) * kv::size_of(IN)
                                       : a.v + (t * a.v_stride + (h - turned) * a.v_head) * kv::size_of(IN);
@@ -80,35 +81,15 @@ __global__ __launch_bounds__(64 * kRopeWaves) void rope_kernel(RopeArgs a, const
   };
   uint32_t h0 = part * each + first;
   load(h0);
-  int pos;
-  uint8_t* to = nullptr;  // where the row's keys go
-  if constexpr (DST != 0) {
-    kv::Seq q;
-    if (!kv::sequence_of(st, (int) t, pg.page, q)) return;
-    pos = q.len - (q.row0 + q.rows - (int) t);
-    if ((int) t < q.row0 || (int) t >= q.row0 + q.rows || pos < 0 || pos >= q.end) return;
-    const uint32_t id = (uint32_t) gload<int>(q.table + (uint32_t) pos / pg.page);
-    if (id < pg.pages) to = pg.data + ((uint64_t) id * a.kv_heads * pg.page + ((uint32_t) pos & (pg.page - 1))) * a.dim * kv::size_of(DST);
-  } else {
-    pos = positions[t];
-  }
+  // (what does not hang on the position is on its way while that is looked up)
   const uint32_t half = a.rot / 2;
   const bool pairs = a.layout == OSMOS_ROPE_PAIRS;
   const uint32_t mine = g * 8 >= a.rot ? 0 : a.rot - g * 8;  // the lane's first values that turn
-  float c[8], s[8];
+  double turns[8];
 #pragma unroll
   for (int j = 0; j < 8; j++) {
     const uint32_t e = g * 8 + j;
-    c[j] = 1.0f, s[j] = 0.0f;
-    if ((uint32_t) j < mine) {
-      if (pairs && (j & 1)) {
-        c[j] = c[j - 1], s[j] = -s[j - 1];
-      } else {
-        sin_cos((double) pos * a.turns[pairs ? e / 2 : e < half ? e : e - half], s[j], c[j]);
-        c[j] *= a.scale, s[j] *= a.scale;
-        if (pairs || e < half) s[j] = -s[j];
-      }
-    }
+    turns[j] = (uint32_t) j >= mine || (pairs && j & 1) ? 0.0 : a.turns[pairs ? e / 2 : e < half ? e : e - half];
   }
   float wq[8], wk[8];
   if (a.q_weight || a.k_weight)
@@ -117,6 +98,34 @@ __global__ __launch_bounds__(64 * kRopeWaves) void rope_kernel(RopeArgs a, const
       wq[j] = a.q_weight && active ? __fadd_rn(a.q_weight[g * 8 + j], a.offset) : 1.0f;
       wk[j] = a.k_weight && active ? __fadd_rn(a.k_weight[g * 8 + j], a.offset) : 1.0f;
     }
+  int pos;
+  uint32_t id = 0;  // (the row's page)
+  if constexpr (DST != 0) {
+    kv::Seq q;
+    if (!kv::sequence_of(st, (int) t, pg.page, q)) return;
+    pos = q.len - (q.row0 + q.rows - (int) t);
+    if ((int) t < q.row0 || (int) t >= q.row0 + q.rows || pos < 0 || pos >= q.end) return;
+    id = (uint32_t) gload<int>(q.table + (uint32_t) pos / pg.page);
+  } else {
+    pos = positions[t];
+  }
+  float c[8], s[8];
+#pragma unroll
+  for (int j = 0; j < 8; j++) {
+    c[j] = 1.0f, s[j] = 0.0f;
+    if ((uint32_t) j < mine) {
+      if (pairs && (j & 1)) {
+        c[j] = c[j - 1], s[j] = -s[j - 1];
+      } else {
+        sin_cos((double) pos * turns[j], s[j], c[j]);
+        c[j] *= a.scale, s[j] *= a.scale;
+        if (pairs || g * 8 + j < half) s[j] = -s[j];
+      }
+    }
+  }
+  uint8_t* to = nullptr;  // where the row's keys go
+  if constexpr (DST != 0)
+    if (id < pg.pages) to = pg.data + ((uint64_t) id * a.kv_heads * pg.page + ((uint32_t) pos & (pg.page - 1))) * a.dim * kv::size_of(DST);
   float* row = lds[wave];
   for (;;) {
 #pragma unroll
@@ -170,7 +179,7 @@ __global__ __launch_bounds__(64 * kRopeWaves) void rope_kernel(RopeArgs a, const
         } else if (to) {
           const bool second = h >= turned;
           const uint32_t hh = h - (second ? turned : a.heads);
-          if (DST == OSMOS_F8 && pg.scale) kv::divide8(y, pg.scale[(second ? a.kv_heads : 0) + hh]);
+          if (DST == OSMOS_F8 && pg.scale) kv::divide8(y, scale[i]);
           kv::store8<DST>(to + (second ? pg.plane : 0) + ((uint64_t) hh * pg.page * a.dim + g * 8) * kv::size_of(DST), y);
         }
       }
