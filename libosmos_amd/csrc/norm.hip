@@ -50,9 +50,6 @@ __device__ inline void store(uint32_t type, void* p, uint64_t at, const float* x
     *(typename Halves<N>::B*) ((__bf16*) p + at) = v;
   }
 }
-__device__ inline float load1(uint32_t type, const void* p, uint64_t at) {
-  return type == OSMOS_F32 ? ((const float*) p)[at] : type == OSMOS_F16 ? (float) ((const _Float16*) p)[at] : (float) ((const __bf16*) p)[at];
-}
 __device__ inline void store1(uint32_t type, void* p, uint64_t at, float x) {
   if (type == OSMOS_F32) ((float*) p)[at] = x;
   else if (type == OSMOS_F16) ((_Float16*) p)[at] = (_Float16) x;
@@ -62,8 +59,19 @@ __device__ inline void store1(uint32_t type, void* p, uint64_t at, float x) {
 template <int N, bool TAIL>
 __device__ inline void load_part(uint32_t type, const void* p, uint64_t at, uint32_t left, float* x) {
   if (!TAIL || left >= N) return load<N>(type, p, at, x);
+  uint32_t w[N];  // (all of them on their way together: one after the other 700 rows of 4999 take 8.9 us, so 7.5)
+  if (type == OSMOS_F32) {
 #pragma unroll
-  for (int i = 0; i < N; i++) x[i] = (uint32_t) i < left ? load1(type, p, at + i) : 0.0f;
+    for (int i = 0; i < N; i++) w[i] = gload<uint32_t>((const uint32_t*) p + at + ((uint32_t) i < left ? i : 0));
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; i++) w[i] = gload<uint16_t>((const uint16_t*) p + at + ((uint32_t) i < left ? i : 0));
+  }
+#pragma unroll
+  for (int i = 0; i < N; i++) {
+    const float v = type == OSMOS_F32 ? __uint_as_float(w[i]) : type == OSMOS_F16 ? __half2float(__ushort_as_half((unsigned short) w[i])) : __uint_as_float(w[i] << 16);
+    x[i] = (uint32_t) i < left ? v : 0.0f;
+  }
 }
 template <int N, bool TAIL>
 __device__ inline void store_part(uint32_t type, void* p, uint64_t at, uint32_t left, const float* x) {

@@ -49,13 +49,21 @@ __device__ inline void store8_as(uint32_t type, void* p, const float (&x)[8]) {
   else kv::store8<OSMOS_BF16>(p, x);
 }
 
+// a wave's LDS writes before its reads that follow (the wave's own: it does not wait for others)
+__device__ inline void wave_order() {
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
 constexpr int kRopeWaves = 4;
 
 // a wave takes a row, or a part of its heads: `group` lanes a head, 8 values a lane, so that a lane has the same values of all its
-// heads and makes their sines and cosines once; kAhead: heads it holds the loads of. a half layout's other values come from the other lane by LDS
+// heads. the wave makes each of the row's angles once, a lane one or two, and hands them round by LDS; kAhead: heads it holds the loads of. a half layout's other values come from the other lane by LDS
 template <uint32_t IN, uint32_t DST, int kAhead>
 __global__ __launch_bounds__(64 * kRopeWaves) void rope_kernel(RopeArgs a, const int32_t* __restrict__ positions, kv::Step st, Pages pg) {
   __shared__ float lds[kRopeWaves][64 * 8];
+  __shared__ float2 angle[kRopeWaves][OSMOS_ATTN_MAX_DIM / 2];
   const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x / 64;
   const uint32_t unit = blockIdx.x * kRopeWaves + wave, t = unit / a.parts, part = unit - t * a.parts;
   if (t >= a.n) return;
@@ -85,12 +93,9 @@ __global__ __launch_bounds__(64 * kRopeWaves) void rope_kernel(RopeArgs a, const
   const uint32_t half = a.rot / 2;
   const bool pairs = a.layout == OSMOS_ROPE_PAIRS;
   const uint32_t mine = g * 8 >= a.rot ? 0 : a.rot - g * 8;  // the lane's first values that turn
-  double turns[8];
+  double turns[2];  // (a lane's angles: pairs lane and lane + 64)
 #pragma unroll
-  for (int j = 0; j < 8; j++) {
-    const uint32_t e = g * 8 + j;
-    turns[j] = (uint32_t) j >= mine || (pairs && j & 1) ? 0.0 : a.turns[pairs ? e / 2 : e < half ? e : e - half];
-  }
+  for (int i = 0; i < 2; i++) turns[i] = lane + 64 * i < half ? a.turns[lane + 64 * i] : 0.0;
   float wq[8], wk[8];
   if (a.q_weight || a.k_weight)
 #pragma unroll
@@ -109,18 +114,22 @@ __global__ __launch_bounds__(64 * kRopeWaves) void rope_kernel(RopeArgs a, const
   } else {
     pos = positions[t];
   }
+#pragma unroll
+  for (int i = 0; i < 2; i++)
+    if (64 * i < (int) half) {
+      float sine, cosine;
+      sin_cos((double) pos * turns[i], sine, cosine);
+      if (lane + 64 * i < half) angle[wave][lane + 64 * i] = make_float2(cosine * a.scale, sine * a.scale);
+    }
+  wave_order();
   float c[8], s[8];
 #pragma unroll
   for (int j = 0; j < 8; j++) {
+    const uint32_t e = g * 8 + j;
     c[j] = 1.0f, s[j] = 0.0f;
     if ((uint32_t) j < mine) {
-      if (pairs && (j & 1)) {
-        c[j] = c[j - 1], s[j] = -s[j - 1];
-      } else {
-        sin_cos((double) pos * turns[j], s[j], c[j]);
-        c[j] *= a.scale, s[j] *= a.scale;
-        if (pairs || g * 8 + j < half) s[j] = -s[j];
-      }
+      const float2 v = angle[wave][pairs ? e / 2 : e < half ? e : e - half];
+      c[j] = v.x, s[j] = (pairs ? !(j & 1) : e < half) ? -v.y : v.y;
     }
   }
   uint8_t* to = nullptr;  // where the row's keys go
@@ -147,13 +156,10 @@ __global__ __launch_bounds__(64 * kRopeWaves) void rope_kernel(RopeArgs a, const
 #pragma unroll
         for (int j = 0; j < 8; j++) z[j] = y[j ^ 1];
       } else {
-        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-        __builtin_amdgcn_wave_barrier();
+        wave_order();
         *(kv::f32x4*) (row + lane * 8) = kv::f32x4{y[0], y[1], y[2], y[3]};
         *(kv::f32x4*) (row + lane * 8 + 4) = kv::f32x4{y[4], y[5], y[6], y[7]};
-        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-        __builtin_amdgcn_wave_barrier();
-        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+        wave_order();
         const float* head = row + (lane - g) * 8;
         if (half % 8 == 0) {
           const uint32_t e = g * 8 < half ? g * 8 + half : g * 8 < a.rot ? g * 8 - half : g * 8;
