@@ -150,7 +150,7 @@ constexpr int kValues = 8192;  // bf16: the values from 2^-24 to 2^8 of either s
 struct ValueLds : ScanLds {
   uint32_t value[kValues];
 };
-template <uint32_t T> using ScanOf = std::conditional_t<T == OSMOS_BF16, ValueLds, ScanLds>;
+template <bool VALUES> using ScanOf = std::conditional_t<VALUES, ValueLds, ScanLds>;
 struct PlanLds {
   Plan plan;
   Prefix prefix;
@@ -164,10 +164,9 @@ struct DrawLds {
   uint64_t word[kSampleWaves], found[4], sum;
   uint32_t at, crowded;
 };
-template <uint32_t T>
 struct WholeLds : PlanLds {
   union {
-    ScanOf<T> scan;
+    ScanLds scan;
     DrawLds draw;
   };
   uint64_t list[kList];
@@ -350,12 +349,11 @@ struct Near {
 };
 
 // a slice's first place and, but for a greedy row, its bins (into l.count and, unless k is small, l.mass): its tokens are one round, but
-// for bf16.
-// bf16's tokens are few values, often: they are counted by value, two a word, and each value is put into its bin once
-template <uint32_t T, typename R, typename L>
+// by VALUES. bf16's tokens are few values, often: by VALUES they are counted by value, two a word, and each value is put into its bin
+// once
+template <uint32_t T, bool VALUES, typename R, typename L>
 __device__ inline void scan_slice(R& row, const Order<T>& order, float temperature, int32_t k, L& l, uint64_t& first, double& top, uint32_t& valid) {
   constexpr uint32_t kLeastBits = 0x3380, kSpan = kValues / 2;  // (2^-24; the first and the last of the span stand for what is outside)
-  constexpr bool by_value = T == OSMOS_BF16;
   const uint32_t tid = threadIdx.x;
   const float none = -__builtin_inff();
   const bool warm = temperature > 0.0f, mass = !few(k);
@@ -364,28 +362,32 @@ __device__ inline void scan_slice(R& row, const Order<T>& order, float temperatu
   if (tid == 0) l.index = ~0u;
   float best = none;
   uint32_t outside = 0;  // whether some of bf16's are not among its values
-  if constexpr (by_value) {
+  if constexpr (VALUES) {
 #pragma unroll
     for (int i = 0; i < kValues; i += kSampleThreads) l.value[i + tid] = 0;
     __syncthreads();
     for (uint32_t round = row.begin;;) {
 #pragma unroll
-      for (uint32_t i = 0; i < sizeof(row.x) / 4; i++) {
-        typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
-        const uint32_t w = row.x[i / 4].w[i % 4], size = w & 0x7FFF7FFFu;
-        u16x2 v = __builtin_bit_cast(u16x2, size);
-        v = __builtin_elementwise_min(__builtin_elementwise_max(v, u16x2{kLeastBits, kLeastBits}), u16x2{kLeastBits + kSpan - 1, kLeastBits + kSpan - 1}) -
-            u16x2{kLeastBits, kLeastBits};
-        const uint32_t at = __builtin_bit_cast(uint32_t, v) << 2 | (w >> 1 & 0x40004000u);  // (4096 values of 4 bytes a sign)
-        atomicAdd((uint32_t*) ((uint8_t*) l.value + (at & 0xFFFF)), 1u);
-        atomicAdd((uint32_t*) ((uint8_t*) l.value + (at >> 16)), 1u);
+      for (uint32_t k = 0; k < sizeof(row.x) / sizeof(row.x[0]); k++) {
+        if (round + (k * kSampleThreads + tid) * kPer<T> >= row.end) break;
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+          typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
+          const uint32_t w = row.x[k].w[i], size = w & 0x7FFF7FFFu;
+          u16x2 v = __builtin_bit_cast(u16x2, size);
+          v = __builtin_elementwise_min(__builtin_elementwise_max(v, u16x2{kLeastBits, kLeastBits}), u16x2{kLeastBits + kSpan - 1, kLeastBits + kSpan - 1}) -
+              u16x2{kLeastBits, kLeastBits};
+          const uint32_t at = __builtin_bit_cast(uint32_t, v) << 2 | (w >> 1 & 0x40004000u);  // (4096 values of 4 bytes a sign)
+          atomicAdd((uint32_t*) ((uint8_t*) l.value + (at & 0xFFFF)), 1u);
+          atomicAdd((uint32_t*) ((uint8_t*) l.value + (at >> 16)), 1u);
+        }
       }
       if ((round += row.kRound) >= row.end) break;
       row.load(round);
     }
     __syncthreads();
-    // (what is past the end is in the last)
-    outside = l.value[0] | l.value[kSpan - 1] | l.value[kSpan] | (l.value[kValues - 1] - ((row.end - row.begin + row.kRound - 1) / row.kRound * row.kRound - (row.end - row.begin)));
+    // (what a last, partial piece has past the end is in the last)
+    outside = l.value[0] | l.value[kSpan - 1] | l.value[kSpan] | (l.value[kValues - 1] - (row.begin - row.end) % kPer<T>);
     if (outside) {
       row.again([&](float x, uint32_t) { best = fmaxf(best, x); });
     } else {
@@ -429,7 +431,7 @@ __device__ inline void scan_slice(R& row, const Order<T>& order, float temperatu
       valid += x > none ? n : 0;
     }
   };
-  if constexpr (by_value) {
+  if constexpr (VALUES) {
     if (outside)
       row.again([&](float x, uint32_t) {
         const uint32_t v = (__float_as_uint(x) >> 16 & 0x7FFF) - kLeastBits;
@@ -449,21 +451,21 @@ __device__ inline void scan_slice(R& row, const Order<T>& order, float temperatu
 }
 
 // 16 bytes of a slice a thread and round, and of a row that is one slice
-constexpr int kPieces = 4;
-template <uint32_t T> constexpr int kRowPieces = T == OSMOS_F32 ? 8 : 4;
-template <uint32_t T>
+template <uint32_t T, bool VALUES> constexpr int kPieces = VALUES ? 4 : 16 / kPer<T>;
+template <uint32_t T> constexpr int kRowPieces = 32 / kPer<T>;
+template <uint32_t T, bool VALUES>
 __global__ __launch_bounds__(kSampleThreads, 8) void scan_kernel(SampleArgs a) {
-  __shared__ ScanOf<T> l;
+  __shared__ ScanOf<VALUES> l;
   const uint32_t t = blockIdx.x / a.slices, s = blockIdx.x - t * a.slices, begin = s * a.slice, tid = threadIdx.x;
   const uint32_t end = begin + a.slice < a.vocab ? begin + a.slice : a.vocab;
-  Tokens<T, kPieces> row = {(const uint8_t*) a.logits + t * a.stride * kv::size_of(T), begin, end};
+  Tokens<T, kPieces<T, VALUES>> row = {(const uint8_t*) a.logits + t * a.stride * kv::size_of(T), begin, end};
   Part* part = (Part*) a.parts + blockIdx.x;
   const Order<T> order = {a.bits};
   const int32_t k = a.top_k ? a.top_k[t] : 0;
   uint64_t first;
   double top;
   uint32_t valid;
-  scan_slice<T>(row, order, a.temperature ? a.temperature[t] : 1.0f, k, l, first, top, valid);
+  scan_slice<T, VALUES>(row, order, a.temperature ? a.temperature[t] : 1.0f, k, l, first, top, valid);
   if (valid) {
     part->count[tid] = l.count[tid];
     if (!few(k)) part->mass[tid] = l.mass[tid];
@@ -582,7 +584,7 @@ __device__ inline void make_plan(const SampleArgs& a, uint32_t t, const Wish& wi
   __syncthreads();
 }
 
-constexpr uint32_t kMostSlices = OSMOS_SAMPLE_MAX_VOCAB / (kSampleThreads * 4 * kPieces);
+constexpr uint32_t kSlice = 16384, kValueSlice = 32768, kMostSlices = OSMOS_SAMPLE_MAX_VOCAB / kSlice;
 constexpr int kAtOnce = 8;  // slices whose bins are loaded together
 template <uint32_t T>
 __global__ __launch_bounds__(kSampleThreads) void plan_kernel(SampleArgs a) {
@@ -658,15 +660,15 @@ __device__ inline bool planned(const Plan& p, float x) {
   return slot_of(p, Scale{p.by, p.top}.bin_of(x)) >= 0;
 }
 
-constexpr int kListThreads = 256;
+constexpr int kListThreads = 256, kListPieces = 4;
 template <uint32_t T>
 __global__ __launch_bounds__(kListThreads) void list_kernel(SampleArgs a, uint32_t blocks) {
   __shared__ uint64_t list[kList];
   __shared__ uint32_t listed, start;
-  constexpr uint32_t each = kListThreads * kPer<T> * kPieces;
+  constexpr uint32_t each = kListThreads * kPer<T> * kListPieces;
   const uint32_t t = blockIdx.x / blocks, begin = (blockIdx.x - t * blocks) * each;
   RowPlan* row_plan = (RowPlan*) a.plans + t;
-  Tokens<T, kPieces, kListThreads> row = {(const uint8_t*) a.logits + t * a.stride * kv::size_of(T), begin,
+  Tokens<T, kListPieces, kListThreads> row = {(const uint8_t*) a.logits + t * a.stride * kv::size_of(T), begin,
                                           begin + each < a.vocab ? begin + each : a.vocab};
   row.load(begin);
   const Plan p = row_plan->plan;
@@ -947,7 +949,7 @@ __global__ __launch_bounds__(kSampleThreads) void draw_kernel(SampleArgs a) {
 // a row of one slice
 template <uint32_t T>
 __global__ __launch_bounds__(kSampleThreads) void sample_kernel(SampleArgs a) {
-  __shared__ WholeLds<T> l;
+  __shared__ WholeLds l;
   const uint32_t t = blockIdx.x;
   Tokens<T, kRowPieces<T>> row = {(const uint8_t*) a.logits + t * a.stride * kv::size_of(T), 0, a.vocab};
   const Order<T> order = {a.bits};
@@ -955,7 +957,7 @@ __global__ __launch_bounds__(kSampleThreads) void sample_kernel(SampleArgs a) {
   uint64_t first;
   double top;
   uint32_t valid;
-  scan_slice<T>(row, order, wish.temperature, wish.k, l.scan, first, top, valid);
+  scan_slice<T, false>(row, order, wish.temperature, wish.k, l.scan, first, top, valid);
   Sum bin = {0, 0};
   if (valid) bin = {l.scan.count[threadIdx.x], l.scan.mass[threadIdx.x]};
   make_plan<T>(a, t, wish, order, l, first, top, valid, bin);
@@ -1005,15 +1007,19 @@ __global__ __launch_bounds__(kSampleThreads) void probs_kernel(SampleArgs a, uin
 }
 
 inline int index_bits(uint32_t vocab) { return vocab > 1 ? 32 - __builtin_clz(vocab - 1) : 0; }
-// a row of up to 32768 tokens is one slice. bf16's slices cost the same whatever they hold (their values are put into bins at the
-// end): as long as there are 512 of them
+// a row of up to 32768 tokens is one slice. VALUES: bf16's tokens are counted by value, where there are many: a slice then costs the same
+// whatever it holds (its values are put into bins at the end), so it is as long as leaves 512 of them. 256 / 128 / 64 / 1 rows of
+// 129024: 62 / 49 / 38 / 40 us by values, 76 / 50 / 38 / 30 token by token
+constexpr uint32_t kRow = 32768;
+inline bool by_values(const OsmosSample* a) {
+  return a->type == OSMOS_BF16 && a->vocab > kRow && (uint64_t) a->n * ((a->vocab + kValueSlice - 1) / kValueSlice) >= 512;
+}
 inline uint32_t slice_of(const OsmosSample* a) {
-  constexpr uint32_t round = kSampleThreads * kPieces * 4, row = 32768;
-  if (a->vocab <= row) return row;
-  if (a->type == OSMOS_F32) return round;
-  const uint32_t rounds = (a->vocab + row - 1) / row;
-  const uint64_t each = a->type == OSMOS_BF16 ? (uint64_t) a->n * rounds / 512 : 1;
-  return row * (uint32_t) (each < 1 ? 1 : each < rounds ? each : rounds);
+  if (a->vocab <= kRow) return kRow;
+  if (!by_values(a)) return kSlice;
+  const uint32_t rounds = (a->vocab + kValueSlice - 1) / kValueSlice;
+  const uint64_t each = (uint64_t) a->n * rounds / 512;
+  return kValueSlice * (uint32_t) (each < 1 ? 1 : each < rounds ? each : rounds);
 }
 inline uint32_t slices_of(const OsmosSample* a) { return (a->vocab + slice_of(a) - 1) / slice_of(a); }
 inline uint64_t round256(uint64_t n) { return (n + 255) / 256 * 256; }
@@ -1022,16 +1028,16 @@ struct SampleRoom {
 };
 inline SampleRoom room_of(const OsmosSample* a) {
   const uint64_t rows = a->n, slices = slices_of(a);
-  return {slices > 1 ? round256(rows * slices * sizeof(Part)) : 0, slices > 1 ? round256(rows * sizeof(RowPlan)) : 0,
+  return {a->vocab > kRow ? round256(rows * slices * sizeof(Part)) : 0, a->vocab > kRow ? round256(rows * sizeof(RowPlan)) : 0,
           a->probs ? round256(rows * sizeof(Drawn)) : 0};
 }
 
-template <uint32_t T>
+template <uint32_t T, bool VALUES>
 bool sample_launch(const SampleArgs& a, hipStream_t s) {
-  if (a.slices > 1) {
-    scan_kernel<T><<<a.n * a.slices, kSampleThreads, 0, s>>>(a);
+  if (a.vocab > kRow) {
+    scan_kernel<T, VALUES><<<a.n * a.slices, kSampleThreads, 0, s>>>(a);
     plan_kernel<T><<<a.n, kSampleThreads, 0, s>>>(a);
-    const uint32_t list_each = kListThreads * kPer<T> * kPieces, blocks = (a.vocab + list_each - 1) / list_each;
+    const uint32_t list_each = kListThreads * kPer<T> * kListPieces, blocks = (a.vocab + list_each - 1) / list_each;
     list_kernel<T><<<a.n * blocks, kListThreads, 0, s>>>(a, blocks);
     draw_kernel<T><<<a.n, kSampleThreads, 0, s>>>(a);
   } else {
@@ -1064,6 +1070,8 @@ extern "C" OSM_API bool osmos_sample(const OsmosSample* a, void* workspace, uint
   const rows::SampleArgs b = {a->logits, a->u, a->temperature, a->top_p, a->min_p, a->top_k, a->token, a->kept, a->prob, a->probs, a->stride,
                               a->n, a->vocab, rows::slices_of(a), rows::slice_of(a), rows::index_bits(a->vocab), w, w + r.parts,
                               w + r.parts + r.plans};
-  return a->type == OSMOS_F32 ? rows::sample_launch<OSMOS_F32>(b, (hipStream_t) stream)
-         : a->type == OSMOS_F16 ? rows::sample_launch<OSMOS_F16>(b, (hipStream_t) stream) : rows::sample_launch<OSMOS_BF16>(b, (hipStream_t) stream);
+  const hipStream_t on = (hipStream_t) stream;
+  return a->type == OSMOS_F32 ? rows::sample_launch<OSMOS_F32, false>(b, on)
+         : a->type == OSMOS_F16 ? rows::sample_launch<OSMOS_F16, false>(b, on)
+         : rows::by_values(a) ? rows::sample_launch<OSMOS_BF16, true>(b, on) : rows::sample_launch<OSMOS_BF16, false>(b, on);
 }

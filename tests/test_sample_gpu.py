@@ -48,7 +48,7 @@ def _one(l, t, k, p, m, u):
     return int(order[at]), w[at] / c[-1], n, probs, margin
 
 
-def _check(logits, u, temperature=None, top_k=None, top_p=None, min_p=None, what="", vocab=None, exact=False):
+def _check(logits, u, temperature=None, top_k=None, top_p=None, min_p=None, what="", only=None, exact=False):
     n, dev = logits.shape[0], "cuda"
     f = lambda v, t: None if v is None else torch.tensor(v, dtype=t, device=dev) if isinstance(v, list) else v  # noqa: E731
     u, temperature, top_p, min_p, top_k = f(u, F32), f(temperature, F32), f(top_p, F32), f(min_p, F32), f(top_k, torch.int32)
@@ -62,8 +62,11 @@ def _check(logits, u, temperature=None, top_k=None, top_p=None, min_p=None, what
     assert torch.equal(token, again), what
     host = lambda x, d: np.full(n, d) if x is None else x.double().cpu().numpy()  # noqa: E731
     par = zip(host(temperature, 1.0), host(top_k, 0), host(top_p, 1.0), host(min_p, 0.0), host(u, 0.0))
-    l = logits.float().cpu().numpy()
+    at = range(n) if only is None else only
+    l = dict(zip(at, logits[torch.tensor(list(at), device=dev)].float().cpu().numpy()))
     for i, (t, k, p, m, v) in enumerate(par):
+        if i not in l:
+            continue
         tok, pr, ke, want, margin = _one(l[i], t, int(k), p, m, v)
         note = "%s row %d: T %g k %d p %g min %g u %g" % (what, i, t, k, p, m, v)
         assert exact or margin > 1e-9, note
@@ -99,6 +102,34 @@ def test_mixed(n, vocab, kind):
     print(n, vocab, kind, flush=True)
     x, u = _logits(n, vocab, kind, vocab + n)
     _check(x, u, what="mixed", **_params(n, vocab, vocab))
+
+
+@pytest.mark.parametrize("n,vocab", [(270, 40009), (600, 65544), (180, 98311)])
+def test_many_rows_by_value(n, vocab):
+    """bf16 rows in such numbers that their tokens are counted by value, in slices of one round and of more; values outside the
+    counted range (256 and more, under 2^-24, zeros, infinities, NaN) among them, and rows of nothing else"""
+    print(n, vocab, flush=True)
+    x, u = _logits(n, vocab, BF16, n)
+    p = _params(n, vocab, n)
+    only = [0, 1, 2, 3, 4, 5, 6, 7, 8, 9, n // 2, n - 1]
+    for i in (1, n - 1):
+        x[i, ::3] = -math.inf
+    x[2, 5::7] = 1e-9
+    x[2, 6::7] = 0.0
+    x[3, 1000], x[3, vocab - 1], x[3, 2000:2100] = 300.0, 300.0, 299.0
+    x[4] = -500.0
+    x[4, 777::5] = -499.0
+    x[5] = -0.0
+    x[6] = math.nan
+    x[6, vocab - 3] = 3.0
+    x[7] = -math.inf
+    x[8, 11], x[8, 12] = math.inf, math.nan
+    x[9, 40::2] = torch.finfo(BF16).min
+    for i in (2, 3, 4, 5):
+        p["temperature"][i] = 1.0
+    p["temperature"][n // 2] = 0.0
+    _check(x, u, what="by value", only=only, exact=True, **p)
+    _check(x, u, what="by value, no limits", only=only, exact=True)
 
 
 def test_largest_vocab():
