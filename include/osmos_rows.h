@@ -3,7 +3,8 @@
    (osmos_attn.h); and the choice of the next token from a row of logits. no counterpart in the reference's kernel ABI.
 
    types are osmos_attn.h's (OSMOS_F32, _F16, _BF16). every call is queued on `stream` (a hipStream_t) and never waited
-   for, allocates nothing and may be captured into a graph; false = refused, nothing queued. */
+   for, allocates nothing and may be captured into a graph; false = refused, nothing queued (among what is: more rows than a
+   launch of fewer than 2^32 threads holds, at 64 a row or more, 1024 for osmos_sample). */
 #ifndef OSMOS_ROWS_H
 #define OSMOS_ROWS_H
 
@@ -103,8 +104,8 @@ bool osmos_rope_append(const OsmosRope *a, const OsmosKv *kv, uint32_t layer, co
      of those the first whose weights sum up to top_p of theirs (1 or more: all; at least one token), and
      those of at least min_p times the greatest weight (0 or less: all);
    drawn is the first kept token whose running sum of weights passes u (0 <= u < 1) times the kept ones' sum. temperature 0,
-   less or NaN: the first token. a logit of -infinity or NaN is never chosen nor kept, +infinity counts as the greatest float; a
-   row of nothing else gives token -1, prob 0, kept 0. weights under 2^-44 of the greatest count as zero in the sums. NaN
+   less or NaN: the first token. a logit of -infinity or NaN is never chosen nor kept, +infinity counts as its type's
+   greatest value; a row of nothing else gives token -1, prob 0, kept 0. weights under 2^-44 of the greatest count as zero in the sums. NaN
    in top_p or min_p: that limit does not hold; u is clamped into its range, NaN counts as 0.
    the same call gives the same answer, and a row's answer does not depend on the other rows. */
 #define OSMOS_SAMPLE_MAX_VOCAB (1u << 20)

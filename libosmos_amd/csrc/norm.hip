@@ -231,6 +231,7 @@ bool norm_launch(const OsmosNorm* a, hipStream_t s) {
   const uint32_t each = all < 1 ? 1 : all < 4 ? (uint32_t) all : 4, waves = (pieces + 64 * each - 1) / (64 * each);
   b.waves = waves > 16 ? 16 : waves;
   const uint32_t k = (pieces + b.waves * 64 - 1) / (b.waves * 64);
+  if (!launches(b.waves > 1 ? rows : (rows + 3) / 4, b.waves > 1 ? b.waves * 64 : 256)) return false;
   auto* kernel = a->dim % per<T>() ? norm_of<T, true>(k) : norm_of<T, false>(k);
   if (b.waves > 1) kernel<<<rows, b.waves * 64, 0, s>>>(b);
   else kernel<<<(rows + 3) / 4, 256, 0, s>>>(b);

@@ -212,6 +212,7 @@ bool rope_launch(const OsmosRope* o, const int32_t* pos, const kv::Step& st, con
   const uint32_t all = a.heads + a.kv_heads * (dst ? 2 : 1), rounds = (all * a.group + 63) / 64;
   a.parts = 4096 / a.n < 1 ? 1 : 4096 / a.n < rounds ? 4096 / a.n : rounds;
   const uint64_t waves = (uint64_t) a.n * a.parts;
+  if (!launches((waves + kRopeWaves - 1) / kRopeWaves, 64 * kRopeWaves)) return false;
   const uint32_t grid = (uint32_t) ((waves + kRopeWaves - 1) / kRopeWaves);
   const bool one = a.parts == rounds;
   auto* kernel = o->type == OSMOS_F32 ? one ? rope_of<OSMOS_F32, 1>(dst) : rope_of<OSMOS_F32, 4>(dst)

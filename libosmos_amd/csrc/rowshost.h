@@ -16,6 +16,9 @@ inline bool rows_ok(const void* p, uint32_t type, uint64_t stride, uint32_t n, u
   return p && aligned(p, kv::size_of(type)) && stride <= (1ull << 40) && (n == 1 || stride >= row);
 }
 
+// a launch has fewer than 2^32 threads
+inline bool launches(uint64_t blocks, uint32_t threads) { return blocks && blocks * threads <= 0xFFFFFFFFull; }
+
 inline bool norm_ok(const OsmosNorm* a) {
   if (!a || !a->n || a->n > 0x7FFFFFF0u || !a->dim || a->dim > OSMOS_NORM_MAX_DIM || !kv::row_type(a->type)) return false;
   if (!rows_ok(a->x, a->type, a->x_stride, a->n, a->dim)) return false;

@@ -535,7 +535,8 @@ __device__ inline void make_plan(const SampleArgs& a, uint32_t t, const Wish& wi
     int f[4] = {0, kBins, kBins, kBins}, g[4] = {by_k ? k_bin : kBins - 1, -1, -1, -1};
     if (!small) {
       uint64_t least_m = all, most_m = all;
-      if (by_k) f[2] = g[2] = k_bin, least_m = before[k_bin] + 1, most_m = before[k_bin + 1];
+      // (tokens of less than 2^-43 of the greatest's weight add nothing to a sum: a bin's tokens may end where they begin)
+      if (by_k) f[2] = g[2] = k_bin, least_m = before[k_bin] > 1 ? before[k_bin] : 1, most_m = before[k_bin + 1];
       if (by_p) {
         f[1] = reaches(before, p_goal(part, least_m));
         g[1] = least_m == most_m ? f[1] : reaches(before, p_goal(part, most_m));
@@ -1034,20 +1035,20 @@ inline SampleRoom room_of(const OsmosSample* a) {
 
 template <uint32_t T, bool VALUES>
 bool sample_launch(const SampleArgs& a, hipStream_t s) {
+  constexpr uint32_t list_each = kListThreads * kPer<T> * kListPieces, probs_each = kSampleThreads * kPer<T>;
+  const uint64_t blocks = (a.vocab + list_each - 1) / list_each, chunks = (a.vocab + probs_each - 1) / probs_each;
+  if (!launches((uint64_t) a.n * a.slices, kSampleThreads) || !launches(a.n * blocks, kListThreads) ||
+      (a.probs && !launches(a.n * chunks, kSampleThreads)))
+    return false;
   if (a.vocab > kRow) {
     scan_kernel<T, VALUES><<<a.n * a.slices, kSampleThreads, 0, s>>>(a);
     plan_kernel<T><<<a.n, kSampleThreads, 0, s>>>(a);
-    const uint32_t list_each = kListThreads * kPer<T> * kListPieces, blocks = (a.vocab + list_each - 1) / list_each;
-    list_kernel<T><<<a.n * blocks, kListThreads, 0, s>>>(a, blocks);
+    list_kernel<T><<<(uint32_t) (a.n * blocks), kListThreads, 0, s>>>(a, (uint32_t) blocks);
     draw_kernel<T><<<a.n, kSampleThreads, 0, s>>>(a);
   } else {
     sample_kernel<T><<<a.n, kSampleThreads, 0, s>>>(a);
   }
-  if (a.probs) {
-    const uint32_t each = kSampleThreads * kPer<T>;
-    const uint32_t chunks = (a.vocab + each - 1) / each;
-    probs_kernel<T><<<a.n * chunks, kSampleThreads, 0, s>>>(a, chunks);
-  }
+  if (a.probs) probs_kernel<T><<<(uint32_t) (a.n * chunks), kSampleThreads, 0, s>>>(a, (uint32_t) chunks);
   return hipGetLastError() == hipSuccess;
 }
 

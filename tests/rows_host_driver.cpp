@@ -11,4 +11,5 @@ bool host_rope_append(const OsmosRope* a, const OsmosKv* kv, uint32_t layer, con
 }
 bool host_turns(const OsmosRopeScaling* s, uint32_t rot, double* turns, float* scale) { return rows::turns_of(s, rot, turns, scale); }
 bool host_sample(const OsmosSample* a) { return rows::sample_ok(a); }
+bool host_launches(uint64_t blocks, uint32_t threads) { return rows::launches(blocks, threads); }
 }

@@ -22,7 +22,7 @@ def H(tmp_path_factory):
     subprocess.run(["g++", "-O2", "-std=c++17", "-Wall", "-Werror", "-shared", "-fPIC", os.path.join(HERE, "rows_host_driver.cpp"),
                     "-o", lib], check=True)
     h = ctypes.CDLL(lib)
-    for f in ("host_norm", "host_rope", "host_rope_append", "host_turns", "host_sample"):
+    for f in ("host_norm", "host_rope", "host_rope_append", "host_turns", "host_sample", "host_launches"):
         getattr(h, f).restype = ctypes.c_bool
     h.host_rope_append.argtypes = [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_uint32, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_uint64,
                                    ctypes.c_uint64]
@@ -149,6 +149,16 @@ def test_sample_good(H, o):
 def test_sample_bad(H, o):
     assert not H.host_sample(R(_sample(**o)))
     assert not capi.lib().osmos_sample(R(_sample(**o)), None, 0, None)
+
+
+def test_more_rows_than_a_launch_holds():
+    """refused before anything is queued (2^32 threads and more)"""
+    fits = lambda blocks, threads: H.host_launches(ctypes.c_uint64(blocks), ctypes.c_uint32(threads))  # noqa: E731
+    assert fits(1, 1024) and fits(4194303, 1024) and not fits(4194304, 1024) and not fits(0, 64) and not fits(1 << 40, 64)
+    n = 0x3FFFFFF
+    assert not capi.lib().osmos_norm(R(_norm(n=1 << 30, dim=32, x_stride=32, add_stride=32, sum_stride=32, out_stride=32)), None)
+    assert not capi.lib().osmos_rope(R(_rope(n=1 << 27, kv_heads=0)), ctypes.c_void_p(A), None)
+    assert not capi.lib().osmos_sample(R(_sample(n=n >> 3, vocab=8, stride=8)), ctypes.c_void_p(A), 1 << 40, None)
 
 
 def test_no_workspace(H):

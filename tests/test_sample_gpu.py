@@ -213,6 +213,20 @@ def test_magnitudes(scale):
     _check(x - 1000.0 * min(scale, 1e6), u, temperature=[scale] * 6, top_k=[77] * 6, what="size %g, far from zero" % scale, exact=True)
 
 
+@pytest.mark.parametrize("vocab", [4000, 40000])
+def test_weights_of_almost_nothing(vocab):
+    """limits that end among tokens of 2^-43 of the greatest weight and less, which add little or nothing to the sums"""
+    x = torch.full((6, vocab), -60.0, device="cuda")
+    x[:, 7] = 0.0
+    x[:, 100:3100] = -29.4 - 1.1e-3 * torch.arange(3000, device="cuda")
+    u = [0.3, 0.9, 0.99999, 0.5, 0.99999994, 0.0]
+    got = _check(x, u, top_k=[1500, 2900, 3001, 1025, 40, vocab - 1], what="k", exact=True)
+    assert got.tolist() == [7] * 6
+    x[3:, 8] = -0.5
+    _check(x, u, top_k=[1500, 2900, 3001, 1025, 2000, 2500], top_p=[0.5, 0.99, 0.999999, 0.9, 0.7, 0.3], what="k, p", exact=True)
+    _check(x, u, top_k=[1500, 0, 3001, 1025, 2000, 2500], min_p=[1e-13, 2e-13, 5e-14, 1e-13, 1.0, 0.6], what="k, min-p", exact=True)
+
+
 def test_a_row_alone():
     x, u = _logits(64, 70001, F32, 19)
     p = _params(64, 70001, 23)
