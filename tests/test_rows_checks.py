@@ -151,7 +151,7 @@ def test_sample_bad(H, o):
     assert not capi.lib().osmos_sample(R(_sample(**o)), None, 0, None)
 
 
-def test_more_rows_than_a_launch_holds():
+def test_more_rows_than_a_launch_holds(H):
     """refused before anything is queued (2^32 threads and more)"""
     fits = lambda blocks, threads: H.host_launches(ctypes.c_uint64(blocks), ctypes.c_uint32(threads))  # noqa: E731
     assert fits(1, 1024) and fits(4194303, 1024) and not fits(4194304, 1024) and not fits(0, 64) and not fits(1 << 40, 64)
