@@ -302,7 +302,7 @@ struct Tokens {
         for (uint32_t j = 0; j < kPer<T>; j++) hits = hits + hits + in(x[k].at(j));  // (the first one's bit the highest)
     };
     static_assert(P * kPer<T> <= 32);
-    // (& and |: as && and || each comparison is a branch, and 33 million 16-bit logits take 16.4 us, so 11)
+    // (& and |: as && and || each comparison is a branch, and 33 million 16-bit logits take 16.4 us, so 15.8; 13 instructions a token, so 7)
     if (spans == 1) test([&](float v) { return (v >= l0) & (v <= h0); });
     else if (spans == 2) test([&](float v) { return ((v >= l0) & (v <= h0)) | ((v >= l1) & (v <= h1)); });
     else test([&](float v) { return ((v >= l0) & (v <= h0)) | ((v >= l1) & (v <= h1)) | ((v >= l2) & (v <= h2)) | ((v >= l3) & (v <= h3)); });
@@ -573,7 +573,7 @@ __device__ inline void make_plan(const SampleArgs& a, uint32_t t, const Wish& wi
     if (tid < 4) {
       const int a0 = tid == 0 ? from[0] : tid == 1 ? from[1] : tid == 2 ? from[2] : from[3], a1 = tid == 0 ? to[0] : tid == 1 ? to[1] : tid == 2 ? to[2] : to[3];
       const double lo = (top - a1 - 0.5) / sc.by, hi = (top - a0 + 0.5) / sc.by;
-      const float fl = (float) (lo - 1e-6 * fabs(lo)), fh = (float) (hi + 1e-6 * fabs(hi));
+      const float fl = (float) (lo - 1e-6 * fabs(lo) - 3e-45), fh = (float) (hi + 1e-6 * fabs(hi) + 3e-45);  // (two of float's least steps)
       p.from[tid] = a0, p.to[tid] = a1, p.slot[tid] = tid == 0 ? slot[0] : tid == 1 ? slot[1] : tid == 2 ? slot[2] : slot[3];
       p.low[tid] = a0 >= kBins ? __builtin_inff() : fl == fl ? fl : -__builtin_inff();
       p.high[tid] = a0 >= kBins ? -__builtin_inff() : fh < kGreatest<T> ? fh : __builtin_inff();

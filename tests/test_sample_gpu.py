@@ -227,6 +227,18 @@ def test_weights_of_almost_nothing(vocab):
     _check(x, u, top_k=[1500, 0, 3001, 1025, 2000, 2500], min_p=[1e-13, 2e-13, 5e-14, 1e-13, 1.0, 0.6], what="k, min-p", exact=True)
 
 
+def test_denormal_logits():
+    """logits and temperatures among float's least values"""
+    for scale in (1e-38, 1e-41, 1e-43):
+        for vocab in (3000, 50001):
+            x, u = _logits(4, vocab, F32, 37)
+            x = (x.double() * scale).float()
+            t = [float(np.float32(scale))] * 4
+            _check(x, u, temperature=t, what="size %g" % scale, exact=True)
+            _check(x, u, temperature=t, top_p=[0.9] * 4, min_p=[0.0, 0.01, 0.1, 0.5], what="size %g" % scale, exact=True)
+            _check(x, u, temperature=t, top_k=[40, 2000, 5, 1], what="size %g" % scale, exact=True)
+
+
 def test_a_row_alone():
     x, u = _logits(64, 70001, F32, 19)
     p = _params(64, 70001, 23)
