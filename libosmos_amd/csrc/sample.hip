@@ -553,26 +553,30 @@ __device__ inline void make_plan(const SampleArgs& a, uint32_t t, const Wish& wi
       f[0] = reaches(before, u_goal(drawn, least_m));
       g[0] = least_m == most_m ? f[0] : reaches(before, u_goal(drawn, most_m));
     }
-    // (spans that touch are one; in ascending order, those that are left first)
-    int from[4], to[4], slots = 0, slot[4];
-    uint32_t taken = 0;
+    // in ascending order, spans that touch as one
+    auto sort = [&](int i, int j) {
+      const bool swap = f[j] < f[i];
+      const int a0 = swap ? f[j] : f[i], a1 = swap ? g[j] : g[i], b0 = swap ? f[i] : f[j], b1 = swap ? g[i] : g[j];
+      f[i] = a0, g[i] = a1, f[j] = b0, g[j] = b1;
+    };
+    if (!small) sort(0, 1), sort(2, 3), sort(0, 2), sort(1, 3), sort(1, 2);
+    int from[4] = {f[0], kBins, kBins, kBins}, to[4] = {g[0], kBins, kBins, kBins}, last = 0;
 #pragma unroll
-    for (int n = 0; n < 4; n++) {
-      int a0 = kBins, a1 = -1;
+    for (int i = 1; i < 4; i++) {
+      if (f[i] >= kBins) continue;
 #pragma unroll
-      for (int i = 0; i < 4; i++)
-        if (!(taken >> i & 1) && f[i] < a0) a0 = f[i], a1 = g[i];
-#pragma unroll
-      for (int twice = 0; twice < 3; twice++)
-#pragma unroll
-        for (int i = 0; i < 4; i++)
-          if (f[i] <= a1 + 1 && f[i] >= a0 && !(taken >> i & 1)) taken |= 1u << i, a1 = g[i] > a1 ? g[i] : a1;
-      from[n] = a0, to[n] = a0 < kBins ? a1 : kBins, slot[n] = slots;
-      slots += a0 < kBins ? a1 - a0 + 1 : 0;
+      for (int n = 3; n >= 0; n--) {
+        if (n != last) continue;
+        if (f[i] <= to[n] + 1) to[n] = g[i] > to[n] ? g[i] : to[n];
+        else if (n < 3) from[n + 1 < 4 ? n + 1 : 3] = f[i], to[n + 1 < 4 ? n + 1 : 3] = g[i], last = n + 1;
+      }
     }
+    int slots = 0, slot[4];
+#pragma unroll
+    for (int n = 0; n < 4; n++) slot[n] = slots, slots += from[n] < kBins ? to[n] - from[n] + 1 : 0;
     if (tid < 4) {
       const int a0 = tid == 0 ? from[0] : tid == 1 ? from[1] : tid == 2 ? from[2] : from[3], a1 = tid == 0 ? to[0] : tid == 1 ? to[1] : tid == 2 ? to[2] : to[3];
-      const double lo = (top - a1 - 0.5) / sc.by, hi = (top - a0 + 0.5) / sc.by;
+      const double unit = 1.0 / sc.by, lo = (top - a1 - 0.5) * unit, hi = (top - a0 + 0.5) * unit;
       const float fl = (float) (lo - 1e-6 * fabs(lo) - 3e-45), fh = (float) (hi + 1e-6 * fabs(hi) + 3e-45);  // (two of float's least steps)
       p.from[tid] = a0, p.to[tid] = a1, p.slot[tid] = tid == 0 ? slot[0] : tid == 1 ? slot[1] : tid == 2 ? slot[2] : slot[3];
       p.low[tid] = a0 >= kBins ? __builtin_inff() : fl == fl ? fl : -__builtin_inff();
