@@ -302,7 +302,7 @@ struct Tokens {
         for (uint32_t j = 0; j < kPer<T>; j++) hits = hits + hits + in(x[k].at(j));  // (the first one's bit the highest)
     };
     static_assert(P * kPer<T> <= 32);
-    // (& and |: as && and || each comparison is a branch, and 33 million 16-bit logits take 16.4 us, so 15.8; 13 instructions a token, so 7)
+    // (& and |: as && and || each comparison is a branch, 13 instructions a token in all, and 33 million bf16 logits take 16.4 us, so 15.8)
     if (spans == 1) test([&](float v) { return (v >= l0) & (v <= h0); });
     else if (spans == 2) test([&](float v) { return ((v >= l0) & (v <= h0)) | ((v >= l1) & (v <= h1)); });
     else test([&](float v) { return ((v >= l0) & (v <= h0)) | ((v >= l1) & (v <= h1)) | ((v >= l2) & (v <= h2)) | ((v >= l3) & (v <= h3)); });
