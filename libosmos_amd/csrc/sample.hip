@@ -126,7 +126,7 @@ struct Plan {
   int done, small, by_p;    // done: the row's token is given already; small: all bins up to to[0] are listed, whatever their weights
   int split;                // a listed bin's parts, as a power of two
   int from[4], to[4], slot[4];  // the listed bins, apart from one another (kBins: none); how many are listed before a span's
-  float low[4], high[4];    // these spans' logits, a little wide
+  float low[4], high[4];    // these spans' logits, a little wide; low is finite: -infinity is no token, and stands past a row's end
 };
 // a row's bins' prefix sums: weights (of kOne the first bin's middle) and tokens
 struct Prefix {
@@ -289,7 +289,8 @@ struct Tokens {
 #pragma unroll
       for (uint32_t j = 0; j < kPer<T>; j++) f(x[k].at(j), at + (k * N + threadIdx.x) * kPer<T> + j);
   }
-  // those of a plan's spans' logits: most threads have none, so they are read again
+  // those of a plan's spans' logits: most threads have none, so they are read again (what a piece has past the end is -infinity, less
+  // than any low)
   template <typename F>
   __device__ inline void loaded_between(uint32_t at, const Plan& p, F f) const {
     const float l0 = p.low[0], h0 = p.high[0], l1 = p.low[1], h1 = p.high[1], l2 = p.low[2], h2 = p.high[2], l3 = p.low[3], h3 = p.high[3];
@@ -579,7 +580,7 @@ __device__ inline void make_plan(const SampleArgs& a, uint32_t t, const Wish& wi
       const double unit = 1.0 / sc.by, lo = (top - a1 - 0.5) * unit, hi = (top - a0 + 0.5) * unit;
       const float fl = (float) (lo - 1e-6 * fabs(lo) - 3e-45), fh = (float) (hi + 1e-6 * fabs(hi) + 3e-45);  // (two of float's least steps)
       p.from[tid] = a0, p.to[tid] = a1, p.slot[tid] = tid == 0 ? slot[0] : tid == 1 ? slot[1] : tid == 2 ? slot[2] : slot[3];
-      p.low[tid] = a0 >= kBins ? __builtin_inff() : fl == fl ? fl : -__builtin_inff();
+      p.low[tid] = a0 >= kBins ? __builtin_inff() : fl > -kGreatest<T> ? fl : -kGreatest<T>;
       p.high[tid] = a0 >= kBins ? -__builtin_inff() : fh < kGreatest<T> ? fh : __builtin_inff();
     }
     if (tid == 0) {
