@@ -124,6 +124,8 @@ struct Plan {
   uint32_t k;               // top_k where it limits, or 0; k_bin kBins: among tokens of no weight
   int k_bin, m_bin;         // kBins: none
   int done, small, by_p;    // done: the row's token is given already; small: all bins up to to[0] are listed, whatever their weights
+  int far;                  // min_p alone ends the kept tokens, and past the bins: those from there on are counted, into `past`
+  uint32_t past;
   int split;                // a listed bin's parts, as a power of two
   int from[4], to[4], slot[4];  // the listed bins, apart from one another (kBins: none); how many are listed before a span's
   float low[4], high[4];    // these spans' logits, a little wide; low is finite: -infinity is no token, and stands past a row's end
@@ -575,18 +577,22 @@ __device__ inline void make_plan(const SampleArgs& a, uint32_t t, const Wish& wi
     int slots = 0, slot[4];
 #pragma unroll
     for (int n = 0; n < 4; n++) slot[n] = slots, slots += from[n] < kBins ? to[n] - from[n] + 1 : 0;
+    // (tokens past the bins add nothing to a sum: a min_p there says only how many of them are kept, which top_p or a top_k in the bins
+    // settles by itself. such a plan's one span is the token's, and the fourth has the logits between the bins and the edge)
+    const bool far = a.kept && min_p > 0.0f && m_bin == kBins && !by_p && k_bin == kBins;
     if (tid < 4) {
       const int a0 = tid == 0 ? from[0] : tid == 1 ? from[1] : tid == 2 ? from[2] : from[3], a1 = tid == 0 ? to[0] : tid == 1 ? to[1] : tid == 2 ? to[2] : to[3];
-      const double unit = 1.0 / sc.by, lo = (top - a1 - 0.5) * unit, hi = (top - a0 + 0.5) * unit;
+      const bool beyond = far && tid == 3, none = a0 >= kBins && !beyond;
+      const double unit = 1.0 / sc.by, lo = (beyond ? edge : top - a1 - 0.5) * unit, hi = (top - a0 + 0.5) * unit;
       const float fl = (float) (lo - 1e-6 * fabs(lo) - 3e-45), fh = (float) (hi + 1e-6 * fabs(hi) + 3e-45);  // (two of float's least steps)
       p.from[tid] = a0, p.to[tid] = a1, p.slot[tid] = tid == 0 ? slot[0] : tid == 1 ? slot[1] : tid == 2 ? slot[2] : slot[3];
-      p.low[tid] = a0 >= kBins ? __builtin_inff() : fl > -kGreatest<T> ? fl : -kGreatest<T>;
-      p.high[tid] = a0 >= kBins ? -__builtin_inff() : fh < kGreatest<T> ? fh : __builtin_inff();
+      p.low[tid] = none ? __builtin_inff() : fl > -kGreatest<T> ? fl : -kGreatest<T>;
+      p.high[tid] = none ? -__builtin_inff() : fh < kGreatest<T> ? fh : __builtin_inff();
     }
     if (tid == 0) {
       p.by = sc.by, p.top = top, p.part = part, p.draw = drawn, p.edge = edge;
       p.all = all, p.valid = valid, p.listed = 0, p.k = limit, p.k_bin = k_bin, p.m_bin = m_bin;
-      p.done = 0, p.small = small, p.by_p = by_p;
+      p.done = 0, p.small = small, p.by_p = by_p, p.far = far, p.past = 0;
       p.split = small ? 0 : 10 - (slots > 1 ? 32 - __builtin_clz(slots - 1) : 0);
     }
   }
@@ -664,9 +670,12 @@ __device__ inline int slot_of(const Plan& p, int b) {
   for (int i = 0; i < 4; i++) slot = b >= p.from[i] && b <= p.to[i] ? p.slot[i] + b - p.from[i] : slot;
   return b < kBins ? slot : -1;
 }
-template <uint32_t T>
-__device__ inline bool planned(const Plan& p, float x) {
-  return slot_of(p, Scale{p.by, p.top}.bin_of(x)) >= 0;
+// whether a token is of the plan's bins; one past all bins that min_p keeps is counted
+__device__ inline bool planned(const Plan& p, float x, uint32_t& past) {
+  const Scale sc = {p.by, p.top};
+  const int b = sc.bin_of(x);
+  if (p.far && b == kBins && sc.y(x) >= p.edge) past++;
+  return slot_of(p, b) >= 0;
 }
 
 // the planned bins' tokens of a row, in any order: 48 rows of 151001 floats 8 us, 256 of 129024 bf16 15.5 (4.3 TB/s)
@@ -674,7 +683,7 @@ constexpr int kListThreads = 256, kListPieces = 4;
 template <uint32_t T>
 __global__ __launch_bounds__(kListThreads) void list_kernel(SampleArgs a, uint32_t blocks) {
   __shared__ uint64_t list[kList];
-  __shared__ uint32_t listed, start;
+  __shared__ uint32_t listed, start, past;
   constexpr uint32_t each = kListThreads * kPer<T> * kListPieces;
   const uint32_t t = blockIdx.x / blocks, begin = (blockIdx.x - t * blocks) * each;
   RowPlan* row_plan = (RowPlan*) a.plans + t;
@@ -684,14 +693,17 @@ __global__ __launch_bounds__(kListThreads) void list_kernel(SampleArgs a, uint32
   const Plan p = row_plan->plan;
   if (p.done) return;
   const Order<T> order = {a.bits};
-  if (threadIdx.x == 0) listed = 0;
+  if (threadIdx.x == 0) listed = 0, past = 0;
   __syncthreads();
+  uint32_t own_past = 0;
   row.loaded_between(begin, p, [&](float x, uint32_t i) {
-    if (!planned<T>(p, x)) return;
+    if (!planned(p, x, own_past)) return;
     const uint32_t at = atomicAdd(&listed, 1u);
     if (at < kList) list[at] = order.place(x, i);
   });
+  if (own_past) atomicAdd(&past, own_past);
   __syncthreads();
+  if (threadIdx.x == 0 && past) atomicAdd(&row_plan->plan.past, past);
   if (!listed) return;
   if (threadIdx.x == 0) start = atomicAdd(&row_plan->plan.listed, listed);
   __syncthreads();
@@ -929,6 +941,7 @@ __device__ inline void draw(const SampleArgs& a, uint32_t t, const Order<T>& ord
     const uint64_t goal = u_goal(p.draw, cut.m);
     d = cut_at(first_of([&](uint32_t i) { return l.weight[i] >= goal; }));
   }
+  if (p.far && prefix.ahead[kBins] + p.past < cut.n) cut.n = prefix.ahead[kBins] + p.past;
   const double share = kOne / (double) cut.m;
   if (tid == 0) {
     const double z = sc.y(order.logit(d.place)), middle = __builtin_rint(z);
@@ -972,11 +985,13 @@ __global__ __launch_bounds__(kSampleThreads) void sample_kernel(SampleArgs a) {
   if (valid) bin = {l.scan.count[threadIdx.x], l.scan.mass[threadIdx.x]};
   make_plan<T>(a, t, wish, order, l, first, top, valid, bin);
   if (l.plan.done) return;
+  uint32_t past = 0;
   row.loaded_between(0, l.plan, [&](float x, uint32_t i) {
-    if (!planned<T>(l.plan, x)) return;
+    if (!planned(l.plan, x, past)) return;
     const uint32_t at = atomicAdd(&l.plan.listed, 1u);
     if (at < kList) l.list[at] = order.place(x, i);
   });
+  if (past) atomicAdd(&l.plan.past, past);
   __syncthreads();
   uint64_t at[2] = {l.list[threadIdx.x], l.list[threadIdx.x + kSampleThreads]};
   draw<T>(a, t, order, l.plan, l.prefix, l.list, at, l.draw);
