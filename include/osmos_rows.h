@@ -48,8 +48,9 @@ typedef struct OsmosNorm
 bool osmos_norm(const OsmosNorm *a, void *stream);
 
 /* rotary positions: a head's pair i < rot / 2 turned by position x turns[i] whole turns, (a, b) -> (a c - b s, b c + a s) with
-   c and s the angle's cosine and sine times `scale`; the values from rot on stay. the angle is in float64, so that far
-   positions turn as exactly as near ones. */
+   c and s the angle's cosine and sine times `scale`; the values from rot on stay. the product is formed exactly and its
+   fraction of a turn in float64, so that far positions turn by turns[i] as exactly as near ones, up to 2^53 turns (a table's
+   own rounding to float64 grows with the position: osmos_rope_turns' first pair is 2^-24 of a turn off at 2^31 at most). */
 #define OSMOS_ROPE_HALVES 0u /* pair i: values i and i + rot / 2 */
 #define OSMOS_ROPE_PAIRS 1u  /* pair i: values 2 i and 2 i + 1 */
 

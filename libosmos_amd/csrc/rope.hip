@@ -6,10 +6,11 @@
 namespace osm {
 namespace rows {
 
-// sine and cosine of t turns: the fraction of a quarter turn in float64, then the series on [-pi/4, pi/4] in float (the
-// first terms left out are under 2^-29 of the results')
-__device__ inline void sin_cos(double t, float& s, float& c) {
-  const double q = 4.0 * (t - __builtin_rint(t)), k = __builtin_rint(q);
+// sine and cosine of pos x turn turns: the product exactly (what its rounding leaves is added to its fraction: at position 2^31 the
+// rounding alone is up to 2^-25 of a turn, more than the angle's own to float), the fraction of a quarter turn in float64, then the
+// series on [-pi/4, pi/4] in float (the first terms left out are under 2^-28.5 of the results')
+__device__ inline void sin_cos(double pos, double turn, float& s, float& c) {
+  const double t = pos * turn, q = 4.0 * (t - __builtin_rint(t) + __builtin_fma(pos, turn, -t)), k = __builtin_rint(q);
   const float x = (float) ((q - k) * 1.5707963267948966), z = x * x;
   float a = __builtin_fmaf(z, 2.7557319e-6f, -1.9841270e-4f);
   a = __builtin_fmaf(z, a, 8.3333333e-3f);
@@ -20,7 +21,7 @@ __device__ inline void sin_cos(double t, float& s, float& c) {
   b = __builtin_fmaf(z, b, 4.1666668e-2f);
   b = __builtin_fmaf(z, b, -0.5f);
   b = __builtin_fmaf(z, b, 1.0f);
-  const int n = (int) k;  // (-2 .. 2)
+  const int n = (int) k;  // (-4 .. 4 where the turns are under 2^53)
   s = n & 1 ? b : a, c = n & 1 ? a : b;
   s = n & 2 ? -s : s, c = (n + 1) & 2 ? -c : c;
 }
@@ -120,7 +121,7 @@ __global__ __launch_bounds__(64 * kRopeWaves) void rope_kernel(RopeArgs a, const
   for (int i = 0; i < 2; i++)
     if (64 * i < (int) half) {
       float sine, cosine;
-      sin_cos((double) pos * turns[i], sine, cosine);
+      sin_cos((double) pos, turns[i], sine, cosine);
       if (lane + 64 * i < half) angle[wave][lane + 64 * i] = make_float2(cosine * a.scale, sine * a.scale);
     }
   wave_order();
