@@ -87,6 +87,7 @@ inline bool turns_of(const OsmosRopeScaling* s, uint32_t rot, double* turns, flo
     const double at = rot / (2.0 * log(base));
     first = floor(at * log(s->context / (two_pi * s->high))), last = ceil(at * log(s->context / (two_pi * s->low)));
     first = first < 0 ? 0 : first, last = last > rot - 1.0 ? rot - 1.0 : last;
+    if (last <= 0) first = -1, last = 0;  // (a context so short that the first pair makes no more than `slow`: all divided)
     if (last - first < 0.001) last = first + 0.001;
   }
   for (uint32_t i = 0; i < rot / 2; i++) {
