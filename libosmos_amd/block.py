@@ -25,6 +25,7 @@ def _weight(norm, dim):
     import torch
     if norm is not None and (norm.dtype != torch.float32 or tuple(norm.shape) != (dim,) or not norm.is_contiguous() or not norm.is_cuda):
         raise TypeError("norm is a contiguous float32 device tensor of dim values")
+    row_calls._on_device((norm,))
     return norm
 
 
@@ -41,8 +42,10 @@ def _tiles(norm, eps, x, add, x16, overflow, stream):
     _need(capi.lib().osmos_norm(ctypes.byref(d), stream), "osmos_norm")
 
 
-def _check_rows(owner, named, shape):
+def _check_rows(owner, named, shape, device):
     import torch
+    if torch.cuda.current_device() != device.index:
+        raise RuntimeError("%s.forward: its buffers are on %s, which is not current" % (owner, device))
     for t, name in named:
         if t is None:
             continue
@@ -50,6 +53,8 @@ def _check_rows(owner, named, shape):
             raise TypeError("%s.forward: %s is a contiguous float32 device tensor" % (owner, name))
         if tuple(t.shape) != shape:
             raise ValueError("%s.forward: %s is (rows of the step, dim)" % (owner, name))
+        if t.device != device:
+            raise ValueError("%s.forward: %s is on another device than the buffers (%s, %s)" % (owner, name, t.device, device))
 
 
 class AttentionLayer:
@@ -116,7 +121,7 @@ class AttentionLayer:
         if getattr(calls, "owner", None) is not self:
             raise ValueError("AttentionLayer.forward: calls of another layer")
         L, n, b, (append, attention) = capi.lib(), calls.n, calls.buffers, calls
-        _check_rows("AttentionLayer", ((x, "x"), (out, "out"), (add, "add")), (n, self.dim))
+        _check_rows("AttentionLayer", ((x, "x"), (out, "out"), (add, "add")), (n, self.dim), b["qkv"].device)
         _tiles(self.norm, self.eps, x, add, b["x16"], self.overflow, stream)
         stride = b["qkv"].stride(0)
         for ((t, w), rows), y in zip(self.w, (b["q"], b["k"], b["v"])):
@@ -163,7 +168,7 @@ class TokenHead:
         if getattr(calls, "owner", None) is not self:
             raise ValueError("TokenHead.forward: calls of another head")
         (x16, logits), n = calls.buffers, calls.n
-        _check_rows("TokenHead", ((x, "x"), (add, "add")), (n, self.dim))
+        _check_rows("TokenHead", ((x, "x"), (add, "add")), (n, self.dim), logits.device)
         _tiles(self.norm, self.eps, x, add, x16, self.overflow, stream)
         _need(capi.lib().mm_run(self.w[0], capi.addr(self.w[1]), self.vocab, self.dim, capi.addr(x16), n, capi.addr(logits), self.vocab,
                                 stream), "mm_run")
