@@ -124,8 +124,8 @@ typedef struct OsmosSample
   uint32_t type, n, vocab;
 } OsmosSample;
 
-/* the device memory (256-byte aligned) that the call needs as its workspace, 0 for none; a workspace is written before it is
-   read, and calls that share one are ordered on one stream */
+/* the device memory (256-byte aligned) that the call needs as its workspace, 0 for none; what a workspace holds before a call
+   does not matter, and calls that share one are ordered on one stream */
 uint64_t osmos_sample_workspace(const OsmosSample *a);
 bool osmos_sample(const OsmosSample *a, void *workspace, uint64_t workspace_bytes, void *stream);
 
