@@ -20,8 +20,8 @@ extern "C" {
 #define OSMOS_NORM_MAX_DIM 65536u
 
 /* s = x + add (float, rounded once); y = (s r) (weight + offset), each product rounded, with r = 1 / sqrt(mean of s^2 + eps)
-   rounded once from float64 (the squares and their sum are in float64: a row's values never depend on the order of its sum,
-   on the other rows or on what else is written). n rows of dim values, row t at x + t x_stride (values). outputs, any of them:
+   rounded once from float64 (the squares are exact and summed in float64, in an order that type and dim alone fix: a row's bits
+   do not depend on the other rows, on their number or on what else is written). n rows of dim values, row t at x + t x_stride (values). outputs, any of them:
      sum      s, rounded once to `type`; may be x or add (in place)
      out      y, rounded once to out_type
      x16      y as mm_x16's tiles (include/osmos/gpu/mm.h), the bytes that mm_x16 makes of float rows y, the rows past n up to a
@@ -50,7 +50,7 @@ bool osmos_norm(const OsmosNorm *a, void *stream);
 /* rotary positions: a head's pair i < rot / 2 turned by position x turns[i] whole turns, (a, b) -> (a c - b s, b c + a s) with
    c and s the angle's cosine and sine times `scale`; the values from rot on stay. the product is formed exactly and its
    fraction of a turn in float64, so that far positions turn by turns[i] as exactly as near ones, up to 2^53 turns (a table's
-   own rounding to float64 grows with the position: osmos_rope_turns' first pair is 2^-24 of a turn off at 2^31 at most). */
+   own rounding to float64 grows with the position: osmos_rope_turns' first pair, unscaled, is 2^-25 of a turn off at 2^31). */
 #define OSMOS_ROPE_HALVES 0u /* pair i: values i and i + rot / 2 */
 #define OSMOS_ROPE_PAIRS 1u  /* pair i: values 2 i and 2 i + 1 */
 
@@ -103,11 +103,13 @@ bool osmos_rope_append(const OsmosRope *a, const OsmosKv *kv, uint32_t layer, co
    tokens stand in the order of their logits, the greatest first, the lower index first among equals; of these are kept
      the first top_k (0 or less: all),
      of those the first whose weights sum up to top_p of theirs (1 or more: all; at least one token), and
-     those of at least min_p times the greatest weight (0 or less: all);
+     those of at least min_p times the greatest weight (0 or less: all; over 1: as 1);
    drawn is the first kept token whose running sum of weights passes u (0 <= u < 1) times the kept ones' sum. temperature 0,
    less or NaN: the first token. a logit of -infinity or NaN is never chosen nor kept, +infinity counts as its type's
-   greatest value; a row of nothing else gives token -1, prob 0, kept 0. weights under 2^-44 of the greatest count as zero in the sums. NaN
-   in top_p or min_p: that limit does not hold; u is clamped into its range, NaN counts as 0.
+   greatest value; a row of nothing else gives token -1, prob 0, kept 0. the sums are whole numbers of 2^-42 of the greatest weight: a
+   weight under 2^-44.5 of it counts as zero, and the tokens of each 23rd of an octave are summed and then rounded to such a unit, so
+   that one of under 2^-43 by itself adds nothing. NaN in top_p or min_p: that limit does not hold; u is clamped into its range, NaN
+   counts as 0. outputs overlap neither inputs nor one another.
    the same call gives the same answer, and a row's answer does not depend on the other rows. */
 #define OSMOS_SAMPLE_MAX_VOCAB (1u << 20)
 typedef struct OsmosSample

@@ -109,7 +109,7 @@ struct NormArgs {
 
 // a row a workgroup (short ones: a wave), its values in registers between the sum of their squares and their stores: K pieces of 16
 // bytes a thread. bound by memory where the rows are many: 4096 rows of 6144 floats and as many to add, the sums and f16 tiles
-// written, 73 us for 352 MB (4.8 TB/s, what a large copy reaches); by latency where they are few: one row of 4096 3.0 us, the launch,
+// written, 69 us for 352 MB (5.1 TB/s, more than a large copy reaches); by latency where they are few: one row of 4096 3.0 us, the launch,
 // one trip to memory, the sum over the row (lane moves, then LDS) and the stores
 template <uint32_t T, int K, bool TAIL>
 __global__ __launch_bounds__(1024) void norm_kernel(NormArgs a) {
@@ -231,9 +231,10 @@ bool norm_launch(const OsmosNorm* a, hipStream_t s) {
   const uint32_t pieces = (a->dim + per<T>() - 1) / per<T>(), rows = a->x16 ? (a->n + 15) / 16 * 16 : a->n;
   NormArgs b = {a->x, a->add, a->sum, a->weight, a->out, (_Float16*) a->x16, a->overflow, a->codes, a->scales, a->x_stride, a->add_stride,
                 a->sum_stride, a->out_stride, a->weight_type, a->out_type, a->n, a->dim, a->eps, a->offset, 1.0 / a->dim, 0, a->x16 != nullptr};
-  // a piece a thread as far as 16 waves go: 1 (2, 4, 8) pieces a thread where the rows are many take 73 us (72, 80, 85) for 4096 rows of
-  // 6144 floats into tiles, 50 (53, 57, 58) for 8192 of 4096 bf16, 13.0 (12.9, 12.3, 13.0) for 1000 of 4096 floats; one row of
-  // 4096 3.6 (4 pieces: 4.3)
+  // as many waves as there are pieces for, 16 at most (then 2 pieces a thread and more). for such waves (a half, a quarter, an eighth of
+  // them, 16 at most), sums written too: one row of 4096 floats into tiles 3.7 us (3.6, 4.4, 6.9), 48 of 2048 3.5 (3.8, 4.7, 7.4), 1000
+  // of 4096 12.7 (10.5, 11.2, 13.9), 4096 of 6144 68.5 (68.8, 72.9, 83.0), 8192 bf16 rows of 4096 into rows 39.7 (41.7, 43.2, 46.0): the
+  // best, or 3 % from it, but for the 1000 rows
   const uint32_t waves = (pieces + 63) / 64;
   b.waves = waves > 16 ? 16 : waves;
   const uint32_t k = (pieces + b.waves * 64 - 1) / (b.waves * 64);

@@ -305,7 +305,7 @@ struct Tokens {
         for (uint32_t j = 0; j < kPer<T>; j++) hits = hits + hits + in(x[k].at(j));  // (the first one's bit the highest)
     };
     static_assert(P * kPer<T> <= 32);
-    // (& and |: as && and || each comparison is a branch, 13 instructions a token in all, and 33 million bf16 logits take 16.4 us, so 15.8)
+    // (& and |: as && and || each comparison is a branch, 13 instructions a bf16 token in all instead of 11)
     if (spans == 1) test([&](float v) { return (v >= l0) & (v <= h0); });
     else if (spans == 2) test([&](float v) { return ((v >= l0) & (v <= h0)) | ((v >= l1) & (v <= h1)); });
     else test([&](float v) { return ((v >= l0) & (v <= h0)) | ((v >= l1) & (v <= h1)) | ((v >= l2) & (v <= h2)) | ((v >= l3) & (v <= h3)); });
@@ -456,8 +456,8 @@ __device__ inline void scan_slice(R& row, const Order<T>& order, float temperatu
 // 16 bytes of a slice a thread and round, and of a row that is one slice
 template <uint32_t T, bool VALUES> constexpr int kPieces = VALUES ? 4 : 16 / kPer<T>;
 template <uint32_t T> constexpr int kRowPieces = 32 / kPer<T>;
-// bound by its vector and LDS instructions: some 25 and two atomics a token (48 rows of 151001 floats 14.5 us); by value 5 and one (256 rows
-// of 129024 bf16 25.5 us; token by token the call takes 13 us more)
+// bound by its vector and LDS instructions: in all 33 and 3 a token, of which two are atomics (48 rows of 151001 floats 14.5 us); by value
+// 12 and 1.8 (256 rows of 129024 bf16 25.3 us; token by token the call takes 16 us more)
 template <uint32_t T, bool VALUES>
 __global__ __launch_bounds__(kSampleThreads, 8) void scan_kernel(SampleArgs a) {
   __shared__ ScanOf<VALUES> l;
@@ -678,7 +678,7 @@ __device__ inline bool planned(const Plan& p, float x, uint32_t& past) {
   return slot_of(p, b) >= 0;
 }
 
-// the planned bins' tokens of a row, in any order: 48 rows of 151001 floats 8 us, 256 of 129024 bf16 15.5 (4.3 TB/s)
+// the planned bins' tokens of a row, in any order: 48 rows of 151001 floats 8.4 us, 256 of 129024 bf16 16.2 (4.1 TB/s)
 constexpr int kListThreads = 256, kListPieces = 4;
 template <uint32_t T>
 __global__ __launch_bounds__(kListThreads) void list_kernel(SampleArgs a, uint32_t blocks) {
@@ -769,7 +769,8 @@ __device__ Cut find(Near<T>& row, const Scale& sc, const Prefix& prefix, DrawLds
 }
 
 // bins of more tokens than the list or a part holds, or limits that leave a bound over many bins: one by one, each bin looked
-// through as often as it takes
+// through as often as it takes, by one workgroup a row: 64 rows of 128256 floats (normal, deviation 1.5), top_p 0.9, are 44 us at a
+// temperature of 0.7 and 201 at 1.5, where the limits' bins hold some 2500 tokens; of 262144 (2.5), top_p 0.95, 55 and 363
 template <uint32_t T>
 __device__ __attribute__((noinline)) void draw_slowly(const void* logits, uint32_t vocab, const Order<T>& order, const Plan& p, Prefix& prefix,
                                                       const uint64_t* list, DrawLds& l, Cut& cut, Cut& d, double& least_y) {
@@ -1034,7 +1035,7 @@ __global__ __launch_bounds__(kSampleThreads) void probs_kernel(SampleArgs a, uin
 inline int index_bits(uint32_t vocab) { return vocab > 1 ? 32 - __builtin_clz(vocab - 1) : 0; }
 // a row of up to 32768 tokens is one slice. VALUES: bf16's tokens are counted by value, where there are many: a slice then costs the same
 // whatever it holds (its values are put into bins at the end), so it is as long as leaves 512 of them. 256 / 128 / 64 / 1 rows of
-// 129024: 62 / 49 / 38 / 40 us by values, 76 / 50 / 38 / 30 token by token
+// 129024: 60 / 44 / 35 / 29 us by values, 76 / 49 / 37 / 28 token by token
 constexpr uint32_t kRow = 32768;
 inline bool by_values(const OsmosSample* a) {
   return a->type == OSMOS_BF16 && a->vocab > kRow && (uint64_t) a->n * ((a->vocab + kValueSlice - 1) / kValueSlice) >= 512;
