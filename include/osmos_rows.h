@@ -21,7 +21,8 @@ extern "C" {
 
 /* s = x + add (float, rounded once); y = (s r) (weight + offset), each product rounded, with r = 1 / sqrt(mean of s^2 + eps)
    rounded once from float64 (the squares are exact and summed in float64, in an order that type and dim alone fix: a row's bits
-   do not depend on the other rows, on their number or on what else is written). n rows of dim values, row t at x + t x_stride (values). outputs, any of them:
+   do not depend on the other rows, on their number or on what else is written). n rows of dim values, row t at x + t x_stride
+   (values). outputs, any of them:
      sum      s, rounded once to `type`; may be x or add (in place)
      out      y, rounded once to out_type
      x16      y as mm_x16's tiles (include/osmos/gpu/mm.h), the bytes that mm_x16 makes of float rows y, the rows past n up to a
